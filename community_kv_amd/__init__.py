@@ -14,6 +14,14 @@ from community_kv_amd.config import CommunityKVConfig, GraphAggregation, Partiti
 from community_kv_amd.graph.partition import leiden_max_iterations, partition_graphs, partition_query_groups
 from community_kv_amd.runtime import CommunityKVRuntime
 
+# the 8-bit cache has no counterpart in the reference, whose __all__ this keeps
+from community_kv_amd.attention.quantized import (  # noqa: F401
+    QuantizedKVCache,
+    evict,
+    quantized_append,
+    quantized_attention,
+)
+
 __all__ = [
     "ATTENTION_IMPLEMENTATION",
     "CommunityKVAttention",

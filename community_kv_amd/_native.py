@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(PACKAGE_DIR, "libckv_amd.so")
 SOURCES = [os.path.join(PACKAGE_DIR, "csrc", name)
            for name in ("ckv_decode.hip", "ckv_select.hip", "ckv_attend.hip", "ckv_prefill.hip", "ckv_diag.hip",
                                 "ckv_state.hip", "ckv_adjacency.hip", "ckv_leiden.hip", "ckv_noalloc.hip",
-                                "ckv_select_large.hip")]
+                                "ckv_select_large.hip", "ckv_quant.hip", "ckv_quant_attend.hip")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HIP_FLAGS = [
     "--offload-arch=gfx950",
@@ -39,7 +39,7 @@ FILE_FLAGS = {"ckv_prefill.hip": ["-fno-honor-nans"]}
 
 ABI_VERSION = 3
 
-CKV_BF16, CKV_F32, CKV_E4M3 = 0, 1, 2
+CKV_BF16, CKV_F32, CKV_E4M3, CKV_F16 = 0, 1, 2, 3
 CKV_SELECT_BUDGET, CKV_SELECT_TOPK = 0, 1
 CKV_ASSIGN_NONE, CKV_ASSIGN_DELTA_Q, CKV_ASSIGN_NEAREST = 0, 1, 2
 
@@ -95,6 +95,11 @@ EXPORTED_SYMBOLS = (
     "ckv_adjacency_workspace_bytes",
     "ckv_adjacency_capacity",
     "ckv_build_adjacency",
+    "ckv_quant_append",
+    "ckv_quant_attention_workspace_bytes",
+    "ckv_quant_attention",
+    "ckv_quant_evict_workspace_bytes",
+    "ckv_quant_evict",
     "ckv_host_numerics",
     "ckv_device_numerics",
     "ckv_latency_probe",
@@ -178,6 +183,16 @@ class StateBuildArgs(ctypes.Structure):
                 ("community_weight", _p), ("total_weight", _p), ("token_communities", _p), ("workspace", _p),
                 ("topk_indices", _p), ("topk_scores", _p), ("topk_heads", _i32), ("topk_rows", _i32),
                 ("topk_kappa", _i32), ("topk_group", _i32), ("topk_row0", _i32), ("lam", _f32)]
+
+
+class QuantCache(ctypes.Structure):
+    _fields_ = [("key_codes", _p), ("value_codes", _p), ("key_scales", _p), ("value_scales", _p), ("positions", _p),
+                ("weights", _p), ("cursors", _p), ("counters", _p), ("capacity", _i32), ("batch", _i32),
+                ("kv_heads", _i32), ("block", _i32)]
+
+
+class QuantRows(ctypes.Structure):
+    _fields_ = [("data", _p), ("batch_stride", _i64), ("head_stride", _i64), ("token_stride", _i64)]
 
 
 def build(verbose: bool = False) -> str:
@@ -305,6 +320,17 @@ def lib() -> ctypes.CDLL:
     handle.ckv_adjacency_capacity.restype = ctypes.c_int64
     handle.ckv_build_adjacency.argtypes = [_p, _p, _p, _i32, _i32, _i32, _i32, _f32, _p, _p, _p, _p, _p, _p]
     handle.ckv_build_adjacency.restype = ctypes.c_int
+    quant, rows = ctypes.POINTER(QuantCache), ctypes.POINTER(QuantRows)
+    handle.ckv_quant_append.argtypes = [quant, rows, rows, _i32, _p, _i32, _p]
+    handle.ckv_quant_append.restype = ctypes.c_int
+    handle.ckv_quant_attention_workspace_bytes.argtypes = [quant, _i32, _i32, _i32]
+    handle.ckv_quant_attention_workspace_bytes.restype = ctypes.c_size_t
+    handle.ckv_quant_attention.argtypes = [quant, rows, _i32, _i32, _p, _i32, _f32, _i32, _i32, _p, _p, _p, _p]
+    handle.ckv_quant_attention.restype = ctypes.c_int
+    handle.ckv_quant_evict_workspace_bytes.argtypes = [quant, _i32]
+    handle.ckv_quant_evict_workspace_bytes.restype = ctypes.c_size_t
+    handle.ckv_quant_evict.argtypes = [quant, quant, _i32, _i32, _i32, _p, _p]
+    handle.ckv_quant_evict.restype = ctypes.c_int
     handle.ckv_host_numerics.argtypes = [ctypes.c_int, _p, _p, _i64]
     handle.ckv_host_numerics.restype = ctypes.c_int
     handle.ckv_device_numerics.argtypes = [ctypes.c_int, _p, _p, _i64, _p]

@@ -5,6 +5,7 @@ from community_kv_amd.attention.cache import StaticCache, StaticCacheLayer
 from community_kv_amd.attention.decode import DecodeLayerWorkspace, decode_layer
 from community_kv_amd.attention.flash_attention import prefill_attention_topk
 from community_kv_amd.attention.kernels.packed_segments import PackedSegments
+from community_kv_amd.attention.quantized import QuantizedKVCache, evict, quantized_append, quantized_attention
 
 __all__ = [
     "ATTENTION_IMPLEMENTATION",
@@ -12,8 +13,12 @@ __all__ = [
     "DecodeLayerWorkspace",
     "HuggingFaceAttention",
     "PackedSegments",
+    "QuantizedKVCache",
     "StaticCache",
     "StaticCacheLayer",
     "decode_layer",
+    "evict",
     "prefill_attention_topk",
+    "quantized_append",
+    "quantized_attention",
 ]

@@ -1,0 +1,625 @@
+// Attention over the 8-bit KV cache (gfx950).
+//
+//   s_j = softmax_scale * s^K_j * (q . c^K_j),  out = sum_j e^{s_j - lse} s^V_j c^V_j
+//
+// E4M3 codes have four significant bits, so they are exact in bf16, and the
+// products run on v_mfma_f32_16x16x32_bf16 with the codes themselves; block
+// scales multiply the scores and the probabilities, in 32 bits.  Queries and
+// scaled probabilities are split into as many bf16 pieces as their type has
+// significant bits (bf16 queries 1, fp16 2, f32 3), each piece a product of its
+// own into the same 32-bit accumulator.
+//
+// A head's query rows are packed as token * group + query head, so that one
+// read of a key or value serves the whole group.
+#include <hip/hip_runtime.h>
+
+#include <stdio.h>
+
+#include "ckv_quant.h"
+#include "ckv_tile.h"
+
+namespace {
+using namespace ckv;
+
+constexpr int STEP = 32;       // cache rows a wave takes at a time
+constexpr int WAVES = 4;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float RESCALE = 8.0f;  // log2: how far scores may exceed the running maximum before it moves
+
+int fail(int code, const char* message) { return ckv_internal::set_error(code, message); }
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return CKV_OK;
+  static thread_local char message[160];
+  snprintf(message, sizeof(message), "%s: %s", what, hipGetErrorString(e));
+  return fail(CKV_E_LAUNCH, message);
+}
+
+struct AttendArgs {
+  ckv_quant_cache cache;
+  ckv_quant_rows query;
+  const int32_t* counts;
+  void* out;
+  float* lse;
+  float* part_max;   // [batch][kv_heads][row_pad][splits], log2
+  float* part_sum;
+  float* part_acc;   // [batch][kv_heads][splits][row_pad][128]
+  float2* stats;     // [batch][kv_heads][row_pad]: log2 maximum and 1 / sum, or null
+  float scale_log2;  // softmax_scale * log2 e
+  int32_t tokens, group, rows, row_pad, window, splits;
+};
+
+// Two E4M3 codes in the low / high half of `w` as bf16 (exact).
+template <bool HIGH>
+__device__ inline uint32_t codes_to_bf16(uint32_t w) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+}
+
+__device__ inline uint4 codes8_to_bf16(uint32_t lo, uint32_t hi) {
+  return uint4{codes_to_bf16<false>(lo), codes_to_bf16<true>(lo), codes_to_bf16<false>(hi), codes_to_bf16<true>(hi)};
+}
+
+constexpr int pieces(int dt) { return dt == CKV_BF16 ? 1 : dt == CKV_F16 ? 2 : 3; }
+
+// x as a sum of NP bf16 values (each the nearest to what is left).
+template <int NP>
+__device__ inline void split_pair(float a, float b, uint32_t* out, int stride) {
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const uint32_t w = pack_bf16x2_hw(a, b);
+    out[p * stride] = w;
+    a -= ckv_u2f(w << 16);
+    b -= ckv_u2f(w & 0xffff0000u);
+  }
+}
+
+template <int DT>
+__device__ inline void load_query8(const void* base, int64_t index, float* out) {
+  if constexpr (DT == CKV_F16) {
+    const uint4 raw = gload16(reinterpret_cast<const uint16_t*>(base) + index);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] & 0xffffu));
+      out[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
+    }
+  } else {
+    load8<DT>(base, index, out);
+  }
+}
+
+template <int DT>
+__device__ inline void store_out(void* base, int64_t index, float v) {
+  if constexpr (DT == CKV_BF16) reinterpret_cast<uint16_t*>(base)[index] = ckv_f32_to_bf16_bits(v);
+  else if constexpr (DT == CKV_F16) reinterpret_cast<_Float16*>(base)[index] = (_Float16)v;
+  else reinterpret_cast<float*>(base)[index] = v;
+}
+
+__device__ inline int new_count(const AttendArgs& a, int b) {
+  return a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
+}
+
+// The 16 query rows from `row0` as B operands of the four 32-dim steps: lane
+// (L, c) = (lane / 16, lane % 16) holds row c, dims dim_of(step, L) .. + 7 --
+// 16 neighbouring dims a lane for steps 0, 1 and for 2, 3, so that a cache row's
+// codes are read 16 bytes a lane, 64 contiguous bytes for the four lane groups.
+__device__ inline int dim_of(int s, int L) { return 64 * (s >> 1) + 16 * L + 8 * (s & 1); }
+
+template <int DT>
+struct QueryTile {
+  uint4 piece[pieces(DT)][4];
+};
+
+template <int DT>
+__device__ inline void load_query_tile(const AttendArgs& a, int b, int h, int row0, QueryTile<DT>& q) {
+  constexpr int NP = pieces(DT);
+  const int L = (threadIdx.x & 63) >> 4;
+  const int row = row0 + (threadIdx.x & 15);
+  const bool ok = row < a.rows;
+  const int t = ok ? row / a.group : 0, g = ok ? row % a.group : 0;
+  const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
+                       (int64_t)t * a.query.token_stride;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    float v[8];
+    load_query8<DT>(a.query.data, base + dim_of(s, L), v);
+    uint32_t w[NP * 4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split_pair<NP>(ok ? v[2 * i] : 0.0f, ok ? v[2 * i + 1] : 0.0f, w + i, 4);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) q.piece[p][s] = uint4{w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]};
+  }
+}
+
+// Positions that query row `row` may see: [lo, hi].
+__device__ inline void query_range(const AttendArgs& a, int row, int count, int seen, int* lo, int* hi) {
+  const int t = row / a.group;
+  const bool ok = row < a.rows && t < count;
+  const int at = seen - count + t;
+  *hi = ok ? at : -1;
+  *lo = a.window > 0 && at >= a.window ? at - a.window + 1 : 0;  // no position is negative
+}
+
+// One step's rows of a head: keys as A operands (row m of MFMA block j is cache
+// row 8 (m / 4) + 4 j + m % 4 of the step, so that an accumulator lane holds the
+// eight rows 8 L .. 8 L + 7, just what the P operand of the value product
+// takes), values 8 dims a lane of the rows 8 L + u.
+struct StepCodes {
+  uint4 k[2][2];
+  uint2 v[8];
+  float ks, vs;
+};
+
+__device__ inline int step_row(int j, int m) { return 8 * (m >> 2) + 4 * j + (m & 3); }
+
+template <bool WITH_V = true>
+__device__ inline void load_step(const QuantHead& q, int t0, int last, int block_log2, StepCodes& s) {
+  const int lane = threadIdx.x & 63, L = lane >> 4, c = lane & 15;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint8_t* p = q.key_codes + (int64_t)min(t0 + step_row(j, c), last) * D + 16 * L;
+    s.k[j][0] = gload16(p);
+    s.k[j][1] = gload16(p + 64);
+  }
+  const int blk = min(t0 + 8 * L, last) >> block_log2;
+  s.ks = gload_f32(q.key_scales + blk);
+  if constexpr (WITH_V) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+      typedef const __attribute__((address_space(1))) u32x2_t* global_u32x2_ptr;
+      const u32x2_t w = *(global_u32x2_ptr)(q.value_codes + (int64_t)min(t0 + 8 * L + u, last) * D + 8 * c);
+      s.v[u] = uint2{w[0], w[1]};
+    }
+    s.vs = gload_f32(q.value_scales + blk);
+  }
+}
+
+// Scores of a step in log2 units: sc[4 j + i] = row 8 L + 4 j + i against query
+// row c; rows past n and positions outside [lo, hi] are -inf.
+template <int DT>
+__device__ inline void step_scores(const StepCodes& s, const QueryTile<DT>& q, float scale_log2, float* sc) {
+  constexpr int NP = pieces(DT);
+  const float f = s.ks * scale_log2;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      const uint4 w = s.k[j][st >> 1];
+      const uint4 op = (st & 1) ? codes8_to_bf16(w.z, w.w) : codes8_to_bf16(w.x, w.y);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) acc = mfma_bf16(op, q.piece[p][st], acc);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc[4 * j + i] = acc[i] * f;
+  }
+}
+
+// Masks the scores of the step from t0 on: n rows in use; `positions` null where
+// every row in use is seen by every query.
+__device__ inline void mask_step(const int32_t* positions, int t0, int n, int lo, int hi, float* sc) {
+  const int L = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = t0 + 8 * L + i;
+    bool ok = r < n;
+    if (positions) {
+      const int p = gload_i32(positions + min(r, n - 1));
+      ok = ok && p >= lo && p <= hi;
+    }
+    sc[i] = ok ? sc[i] : NEG_INF;
+  }
+}
+
+// B operands of the value product: for dims 8 c + d, the rows 8 L + u.
+__device__ inline void value_operands(const uint2* v, uint4* op) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int pair = 0; pair < 2; ++pair) {  // dims 4 half + 2 pair, + 1
+      uint32_t w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t a = half ? v[2 * u].y : v[2 * u].x, b = half ? v[2 * u + 1].y : v[2 * u + 1].x;
+        // bytes (row 2u, row 2u + 1) of the first dim, then of the second
+        w[u] = __builtin_amdgcn_perm(b, a, pair ? 0x07030602u : 0x05010400u);
+      }
+      op[4 * half + 2 * pair] = uint4{codes_to_bf16<false>(w[0]), codes_to_bf16<false>(w[1]),
+                                      codes_to_bf16<false>(w[2]), codes_to_bf16<false>(w[3])};
+      op[4 * half + 2 * pair + 1] = uint4{codes_to_bf16<true>(w[0]), codes_to_bf16<true>(w[1]),
+                                          codes_to_bf16<true>(w[2]), codes_to_bf16<true>(w[3])};
+    }
+  }
+}
+
+__device__ inline bool has_nan_code(uint32_t w) {
+  // a byte is NaN where its low seven bits are all ones
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+}
+
+__device__ inline uint32_t without_nan_codes(uint32_t w) {
+  const uint32_t is = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // 0x80 in every NaN byte
+  const uint32_t all = (is >> 7) * 0xffu;
+  return w & ~all;
+}
+
+// The running softmax of 16 query rows over the steps of one wave.  m: log2
+// maximum of query row c, the same on the four lane groups; l: sum over this
+// lane's rows alone; o: accumulators, element i of block nb is query row
+// 4 L + i, dim 8 c + nb.
+struct Running {
+  float m, l;
+  f32x4_t o[8];
+};
+
+// Adds a step to a row tile's running softmax.  fix_nan: the step has masked
+// rows and NaN among its values, which `vop` holds as zeros (a product with a
+// masked row's zero probability would spread them) and `v` as they are.
+template <int DT>
+__device__ inline void add_step(const float* sc, float vs, const uint4* vop, bool fix_nan, const uint2* v, Running& r) {
+  constexpr int NP = pieces(DT);
+  float top = sc[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[i]);
+  if (__ballot(top > r.m + RESCALE) != 0) {
+    float t = fmaxf(r.m, top);
+    t = fmaxf(t, xor_f32<16>(t));
+    t = fmaxf(t, xor_f32<32>(t));
+    const float corr = r.m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(r.m - t);
+    const int L = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = __shfl(corr, 4 * L + i, 64);
+#pragma unroll
+      for (int nb = 0; nb < 8; ++nb) r.o[nb][i] *= f;
+    }
+    r.l *= corr;
+    r.m = t;
+  }
+  const float m = r.m == NEG_INF ? 0.0f : r.m;
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(sc[i] - m);
+    r.l += p[i];
+  }
+  uint32_t w[NP * 4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split_pair<NP>(p[2 * i] * vs, p[2 * i + 1] * vs, w + i, 4);
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {
+    const uint4 aop = {w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]};
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) r.o[nb] = mfma_bf16(aop, vop[nb], r.o[nb]);
+  }
+  if (fix_nan) {
+    // values of this step hold NaN, which were taken as zeros above: what is
+    // NaN is a query that sees such a row, in that dim
+    uint32_t one[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      one[i] = (sc[2 * i] == NEG_INF ? 0u : 0x3f80u) | (sc[2 * i + 1] == NEG_INF ? 0u : 0x3f800000u);
+    const uint4 aop = {one[0], one[1], one[2], one[3]};
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) {
+      uint32_t is[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t lo = (nb < 4 ? v[2 * u].x : v[2 * u].y) >> (8 * (nb & 3));
+        const uint32_t hi = (nb < 4 ? v[2 * u + 1].x : v[2 * u + 1].y) >> (8 * (nb & 3));
+        is[u] = ((lo & 0x7fu) == 0x7fu ? 0x3f80u : 0u) | ((hi & 0x7fu) == 0x7fu ? 0x3f800000u : 0u);
+      }
+      const f32x4_t hits = mfma_bf16(aop, uint4{is[0], is[1], is[2], is[3]}, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.o[nb][i] = hits[i] > 0.0f ? __builtin_nanf("") : r.o[nb][i];
+    }
+  }
+}
+
+// One workgroup of four waves takes a part of the cache rows of a (sequence,
+// head) for NR * 16 query rows; its waves take steps in turn and join in LDS.
+template <int DT, int NR>
+__global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const AttendArgs a) {
+  __shared__ float m_s[WAVES][16];
+  __shared__ float l_s[WAVES][16];
+  __shared__ float o_s[WAVES][16 * D];
+  const ckv_quant_cache& c = a.cache;
+  const int b = blockIdx.z / c.kv_heads, h = blockIdx.z % c.kv_heads;
+  const int row0 = blockIdx.x * (16 * NR), split = blockIdx.y;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, L = lane >> 4, col = lane & 15;
+  const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
+  // rows of this part: equal parts of whole rounds of the four waves
+  const int per = ((n + a.splits - 1) / a.splits + WAVES * STEP - 1) / (WAVES * STEP) * (WAVES * STEP);
+  const int lo_row = (int)min((int64_t)split * per, (int64_t)n), hi_row = min(lo_row + per, n);
+  if (split > 0 && lo_row >= n) return;  // the join knows how many parts there are
+  const QuantHead q = quant_head(c, b, h);
+  const int block_log2 = 31 - __clz(c.block);
+  QueryTile<DT> query[NR];
+  Running run[NR];
+  int lo[NR], hi[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    load_query_tile<DT>(a, b, h, row0 + 16 * r, query[r]);
+    query_range(a, row0 + 16 * r + col, count, seen, &lo[r], &hi[r]);
+    run[r].m = NEG_INF;
+    run[r].l = 0.0f;
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) run[r].o[nb] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  // with one new token and no window every row in use is at or before it
+  const bool by_position = a.window > 0 || a.tokens > 1 || count < a.tokens;
+  StepCodes cur;
+  for (int t0 = lo_row + wave * STEP; t0 < hi_row; t0 += WAVES * STEP) {
+    load_step(q, t0, n - 1, block_log2, cur);
+    const bool tail = t0 + STEP > n;
+    bool fix_nan = false;
+    uint2 raw[8];
+    if (tail || by_position) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) raw[u] = cur.v[u];
+      bool nan = false;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) nan = nan || has_nan_code(raw[u].x) || has_nan_code(raw[u].y);
+      fix_nan = __ballot(nan) != 0;
+      if (fix_nan) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) cur.v[u] = uint2{without_nan_codes(raw[u].x), without_nan_codes(raw[u].y)};
+      }
+    }
+    uint4 vop[8];
+    value_operands(cur.v, vop);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      float sc[8];
+      step_scores<DT>(cur, query[r], a.scale_log2, sc);
+      if (tail || by_position) mask_step(by_position ? q.positions : nullptr, t0, n, lo[r], hi[r], sc);
+      add_step<DT>(sc, cur.vs, vop, fix_nan, raw, run[r]);
+    }
+  }
+  // join the waves, one tile of 16 query rows after the other
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    float l = add_xor16(run[r].l);
+    l = add_xor32(l);
+    __syncthreads();
+    if (L == 0) {
+      m_s[wave][col] = run[r].m;
+      l_s[wave][col] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float4* p = reinterpret_cast<float4*>(&o_s[wave][(4 * L + i) * D + 8 * col]);
+      p[0] = float4{run[r].o[0][i], run[r].o[1][i], run[r].o[2][i], run[r].o[3][i]};
+      p[1] = float4{run[r].o[4][i], run[r].o[5][i], run[r].o[6][i], run[r].o[7][i]};
+    }
+    __syncthreads();
+    for (int x = tid; x < 16 * D; x += 64 * WAVES) {
+      const int i = x >> 7, d = x & (D - 1), row = row0 + 16 * r + i;
+      if (row >= a.rows) continue;
+      float m = m_s[0][i];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) m = fmaxf(m, m_s[w][i]);
+      const float at = m == NEG_INF ? 0.0f : m;
+      float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        // a wave without a row has zeros and a maximum of -inf
+        const float f = __builtin_amdgcn_exp2f(m_s[w][i] - at);
+        sum += l_s[w][i] * f;
+        acc += o_s[w][x] * f;
+      }
+      const int64_t bh = (int64_t)b * c.kv_heads + h;
+      if (a.splits == 1) {
+        const int t = row / a.group, g = row % a.group;
+        const int64_t hq = (int64_t)h * a.group + g, heads = (int64_t)c.kv_heads * a.group;
+        store_out<DT>(a.out, (((int64_t)b * a.tokens + t) * heads + hq) * D + d, sum == 0.0f ? 0.0f : acc / sum);
+        if (d == 0) {
+          a.lse[((int64_t)b * heads + hq) * a.tokens + t] = sum == 0.0f ? NEG_INF : (m + __log2f(sum)) * LN2;
+          if (a.stats) a.stats[bh * a.row_pad + row] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
+        }
+      } else {
+        a.part_acc[((bh * a.splits + split) * a.row_pad + row) * D + d] = acc;
+        if (d == 0) {
+          a.part_max[(bh * a.row_pad + row) * a.splits + split] = m;
+          a.part_sum[(bh * a.row_pad + row) * a.splits + split] = sum;
+        }
+      }
+    }
+  }
+}
+
+// Joins the parts of one query row (a workgroup of 128 threads, a dim each).
+template <int DT>
+__global__ __launch_bounds__(D) void attend_join_kernel(const AttendArgs a) {
+  const ckv_quant_cache& c = a.cache;
+  const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, d = threadIdx.x;
+  const int n = quant_length(c, b);
+  const int per = ((n + a.splits - 1) / a.splits + WAVES * STEP - 1) / (WAVES * STEP) * (WAVES * STEP);
+  const int parts = n > 0 ? (n + per - 1) / per : 1;
+  const int64_t bh = (int64_t)b * c.kv_heads + h;
+  const float* pm = a.part_max + (bh * a.row_pad + row) * a.splits;
+  const float* pl = a.part_sum + (bh * a.row_pad + row) * a.splits;
+  float m = NEG_INF;
+  for (int s = 0; s < parts; ++s) m = fmaxf(m, pm[s]);
+  const float at = m == NEG_INF ? 0.0f : m;
+  float sum = 0.0f, acc = 0.0f;
+  for (int s = 0; s < parts; ++s) {
+    const float f = __builtin_amdgcn_exp2f(pm[s] - at);
+    sum += pl[s] * f;
+    acc += a.part_acc[((bh * a.splits + s) * a.row_pad + row) * D + d] * f;
+  }
+  const int t = row / a.group, g = row % a.group;
+  const int64_t hq = (int64_t)h * a.group + g, heads = (int64_t)c.kv_heads * a.group;
+  store_out<DT>(a.out, (((int64_t)b * a.tokens + t) * heads + hq) * D + d, sum == 0.0f ? 0.0f : acc / sum);
+  if (d == 0) {
+    a.lse[((int64_t)b * heads + hq) * a.tokens + t] = sum == 0.0f ? NEG_INF : (m + __log2f(sum)) * LN2;
+    if (a.stats) a.stats[bh * a.row_pad + row] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
+  }
+}
+
+// Received weight: a wave owns 32 cache rows of a (sequence, head), goes over
+// all query rows with the scores computed again, and adds up what each row got
+// (no atomics: one owner a row, a fixed order).
+template <int DT>
+__global__ __launch_bounds__(64 * WAVES) void weights_kernel(const AttendArgs a) {
+  const ckv_quant_cache& c = a.cache;
+  const int h = blockIdx.y, b = blockIdx.z, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, L = lane >> 4, col = lane & 15;
+  const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
+  const int64_t first = ((int64_t)blockIdx.x * WAVES + wave) * STEP;
+  if (first >= n) return;
+  const int t0 = (int)first;
+  const QuantHead q = quant_head(c, b, h);
+  const bool by_position = a.window > 0 || a.tokens > 1 || count < a.tokens;
+  StepCodes s;
+  load_step<false>(q, t0, n - 1, 31 - __clz(c.block), s);
+  const float2* stats = a.stats + ((int64_t)b * c.kv_heads + h) * a.row_pad;
+  float got[8] = {};
+  for (int row0 = 0; row0 < a.rows; row0 += 16) {
+    QueryTile<DT> query;
+    load_query_tile<DT>(a, b, h, row0, query);
+    int lo, hi;
+    query_range(a, row0 + col, count, seen, &lo, &hi);
+    const float2 st = row0 + col < a.rows ? stats[row0 + col] : float2{0.0f, 0.0f};
+    float sc[8];
+    step_scores<DT>(s, query, a.scale_log2, sc);
+    mask_step(by_position ? q.positions : nullptr, t0, n, lo, hi, sc);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      got[i] += sc[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(sc[i] - st.x) * st.y;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float x = got[i];
+    x = add_xor_f32<1>(x);
+    x = add_xor_f32<2>(x);
+    x = add_xor_f32<4>(x);
+    x = x + xor_f32<8>(x);
+    const int row = t0 + 8 * L + i;
+    if (col == 0 && row < n) q.weights[row] += x;
+  }
+}
+
+// Query rows a workgroup: 16 while that holds all of them, else 32.
+template <int DT>
+int row_tiles(int rows) { return rows > 16 && DT == CKV_BF16 ? 2 : 1; }
+
+// Parts that the rows of a (sequence, head) are split into.
+int parts_of(const ckv_quant_cache* c, int row_blocks) {
+  const int64_t heads = (int64_t)c->batch * c->kv_heads * row_blocks;
+  const int64_t most = ((int64_t)c->capacity + WAVES * STEP - 1) / (WAVES * STEP);
+  int64_t want = (1024 + heads - 1) / heads;
+  if (want > 64) want = 64;
+  if (want > most) want = most;
+  return (int)(want < 1 ? 1 : want);
+}
+
+struct AttendLayout {
+  int splits, row_pad;
+  size_t stats, max, sum, acc, bytes;
+  AttendLayout(const ckv_quant_cache* c, int rows, bool accumulate) {
+    row_pad = (rows + 15) / 16 * 16;
+    splits = parts_of(c, row_pad / 16);
+    const size_t heads = (size_t)c->batch * c->kv_heads;
+    stats = 0;
+    size_t at = accumulate ? heads * row_pad * sizeof(float2) : 0;
+    max = at;
+    if (splits > 1) at += heads * row_pad * splits * sizeof(float);
+    sum = at;
+    if (splits > 1) at += heads * row_pad * splits * sizeof(float);
+    acc = at;
+    if (splits > 1) at += heads * row_pad * splits * D * sizeof(float);
+    bytes = at;
+  }
+};
+
+template <int DT, int NR>
+void launch_split(const AttendArgs& a, hipStream_t s) {
+  const dim3 grid((a.rows + 16 * NR - 1) / (16 * NR), a.splits, a.cache.batch * a.cache.kv_heads);
+  attend_split_kernel<DT, NR><<<grid, 64 * WAVES, 0, s>>>(a);
+}
+
+template <int DT>
+int launch_attend(const AttendArgs& a, bool accumulate, hipStream_t s) {
+  if (row_tiles<DT>(a.rows) == 2) launch_split<DT, 2>(a, s);
+  else launch_split<DT, 1>(a, s);
+  int rc = launched("ckv_quant_attention");
+  if (rc) return rc;
+  if (a.splits > 1) {
+    attend_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), D, 0, s>>>(a);
+    rc = launched("ckv_quant_attention");
+    if (rc) return rc;
+  }
+  if (accumulate) {
+    const dim3 grid((a.cache.capacity + WAVES * STEP - 1) / (WAVES * STEP), a.cache.kv_heads, a.cache.batch);
+    weights_kernel<DT><<<grid, 64 * WAVES, 0, s>>>(a);
+    rc = launched("ckv_quant_attention");
+  }
+  return rc;
+}
+
+}  // namespace
+
+extern "C" size_t ckv_quant_attention_workspace_bytes(const ckv_quant_cache* cache, int32_t query_heads,
+                                                      int32_t tokens, int32_t accumulate) {
+  if (!cache || cache->batch <= 0 || cache->kv_heads <= 0 || cache->capacity <= 0 || tokens <= 0 ||
+      query_heads <= 0 || query_heads % cache->kv_heads)
+    return 0;
+  const int64_t rows = (int64_t)tokens * (query_heads / cache->kv_heads);
+  if (rows > (1 << 24)) return 0;
+  return AttendLayout(cache, (int)rows, accumulate != 0).bytes;
+}
+
+extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant_rows* query, int32_t query_heads,
+                                   int32_t tokens, const int32_t* counts, int32_t dtype, float softmax_scale,
+                                   int32_t window, int32_t accumulate, void* out, float* lse, void* workspace,
+                                   void* stream) {
+  int rc = validate_quant_cache(cache, "ckv_quant_attention");
+  if (rc) return rc;
+  if (dtype != CKV_BF16 && dtype != CKV_F16 && dtype != CKV_F32)
+    return fail(CKV_E_INVALID, "ckv_quant_attention: dtype must be bf16, fp16 or f32");
+  if (!query || !query->data || !out || !lse) return fail(CKV_E_INVALID, "ckv_quant_attention: null argument");
+  if (query_heads <= 0 || query_heads % cache->kv_heads)
+    return fail(CKV_E_INVALID, "ckv_quant_attention: query heads must be a multiple of the cache's heads");
+  const int group = query_heads / cache->kv_heads;
+  if (group > CKV_MAX_GROUP) return fail(CKV_E_LIMIT, "ckv_quant_attention: group size exceeds 16");
+  if (tokens <= 0 || window < 0) return fail(CKV_E_INVALID, "ckv_quant_attention: tokens must be positive, window not negative");
+  if ((int64_t)tokens * group > (1 << 24)) return fail(CKV_E_LIMIT, "ckv_quant_attention: more than 2^24 query rows a head");
+  if (!(softmax_scale > 0.0f) || softmax_scale > 1e30f)
+    return fail(CKV_E_INVALID, "ckv_quant_attention: softmax_scale must be positive");
+  const int unit = dtype == CKV_F32 ? 4 : 8;
+  if (((uintptr_t)query->data & 15) || query->batch_stride % unit || query->head_stride % unit ||
+      query->token_stride % unit)
+    return fail(CKV_E_INVALID, "ckv_quant_attention: query rows must be 16-byte aligned");
+  if (accumulate && !cache->weights) return fail(CKV_E_INVALID, "ckv_quant_attention: the cache keeps no weights");
+  if ((int64_t)cache->batch * cache->kv_heads > 65535)
+    return fail(CKV_E_LIMIT, "ckv_quant_attention: more than 65535 heads over the batch");
+  const AttendLayout lay(cache, tokens * group, accumulate != 0);
+  if (lay.bytes && (!workspace || ((uintptr_t)workspace & 15)))
+    return fail(CKV_E_INVALID, "ckv_quant_attention: workspace");
+  char* ws = reinterpret_cast<char*>(workspace);
+  AttendArgs a{};
+  a.cache = *cache;
+  a.query = *query;
+  a.counts = counts;
+  a.out = out;
+  a.lse = lse;
+  a.part_max = reinterpret_cast<float*>(ws + lay.max);
+  a.part_sum = reinterpret_cast<float*>(ws + lay.sum);
+  a.part_acc = reinterpret_cast<float*>(ws + lay.acc);
+  a.stats = accumulate ? reinterpret_cast<float2*>(ws + lay.stats) : nullptr;
+  a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
+  a.tokens = tokens;
+  a.group = group;
+  a.rows = tokens * group;
+  a.row_pad = lay.row_pad;
+  a.window = window;
+  a.splits = lay.splits;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == CKV_BF16) return launch_attend<CKV_BF16>(a, accumulate != 0, s);
+  if (dtype == CKV_F16) return launch_attend<CKV_F16>(a, accumulate != 0, s);
+  return launch_attend<CKV_F32>(a, accumulate != 0, s);
+}

@@ -36,6 +36,9 @@
  *                           (graph/leiden/algorithm.py:51-161)
  *   ckv_leiden_run          run_leiden() (graph/leiden/algorithm.py:51-161), every level in one call
  *   ckv_dense_communities   the dense relabelling after it (graph/partition.py:252-286)
+ *   ckv_quant_append,       (no reference counterpart) the 8-bit KV cache: block-scaled E4M3 write,
+ *   ckv_quant_attention,    attention over it, and eviction of its least attended rows
+ *   ckv_quant_evict
  *   ckv_aggregate_coo       aggregate_coo() of the same extension (bindings.cpp:118-170,
  *                           aggregate_upper_coo in aggregate.cu:88-184)
  *   ckv_densify_count,      _densify_per_graph() (graph/leiden/algorithm.py:30-48), as two calls
@@ -71,7 +74,7 @@ enum ckv_status {
   CKV_E_LAUNCH = 3     /* the HIP runtime reported a launch error */
 };
 
-enum ckv_dtype { CKV_BF16 = 0, CKV_F32 = 1, CKV_E4M3 = 2 };
+enum ckv_dtype { CKV_BF16 = 0, CKV_F32 = 1, CKV_E4M3 = 2, CKV_F16 = 3 };  /* CKV_F16: ckv_quant_* only */
 enum ckv_selection_mode { CKV_SELECT_BUDGET = 0, CKV_SELECT_TOPK = 1 };
 enum ckv_assignment { CKV_ASSIGN_NONE = 0, CKV_ASSIGN_DELTA_Q = 1, CKV_ASSIGN_NEAREST = 2 };
 
@@ -562,6 +565,80 @@ size_t ckv_decode_static_scratch_limit(void);
 int ckv_dense_decode(const ckv_kv_cache* kv, int32_t seq_len, float softmax_scale,
                      float* partial_max, float* partial_sum, float* partial_acc,
                      void* output, float* lse, void* stream);
+
+/* 8-bit KV cache of one layer (no reference counterpart; the reference's cache
+ * is bf16).  Codes are OCP E4M3, row-major and dense; a block of `block` rows
+ * of one sequence and head has one scale for its keys and one for its values,
+ * and a value is code * scale.  A cache is a set of (position, key, value)
+ * rows: every mask goes by position, so rows may stand in any order. */
+typedef struct ckv_quant_cache {
+  void* key_codes;         /* [batch][kv_heads][capacity][128] E4M3 */
+  void* value_codes;       /* same */
+  float* key_scales;       /* [batch][kv_heads][capacity / block] */
+  float* value_scales;     /* same */
+  int32_t* positions;      /* [batch][kv_heads][capacity] */
+  float* weights;          /* [batch][kv_heads][capacity] attention received, or null */
+  int32_t* cursors;        /* [3][batch]: rows in use, tokens ever appended, overflow (1: tokens were dropped) */
+  uint32_t* counters;      /* [batch][kv_heads + 1], zero before first use; the kernels leave it zero */
+  int32_t capacity;        /* rows, a multiple of block */
+  int32_t batch;
+  int32_t kv_heads;
+  int32_t block;           /* 16, 32, 64 or 128 */
+} ckv_quant_cache;
+
+/* New rows or queries: element (b, head, t, d) at
+ * data[b*batch_stride + head*head_stride + t*token_stride + d], strides in
+ * elements and multiples of 8 (CKV_F32: of 4), data 16-byte aligned. */
+typedef struct ckv_quant_rows {
+  const void* data;
+  int64_t batch_stride;
+  int64_t head_stride;
+  int64_t token_stride;
+} ckv_quant_rows;
+
+/* Appends the first counts[b] (null: all) of `tokens` new tokens to every
+ * sequence: row lengths[b] + t takes token t at position seen[b] + t; rows past
+ * the capacity are dropped and set overflow[b].  A block's scale is the
+ * smallest power of two s >= 2^-64 with |x| <= 448 s for every finite value
+ * written into the block so far (a block's first row starts it afresh; the
+ * scale never shrinks); a code is x / s rounded to nearest even, and when a
+ * scale grows the block's earlier codes become round(code * s_old / s_new),
+ * exact unless the result is an E4M3 subnormal.  A value that is not finite
+ * becomes NaN.  weights (if any) of the new rows are zeroed.  dtype: CKV_BF16,
+ * CKV_F16 or CKV_F32.  Rows at and past the new length are left as they are. */
+int ckv_quant_append(const ckv_quant_cache* cache, const ckv_quant_rows* key, const ckv_quant_rows* value,
+                     int32_t tokens, const int32_t* counts, int32_t dtype, void* stream);
+
+/* Attention of the newest tokens over the cache: query t < counts[b] (null:
+ * tokens) of sequence b stands at position seen[b] - counts[b] + t and attends
+ * the rows of its KV head (query head / group) whose position is at most its
+ * own and, with window > 0, above its own minus window.  out
+ * [batch][tokens][query_heads][128] in the queries' dtype, lse
+ * [batch][query_heads][tokens] (natural log); a query that attends no row, or
+ * with t >= counts[b], gives zeros and -inf.  accumulate adds to
+ * weights[b][h][row] the probabilities that the head's queries gave the row
+ * (fixed summation order).  workspace:
+ * ckv_quant_attention_workspace_bytes() bytes, this call's alone. */
+size_t ckv_quant_attention_workspace_bytes(const ckv_quant_cache* cache, int32_t query_heads, int32_t tokens,
+                                           int32_t accumulate);
+int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant_rows* query, int32_t query_heads,
+                        int32_t tokens, const int32_t* counts, int32_t dtype, float softmax_scale, int32_t window,
+                        int32_t accumulate, void* out, float* lse, void* workspace, void* stream);
+
+/* Reduces every sequence of more than `keep` rows to `keep` rows a head: those
+ * with position < num_sink or >= seen - recent, then the largest weights (NaN
+ * above all), equal ones by the lower row (num_sink + recent <= keep; more
+ * protected rows than that are taken by the lower row).  Kept rows below
+ * `keep` stay; the j-th freed row below it takes the j-th kept row from above,
+ * written by ckv_quant_append's scale rule.  Positions and weights move with
+ * their rows, lengths become min(length, keep), rows at and past the new
+ * length are left as they are.  into (null: in place): the rows go to another
+ * cache of the same batch, heads and block and at least min(keep, capacity)
+ * rows, whose cursors are set, and `cache` stays as it is.  workspace:
+ * ckv_quant_evict_workspace_bytes() bytes, this call's alone. */
+size_t ckv_quant_evict_workspace_bytes(const ckv_quant_cache* cache, int32_t keep);
+int ckv_quant_evict(const ckv_quant_cache* cache, const ckv_quant_cache* into, int32_t keep, int32_t num_sink,
+                    int32_t recent, void* workspace, void* stream);
 
 /* Diagnostic, no counterpart in the reference: latency probes behind the
  * decode step's measured cost model (bench.py --workload floor).  kind 0: one
