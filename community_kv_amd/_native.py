@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(PACKAGE_DIR, "libckv_amd.so")
 SOURCES = [os.path.join(PACKAGE_DIR, "csrc", name)
            for name in ("ckv_decode.hip", "ckv_select.hip", "ckv_attend.hip", "ckv_prefill.hip", "ckv_diag.hip",
                                 "ckv_state.hip", "ckv_adjacency.hip", "ckv_leiden.hip", "ckv_noalloc.hip",
-                                "ckv_select_large.hip", "ckv_quant.hip", "ckv_quant_attend.hip")]
+                                "ckv_select_large.hip", "ckv_quant.hip", "ckv_quant_attend.hip", "ckv_quant_rows.hip")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HIP_FLAGS = [
     "--offload-arch=gfx950",
@@ -323,7 +323,7 @@ def lib() -> ctypes.CDLL:
     quant, rows = ctypes.POINTER(QuantCache), ctypes.POINTER(QuantRows)
     handle.ckv_quant_append.argtypes = [quant, rows, rows, _i32, _p, _i32, _p]
     handle.ckv_quant_append.restype = ctypes.c_int
-    handle.ckv_quant_attention_workspace_bytes.argtypes = [quant, _i32, _i32, _i32]
+    handle.ckv_quant_attention_workspace_bytes.argtypes = [quant, _i32, _i32, _i32, _i32]
     handle.ckv_quant_attention_workspace_bytes.restype = ctypes.c_size_t
     handle.ckv_quant_attention.argtypes = [quant, rows, _i32, _i32, _p, _i32, _f32, _i32, _i32, _p, _p, _p, _p]
     handle.ckv_quant_attention.restype = ctypes.c_int

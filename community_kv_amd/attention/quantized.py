@@ -255,7 +255,7 @@ def quantized_attention(query: torch.Tensor, cache: QuantizedKVCache, *, softmax
         return out, lse
     lib = nat.lib()
     struct = ctypes.byref(cache._struct)
-    size = lib.ckv_quant_attention_workspace_bytes(struct, heads, tokens, accumulate)
+    size = lib.ckv_quant_attention_workspace_bytes(struct, heads, tokens, _DTYPES[query.dtype], accumulate)
     workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     rows, query = _rows(query)
     _call(device, lib.ckv_quant_attention, struct, ctypes.byref(rows), heads, tokens, nat.ptr(counts),

@@ -13,18 +13,14 @@
 // read of a key or value serves the whole group.
 #include <hip/hip_runtime.h>
 
-#include <stdio.h>
-
-#include "ckv_quant.h"
-#include "ckv_tile.h"
+#include "ckv_quant_attend.h"
 
 namespace {
 using namespace ckv;
 
-constexpr int STEP = 32;       // cache rows a wave takes at a time
+constexpr int STEP = 32;  // cache rows a wave takes at a time
 constexpr int WAVES = 4;
-constexpr float LN2 = 0.6931471805599453f;
-constexpr float RESCALE = 8.0f;  // log2: how far scores may exceed the running maximum before it moves
+static_assert(PART_UNIT % (WAVES * STEP) == 0, "parts are whole rounds of the waves");
 
 int fail(int code, const char* message) { return ckv_internal::set_error(code, message); }
 
@@ -34,71 +30,6 @@ int launched(const char* what) {
   static thread_local char message[160];
   snprintf(message, sizeof(message), "%s: %s", what, hipGetErrorString(e));
   return fail(CKV_E_LAUNCH, message);
-}
-
-struct AttendArgs {
-  ckv_quant_cache cache;
-  ckv_quant_rows query;
-  const int32_t* counts;
-  void* out;
-  float* lse;
-  float* part_max;   // [batch][kv_heads][row_pad][splits], log2
-  float* part_sum;
-  float* part_acc;   // [batch][kv_heads][splits][row_pad][128]
-  float2* stats;     // [batch][kv_heads][row_pad]: log2 maximum and 1 / sum, or null
-  float scale_log2;  // softmax_scale * log2 e
-  int32_t tokens, group, rows, row_pad, window, splits;
-};
-
-// Two E4M3 codes in the low / high half of `w` as bf16 (exact).
-template <bool HIGH>
-__device__ inline uint32_t codes_to_bf16(uint32_t w) {
-  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
-}
-
-__device__ inline uint4 codes8_to_bf16(uint32_t lo, uint32_t hi) {
-  return uint4{codes_to_bf16<false>(lo), codes_to_bf16<true>(lo), codes_to_bf16<false>(hi), codes_to_bf16<true>(hi)};
-}
-
-constexpr int pieces(int dt) { return dt == CKV_BF16 ? 1 : dt == CKV_F16 ? 2 : 3; }
-
-// x as a sum of NP bf16 values (each the nearest to what is left).
-template <int NP>
-__device__ inline void split_pair(float a, float b, uint32_t* out, int stride) {
-#pragma unroll
-  for (int p = 0; p < NP; ++p) {
-    const uint32_t w = pack_bf16x2_hw(a, b);
-    out[p * stride] = w;
-    a -= ckv_u2f(w << 16);
-    b -= ckv_u2f(w & 0xffff0000u);
-  }
-}
-
-template <int DT>
-__device__ inline void load_query8(const void* base, int64_t index, float* out) {
-  if constexpr (DT == CKV_F16) {
-    const uint4 raw = gload16(reinterpret_cast<const uint16_t*>(base) + index);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      out[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] & 0xffffu));
-      out[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
-    }
-  } else {
-    load8<DT>(base, index, out);
-  }
-}
-
-template <int DT>
-__device__ inline void store_out(void* base, int64_t index, float v) {
-  if constexpr (DT == CKV_BF16) reinterpret_cast<uint16_t*>(base)[index] = ckv_f32_to_bf16_bits(v);
-  else if constexpr (DT == CKV_F16) reinterpret_cast<_Float16*>(base)[index] = (_Float16)v;
-  else reinterpret_cast<float*>(base)[index] = v;
-}
-
-__device__ inline int new_count(const AttendArgs& a, int b) {
-  return a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
 }
 
 // The 16 query rows from `row0` as B operands of the four 32-dim steps: lane
@@ -113,7 +44,7 @@ struct QueryTile {
 };
 
 template <int DT>
-__device__ inline void load_query_tile(const AttendArgs& a, int b, int h, int row0, QueryTile<DT>& q) {
+__device__ inline void load_query_tile(const QuantAttendArgs& a, int b, int h, int row0, QueryTile<DT>& q) {
   constexpr int NP = pieces(DT);
   const int L = (threadIdx.x & 63) >> 4;
   const int row = row0 + (threadIdx.x & 15);
@@ -131,15 +62,6 @@ __device__ inline void load_query_tile(const AttendArgs& a, int b, int h, int ro
 #pragma unroll
     for (int p = 0; p < NP; ++p) q.piece[p][s] = uint4{w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]};
   }
-}
-
-// Positions that query row `row` may see: [lo, hi].
-__device__ inline void query_range(const AttendArgs& a, int row, int count, int seen, int* lo, int* hi) {
-  const int t = row / a.group;
-  const bool ok = row < a.rows && t < count;
-  const int at = seen - count + t;
-  *hi = ok ? at : -1;
-  *lo = a.window > 0 && at >= a.window ? at - a.window + 1 : 0;  // no position is negative
 }
 
 // One step's rows of a head: keys as A operands (row m of MFMA block j is cache
@@ -322,7 +244,7 @@ __device__ inline void add_step(const float* sc, float vs, const uint4* vop, boo
 // One workgroup of four waves takes a part of the cache rows of a (sequence,
 // head) for NR * 16 query rows; its waves take steps in turn and join in LDS.
 template <int DT, int NR>
-__global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const QuantAttendArgs a) {
   __shared__ float m_s[WAVES][16];
   __shared__ float l_s[WAVES][16];
   __shared__ float o_s[WAVES][16 * D];
@@ -331,8 +253,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const AttendAr
   const int row0 = blockIdx.x * (16 * NR), split = blockIdx.y;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, L = lane >> 4, col = lane & 15;
   const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
-  // rows of this part: equal parts of whole rounds of the four waves
-  const int per = ((n + a.splits - 1) / a.splits + WAVES * STEP - 1) / (WAVES * STEP) * (WAVES * STEP);
+  const int per = part_rows(n, a.splits);
   const int lo_row = (int)min((int64_t)split * per, (int64_t)n), hi_row = min(lo_row + per, n);
   if (split > 0 && lo_row >= n) return;  // the join knows how many parts there are
   const QuantHead q = quant_head(c, b, h);
@@ -413,11 +334,11 @@ __global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const AttendAr
       }
       const int64_t bh = (int64_t)b * c.kv_heads + h;
       if (a.splits == 1) {
-        const int t = row / a.group, g = row % a.group;
-        const int64_t hq = (int64_t)h * a.group + g, heads = (int64_t)c.kv_heads * a.group;
-        store_out<DT>(a.out, (((int64_t)b * a.tokens + t) * heads + hq) * D + d, sum == 0.0f ? 0.0f : acc / sum);
+        int64_t at_out, at_lse;
+        output_index(a, b, h, row, &at_out, &at_lse);
+        store_out<DT>(a.out, at_out + d, sum == 0.0f ? 0.0f : acc / sum);
         if (d == 0) {
-          a.lse[((int64_t)b * heads + hq) * a.tokens + t] = sum == 0.0f ? NEG_INF : (m + __log2f(sum)) * LN2;
+          a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + __log2f(sum)) * LN2;
           if (a.stats) a.stats[bh * a.row_pad + row] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
         }
       } else {
@@ -433,11 +354,11 @@ __global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const AttendAr
 
 // Joins the parts of one query row (a workgroup of 128 threads, a dim each).
 template <int DT>
-__global__ __launch_bounds__(D) void attend_join_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(D) void attend_join_kernel(const QuantAttendArgs a) {
   const ckv_quant_cache& c = a.cache;
   const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, d = threadIdx.x;
   const int n = quant_length(c, b);
-  const int per = ((n + a.splits - 1) / a.splits + WAVES * STEP - 1) / (WAVES * STEP) * (WAVES * STEP);
+  const int per = part_rows(n, a.splits);
   const int parts = n > 0 ? (n + per - 1) / per : 1;
   const int64_t bh = (int64_t)b * c.kv_heads + h;
   const float* pm = a.part_max + (bh * a.row_pad + row) * a.splits;
@@ -451,11 +372,11 @@ __global__ __launch_bounds__(D) void attend_join_kernel(const AttendArgs a) {
     sum += pl[s] * f;
     acc += a.part_acc[((bh * a.splits + s) * a.row_pad + row) * D + d] * f;
   }
-  const int t = row / a.group, g = row % a.group;
-  const int64_t hq = (int64_t)h * a.group + g, heads = (int64_t)c.kv_heads * a.group;
-  store_out<DT>(a.out, (((int64_t)b * a.tokens + t) * heads + hq) * D + d, sum == 0.0f ? 0.0f : acc / sum);
+  int64_t at_out, at_lse;
+  output_index(a, b, h, row, &at_out, &at_lse);
+  store_out<DT>(a.out, at_out + d, sum == 0.0f ? 0.0f : acc / sum);
   if (d == 0) {
-    a.lse[((int64_t)b * heads + hq) * a.tokens + t] = sum == 0.0f ? NEG_INF : (m + __log2f(sum)) * LN2;
+    a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + __log2f(sum)) * LN2;
     if (a.stats) a.stats[bh * a.row_pad + row] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
   }
 }
@@ -464,7 +385,7 @@ __global__ __launch_bounds__(D) void attend_join_kernel(const AttendArgs a) {
 // all query rows with the scores computed again, and adds up what each row got
 // (no atomics: one owner a row, a fixed order).
 template <int DT>
-__global__ __launch_bounds__(64 * WAVES) void weights_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendArgs a) {
   const ckv_quant_cache& c = a.cache;
   const int h = blockIdx.y, b = blockIdx.z, wave = threadIdx.x >> 6;
   const int lane = threadIdx.x & 63, L = lane >> 4, col = lane & 15;
@@ -507,53 +428,68 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const AttendArgs a)
 template <int DT>
 int row_tiles(int rows) { return rows > 16 && DT == CKV_BF16 ? 2 : 1; }
 
-// Parts that the rows of a (sequence, head) are split into.
-int parts_of(const ckv_quant_cache* c, int row_blocks) {
+// Parts that the rows of a (sequence, head) are split into: enough workgroups
+// to fill the chip (1,024 of the few-row kernel's, four a compute unit; 256 of
+// the many-row kernel's, which has a compute unit to itself).
+int parts_of(const ckv_quant_cache* c, int64_t row_blocks, int64_t workgroups) {
   const int64_t heads = (int64_t)c->batch * c->kv_heads * row_blocks;
-  const int64_t most = ((int64_t)c->capacity + WAVES * STEP - 1) / (WAVES * STEP);
-  int64_t want = (1024 + heads - 1) / heads;
+  const int64_t most = ((int64_t)c->capacity + PART_UNIT - 1) / PART_UNIT;
+  int64_t want = (workgroups + heads - 1) / heads;
   if (want > 64) want = 64;
   if (want > most) want = most;
   return (int)(want < 1 ? 1 : want);
 }
 
+constexpr int64_t MAX_ROWS = 1 << 22;  // query rows of a head: the grids' second dimension holds their blocks
+
 struct AttendLayout {
   int splits, row_pad;
-  size_t stats, max, sum, acc, bytes;
-  AttendLayout(const ckv_quant_cache* c, int rows, bool accumulate) {
+  bool many;
+  size_t stats, ranges, max, sum, acc, bytes;
+  AttendLayout(const ckv_quant_cache* c, int rows, int dtype, bool accumulate) {
     row_pad = (rows + 15) / 16 * 16;
-    splits = parts_of(c, row_pad / 16);
+    many = rows > FEW_ROWS;
+    const int64_t block = many ? many_row_block(dtype) : 16;
+    splits = parts_of(c, (rows + block - 1) / block, many ? 256 : 1024);
     const size_t heads = (size_t)c->batch * c->kv_heads;
-    stats = 0;
-    size_t at = accumulate ? heads * row_pad * sizeof(float2) : 0;
-    max = at;
-    if (splits > 1) at += heads * row_pad * splits * sizeof(float);
-    sum = at;
-    if (splits > 1) at += heads * row_pad * splits * sizeof(float);
-    acc = at;
-    if (splits > 1) at += heads * row_pad * splits * D * sizeof(float);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+      const size_t here = at;
+      at += (bytes + 15) & ~(size_t)15;
+      return here;
+    };
+    stats = take(accumulate ? heads * row_pad * sizeof(float2) : 0);
+    ranges = take(many ? heads * ((c->capacity + RANGE_TILE - 1) / RANGE_TILE) * sizeof(int2) : 0);
+    const size_t parts = splits > 1 ? heads * row_pad * splits * sizeof(float) : 0;
+    max = take(parts);
+    sum = take(parts);
+    acc = take(parts * D);
     bytes = at;
   }
 };
 
 template <int DT, int NR>
-void launch_split(const AttendArgs& a, hipStream_t s) {
+void launch_split(const QuantAttendArgs& a, hipStream_t s) {
   const dim3 grid((a.rows + 16 * NR - 1) / (16 * NR), a.splits, a.cache.batch * a.cache.kv_heads);
   attend_split_kernel<DT, NR><<<grid, 64 * WAVES, 0, s>>>(a);
 }
 
 template <int DT>
-int launch_attend(const AttendArgs& a, bool accumulate, hipStream_t s) {
-  if (row_tiles<DT>(a.rows) == 2) launch_split<DT, 2>(a, s);
-  else launch_split<DT, 1>(a, s);
-  int rc = launched("ckv_quant_attention");
-  if (rc) return rc;
-  if (a.splits > 1) {
+int launch_attend(const QuantAttendArgs& a, bool many, bool accumulate, hipStream_t s) {
+  int rc;
+  if (many) {
+    rc = launch_many_rows(a, DT, s);
+  } else {
+    if (row_tiles<DT>(a.rows) == 2) launch_split<DT, 2>(a, s);
+    else launch_split<DT, 1>(a, s);
+    rc = launched("ckv_quant_attention");
+  }
+  if (!rc && a.splits > 1) {
     attend_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), D, 0, s>>>(a);
     rc = launched("ckv_quant_attention");
-    if (rc) return rc;
   }
-  if (accumulate) {
+  if (!rc && accumulate) {
+    if (many) return launch_many_rows_weights(a, DT, s);
     const dim3 grid((a.cache.capacity + WAVES * STEP - 1) / (WAVES * STEP), a.cache.kv_heads, a.cache.batch);
     weights_kernel<DT><<<grid, 64 * WAVES, 0, s>>>(a);
     rc = launched("ckv_quant_attention");
@@ -564,13 +500,13 @@ int launch_attend(const AttendArgs& a, bool accumulate, hipStream_t s) {
 }  // namespace
 
 extern "C" size_t ckv_quant_attention_workspace_bytes(const ckv_quant_cache* cache, int32_t query_heads,
-                                                      int32_t tokens, int32_t accumulate) {
+                                                      int32_t tokens, int32_t dtype, int32_t accumulate) {
   if (!cache || cache->batch <= 0 || cache->kv_heads <= 0 || cache->capacity <= 0 || tokens <= 0 ||
       query_heads <= 0 || query_heads % cache->kv_heads)
     return 0;
   const int64_t rows = (int64_t)tokens * (query_heads / cache->kv_heads);
-  if (rows > (1 << 24)) return 0;
-  return AttendLayout(cache, (int)rows, accumulate != 0).bytes;
+  if (rows > MAX_ROWS) return 0;
+  return AttendLayout(cache, (int)rows, dtype, accumulate != 0).bytes;
 }
 
 extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant_rows* query, int32_t query_heads,
@@ -587,7 +523,8 @@ extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant
   const int group = query_heads / cache->kv_heads;
   if (group > CKV_MAX_GROUP) return fail(CKV_E_LIMIT, "ckv_quant_attention: group size exceeds 16");
   if (tokens <= 0 || window < 0) return fail(CKV_E_INVALID, "ckv_quant_attention: tokens must be positive, window not negative");
-  if ((int64_t)tokens * group > (1 << 24)) return fail(CKV_E_LIMIT, "ckv_quant_attention: more than 2^24 query rows a head");
+  if ((int64_t)tokens * group > MAX_ROWS)
+    return fail(CKV_E_LIMIT, "ckv_quant_attention: more than 2^22 query rows a head");
   if (!(softmax_scale > 0.0f) || softmax_scale > 1e30f)
     return fail(CKV_E_INVALID, "ckv_quant_attention: softmax_scale must be positive");
   const int unit = dtype == CKV_F32 ? 4 : 8;
@@ -597,11 +534,11 @@ extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant
   if (accumulate && !cache->weights) return fail(CKV_E_INVALID, "ckv_quant_attention: the cache keeps no weights");
   if ((int64_t)cache->batch * cache->kv_heads > 65535)
     return fail(CKV_E_LIMIT, "ckv_quant_attention: more than 65535 heads over the batch");
-  const AttendLayout lay(cache, tokens * group, accumulate != 0);
+  const AttendLayout lay(cache, tokens * group, dtype, accumulate != 0);
   if (lay.bytes && (!workspace || ((uintptr_t)workspace & 15)))
     return fail(CKV_E_INVALID, "ckv_quant_attention: workspace");
   char* ws = reinterpret_cast<char*>(workspace);
-  AttendArgs a{};
+  QuantAttendArgs a{};
   a.cache = *cache;
   a.query = *query;
   a.counts = counts;
@@ -611,6 +548,7 @@ extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant
   a.part_sum = reinterpret_cast<float*>(ws + lay.sum);
   a.part_acc = reinterpret_cast<float*>(ws + lay.acc);
   a.stats = accumulate ? reinterpret_cast<float2*>(ws + lay.stats) : nullptr;
+  a.ranges = lay.many ? reinterpret_cast<int2*>(ws + lay.ranges) : nullptr;
   a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
   a.tokens = tokens;
   a.group = group;
@@ -619,7 +557,7 @@ extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant
   a.window = window;
   a.splits = lay.splits;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == CKV_BF16) return launch_attend<CKV_BF16>(a, accumulate != 0, s);
-  if (dtype == CKV_F16) return launch_attend<CKV_F16>(a, accumulate != 0, s);
-  return launch_attend<CKV_F32>(a, accumulate != 0, s);
+  if (dtype == CKV_BF16) return launch_attend<CKV_BF16>(a, lay.many, accumulate != 0, s);
+  if (dtype == CKV_F16) return launch_attend<CKV_F16>(a, lay.many, accumulate != 0, s);
+  return launch_attend<CKV_F32>(a, lay.many, accumulate != 0, s);
 }

@@ -1,0 +1,673 @@
+// Attention of many query rows (prompts and pieces of prompts) over the 8-bit
+// KV cache, and the weight that every cache row received from them (gfx950).
+//
+// attend_rows_kernel: a workgroup of W waves takes 32 W packed query rows of a
+// KV head (row = token * group + query head).  Tiles of 64 cache rows are
+// converted once for the whole workgroup: codes come from memory into registers
+// two tiles ahead, become bf16 with the block's power of two folded in (one
+// v_cvt_scalef32_pk_bf16_fp8 a pair, exact), and are stored to LDS for the
+// next tile.  Each wave computes S^T = K Q^T with v_mfma_f32_32x32x16_bf16, which
+// leaves one query row in a lane (lane % 32) and 16 of 32 cache rows in each half of
+// the wave, so the softmax is per-lane work; O^T = V^T P^T takes the same layout,
+// with V^T by transposing LDS reads.
+//
+// Tiles that no query of the workgroup sees are skipped by their least and
+// largest position, which range_kernel writes beforehand; rows may stand in
+// any order.
+#include <hip/hip_runtime.h>
+
+#include "ckv_quant_attend.h"
+
+namespace {
+using namespace ckv;
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+constexpr int KEYS = RANGE_TILE;     // cache rows of an LDS tile
+constexpr int K_STRIDE = D + 8;      // 17 chunks of 16 bytes: b128 reads of 16 lanes hit distinct banks
+constexpr int V_STRIDE = D + 32;     // 20 chunks: transposed b64 reads hit distinct banks
+constexpr int K_TILE = KEYS * K_STRIDE;
+constexpr int V_TILE = KEYS * V_STRIDE;
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return CKV_OK;
+  static thread_local char message[160];
+  snprintf(message, sizeof(message), "%s: %s", what, hipGetErrorString(e));
+  return ckv_internal::set_error(CKV_E_LAUNCH, message);
+}
+
+__device__ inline f32x16_t mfma32(uint4 a, uint4 b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                 0, 0, 0);
+}
+
+// Largest of three without the moves that quiet a NaN first; a NaN operand is
+// passed over.
+__device__ inline float max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
+
+// Two codes as bf16 times the power of two in `scale`'s exponent (exact).
+template <bool HIGH>
+__device__ inline uint32_t scaled_codes(uint32_t w, float scale) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HIGH));
+}
+
+__device__ inline uint4 scaled_codes8(uint32_t lo, uint32_t hi, float scale) {
+  return uint4{scaled_codes<false>(lo, scale), scaled_codes<true>(lo, scale), scaled_codes<false>(hi, scale),
+               scaled_codes<true>(hi, scale)};
+}
+
+// What a scale holds beyond its power of two: 1 but for a cache from elsewhere.
+__device__ inline float mantissa_of(float scale) { return ckv_u2f((ckv_f2u(scale) & 0x7fffffu) | 0x3f800000u); }
+
+__device__ inline bool has_nan_code(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
+
+// Least and largest position of every 64 rows in use.
+__global__ __launch_bounds__(256) void range_kernel(const QuantAttendArgs a) {
+  const ckv_quant_cache& c = a.cache;
+  const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
+  const int n = quant_length(c, b);
+  const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (tile * KEYS >= n) return;
+  const int64_t row = tile * KEYS + lane;
+  const int32_t p = quant_head(c, b, h).positions[min(row, (int64_t)n - 1)];
+  const int top = wave_max_i32(p), low = -wave_max_i32(-p);
+  const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
+  if (lane == 0) a.ranges[((int64_t)b * c.kv_heads + h) * tiles + tile] = int2{low, top};
+}
+
+struct TileRef {
+  int tile, lo, hi;  // -1: none; its least and largest position
+};
+
+// Goes over the tiles of [first, last) that hold a position in [lo, hi], in
+// order; every wave of a workgroup sees the same.
+struct TileWalk {
+  const int2* ranges;
+  int base, last, lo, hi;
+  uint64_t bits;
+  int2 mine;
+  __device__ TileWalk(const int2* r, int first, int end, int low, int high)
+      : ranges(r), base(first - 64), last(end), lo(low), hi(high), bits(0) {}
+  __device__ TileRef next() {
+    while (bits == 0) {
+      base += 64;
+      if (base >= last) return TileRef{-1, 0, 0};
+      const int t = base + (int)(threadIdx.x & 63);
+      bool need = false;
+      if (t < last) {
+        mine = ranges[t];
+        need = mine.x <= hi && mine.y >= lo;
+      }
+      bits = __ballot(need);
+    }
+    const int i = __ffsll((unsigned long long)bits) - 1;
+    bits &= bits - 1;
+    return TileRef{base + i, __builtin_amdgcn_readlane(mine.x, i), __builtin_amdgcn_readlane(mine.y, i)};
+  }
+};
+
+// The codes of one tensor of a tile, C = 16-byte pieces a thread: piece i of
+// thread t is 16 (t % 8) .. + 15 of row t / 8 + i * threads / 8.
+template <int W>
+struct TileCodes {
+  static constexpr int C = 8 / W;
+  uint4 w[C];
+  float scale[C];
+};
+
+template <int W>
+__device__ inline void load_codes(const uint8_t* codes, const float* scales, int tile, int n, int block_log2,
+                                  TileCodes<W>& t) {
+#pragma unroll
+  for (int i = 0; i < TileCodes<W>::C; ++i) {
+    const int row = min(tile * KEYS + (int)(threadIdx.x >> 3) + i * 8 * W, n - 1);
+    t.w[i] = gload16(codes + (int64_t)row * D + 16 * (threadIdx.x & 7));
+    t.scale[i] = gload_f32(scales + (row >> block_log2));
+  }
+}
+
+template <int W>
+__device__ inline void store_codes(const TileCodes<W>& t, uint16_t* tile, int stride, float* mantissa) {
+#pragma unroll
+  for (int i = 0; i < TileCodes<W>::C; ++i) {
+    const int row = (threadIdx.x >> 3) + i * 8 * W, chunk = threadIdx.x & 7;
+    uint4* p = reinterpret_cast<uint4*>(tile + row * stride + 16 * chunk);
+    p[0] = scaled_codes8(t.w[i].x, t.w[i].y, t.scale[i]);
+    p[1] = scaled_codes8(t.w[i].z, t.w[i].w, t.scale[i]);
+    if (chunk == 0 && (row & 15) == 0) mantissa[row >> 4] = mantissa_of(t.scale[i]);
+  }
+}
+
+template <int W>
+struct RowsLds {
+  uint16_t k[2][K_TILE];
+  uint16_t v[2][V_TILE];
+  int32_t pos[2][KEYS];
+  float k_mantissa[4][4];  // a ring: a tile's are read after its stage is filled anew
+  float v_mantissa[2][4];
+  int nan[2];  // tile whose values hold a NaN code, per stage
+};
+
+// Replaces the NaN of a pair of bf16 by zeros and tells them as ones.
+__device__ inline uint32_t split_nan(uint32_t w, uint32_t* is) {
+  const bool lo = (w & 0x7fffu) > 0x7f80u, hi = (w & 0x7fff0000u) > 0x7f800000u;
+  *is = (lo ? 0x3f80u : 0u) | (hi ? 0x3f800000u : 0u);
+  return w & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
+}
+
+template <int DT, int W>
+__global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendArgs a) {
+  constexpr int NP = pieces(DT);
+  extern __shared__ __align__(16) unsigned char lds_raw[];
+  RowsLds<W>& lds = *reinterpret_cast<RowsLds<W>*>(lds_raw);
+  const ckv_quant_cache& c = a.cache;
+  const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
+  // the blocks of the newest rows see the most: they go first
+  const int block0 = (int)(gridDim.y - 1 - blockIdx.y) * 32 * W;
+  const int split = blockIdx.z;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
+  const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
+  const int per = part_rows(n, a.splits);
+  const int lo_row = (int)min((int64_t)split * per, (int64_t)n), hi_row = min(lo_row + per, n);
+  if (split > 0 && lo_row >= n) return;
+  const QuantHead q = quant_head(c, b, h);
+  const int block_log2 = 31 - __clz(c.block);
+  const int row = block0 + 32 * wave + (lane & 31);
+  int lo, hi;
+  query_range(a, row, count, seen, &lo, &hi);
+  // of the whole workgroup (rows are in order of their positions), and of this wave
+  const int t_first = block0 / a.group, t_last = min((min(block0 + 32 * W, a.rows) - 1) / a.group, count - 1);
+  int walk_lo = 0, walk_hi = -1, unused;
+  if (t_first <= t_last) {
+    query_range(a, t_first * a.group, count, seen, &walk_lo, &unused);
+    query_range(a, t_last * a.group, count, seen, &unused, &walk_hi);
+  }
+  // every query of this wave sees all of a tile whose positions are in [all_lo, all_hi]
+  const int w_first = (block0 + 32 * wave) / a.group;
+  const int w_last = min((min(block0 + 32 * wave + 32, a.rows) - 1) / a.group, count - 1);
+  int all_lo = 0, all_hi = 0x7fffffff;  // a wave without a query masks nothing: its rows are dropped at the end
+  if (w_first <= w_last) {
+    query_range(a, w_first * a.group, count, seen, &unused, &all_hi);
+    query_range(a, w_last * a.group, count, seen, &all_lo, &unused);
+  }
+
+  uint4 qreg[NP][8];
+  {
+    const bool ok = row < a.rows;
+    const int t = ok ? row / a.group : 0, g = ok ? row % a.group : 0;
+    const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
+                         (int64_t)t * a.query.token_stride;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      float v[8];
+      load_query8<DT>(a.query.data, base + 16 * s + 8 * half, v);
+      uint32_t w[NP * 4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) split_pair<NP>(ok ? v[2 * i] : 0.0f, ok ? v[2 * i + 1] : 0.0f, w + i, 4);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) qreg[p][s] = uint4{w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]};
+    }
+  }
+
+  const float sl2 = a.scale_log2;
+  const float grow_by = RESCALE / sl2;
+  float m = NEG_INF;  // running maximum of the unscaled scores, shared by a row's two lanes
+  float l = 0.0f;     // this lane's share of the sum
+  f32x16_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = f32x16_t{};
+
+  const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
+  TileWalk walk(a.ranges + (int64_t)bh * tiles, lo_row / KEYS, (hi_row + KEYS - 1) / KEYS, walk_lo, walk_hi);
+
+  // Scores of the tile staged in `stage`: accumulator i holds cache rows
+  // 32 i + 8 (v / 4) + 4 half + v % 4.
+  auto qk_tile = [&](int stage, f32x16_t (&acc)[2]) __attribute__((always_inline)) {
+    const uint16_t* k_s = lds.k[stage];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) acc[i] = f32x16_t{};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 kf = *reinterpret_cast<const uint4*>(k_s + (32 * i + (lane & 31)) * K_STRIDE + 16 * s + 8 * half);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) acc[i] = mfma32(kf, qreg[p][s], acc[i]);
+      }
+    }
+  };
+
+  // One bf16 piece: the next tile's scores are computed beside this tile's
+  // exponentials, so keys are staged a tile ahead of values.
+  constexpr bool AHEAD = NP == 1;
+  const TileRef none{-1, 0, 0};
+  TileRef here = walk.next();
+  TileRef next = here.tile < 0 ? none : walk.next();
+  TileRef third = next.tile < 0 ? none : walk.next();
+  TileCodes<W> kc, vc;
+  auto stage_values = [&](int tile, int stage) __attribute__((always_inline)) {
+    store_codes<W>(vc, lds.v[stage], V_STRIDE, lds.v_mantissa[stage]);
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < TileCodes<W>::C; ++i)
+      nan = nan || has_nan_code(vc.w[i].x) || has_nan_code(vc.w[i].y) || has_nan_code(vc.w[i].z) ||
+            has_nan_code(vc.w[i].w);
+    if (nan) lds.nan[stage] = tile;
+    if (tid < KEYS) {
+      const int r = tile * KEYS + tid;
+      lds.pos[stage][tid] = r < n ? gload_i32(q.positions + r) : 0x7fffffff;
+    }
+  };
+  if (tid < 2) lds.nan[tid] = -1;
+  __syncthreads();
+  int kstage = 0, vstage = 0, slot = 0;
+  f32x16_t sa[2], sb[2];
+  if (here.tile >= 0) {
+    load_codes<W>(q.key_codes, q.key_scales, here.tile, n, block_log2, kc);
+    load_codes<W>(q.value_codes, q.value_scales, here.tile, n, block_log2, vc);
+    store_codes<W>(kc, lds.k[0], K_STRIDE, lds.k_mantissa[0]);
+    stage_values(here.tile, 0);
+    if (next.tile >= 0) {
+      load_codes<W>(q.key_codes, q.key_scales, next.tile, n, block_log2, kc);
+      load_codes<W>(q.value_codes, q.value_scales, next.tile, n, block_log2, vc);
+    }
+    if (AHEAD && next.tile >= 0) {
+      store_codes<W>(kc, lds.k[1], K_STRIDE, lds.k_mantissa[1]);
+      if (third.tile >= 0) load_codes<W>(q.key_codes, q.key_scales, third.tile, n, block_log2, kc);
+    }
+    __syncthreads();
+    if (AHEAD) qk_tile(0, sa);
+  }
+  if (AHEAD) __syncthreads();
+
+  // One tile.  AHEAD: `cur` holds its scores, its values are in v[vstage], the
+  // next tile's keys in k[kstage ^ 1]; kc holds the third tile's keys, vc the
+  // next tile's values.  Otherwise its keys are in k[kstage] and kc holds the
+  // next tile's.
+  auto tile_step = [&](f32x16_t (&cur)[2], f32x16_t (&nxt)[2]) __attribute__((always_inline)) {
+    const TileRef fourth = third.tile < 0 ? none : walk.next();
+    const float4 km = *reinterpret_cast<const float4*>(lds.k_mantissa[slot]);
+    if (!AHEAD) qk_tile(kstage, cur);
+    const float4 vm = *reinterpret_cast<const float4*>(lds.v_mantissa[vstage]);
+    const bool nan = lds.nan[vstage] == here.tile;
+    // the stages that the last tile used are free: fill them
+    if (next.tile >= 0) stage_values(next.tile, vstage ^ 1);
+    const int key_tile = AHEAD ? third.tile : next.tile;
+    const int load_key = AHEAD ? fourth.tile : third.tile;
+    // (AHEAD: this tile's keys were read for `cur` already, so their stage is free)
+    if (key_tile >= 0) {
+      const int to = AHEAD ? kstage : kstage ^ 1;
+      store_codes<W>(kc, lds.k[to], K_STRIDE, lds.k_mantissa[(slot + (AHEAD ? 2 : 1)) & 3]);
+    }
+    if (load_key >= 0) load_codes<W>(q.key_codes, q.key_scales, load_key, n, block_log2, kc);
+    if (third.tile >= 0) load_codes<W>(q.value_codes, q.value_scales, third.tile, n, block_log2, vc);
+
+    if (!(km.x == 1.0f && km.y == 1.0f && km.z == 1.0f && km.w == 1.0f)) {
+      const float mant[4] = {km.x, km.y, km.z, km.w};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) cur[i][v] *= mant[2 * i + (v >> 3)];
+      }
+    }
+    // masks, where some query of this wave does not see some row of the tile
+    const bool masked = here.lo < all_lo || here.hi > all_hi || (here.tile + 1) * KEYS > n;
+    uint32_t hidden = 0;  // bit 16 i + v: this query does not see that row
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int4 p = *reinterpret_cast<const int4*>(&lds.pos[vstage][32 * i + 8 * g + 4 * half]);
+          const int at[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (at[e] < lo || at[e] > hi) {
+              cur[i][4 * g + e] = NEG_INF;
+              hidden |= 1u << (16 * i + 4 * g + e);
+            }
+        }
+      }
+    }
+    float top = max3(cur[0][0], cur[0][1], cur[1][0]);
+#pragma unroll
+    for (int v = 2; v < 16; v += 2) top = max3(top, cur[0][v], cur[0][v + 1]);
+#pragma unroll
+    for (int v = 1; v < 15; v += 2) top = max3(top, cur[1][v], cur[1][v + 1]);
+    top = max3(top, cur[1][15], cur[1][15]);
+    top = max_xor32(top);
+    if (__ballot(top > m + grow_by) != 0) {
+      const float t = fmaxf(m, top);
+      const float f = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((m - t) * sl2);
+      m = t;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] *= f;
+    }
+    const float mc = m == NEG_INF ? 0.0f : m * sl2;
+    if (AHEAD) qk_tile(kstage ^ 1, nxt);  // on the last tile: an old stage, unused
+    uint32_t pb[NP][2][8];
+    const bool plain_values = vm.x == 1.0f && vm.y == 1.0f && vm.z == 1.0f && vm.w == 1.0f;
+    const float vmant[4] = {vm.x, vm.y, vm.z, vm.w};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int v = 0; v < 16; v += 2) {
+        float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v], sl2, -mc));
+        float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v + 1], sl2, -mc));
+        l += p0;
+        l += p1;
+        if (!plain_values) {
+          p0 *= vmant[2 * i + (v >> 3)];
+          p1 *= vmant[2 * i + (v >> 3)];
+        }
+        split_pair<NP>(p0, p1, &pb[0][i][v >> 1], 16);
+      }
+    }
+    const uint16_t* v_s = lds.v[vstage];
+    auto value_pairs = [&](int kk, int db) __attribute__((always_inline)) {
+      const uint16_t* p = v_s + (16 * kk + 4 * half + ((lane & 15) >> 2)) * V_STRIDE + 16 * ((lane >> 4) & 1) +
+                          4 * (lane & 3) + 32 * db;
+      const uint2 x = lds_read_tr16(p), y = lds_read_tr16(p + 8 * V_STRIDE);
+      return uint4{x.x, x.y, y.x, y.y};
+    };
+    if (!(masked && nan)) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        const int i = kk >> 1, vb = 4 * (kk & 1);
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          const uint4 vop = value_pairs(kk, db);
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+            o[db] = mfma32(vop, uint4{pb[p][i][vb], pb[p][i][vb + 1], pb[p][i][vb + 2], pb[p][i][vb + 3]}, o[db]);
+        }
+      }
+    } else {
+      // a masked row's zero times NaN would spread it: zeros in their place, and
+      // NaN where a query sees such a row
+#pragma nounroll
+      for (int kk = 0; kk < 4; ++kk) {
+        uint32_t one[4], w[NP][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int bit = 8 * kk + 2 * e;
+          one[e] = ((hidden >> bit) & 1u ? 0u : 0x3f80u) | ((hidden >> (bit + 1)) & 1u ? 0u : 0x3f800000u);
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+            w[p][e] = kk == 0 ? pb[p][0][e] : kk == 1 ? pb[p][0][4 + e] : kk == 2 ? pb[p][1][e] : pb[p][1][4 + e];
+        }
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          uint4 vop = value_pairs(kk, db), is;
+          vop.x = split_nan(vop.x, &is.x);
+          vop.y = split_nan(vop.y, &is.y);
+          vop.z = split_nan(vop.z, &is.z);
+          vop.w = split_nan(vop.w, &is.w);
+          const f32x16_t hits = mfma32(is, uint4{one[0], one[1], one[2], one[3]}, f32x16_t{});
+#pragma unroll
+          for (int p = 0; p < NP; ++p) o[db] = mfma32(vop, uint4{w[p][0], w[p][1], w[p][2], w[p][3]}, o[db]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[db][e] = hits[e] > 0.0f ? __builtin_nanf("") : o[db][e];
+        }
+      }
+    }
+    __syncthreads();
+    kstage ^= 1;
+    vstage ^= 1;
+    slot = (slot + 1) & 3;
+    here = next;
+    next = third;
+    third = fourth;
+  };
+  while (here.tile >= 0) {
+    if constexpr (AHEAD) {
+      tile_step(sa, sb);
+      if (here.tile < 0) break;
+      tile_step(sb, sa);
+    } else {
+      tile_step(sa, sa);
+    }
+  }
+
+  if (row >= a.rows) return;
+  const float sum = hi < 0 ? 0.0f : add_xor32(l);
+  const float top = m == NEG_INF ? 0.0f : m * sl2;
+  if (a.splits > 1) {
+    float* acc = a.part_acc + (((int64_t)bh * a.splits + split) * a.row_pad + row) * D;
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(acc + 32 * db + 8 * g + 4 * half) =
+            hi < 0 ? float4{0.0f, 0.0f, 0.0f, 0.0f}
+                   : float4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+    }
+    if (half == 0) {
+      a.part_max[((int64_t)bh * a.row_pad + row) * a.splits + split] = m == NEG_INF || hi < 0 ? NEG_INF : top;
+      a.part_sum[((int64_t)bh * a.row_pad + row) * a.splits + split] = sum;
+    }
+    return;
+  }
+  int64_t at_out, at_lse;
+  output_index(a, b, h, row, &at_out, &at_lse);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int db = 0; db < 4; ++db) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int64_t at = at_out + 32 * db + 8 * g + 4 * half;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = sum == 0.0f ? 0.0f : o[db][4 * g + e] * inv;
+      if constexpr (DT == CKV_F32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at) = float4{v[0], v[1], v[2], v[3]};
+      } else {
+        uint32_t w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          w[e] = DT == CKV_BF16 ? pack_bf16x2_hw(v[2 * e], v[2 * e + 1])
+                                : (uint32_t)f16_bits_hw(v[2 * e]) | ((uint32_t)f16_bits_hw(v[2 * e + 1]) << 16);
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at) = uint2{w[0], w[1]};
+      }
+    }
+  }
+  if (half == 0) {
+    a.lse[at_lse] = sum == 0.0f ? NEG_INF : (top + __log2f(sum)) * LN2;
+    if (a.stats) a.stats[(int64_t)bh * a.row_pad + row] = float2{top, inv};
+  }
+}
+
+template <int DT>
+constexpr int rows_waves() { return DT == CKV_BF16 ? 8 : 4; }
+
+template <int DT>
+int launch_rows(const QuantAttendArgs& a, hipStream_t s) {
+  constexpr int W = rows_waves<DT>();
+  const ckv_quant_cache& c = a.cache;
+  const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
+  range_kernel<<<dim3((uint32_t)((tiles + 3) / 4), c.kv_heads, c.batch), 256, 0, s>>>(a);
+  int rc = launched("ckv_quant_attention");
+  if (rc) return rc;
+  auto kernel = attend_rows_kernel<DT, W>;
+  static bool ready[64] = {};  // one flag a device; setting it twice does no harm
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !ready[device]) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RowsLds<W>));
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return ckv_internal::set_error(CKV_E_LAUNCH, hipGetErrorString(e));
+    }
+    if (device >= 0 && device < 64) ready[device] = true;
+  }
+  const dim3 grid(c.batch * c.kv_heads, (a.rows + 32 * W - 1) / (32 * W), a.splits);
+  kernel<<<grid, 64 * W, sizeof(RowsLds<W>), s>>>(a);
+  return launched("ckv_quant_attention");
+}
+
+// Received weight.  A wave keeps 64 cache rows as A operands in registers and
+// goes over a share of the query rows, 32 a step, straight from memory: with
+// the scores' layout as above a lane adds up its rows' probabilities over the
+// queries lane % 32, and the lanes are added once at the end.  The queries are
+// shared out over `shares` workgroups a cache row, which leave sums of their
+// own for weights_add_kernel (a fixed order, no atomics).
+constexpr int WT_WAVES = 4;
+
+template <int DT>
+__global__ __launch_bounds__(64 * WT_WAVES) void rows_weights_kernel(const QuantAttendArgs a, float* sums, int shares) {
+  constexpr int NP = pieces(DT);
+  const ckv_quant_cache& c = a.cache;
+  const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
+  const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
+  const int64_t tile = (int64_t)blockIdx.y * WT_WAVES + wave;
+  if (tile * KEYS >= n) return;
+  const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
+  const int2 range = a.ranges[(int64_t)bh * tiles + tile];
+  const QuantHead q = quant_head(c, b, h);
+  const int block_log2 = 31 - __clz(c.block);
+  const int row0 = (int)tile * KEYS;
+  uint4 kop[2][8];
+  float mant[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = min(row0 + 32 * i + (lane & 31), n - 1);
+    const float scale = gload_f32(q.key_scales + (r >> block_log2));
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const uint2 w = *reinterpret_cast<const uint2*>(q.key_codes + (int64_t)r * D + 16 * s + 8 * half);
+      kop[i][s] = scaled_codes8(w.x, w.y, scale);
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+      mant[i][g] = mantissa_of(gload_f32(q.key_scales + (min(row0 + 32 * i + 16 * g, n - 1) >> block_log2)));
+  }
+  const bool plain = mant[0][0] == 1.0f && mant[0][1] == 1.0f && mant[1][0] == 1.0f && mant[1][1] == 1.0f;
+  const bool tail = row0 + KEYS > n;
+  // queries t that see any of the tile: seen - count + t >= least position, and > largest - window
+  const int first_at = seen - count;
+  const int64_t t_lo = max((int64_t)range.x - first_at, (int64_t)0);
+  const int64_t t_hi = a.window > 0 ? min((int64_t)count - 1, (int64_t)range.y + a.window - 1 - first_at) : count - 1;
+  const int steps = (a.rows + 31) / 32;
+  const int step_lo = (int)min(t_lo * a.group / 32, (int64_t)steps);
+  const int step_hi = t_hi < 0 ? 0 : (int)min((t_hi * a.group + a.group - 1) / 32 + 1, (int64_t)steps);
+  const float sl2 = a.scale_log2;
+  const float2* stats = a.stats + (int64_t)bh * a.row_pad;
+  f32x16_t got[2] = {f32x16_t{}, f32x16_t{}};
+  for (int step = step_lo + (int)blockIdx.z; step < step_hi; step += shares) {
+    const int row = 32 * step + (lane & 31);
+    const bool ok = row < a.rows;
+    const int t = ok ? row / a.group : 0, g = ok ? row % a.group : 0;
+    const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
+                         (int64_t)t * a.query.token_stride;
+    const float2 st = ok ? stats[row] : float2{0.0f, 0.0f};
+    f32x16_t acc[2] = {f32x16_t{}, f32x16_t{}};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      float v[8];
+      load_query8<DT>(a.query.data, base + 16 * s + 8 * half, v);
+      uint32_t w[NP * 4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) split_pair<NP>(v[2 * i], v[2 * i + 1], w + i, 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          acc[i] = mfma32(kop[i][s], uint4{w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]}, acc[i]);
+      }
+    }
+    if (!plain) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[i][v] *= mant[i][v >> 3];
+      }
+    }
+    int lo, hi;
+    query_range(a, row, count, seen, &lo, &hi);
+    const bool masked = tail || __ballot(range.x < lo || range.y > hi) != 0;
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int r = row0 + 32 * i + 8 * (v >> 2) + 4 * half + (v & 3);
+          const int p = gload_i32(q.positions + min(r, n - 1));
+          if (r >= n || p < lo || p > hi) acc[i][v] = NEG_INF;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][v], sl2, -st.x));
+        got[i][v] = __builtin_fmaf(p, st.y, got[i][v]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      float x = got[i][v];
+      x = add_xor_f32<1>(x);
+      x = add_xor_f32<2>(x);
+      x = add_xor_f32<4>(x);
+      x = x + xor_f32<8>(x);
+      x = add_xor16(x);
+      const int r = row0 + 32 * i + 8 * (v >> 2) + 4 * half + (v & 3);
+      if ((lane & 31) == 0 && r < n) {
+        if (shares == 1) q.weights[r] += x;
+        else sums[((int64_t)blockIdx.z * gridDim.x + bh) * c.capacity + r] = x;
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void weights_add_kernel(const QuantAttendArgs a, const float* sums, int shares) {
+  const ckv_quant_cache& c = a.cache;
+  const int bh = blockIdx.y, b = bh / c.kv_heads, h = bh % c.kv_heads;
+  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (r >= quant_length(c, b)) return;
+  float x = 0.0f;
+  for (int s = 0; s < shares; ++s) x += sums[((int64_t)s * gridDim.y + bh) * c.capacity + r];
+  quant_head(c, b, h).weights[r] += x;
+}
+
+template <int DT>
+int launch_weights(const QuantAttendArgs& a, hipStream_t s) {
+  const ckv_quant_cache& c = a.cache;
+  const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
+  const int shares = 1;
+  const dim3 grid(c.batch * c.kv_heads, (uint32_t)((tiles + WT_WAVES - 1) / WT_WAVES), shares);
+  rows_weights_kernel<DT><<<grid, 64 * WT_WAVES, 0, s>>>(a, nullptr, shares);
+  return launched("ckv_quant_attention");
+}
+
+}  // namespace
+
+namespace ckv {
+
+int many_row_block(int dtype) { return 32 * (dtype == CKV_BF16 ? rows_waves<CKV_BF16>() : rows_waves<CKV_F32>()); }
+
+int launch_many_rows(const QuantAttendArgs& a, int dtype, hipStream_t stream) {
+  if (dtype == CKV_BF16) return launch_rows<CKV_BF16>(a, stream);
+  if (dtype == CKV_F16) return launch_rows<CKV_F16>(a, stream);
+  return launch_rows<CKV_F32>(a, stream);
+}
+
+int launch_many_rows_weights(const QuantAttendArgs& a, int dtype, hipStream_t stream) {
+  if (dtype == CKV_BF16) return launch_weights<CKV_BF16>(a, stream);
+  if (dtype == CKV_F16) return launch_weights<CKV_F16>(a, stream);
+  return launch_weights<CKV_F32>(a, stream);
+}
+
+}  // namespace ckv

@@ -620,7 +620,7 @@ int ckv_quant_append(const ckv_quant_cache* cache, const ckv_quant_rows* key, co
  * (fixed summation order).  workspace:
  * ckv_quant_attention_workspace_bytes() bytes, this call's alone. */
 size_t ckv_quant_attention_workspace_bytes(const ckv_quant_cache* cache, int32_t query_heads, int32_t tokens,
-                                           int32_t accumulate);
+                                           int32_t dtype, int32_t accumulate);
 int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant_rows* query, int32_t query_heads,
                         int32_t tokens, const int32_t* counts, int32_t dtype, float softmax_scale, int32_t window,
                         int32_t accumulate, void* out, float* lse, void* workspace, void* stream);

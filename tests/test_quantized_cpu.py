@@ -185,10 +185,10 @@ def test_workspace_sizes(lib):
     c = ctypes.byref(_struct())
     assert lib.ckv_quant_evict_workspace_bytes(c, 16) >= 4 * (128 + 16) * 4
     assert lib.ckv_quant_evict_workspace_bytes(c, 0) == lib.ckv_quant_evict_workspace_bytes(None, 4) == 0
-    assert lib.ckv_quant_attention_workspace_bytes(c, 3, 1, 0) == 0
-    assert lib.ckv_quant_attention_workspace_bytes(None, 4, 1, 0) == 0
-    plain = lib.ckv_quant_attention_workspace_bytes(c, 4, 5, 0)
-    assert lib.ckv_quant_attention_workspace_bytes(c, 4, 5, 1) >= plain + 2 * 2 * 10 * 8
+    assert lib.ckv_quant_attention_workspace_bytes(c, 3, 1, nat.CKV_BF16, 0) == 0
+    assert lib.ckv_quant_attention_workspace_bytes(None, 4, 1, nat.CKV_BF16, 0) == 0
+    plain = lib.ckv_quant_attention_workspace_bytes(c, 4, 5, nat.CKV_F32, 0)
+    assert lib.ckv_quant_attention_workspace_bytes(c, 4, 5, nat.CKV_F32, 1) >= plain + 2 * 2 * 10 * 8
 
 
 def test_oracle_block_scale_and_growth():
