@@ -27,6 +27,7 @@ struct QuantAttendArgs {
   float* part_acc;   // [batch][kv_heads][splits][row_pad][128]
   float2* stats;     // [batch][kv_heads][row_pad]: log2 maximum and 1 / sum, or null
   int2* ranges;      // [batch][kv_heads][tiles]: least and largest position of every RANGE_TILE rows, or null
+  float* sums;       // [shares][batch][kv_heads][capacity] received weights, or null
   float scale_log2;  // softmax_scale * log2 e
   int32_t tokens, group, rows, row_pad, window, splits;
 };
@@ -112,5 +113,6 @@ constexpr int FEW_ROWS = 64;
 int launch_many_rows(const QuantAttendArgs& a, int dtype, hipStream_t stream);
 int launch_many_rows_weights(const QuantAttendArgs& a, int dtype, hipStream_t stream);
 int many_row_block(int dtype);  // query rows of one workgroup
+int many_row_shares(const ckv_quant_cache* c, int rows);  // workgroups that share a cache row's queries
 
 }  // namespace ckv

@@ -445,7 +445,7 @@ constexpr int64_t MAX_ROWS = 1 << 22;  // query rows of a head: the grids' secon
 struct AttendLayout {
   int splits, row_pad;
   bool many;
-  size_t stats, ranges, max, sum, acc, bytes;
+  size_t stats, ranges, sums, max, sum, acc, bytes;
   AttendLayout(const ckv_quant_cache* c, int rows, int dtype, bool accumulate) {
     row_pad = (rows + 15) / 16 * 16;
     many = rows > FEW_ROWS;
@@ -460,6 +460,8 @@ struct AttendLayout {
     };
     stats = take(accumulate ? heads * row_pad * sizeof(float2) : 0);
     ranges = take(many ? heads * ((c->capacity + RANGE_TILE - 1) / RANGE_TILE) * sizeof(int2) : 0);
+    const int shares = many && accumulate ? many_row_shares(c, rows) : 1;
+    sums = take(shares > 1 ? heads * c->capacity * shares * sizeof(float) : 0);
     const size_t parts = splits > 1 ? heads * row_pad * splits * sizeof(float) : 0;
     max = take(parts);
     sum = take(parts);
@@ -549,6 +551,7 @@ extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant
   a.part_acc = reinterpret_cast<float*>(ws + lay.acc);
   a.stats = accumulate ? reinterpret_cast<float2*>(ws + lay.stats) : nullptr;
   a.ranges = lay.many ? reinterpret_cast<int2*>(ws + lay.ranges) : nullptr;
+  a.sums = reinterpret_cast<float*>(ws + lay.sums);
   a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
   a.tokens = tokens;
   a.group = group;

@@ -62,6 +62,22 @@ __device__ inline uint4 scaled_codes8(uint32_t lo, uint32_t hi, float scale) {
                scaled_codes<true>(hi, scale)};
 }
 
+// Which positions a query sees: p is one where (uint32_t)(p - lo) <= span.  No
+// position is negative or 2^31 - 1, so a query that sees none has lo -2, span 0.
+struct Seen {
+  int lo;
+  uint32_t span;
+  __device__ Seen(int low, int high) : lo(high < low ? -2 : low), span(high < low ? 0u : (uint32_t)(high - low)) {}
+  // x, or -inf where position p is not seen.  One block of two instructions:
+  // apart, the compiler collects the 32 compares of a tile first and spills them.
+  __device__ void mask(float& x, int p) const {
+    asm("v_cmp_gt_u32 vcc, %1, %2\n\tv_cndmask_b32 %0, %0, %3, vcc"
+        : "+v"(x)
+        : "v"((uint32_t)(p - lo)), "v"(span), "v"(NEG_INF)
+        : "vcc");
+  }
+};
+
 // What a scale holds beyond its power of two: 1 but for a cache from elsewhere.
 __device__ inline float mantissa_of(float scale) { return ckv_u2f((ckv_f2u(scale) & 0x7fffffu) | 0x3f800000u); }
 
@@ -181,6 +197,7 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   const int row = block0 + 32 * wave + (lane & 31);
   int lo, hi;
   query_range(a, row, count, seen, &lo, &hi);
+  const Seen see(lo, hi);
   // of the whole workgroup (rows are in order of their positions), and of this wave
   const int t_first = block0 / a.group, t_last = min((min(block0 + 32 * W, a.rows) - 1) / a.group, count - 1);
   int walk_lo = 0, walk_hi = -1, unused;
@@ -309,6 +326,7 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
     if (third.tile >= 0) load_codes<W>(q.value_codes, q.value_scales, third.tile, n, block_log2, vc);
 
     if (!(km.x == 1.0f && km.y == 1.0f && km.z == 1.0f && km.w == 1.0f)) {
+      asm volatile("");
       const float mant[4] = {km.x, km.y, km.z, km.w};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -318,8 +336,8 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
     }
     // masks, where some query of this wave does not see some row of the tile
     const bool masked = here.lo < all_lo || here.hi > all_hi || (here.tile + 1) * KEYS > n;
-    uint32_t hidden = 0;  // bit 16 i + v: this query does not see that row
     if (masked) {
+      asm volatile("");  // a branch, not selects on every tile
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -327,11 +345,11 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
           const int4 p = *reinterpret_cast<const int4*>(&lds.pos[vstage][32 * i + 8 * g + 4 * half]);
           const int at[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (at[e] < lo || at[e] > hi) {
-              cur[i][4 * g + e] = NEG_INF;
-              hidden |= 1u << (16 * i + 4 * g + e);
-            }
+          for (int e = 0; e < 4; ++e) {
+            float x = cur[i][4 * g + e];
+            see.mask(x, at[e]);
+            cur[i][4 * g + e] = x;
+          }
         }
       }
     }
@@ -352,23 +370,28 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
     }
     const float mc = m == NEG_INF ? 0.0f : m * sl2;
     if (AHEAD) qk_tile(kstage ^ 1, nxt);  // on the last tile: an old stage, unused
-    uint32_t pb[NP][2][8];
-    const bool plain_values = vm.x == 1.0f && vm.y == 1.0f && vm.z == 1.0f && vm.w == 1.0f;
-    const float vmant[4] = {vm.x, vm.y, vm.z, vm.w};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int v = 0; v < 16; v += 2) {
-        float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v], sl2, -mc));
-        float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v + 1], sl2, -mc));
-        l += p0;
-        l += p1;
-        if (!plain_values) {
-          p0 *= vmant[2 * i + (v >> 3)];
-          p1 *= vmant[2 * i + (v >> 3)];
-        }
-        split_pair<NP>(p0, p1, &pb[0][i][v >> 1], 16);
+      for (int v = 0; v < 16; ++v) {
+        cur[i][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v], sl2, -mc));
+        l += cur[i][v];
       }
+    }
+    if (!(vm.x == 1.0f && vm.y == 1.0f && vm.z == 1.0f && vm.w == 1.0f)) {
+      asm volatile("");
+      const float mant[4] = {vm.x, vm.y, vm.z, vm.w};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) cur[i][v] *= mant[2 * i + (v >> 3)];
+      }
+    }
+    uint32_t pb[NP][2][8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int v = 0; v < 16; v += 2) split_pair<NP>(cur[i][v], cur[i][v + 1], &pb[0][i][v >> 1], 16);
     }
     const uint16_t* v_s = lds.v[vstage];
     auto value_pairs = [&](int kk, int db) __attribute__((always_inline)) {
@@ -397,8 +420,10 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
         uint32_t one[4], w[NP][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int bit = 8 * kk + 2 * e;
-          one[e] = ((hidden >> bit) & 1u ? 0u : 0x3f80u) | ((hidden >> (bit + 1)) & 1u ? 0u : 0x3f800000u);
+          const int2 at = *reinterpret_cast<const int2*>(
+              &lds.pos[vstage][16 * kk + 8 * (e >> 1) + 4 * half + 2 * (e & 1)]);
+          one[e] = ((uint32_t)(at.x - see.lo) > see.span ? 0u : 0x3f80u) |
+                   ((uint32_t)(at.y - see.lo) > see.span ? 0u : 0x3f800000u);
 #pragma unroll
           for (int p = 0; p < NP; ++p)
             w[p][e] = kk == 0 ? pb[p][0][e] : kk == 1 ? pb[p][0][4 + e] : kk == 2 ? pb[p][1][e] : pb[p][1][4 + e];
@@ -512,28 +537,55 @@ int launch_rows(const QuantAttendArgs& a, hipStream_t s) {
   return launched("ckv_quant_attention");
 }
 
-// Received weight.  A wave keeps 64 cache rows as A operands in registers and
-// goes over a share of the query rows, 32 a step, straight from memory: with
-// the scores' layout as above a lane adds up its rows' probabilities over the
-// queries lane % 32, and the lanes are added once at the end.  The queries are
-// shared out over `shares` workgroups a cache row, which leave sums of their
-// own for weights_add_kernel (a fixed order, no atomics).
+// Received weight.  A wave keeps 64 cache rows as A operands in registers; the
+// workgroup's four waves (256 cache rows) go over the query rows, 32 a step,
+// staged in LDS a step ahead.  With the scores' layout as above a lane adds up
+// what its cache rows got from the queries lane % 32; the lanes are added once
+// at the end.  The steps are shared out over `shares` workgroups a block of cache
+// rows, which leave sums of their own for weights_add_kernel: one owner a sum
+// and a fixed order, no atomics.  Per step and wave: 16 products of 32 cycles
+// beside 32 x (fma, exp, fma), 24 cycles each, so the vector ALUs bound it.
 constexpr int WT_WAVES = 4;
+constexpr int WT_ROWS = 64;   // query rows of a step
+constexpr int WT_KEYS = WT_WAVES * KEYS;
+
+template <int NP>
+struct WeightsLds {
+  uint16_t q[2][NP][WT_ROWS * K_STRIDE];
+  float2 stats[2][WT_ROWS];
+  int32_t pos[WT_KEYS];
+};
 
 template <int DT>
-__global__ __launch_bounds__(64 * WT_WAVES) void rows_weights_kernel(const QuantAttendArgs a, float* sums, int shares) {
+__global__ __launch_bounds__(64 * WT_WAVES, 2) void rows_weights_kernel(const QuantAttendArgs a, const int shares) {
   constexpr int NP = pieces(DT);
+  __shared__ WeightsLds<NP> lds;
   const ckv_quant_cache& c = a.cache;
   const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
   const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
-  const int64_t tile = (int64_t)blockIdx.y * WT_WAVES + wave;
-  if (tile * KEYS >= n) return;
+  const int64_t tile0 = (int64_t)blockIdx.y * WT_WAVES, tile = tile0 + wave;
+  if (tile0 * KEYS >= n) return;
   const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
-  const int2 range = a.ranges[(int64_t)bh * tiles + tile];
+  const int live_tiles = (n + KEYS - 1) / KEYS;
   const QuantHead q = quant_head(c, b, h);
   const int block_log2 = 31 - __clz(c.block);
   const int row0 = (int)tile * KEYS;
+  const bool live = tile < live_tiles;
+  // least and largest position of this wave's rows, and of the workgroup's
+  int2 range{0x7fffffff, -1}, all{0x7fffffff, -1};
+#pragma unroll
+  for (int w = 0; w < WT_WAVES; ++w) {
+    if (tile0 + w >= live_tiles) break;
+    const int2 r = a.ranges[(int64_t)bh * tiles + tile0 + w];
+    if (w == wave) range = r;
+    all.x = min(all.x, r.x);
+    all.y = max(all.y, r.y);
+  }
+  {
+    const int64_t r = tile0 * KEYS + tid;
+    lds.pos[tid] = r < n ? gload_i32(q.positions + r) : 0x7fffffff;  // nobody sees rows past the last
+  }
   uint4 kop[2][8];
   float mant[2][2];
 #pragma unroll
@@ -550,69 +602,145 @@ __global__ __launch_bounds__(64 * WT_WAVES) void rows_weights_kernel(const Quant
       mant[i][g] = mantissa_of(gload_f32(q.key_scales + (min(row0 + 32 * i + 16 * g, n - 1) >> block_log2)));
   }
   const bool plain = mant[0][0] == 1.0f && mant[0][1] == 1.0f && mant[1][0] == 1.0f && mant[1][1] == 1.0f;
-  const bool tail = row0 + KEYS > n;
-  // queries t that see any of the tile: seen - count + t >= least position, and > largest - window
-  const int first_at = seen - count;
-  const int64_t t_lo = max((int64_t)range.x - first_at, (int64_t)0);
-  const int64_t t_hi = a.window > 0 ? min((int64_t)count - 1, (int64_t)range.y + a.window - 1 - first_at) : count - 1;
-  const int steps = (a.rows + 31) / 32;
-  const int step_lo = (int)min(t_lo * a.group / 32, (int64_t)steps);
-  const int step_hi = t_hi < 0 ? 0 : (int)min((t_hi * a.group + a.group - 1) / 32 + 1, (int64_t)steps);
+  // steps whose queries t see any of some rows: seen - count + t >= least position, and > largest - window
+  const int64_t first_at = (int64_t)seen - count;
+  const int steps = (a.rows + WT_ROWS - 1) / WT_ROWS;
+  auto steps_of = [&](int2 r, int* lo, int* hi) {
+    const int64_t t_lo = max((int64_t)r.x - first_at, (int64_t)0);
+    int64_t t_hi = (int64_t)count - 1;
+    if (a.window > 0) t_hi = min(t_hi, (int64_t)r.y + a.window - 1 - first_at);
+    *lo = (int)min(t_lo * a.group / WT_ROWS, (int64_t)steps);
+    *hi = t_hi < 0 ? 0 : (int)min((t_hi * a.group + a.group - 1) / WT_ROWS + 1, (int64_t)steps);
+  };
+  int step_lo, step_hi, my_lo, my_hi;
+  steps_of(all, &step_lo, &step_hi);
+  steps_of(range, &my_lo, &my_hi);
+  if (!live) my_hi = 0;
   const float sl2 = a.scale_log2;
   const float2* stats = a.stats + (int64_t)bh * a.row_pad;
-  f32x16_t got[2] = {f32x16_t{}, f32x16_t{}};
-  for (int step = step_lo + (int)blockIdx.z; step < step_hi; step += shares) {
-    const int row = 32 * step + (lane & 31);
-    const bool ok = row < a.rows;
-    const int t = ok ? row / a.group : 0, g = ok ? row % a.group : 0;
-    const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
-                         (int64_t)t * a.query.token_stride;
-    const float2 st = ok ? stats[row] : float2{0.0f, 0.0f};
-    f32x16_t acc[2] = {f32x16_t{}, f32x16_t{}};
+  // a thread stages 16 dims of the query rows tid / 8 and tid / 8 + 32 of a step, as they are in memory
+  const int qd = 16 * (tid & 7);
+  constexpr int RAW = DT == CKV_F32 ? 4 : 2;  // 16-byte pieces
+  uint4 raw[2][RAW];
+  float2 next_st{0.0f, 0.0f};
+  auto load = [&](int step) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      float v[8];
-      load_query8<DT>(a.query.data, base + 16 * s + 8 * half, v);
-      uint32_t w[NP * 4];
+    for (int x = 0; x < 2; ++x) {
+      const int row = min(step * WT_ROWS + (tid >> 3) + 32 * x, a.rows - 1);
+      const int t = row / a.group, g = row - t * a.group;
+      const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
+                           (int64_t)t * a.query.token_stride + qd;
+      const char* from = reinterpret_cast<const char*>(a.query.data) + base * (DT == CKV_F32 ? 4 : 2);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split_pair<NP>(v[2 * i], v[2 * i + 1], w + i, 4);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-          acc[i] = mfma32(kop[i][s], uint4{w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]}, acc[i]);
-      }
+      for (int i = 0; i < RAW; ++i) raw[x][i] = gload16(from + 16 * i);
     }
-    if (!plain) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) acc[i][v] *= mant[i][v >> 3];
-      }
+    if (tid < WT_ROWS) {
+      const int r = step * WT_ROWS + tid;
+      next_st = r < a.rows ? stats[r] : float2{0.0f, 0.0f};  // a row past the last gives nothing
     }
-    int lo, hi;
-    query_range(a, row, count, seen, &lo, &hi);
-    const bool masked = tail || __ballot(range.x < lo || range.y > hi) != 0;
-    if (masked) {
+  };
+  auto store = [&](int stage) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+    for (int x = 0; x < 2; ++x) {
+      const int qr = (tid >> 3) + 32 * x;
+      if constexpr (DT == CKV_BF16) {
+        uint4* to = reinterpret_cast<uint4*>(&lds.q[stage][0][qr * K_STRIDE + qd]);
+        to[0] = raw[x][0];
+        to[1] = raw[x][1];
+      } else {
+        uint32_t w[NP * 8];
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int r = row0 + 32 * i + 8 * (v >> 2) + 4 * half + (v & 3);
-          const int p = gload_i32(q.positions + min(r, n - 1));
-          if (r >= n || p < lo || p > hi) acc[i][v] = NEG_INF;
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t* r = reinterpret_cast<const uint32_t*>(&raw[x][0]);
+          float lo, hi;
+          if constexpr (DT == CKV_F16) {
+            lo = (float)__builtin_bit_cast(_Float16, (uint16_t)(r[i] & 0xffffu));
+            hi = (float)__builtin_bit_cast(_Float16, (uint16_t)(r[i] >> 16));
+          } else {
+            lo = ckv_u2f(r[2 * i]);
+            hi = ckv_u2f(r[2 * i + 1]);
+          }
+          split_pair<NP>(lo, hi, w + i, 8);
+        }
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          uint4* to = reinterpret_cast<uint4*>(&lds.q[stage][p][qr * K_STRIDE + qd]);
+          to[0] = uint4{w[8 * p], w[8 * p + 1], w[8 * p + 2], w[8 * p + 3]};
+          to[1] = uint4{w[8 * p + 4], w[8 * p + 5], w[8 * p + 6], w[8 * p + 7]};
         }
       }
     }
+    if (tid < WT_ROWS) lds.stats[stage][tid] = next_st;
+  };
+  f32x16_t got[2] = {f32x16_t{}, f32x16_t{}};
+  int stage = 0;
+  const int first = step_lo + (int)blockIdx.z;
+  if (first < step_hi) {
+    load(first);
+    store(0);
+  }
+  __syncthreads();
+  for (int step = first; step < step_hi; step += shares) {
+    const bool more = step + shares < step_hi;
+    if (more) load(step + shares);
+    if (step >= my_lo && step < my_hi) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+      for (int x = 0; x < 2; ++x) {
+        const int qrow = 32 * x + (lane & 31);
+        f32x16_t acc[2] = {f32x16_t{}, f32x16_t{}};
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][v], sl2, -st.x));
-        got[i][v] = __builtin_fmaf(p, st.y, got[i][v]);
+        for (int s = 0; s < 8; ++s) {
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            const uint4 qop = *reinterpret_cast<const uint4*>(&lds.q[stage][p][qrow * K_STRIDE + 16 * s + 8 * half]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) acc[i] = mfma32(kop[i][s], qop, acc[i]);
+          }
+        }
+        const float2 st = lds.stats[stage][qrow];
+        if (!plain) {
+          asm volatile("");
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[i][v] *= mant[i][v >> 3];
+          }
+        }
+        int lo, hi;
+        query_range(a, step * WT_ROWS + qrow, count, seen, &lo, &hi);
+        if (row0 + KEYS > n || __ballot(range.x < lo || range.y > hi) != 0) {
+          asm volatile("");
+          const Seen see(lo, hi);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int4 p = *reinterpret_cast<const int4*>(&lds.pos[KEYS * wave + 32 * i + 8 * g + 4 * half]);
+              const int at[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float y = acc[i][4 * g + e];
+                see.mask(y, at[e]);
+                acc[i][4 * g + e] = y;
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][v], sl2, -st.x));
+            got[i][v] = __builtin_fmaf(p, st.y, got[i][v]);
+          }
+        }
       }
     }
+    if (more) store(stage ^ 1);
+    __syncthreads();
+    stage ^= 1;
   }
+  if (!live) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -622,34 +750,47 @@ __global__ __launch_bounds__(64 * WT_WAVES) void rows_weights_kernel(const Quant
       x = add_xor_f32<2>(x);
       x = add_xor_f32<4>(x);
       x = x + xor_f32<8>(x);
-      x = add_xor16(x);
-      const int r = row0 + 32 * i + 8 * (v >> 2) + 4 * half + (v & 3);
-      if ((lane & 31) == 0 && r < n) {
-        if (shares == 1) q.weights[r] += x;
-        else sums[((int64_t)blockIdx.z * gridDim.x + bh) * c.capacity + r] = x;
-      }
+      got[i][v] = add_xor16(x);
+    }
+  }
+  // lane 4 g + e of each half writes its rows 8 g + 4 half + e
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float x = got[i][0];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) x = (lane & 15) == v ? got[i][v] : x;
+    const int v = lane & 15;
+    const int r = row0 + 32 * i + 8 * (v >> 2) + 4 * half + (v & 3);
+    if ((lane & 16) == 0 && r < n) {
+      if (shares == 1) q.weights[r] += x;
+      else a.sums[((int64_t)blockIdx.z * gridDim.x + bh) * c.capacity + r] = x;
     }
   }
 }
 
-__global__ __launch_bounds__(256) void weights_add_kernel(const QuantAttendArgs a, const float* sums, int shares) {
+__global__ __launch_bounds__(256) void weights_add_kernel(const QuantAttendArgs a, const int shares) {
   const ckv_quant_cache& c = a.cache;
-  const int bh = blockIdx.y, b = bh / c.kv_heads, h = bh % c.kv_heads;
-  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
+  const int64_t r = (int64_t)blockIdx.y * 256 + threadIdx.x;
   if (r >= quant_length(c, b)) return;
   float x = 0.0f;
-  for (int s = 0; s < shares; ++s) x += sums[((int64_t)s * gridDim.y + bh) * c.capacity + r];
+  for (int s = 0; s < shares; ++s) x += a.sums[((int64_t)s * gridDim.x + bh) * c.capacity + r];
   quant_head(c, b, h).weights[r] += x;
 }
 
 template <int DT>
 int launch_weights(const QuantAttendArgs& a, hipStream_t s) {
   const ckv_quant_cache& c = a.cache;
-  const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
-  const int shares = 1;
-  const dim3 grid(c.batch * c.kv_heads, (uint32_t)((tiles + WT_WAVES - 1) / WT_WAVES), shares);
-  rows_weights_kernel<DT><<<grid, 64 * WT_WAVES, 0, s>>>(a, nullptr, shares);
-  return launched("ckv_quant_attention");
+  const int64_t blocks = ((int64_t)c.capacity + WT_KEYS - 1) / WT_KEYS;
+  const int shares = many_row_shares(&c, a.rows);
+  const dim3 grid(c.batch * c.kv_heads, (uint32_t)blocks, shares);
+  rows_weights_kernel<DT><<<grid, 64 * WT_WAVES, 0, s>>>(a, shares);
+  int rc = launched("ckv_quant_attention");
+  if (!rc && shares > 1) {
+    weights_add_kernel<<<dim3(c.batch * c.kv_heads, (uint32_t)((c.capacity + 255) / 256)), 256, 0, s>>>(a, shares);
+    rc = launched("ckv_quant_attention");
+  }
+  return rc;
 }
 
 }  // namespace
@@ -657,6 +798,15 @@ int launch_weights(const QuantAttendArgs& a, hipStream_t s) {
 namespace ckv {
 
 int many_row_block(int dtype) { return 32 * (dtype == CKV_BF16 ? rows_waves<CKV_BF16>() : rows_waves<CKV_F32>()); }
+
+// Four workgroups a compute unit: the blocks of old cache rows meet more queries
+// than those of new ones, and what is left over evens out.
+int many_row_shares(const ckv_quant_cache* c, int rows) {
+  const int64_t blocks = ((int64_t)c->capacity + WT_KEYS - 1) / WT_KEYS * c->batch * c->kv_heads;
+  const int64_t steps = (rows + WT_ROWS - 1) / WT_ROWS;
+  const int64_t want = (1024 + blocks - 1) / blocks;
+  return (int)(want < 1 ? 1 : want > 32 ? (steps < 32 ? steps : 32) : want > steps ? steps : want);
+}
 
 int launch_many_rows(const QuantAttendArgs& a, int dtype, hipStream_t stream) {
   if (dtype == CKV_BF16) return launch_rows<CKV_BF16>(a, stream);
