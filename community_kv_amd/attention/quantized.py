@@ -109,7 +109,14 @@ class QuantizedKVCache:
                      value_scales: torch.Tensor, positions: torch.Tensor, cursors: torch.Tensor, block: int = 64,
                      weights: torch.Tensor | None = None) -> "QuantizedKVCache":
         """A cache over tensors that the caller has (an imported or restored
-        cache).  Scales must be positive and finite where rows are in use."""
+        cache).  Scales must be powers of two in [2^-64, 2^120], or 0 where no
+        row is in use (checked, which reads the device); the rows in use must
+        have distinct positions in [0, seen) (not checked)."""
+        for name, scales in (("key_scales", key_scales), ("value_scales", value_scales)):
+            mantissa, exponent = torch.frexp(scales)
+            good = (mantissa == 0.5) & (exponent >= -63) & (exponent <= 121)
+            if not bool((good | (scales == 0)).all()):
+                raise ValueError(f"{name} must be powers of two in [2^-64, 2^120], or 0")
         return cls(key_codes=key_codes, value_codes=value_codes, key_scales=key_scales, value_scales=value_scales,
                    positions=positions, cursors=cursors, block=block, weights=weights)
 

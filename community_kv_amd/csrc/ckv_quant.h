@@ -50,28 +50,17 @@ __device__ inline bool finite_f32(float x) { return (ckv_f2u(x) & 0x7f800000u) !
 // |x| where x is finite, else 0: what counts for a block's scale.
 __device__ inline float finite_abs(float x) { return finite_f32(x) ? fabsf(x) : 0.0f; }
 
-// x / s: a scale is a power of two unless the caller brought its own, and then
-// the product with its exact reciprocal is the quotient.
-struct Divider {
-  float s, inv;
-  bool exact;
-  __device__ explicit Divider(float scale) : s(scale) {
-    const uint32_t bits = ckv_f2u(scale);
-    exact = (bits & 0x7fffffu) == 0 && (bits >> 23) >= 2 && (bits >> 23) <= 252;
-    inv = 1.0f / scale;
-  }
-  __device__ float operator()(float x) const { return exact ? x * inv : x / s; }
-};
+// 1 / s of a power of two in [2^-126, 2^126] (exact).
+__device__ inline float inverse_scale(float s) { return ckv_u2f((254u << 23) - ckv_f2u(s)); }
 
-// Four values to E4M3 codes, round to nearest even; what is not finite becomes
-// NaN, and nothing finite exceeds 448 here but by a caller's own scales, where
-// the clamp holds it.
+// Four values of at most 448, or not finite, to E4M3 codes: round to nearest
+// even; what is not finite becomes NaN.
 __device__ inline uint32_t encode4(float a, float b, float c, float d) {
   const float nan = __builtin_nanf("");
-  a = finite_f32(a) ? __builtin_amdgcn_fmed3f(a, -448.0f, 448.0f) : nan;
-  b = finite_f32(b) ? __builtin_amdgcn_fmed3f(b, -448.0f, 448.0f) : nan;
-  c = finite_f32(c) ? __builtin_amdgcn_fmed3f(c, -448.0f, 448.0f) : nan;
-  d = finite_f32(d) ? __builtin_amdgcn_fmed3f(d, -448.0f, 448.0f) : nan;
+  a = finite_f32(a) ? a : nan;
+  b = finite_f32(b) ? b : nan;
+  c = finite_f32(c) ? c : nan;
+  d = finite_f32(d) ? d : nan;
   int w = 0;
   w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, w, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);

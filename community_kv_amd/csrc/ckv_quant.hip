@@ -125,19 +125,19 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendArgs a) {
     amax = block_max256(amax, scratch);
     const float old = row0 < start ? q.scales(tensor)[blk] : 0.0f;
     const float scale = fmaxf(old, block_scale(amax));
-    const Divider div(scale);
+    const float inv = inverse_scale(scale);
 #pragma unroll
     for (int s = 0; s < SWEEPS; ++s) {
       const int row = (int)row0 + 16 * s + (tid >> 4);
       if (row >= lo && row < hi) {
         float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = div(v[s][i]);
+        for (int i = 0; i < 8; ++i) y[i] = v[s][i] * inv;
         *reinterpret_cast<uint2*>(q.codes(tensor) + (int64_t)row * D + col) =
             uint2{encode4(y[0], y[1], y[2], y[3]), encode4(y[4], y[5], y[6], y[7])};
       }
     }
-    if (row0 < start && scale != old) rescale_rows(q.codes(tensor), row0, start - (int)row0, old / scale);
+    if (row0 < start && scale != old) rescale_rows(q.codes(tensor), row0, start - (int)row0, old * inv);
     if (tensor == 0) {
       for (int row = lo + tid; row < hi; row += THREADS) {
         q.positions[row] = seen + (row - start);
@@ -382,8 +382,8 @@ __global__ __launch_bounds__(THREADS) void evict_move_kernel(const EvictArgs a, 
   }
   amax = block_max256(amax, scratch);
   const float scale = any ? fmaxf(old, block_scale(amax)) : old;
-  const Divider div(scale);
-  const float ratio = old / scale;
+  const float inv = inverse_scale(scale);
+  const float ratio = old * inv;
 #pragma unroll
   for (int s = 0; s < SWEEPS; ++s) {
     const int row = row0 + 16 * s + (tid >> 4);
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(THREADS) void evict_move_kernel(const EvictArgs a, 
     decode4(w[s].x, v);
     decode4(w[s].y, v + 4);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = hole[s] ? div(v[i] * scale_of[s]) : v[i] * ratio;
+    for (int i = 0; i < 8; ++i) v[i] *= hole[s] ? scale_of[s] * inv : ratio;
     *p = uint2{encode4(v[0], v[1], v[2], v[3]), encode4(v[4], v[5], v[6], v[7])};
   }
   if (tensor == 0 && (tid & 15) == 0) {

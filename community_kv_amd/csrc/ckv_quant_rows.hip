@@ -78,11 +78,6 @@ struct Seen {
   }
 };
 
-// What a scale holds beyond its power of two: 1 but for a cache from elsewhere.
-__device__ inline float mantissa_of(float scale) { return ckv_u2f((ckv_f2u(scale) & 0x7fffffu) | 0x3f800000u); }
-
-__device__ inline bool has_nan_code(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
-
 // Least and largest position of every 64 rows in use.
 __global__ __launch_bounds__(256) void range_kernel(const QuantAttendArgs a) {
   const ckv_quant_cache& c = a.cache;
@@ -128,8 +123,8 @@ struct TileWalk {
   }
 };
 
-// The codes of one tensor of a tile, C = 16-byte pieces a thread: piece i of
-// thread t is 16 (t % 8) .. + 15 of row t / 8 + i * threads / 8.
+// A thread's share of a tile's codes: piece i is 16 codes of local row
+// tid / 8 + 8 W i, from 16 (tid % 8) on, with its block's scale.
 template <int W>
 struct TileCodes {
   static constexpr int C = 8 / W;
@@ -140,54 +135,53 @@ struct TileCodes {
 template <int W>
 __device__ inline void load_codes(const uint8_t* codes, const float* scales, int tile, int n, int block_log2,
                                   TileCodes<W>& t) {
+  const int first = tile * KEYS;
+  const int last = min(n - 1 - first, KEYS - 1);  // rows past the last one repeat it
+  const uint8_t* base = codes + (int64_t)first * D;
+  const float* scale = scales + (first >> block_log2);
 #pragma unroll
   for (int i = 0; i < TileCodes<W>::C; ++i) {
-    const int row = min(tile * KEYS + (int)(threadIdx.x >> 3) + i * 8 * W, n - 1);
-    t.w[i] = gload16(codes + (int64_t)row * D + 16 * (threadIdx.x & 7));
-    t.scale[i] = gload_f32(scales + (row >> block_log2));
+    const int local = min((int)(threadIdx.x >> 3) + i * 8 * W, last);
+    t.w[i] = gload16(base + local * D + 16 * (threadIdx.x & 7));
+    t.scale[i] = gload_f32(scale + (local >> block_log2));  // a tile's first row opens a block, or halves one of 128
   }
 }
 
 template <int W>
-__device__ inline void store_codes(const TileCodes<W>& t, uint16_t* tile, int stride, float* mantissa) {
+__device__ inline void store_codes(const TileCodes<W>& t, uint16_t* tile, int stride) {
 #pragma unroll
   for (int i = 0; i < TileCodes<W>::C; ++i) {
-    const int row = (threadIdx.x >> 3) + i * 8 * W, chunk = threadIdx.x & 7;
-    uint4* p = reinterpret_cast<uint4*>(tile + row * stride + 16 * chunk);
+    uint4* p = reinterpret_cast<uint4*>(tile + ((threadIdx.x >> 3) + i * 8 * W) * stride + 16 * (threadIdx.x & 7));
     p[0] = scaled_codes8(t.w[i].x, t.w[i].y, t.scale[i]);
     p[1] = scaled_codes8(t.w[i].z, t.w[i].w, t.scale[i]);
-    if (chunk == 0 && (row & 15) == 0) mantissa[row >> 4] = mantissa_of(t.scale[i]);
   }
 }
 
-template <int W>
+// Zeros in place of NaN codes; whether there were any.
+__device__ inline bool drop_nan_codes(uint32_t& w) {
+  const uint32_t is = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  w &= ~((is >> 7) * 0xffu);
+  return is != 0;
+}
+
 struct RowsLds {
   uint16_t k[2][K_TILE];
   uint16_t v[2][V_TILE];
   int32_t pos[2][KEYS];
-  float k_mantissa[4][4];  // a ring: a tile's are read after its stage is filled anew
-  float v_mantissa[2][4];
-  int nan[2];  // tile whose values hold a NaN code, per stage
+  int nan[2];  // the tile, where its values held a NaN code that was staged as zero
 };
-
-// Replaces the NaN of a pair of bf16 by zeros and tells them as ones.
-__device__ inline uint32_t split_nan(uint32_t w, uint32_t* is) {
-  const bool lo = (w & 0x7fffu) > 0x7f80u, hi = (w & 0x7fff0000u) > 0x7f800000u;
-  *is = (lo ? 0x3f80u : 0u) | (hi ? 0x3f800000u : 0u);
-  return w & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
-}
 
 template <int DT, int W>
 __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendArgs a) {
   constexpr int NP = pieces(DT);
   extern __shared__ __align__(16) unsigned char lds_raw[];
-  RowsLds<W>& lds = *reinterpret_cast<RowsLds<W>*>(lds_raw);
+  RowsLds& lds = *reinterpret_cast<RowsLds*>(lds_raw);
   const ckv_quant_cache& c = a.cache;
   const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
   // the blocks of the newest rows see the most: they go first
   const int block0 = (int)(gridDim.y - 1 - blockIdx.y) * 32 * W;
   const int split = blockIdx.z;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
   const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
   const int per = part_rows(n, a.splits);
   const int lo_row = (int)min((int64_t)split * per, (int64_t)n), hi_row = min(lo_row + per, n);
@@ -198,37 +192,39 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   int lo, hi;
   query_range(a, row, count, seen, &lo, &hi);
   const Seen see(lo, hi);
-  // of the whole workgroup (rows are in order of their positions), and of this wave
-  const int t_first = block0 / a.group, t_last = min((min(block0 + 32 * W, a.rows) - 1) / a.group, count - 1);
-  int walk_lo = 0, walk_hi = -1, unused;
-  if (t_first <= t_last) {
-    query_range(a, t_first * a.group, count, seen, &walk_lo, &unused);
-    query_range(a, t_last * a.group, count, seen, &unused, &walk_hi);
-  }
-  // every query of this wave sees all of a tile whose positions are in [all_lo, all_hi]
-  const int w_first = (block0 + 32 * wave) / a.group;
-  const int w_last = min((min(block0 + 32 * wave + 32, a.rows) - 1) / a.group, count - 1);
-  int all_lo = 0, all_hi = 0x7fffffff;  // a wave without a query masks nothing: its rows are dropped at the end
-  if (w_first <= w_last) {
-    query_range(a, w_first * a.group, count, seen, &unused, &all_hi);
-    query_range(a, w_last * a.group, count, seen, &all_lo, &unused);
-  }
+  // Positions that the queries t0 .. t1 see: some of them [some_lo, some_hi], all of them [all_lo, all_hi].
+  auto ranges_of = [&](int first, int rows, int* some_lo, int* some_hi, int* all_lo, int* all_hi) {
+    const int t0 = first / a.group, t1 = min((min(first + rows, a.rows) - 1) / a.group, count - 1);
+    *some_lo = *all_lo = 0;
+    *some_hi = -1;
+    *all_hi = 0x7ffffffe;  // without a query nothing is masked: the rows are dropped at the end
+    if (t0 > t1) return;
+    query_range(a, t0 * a.group, count, seen, some_lo, all_hi);
+    query_range(a, t1 * a.group, count, seen, all_lo, some_hi);
+  };
+  int walk_lo, walk_hi, group_lo, group_hi, wave_lo, wave_hi, unused;
+  ranges_of(block0, 32 * W, &walk_lo, &walk_hi, &group_lo, &group_hi);
+  ranges_of(block0 + 32 * wave, 32, &unused, &unused, &wave_lo, &wave_hi);
 
   uint4 qreg[NP][8];
   {
-    const bool ok = row < a.rows;
-    const int t = ok ? row / a.group : 0, g = ok ? row % a.group : 0;
+    const int qrow = min(row, a.rows - 1);
+    const int t = qrow / a.group, g = qrow % a.group;
     const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
                          (int64_t)t * a.query.token_stride;
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      float v[8];
-      load_query8<DT>(a.query.data, base + 16 * s + 8 * half, v);
-      uint32_t w[NP * 4];
+      if constexpr (DT == CKV_BF16) {
+        qreg[0][s] = gload16(reinterpret_cast<const uint16_t*>(a.query.data) + base + 16 * s + 8 * half);
+      } else {
+        float v[8];
+        load_query8<DT>(a.query.data, base + 16 * s + 8 * half, v);
+        uint32_t w[NP * 4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split_pair<NP>(ok ? v[2 * i] : 0.0f, ok ? v[2 * i + 1] : 0.0f, w + i, 4);
+        for (int i = 0; i < 4; ++i) split_pair<NP>(v[2 * i], v[2 * i + 1], w + i, 4);
 #pragma unroll
-      for (int p = 0; p < NP; ++p) qreg[p][s] = uint4{w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]};
+        for (int p = 0; p < NP; ++p) qreg[p][s] = uint4{w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]};
+      }
     }
   }
 
@@ -239,9 +235,6 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   f32x16_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = f32x16_t{};
-
-  const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
-  TileWalk walk(a.ranges + (int64_t)bh * tiles, lo_row / KEYS, (hi_row + KEYS - 1) / KEYS, walk_lo, walk_hi);
 
   // Scores of the tile staged in `stage`: accumulator i holds cache rows
   // 32 i + 8 (v / 4) + 4 half + v % 4.
@@ -259,84 +252,91 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
       }
     }
   };
+  auto is_masked = [&](const TileRef& t, int all_lo, int all_hi) __attribute__((always_inline)) {
+    return t.lo < all_lo || t.hi > all_hi || (t.tile + 1) * KEYS > n;
+  };
+  TileCodes<W> kc, vc;
+  // Values of a tile to LDS.  Where some query does not see some row, NaN codes
+  // become zeros (a masked row's zero probability times NaN would spread it) and
+  // are made up for afterwards, and the positions are staged too.
+  auto stage_values = [&](const TileRef& t, int stage) __attribute__((always_inline)) {
+    if (is_masked(t, group_lo, group_hi)) {
+      asm volatile("");
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < TileCodes<W>::C; ++i) {
+        nan |= drop_nan_codes(vc.w[i].x);
+        nan |= drop_nan_codes(vc.w[i].y);
+        nan |= drop_nan_codes(vc.w[i].z);
+        nan |= drop_nan_codes(vc.w[i].w);
+      }
+      if (nan) lds.nan[stage] = t.tile;
+      if (tid < KEYS) {
+        const int r = t.tile * KEYS + tid;
+        lds.pos[stage][tid] = r < n ? gload_i32(q.positions + r) : 0x7fffffff;
+      }
+    }
+    store_codes<W>(vc, lds.v[stage], V_STRIDE);
+  };
+  auto load_keys = [&](const TileRef& t) __attribute__((always_inline)) {
+    load_codes<W>(q.key_codes, q.key_scales, t.tile, n, block_log2, kc);
+  };
+  auto load_values = [&](const TileRef& t) __attribute__((always_inline)) {
+    load_codes<W>(q.value_codes, q.value_scales, t.tile, n, block_log2, vc);
+  };
 
   // One bf16 piece: the next tile's scores are computed beside this tile's
-  // exponentials, so keys are staged a tile ahead of values.
+  // exponentials, so keys are staged a tile ahead of values.  Past the last
+  // tile the pipeline stages that tile again, unused.
   constexpr bool AHEAD = NP == 1;
-  const TileRef none{-1, 0, 0};
-  TileRef here = walk.next();
-  TileRef next = here.tile < 0 ? none : walk.next();
-  TileRef third = next.tile < 0 ? none : walk.next();
-  TileCodes<W> kc, vc;
-  auto stage_values = [&](int tile, int stage) __attribute__((always_inline)) {
-    store_codes<W>(vc, lds.v[stage], V_STRIDE, lds.v_mantissa[stage]);
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < TileCodes<W>::C; ++i)
-      nan = nan || has_nan_code(vc.w[i].x) || has_nan_code(vc.w[i].y) || has_nan_code(vc.w[i].z) ||
-            has_nan_code(vc.w[i].w);
-    if (nan) lds.nan[stage] = tile;
-    if (tid < KEYS) {
-      const int r = tile * KEYS + tid;
-      lds.pos[stage][tid] = r < n ? gload_i32(q.positions + r) : 0x7fffffff;
-    }
+  const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
+  TileWalk walk(a.ranges + (int64_t)bh * tiles, lo_row / KEYS, (hi_row + KEYS - 1) / KEYS, walk_lo, walk_hi);
+  int left = 0;  // of here, next, third: tiles that there are
+  TileRef here, next, third;
+  auto advance = [&](const TileRef& after) __attribute__((always_inline)) {
+    const TileRef t = walk.next();
+    if (t.tile < 0) return after;
+    ++left;
+    return t;
   };
+  here = advance(TileRef{-1, 0, 0});
+  next = advance(here);
+  third = advance(next);
+  int kstage = 0, vstage = 0;
+  f32x16_t sa[2], sb[2];
   if (tid < 2) lds.nan[tid] = -1;
   __syncthreads();
-  int kstage = 0, vstage = 0, slot = 0;
-  f32x16_t sa[2], sb[2];
-  if (here.tile >= 0) {
-    load_codes<W>(q.key_codes, q.key_scales, here.tile, n, block_log2, kc);
-    load_codes<W>(q.value_codes, q.value_scales, here.tile, n, block_log2, vc);
-    store_codes<W>(kc, lds.k[0], K_STRIDE, lds.k_mantissa[0]);
-    stage_values(here.tile, 0);
-    if (next.tile >= 0) {
-      load_codes<W>(q.key_codes, q.key_scales, next.tile, n, block_log2, kc);
-      load_codes<W>(q.value_codes, q.value_scales, next.tile, n, block_log2, vc);
-    }
-    if (AHEAD && next.tile >= 0) {
-      store_codes<W>(kc, lds.k[1], K_STRIDE, lds.k_mantissa[1]);
-      if (third.tile >= 0) load_codes<W>(q.key_codes, q.key_scales, third.tile, n, block_log2, kc);
+  if (left > 0) {
+    load_keys(here);
+    load_values(here);
+    store_codes<W>(kc, lds.k[0], K_STRIDE);
+    stage_values(here, 0);
+    load_keys(next);
+    load_values(next);
+    if (AHEAD) {
+      store_codes<W>(kc, lds.k[1], K_STRIDE);
+      load_keys(third);
     }
     __syncthreads();
-    if (AHEAD) qk_tile(0, sa);
+    if (AHEAD) {
+      qk_tile(0, sa);
+      __syncthreads();
+    }
   }
-  if (AHEAD) __syncthreads();
 
   // One tile.  AHEAD: `cur` holds its scores, its values are in v[vstage], the
   // next tile's keys in k[kstage ^ 1]; kc holds the third tile's keys, vc the
   // next tile's values.  Otherwise its keys are in k[kstage] and kc holds the
   // next tile's.
   auto tile_step = [&](f32x16_t (&cur)[2], f32x16_t (&nxt)[2]) __attribute__((always_inline)) {
-    const TileRef fourth = third.tile < 0 ? none : walk.next();
-    const float4 km = *reinterpret_cast<const float4*>(lds.k_mantissa[slot]);
-    if (!AHEAD) qk_tile(kstage, cur);
-    const float4 vm = *reinterpret_cast<const float4*>(lds.v_mantissa[vstage]);
-    const bool nan = lds.nan[vstage] == here.tile;
+    const TileRef fourth = advance(third);
     // the stages that the last tile used are free: fill them
-    if (next.tile >= 0) stage_values(next.tile, vstage ^ 1);
-    const int key_tile = AHEAD ? third.tile : next.tile;
-    const int load_key = AHEAD ? fourth.tile : third.tile;
-    // (AHEAD: this tile's keys were read for `cur` already, so their stage is free)
-    if (key_tile >= 0) {
-      const int to = AHEAD ? kstage : kstage ^ 1;
-      store_codes<W>(kc, lds.k[to], K_STRIDE, lds.k_mantissa[(slot + (AHEAD ? 2 : 1)) & 3]);
-    }
-    if (load_key >= 0) load_codes<W>(q.key_codes, q.key_scales, load_key, n, block_log2, kc);
-    if (third.tile >= 0) load_codes<W>(q.value_codes, q.value_scales, third.tile, n, block_log2, vc);
-
-    if (!(km.x == 1.0f && km.y == 1.0f && km.z == 1.0f && km.w == 1.0f)) {
-      asm volatile("");
-      const float mant[4] = {km.x, km.y, km.z, km.w};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) cur[i][v] *= mant[2 * i + (v >> 3)];
-      }
-    }
-    // masks, where some query of this wave does not see some row of the tile
-    const bool masked = here.lo < all_lo || here.hi > all_hi || (here.tile + 1) * KEYS > n;
-    if (masked) {
+    stage_values(next, vstage ^ 1);
+    store_codes<W>(kc, lds.k[AHEAD ? kstage : kstage ^ 1], K_STRIDE);
+    load_keys(AHEAD ? fourth : third);
+    load_values(third);
+    if (!AHEAD) qk_tile(kstage, cur);
+    if (is_masked(here, wave_lo, wave_hi)) {
       asm volatile("");  // a branch, not selects on every tile
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -369,92 +369,67 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
       for (int i = 0; i < 4; ++i) o[i] *= f;
     }
     const float mc = m == NEG_INF ? 0.0f : m * sl2;
-    if (AHEAD) qk_tile(kstage ^ 1, nxt);  // on the last tile: an old stage, unused
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        cur[i][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v], sl2, -mc));
-        l += cur[i][v];
-      }
-    }
-    if (!(vm.x == 1.0f && vm.y == 1.0f && vm.z == 1.0f && vm.w == 1.0f)) {
-      asm volatile("");
-      const float mant[4] = {vm.x, vm.y, vm.z, vm.w};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) cur[i][v] *= mant[2 * i + (v >> 3)];
-      }
-    }
+    if (AHEAD) qk_tile(kstage ^ 1, nxt);  // on the last tile: unused
     uint32_t pb[NP][2][8];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int v = 0; v < 16; v += 2) split_pair<NP>(cur[i][v], cur[i][v + 1], &pb[0][i][v >> 1], 16);
+      for (int v = 0; v < 16; v += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v], sl2, -mc));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v + 1], sl2, -mc));
+        l += p0;
+        l += p1;
+        split_pair<NP>(p0, p1, &pb[0][i][v >> 1], 16);
+      }
     }
     const uint16_t* v_s = lds.v[vstage];
-    auto value_pairs = [&](int kk, int db) __attribute__((always_inline)) {
-      const uint16_t* p = v_s + (16 * kk + 4 * half + ((lane & 15) >> 2)) * V_STRIDE + 16 * ((lane >> 4) & 1) +
-                          4 * (lane & 3) + 32 * db;
-      const uint2 x = lds_read_tr16(p), y = lds_read_tr16(p + 8 * V_STRIDE);
-      return uint4{x.x, x.y, y.x, y.y};
-    };
-    if (!(masked && nan)) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const int i = kk >> 1, vb = 4 * (kk & 1);
+    for (int kk = 0; kk < 4; ++kk) {
+      const int i = kk >> 1, vb = 4 * (kk & 1);
+      const uint16_t* vrow = v_s + (16 * kk + 4 * half + ((lane & 15) >> 2)) * V_STRIDE + 16 * ((lane >> 4) & 1) +
+                             4 * (lane & 3);
 #pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          const uint4 vop = value_pairs(kk, db);
+      for (int db = 0; db < 4; ++db) {
+        const uint2 x = lds_read_tr16(vrow + 32 * db);
+        const uint2 y = lds_read_tr16(vrow + 8 * V_STRIDE + 32 * db);
 #pragma unroll
-          for (int p = 0; p < NP; ++p)
-            o[db] = mfma32(vop, uint4{pb[p][i][vb], pb[p][i][vb + 1], pb[p][i][vb + 2], pb[p][i][vb + 3]}, o[db]);
-        }
+        for (int p = 0; p < NP; ++p)
+          o[db] = mfma32(uint4{x.x, x.y, y.x, y.y},
+                         uint4{pb[p][i][vb], pb[p][i][vb + 1], pb[p][i][vb + 2], pb[p][i][vb + 3]}, o[db]);
       }
-    } else {
-      // a masked row's zero times NaN would spread it: zeros in their place, and
-      // NaN where a query sees such a row
+    }
+    if (is_masked(here, group_lo, group_hi) && lds.nan[vstage] == here.tile) {
+      asm volatile("");
+      // NaN codes that were staged as zeros: NaN where a query sees their row
 #pragma nounroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t one[4], w[NP][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int2 at = *reinterpret_cast<const int2*>(
-              &lds.pos[vstage][16 * kk + 8 * (e >> 1) + 4 * half + 2 * (e & 1)]);
-          one[e] = ((uint32_t)(at.x - see.lo) > see.span ? 0u : 0x3f80u) |
-                   ((uint32_t)(at.y - see.lo) > see.span ? 0u : 0x3f800000u);
-#pragma unroll
-          for (int p = 0; p < NP; ++p)
-            w[p][e] = kk == 0 ? pb[p][0][e] : kk == 1 ? pb[p][0][4 + e] : kk == 2 ? pb[p][1][e] : pb[p][1][4 + e];
-        }
+      for (int r = 0; r < KEYS; ++r) {
+        if (here.tile * KEYS + r >= n) break;
+        const bool sees = (uint32_t)(lds.pos[vstage][r] - see.lo) <= see.span;
+        const uint8_t* code = q.value_codes + (int64_t)(here.tile * KEYS + r) * D + 4 * half;
 #pragma unroll
         for (int db = 0; db < 4; ++db) {
-          uint4 vop = value_pairs(kk, db), is;
-          vop.x = split_nan(vop.x, &is.x);
-          vop.y = split_nan(vop.y, &is.y);
-          vop.z = split_nan(vop.z, &is.z);
-          vop.w = split_nan(vop.w, &is.w);
-          const f32x16_t hits = mfma32(is, uint4{one[0], one[1], one[2], one[3]}, f32x16_t{});
 #pragma unroll
-          for (int p = 0; p < NP; ++p) o[db] = mfma32(vop, uint4{w[p][0], w[p][1], w[p][2], w[p][3]}, o[db]);
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(code + 32 * db + 8 * g);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[db][e] = hits[e] > 0.0f ? __builtin_nanf("") : o[db][e];
+            for (int e = 0; e < 4; ++e)
+              if (sees && ((w >> (8 * e)) & 0x7fu) == 0x7fu) o[db][4 * g + e] = __builtin_nanf("");
+          }
         }
       }
     }
     __syncthreads();
     kstage ^= 1;
     vstage ^= 1;
-    slot = (slot + 1) & 3;
     here = next;
     next = third;
     third = fourth;
+    --left;
   };
-  while (here.tile >= 0) {
+  while (left > 0) {
     if constexpr (AHEAD) {
       tile_step(sa, sb);
-      if (here.tile < 0) break;
+      if (left == 0) break;
       tile_step(sb, sa);
     } else {
       tile_step(sa, sa);
@@ -525,7 +500,7 @@ int launch_rows(const QuantAttendArgs& a, hipStream_t s) {
   int device = 0;
   if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !ready[device]) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RowsLds<W>));
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RowsLds));
     if (e != hipSuccess) {
       (void)hipGetLastError();
       return ckv_internal::set_error(CKV_E_LAUNCH, hipGetErrorString(e));
@@ -533,7 +508,7 @@ int launch_rows(const QuantAttendArgs& a, hipStream_t s) {
     if (device >= 0 && device < 64) ready[device] = true;
   }
   const dim3 grid(c.batch * c.kv_heads, (a.rows + 32 * W - 1) / (32 * W), a.splits);
-  kernel<<<grid, 64 * W, sizeof(RowsLds<W>), s>>>(a);
+  kernel<<<grid, 64 * W, sizeof(RowsLds), s>>>(a);
   return launched("ckv_quant_attention");
 }
 
@@ -587,7 +562,6 @@ __global__ __launch_bounds__(64 * WT_WAVES, 2) void rows_weights_kernel(const Qu
     lds.pos[tid] = r < n ? gload_i32(q.positions + r) : 0x7fffffff;  // nobody sees rows past the last
   }
   uint4 kop[2][8];
-  float mant[2][2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = min(row0 + 32 * i + (lane & 31), n - 1);
@@ -597,11 +571,7 @@ __global__ __launch_bounds__(64 * WT_WAVES, 2) void rows_weights_kernel(const Qu
       const uint2 w = *reinterpret_cast<const uint2*>(q.key_codes + (int64_t)r * D + 16 * s + 8 * half);
       kop[i][s] = scaled_codes8(w.x, w.y, scale);
     }
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-      mant[i][g] = mantissa_of(gload_f32(q.key_scales + (min(row0 + 32 * i + 16 * g, n - 1) >> block_log2)));
   }
-  const bool plain = mant[0][0] == 1.0f && mant[0][1] == 1.0f && mant[1][0] == 1.0f && mant[1][1] == 1.0f;
   // steps whose queries t see any of some rows: seen - count + t >= least position, and > largest - window
   const int64_t first_at = (int64_t)seen - count;
   const int steps = (a.rows + WT_ROWS - 1) / WT_ROWS;
@@ -698,14 +668,6 @@ __global__ __launch_bounds__(64 * WT_WAVES, 2) void rows_weights_kernel(const Qu
           }
         }
         const float2 st = lds.stats[stage][qrow];
-        if (!plain) {
-          asm volatile("");
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][v] *= mant[i][v >> 3];
-          }
-        }
         int lo, hi;
         query_range(a, step * WT_ROWS + qrow, count, seen, &lo, &hi);
         if (row0 + KEYS > n || __ballot(range.x < lo || range.y > hi) != 0) {

@@ -568,9 +568,11 @@ int ckv_dense_decode(const ckv_kv_cache* kv, int32_t seq_len, float softmax_scal
 
 /* 8-bit KV cache of one layer (no reference counterpart; the reference's cache
  * is bf16).  Codes are OCP E4M3, row-major and dense; a block of `block` rows
- * of one sequence and head has one scale for its keys and one for its values,
- * and a value is code * scale.  A cache is a set of (position, key, value)
- * rows: every mask goes by position, so rows may stand in any order. */
+ * of one sequence and head has one scale for its keys and one for its values, a
+ * power of two in [2^-64, 2^120] (0 where no row is in use), and a value is
+ * code * scale.  A cache is a set of (position, key, value)
+ * rows: every mask goes by position, so rows may stand in any order.  Positions
+ * in use lie in [0, seen). */
 typedef struct ckv_quant_cache {
   void* key_codes;         /* [batch][kv_heads][capacity][128] E4M3 */
   void* value_codes;       /* same */

@@ -71,6 +71,10 @@ def _tensors(cache):
     ("value_codes", torch.zeros(2, 2, 128, 128), TypeError),
     ("key_scales", torch.zeros(2, 2, 5), ValueError),
     ("value_scales", torch.zeros(2, 2, 4, dtype=torch.float64), TypeError),
+    ("key_scales", torch.full((2, 2, 4), 1.5), ValueError),
+    ("value_scales", torch.full((2, 2, 4), float("inf")), ValueError),
+    ("value_scales", torch.full((2, 2, 4), -1.0), ValueError),
+    ("value_scales", torch.full((2, 2, 4), 2.0 ** -65), ValueError),
     ("positions", torch.zeros(2, 2, 128, dtype=torch.int64), TypeError),
     ("cursors", torch.zeros(2, 2, dtype=torch.int32), ValueError),
     ("weights", torch.zeros(2, 2, 128, 2)[..., 0], ValueError),
@@ -80,6 +84,12 @@ def test_from_tensors_refuses(name, value, error):
     assert QuantizedKVCache.from_tensors(**good).key_codes is good["key_codes"]
     with pytest.raises(error):
         QuantizedKVCache.from_tensors(**(good | {name: value}))
+
+
+def test_from_tensors_takes_the_whole_range_of_scales():
+    good = _tensors(_cache())
+    good["key_scales"] = torch.tensor([0.0, 2.0 ** -64, 1.0, 2.0 ** 120]).expand(2, 2, 4).contiguous()
+    QuantizedKVCache.from_tensors(**good)
 
 
 def test_calls_refuse_bad_arguments():
