@@ -25,11 +25,12 @@ struct QuantAttendArgs {
   float* part_max;   // [batch][kv_heads][row_pad][splits], log2
   float* part_sum;
   float* part_acc;   // [batch][kv_heads][splits][row_pad][128]
-  float2* stats;     // [batch][kv_heads][row_pad]: log2 maximum and 1 / sum, or null
+  float2* stats;     // [batch][kv_heads][row_pad]: log2 maximum and 1 / sum (0, 0 without a row), or null
   int2* ranges;      // [batch][kv_heads][tiles]: least and largest position of every RANGE_TILE rows, or null
   float* sums;       // [shares][batch][kv_heads][capacity] received weights, or null
   float scale_log2;  // softmax_scale * log2 e
   int32_t tokens, group, rows, row_pad, window, splits;
+  uint32_t group_magic;  // ceil(2^32 / group), 0 for a group of one
 };
 
 // Two E4M3 codes in the low / high half of `w` as bf16 (exact).
@@ -88,9 +89,14 @@ __host__ __device__ inline int part_rows(int n, int splits) {
   return ((n + splits - 1) / splits + PART_UNIT - 1) / PART_UNIT * PART_UNIT;
 }
 
+// row / group without a division: exact while row * group < 2^32 (rows are below 2^22, groups at most 16).
+__device__ inline int token_of(const QuantAttendArgs& a, int row) {
+  return a.group_magic ? (int)__umulhi((uint32_t)row, a.group_magic) : row;
+}
+
 // Positions that query row `row` may see: [lo, hi].
 __device__ inline void query_range(const QuantAttendArgs& a, int row, int count, int seen, int* lo, int* hi) {
-  const int t = row / a.group;
+  const int t = token_of(a, row);
   const bool ok = row < a.rows && t < count;
   const int at = seen - count + t;
   *hi = ok ? at : -1;
@@ -100,7 +106,7 @@ __device__ inline void query_range(const QuantAttendArgs& a, int row, int count,
 // Where query row `row` of KV head h goes: index of its first output element
 // and of its lse.
 __device__ inline void output_index(const QuantAttendArgs& a, int b, int h, int row, int64_t* out, int64_t* lse) {
-  const int t = row / a.group, g = row % a.group;
+  const int t = token_of(a, row), g = row - t * a.group;
   const int64_t hq = (int64_t)h * a.group + g, heads = (int64_t)a.cache.kv_heads * a.group;
   *out = (((int64_t)b * a.tokens + t) * heads + hq) * D;
   *lse = ((int64_t)b * heads + hq) * a.tokens + t;

@@ -49,7 +49,7 @@ __device__ inline void load_query_tile(const QuantAttendArgs& a, int b, int h, i
   const int L = (threadIdx.x & 63) >> 4;
   const int row = row0 + (threadIdx.x & 15);
   const bool ok = row < a.rows;
-  const int t = ok ? row / a.group : 0, g = ok ? row % a.group : 0;
+  const int t = ok ? token_of(a, row) : 0, g = ok ? row - t * a.group : 0;
   const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
                        (int64_t)t * a.query.token_stride;
 #pragma unroll
@@ -555,6 +555,7 @@ extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant
   a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
   a.tokens = tokens;
   a.group = group;
+  a.group_magic = group > 1 ? (uint32_t)(((1ull << 32) + group - 1) / group) : 0u;
   a.rows = tokens * group;
   a.row_pad = lay.row_pad;
   a.window = window;

@@ -165,9 +165,9 @@ __device__ inline bool drop_nan_codes(uint32_t& w) {
 }
 
 struct RowsLds {
-  uint16_t k[2][K_TILE];
-  uint16_t v[2][V_TILE];
-  int32_t pos[2][KEYS];
+  alignas(16) uint16_t k[2][K_TILE];
+  alignas(16) uint16_t v[2][V_TILE];
+  alignas(16) int32_t pos[2][KEYS];
   int nan[2];  // the tile, where its values held a NaN code that was staged as zero
 };
 
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   const Seen see(lo, hi);
   // Positions that the queries t0 .. t1 see: some of them [some_lo, some_hi], all of them [all_lo, all_hi].
   auto ranges_of = [&](int first, int rows, int* some_lo, int* some_hi, int* all_lo, int* all_hi) {
-    const int t0 = first / a.group, t1 = min((min(first + rows, a.rows) - 1) / a.group, count - 1);
+    const int t0 = token_of(a, first), t1 = min(token_of(a, min(first + rows, a.rows) - 1), count - 1);
     *some_lo = *all_lo = 0;
     *some_hi = -1;
     *all_hi = 0x7ffffffe;  // without a query nothing is masked: the rows are dropped at the end
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   uint4 qreg[NP][8];
   {
     const int qrow = min(row, a.rows - 1);
-    const int t = qrow / a.group, g = qrow % a.group;
+    const int t = token_of(a, qrow), g = qrow - t * a.group;
     const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
                          (int64_t)t * a.query.token_stride;
 #pragma unroll
@@ -512,137 +512,128 @@ int launch_rows(const QuantAttendArgs& a, hipStream_t s) {
   return launched("ckv_quant_attention");
 }
 
-// Received weight.  A wave keeps 64 cache rows as A operands in registers; the
-// workgroup's four waves (256 cache rows) go over the query rows, 32 a step,
+// Received weight.  A wave keeps 32 cache rows as A operands in registers; the
+// workgroup's eight waves (256 cache rows) go over the query rows, 64 a step,
 // staged in LDS a step ahead.  With the scores' layout as above a lane adds up
 // what its cache rows got from the queries lane % 32; the lanes are added once
 // at the end.  The steps are shared out over `shares` workgroups a block of cache
 // rows, which leave sums of their own for weights_add_kernel: one owner a sum
-// and a fixed order, no atomics.  Per step and wave: 16 products of 32 cycles
-// beside 32 x (fma, exp, fma), 24 cycles each, so the vector ALUs bound it.
-constexpr int WT_WAVES = 4;
+// and a fixed order, no atomics.  Four small waves a SIMD overlap one's products
+// with another's exponentials: the counters show the matrix cores busy half of
+// the time and the vector ALUs 70 %.  2,048 queries over 32k rows (32/8 heads)
+// take 582 us; interleaving the two within a wave, half a step apart, took 612,
+// waves of 64 rows, two a SIMD, 10 % more.
+constexpr int WT_WAVES = 8;
 constexpr int WT_ROWS = 64;   // query rows of a step
-constexpr int WT_KEYS = WT_WAVES * KEYS;
+constexpr int WT_KEYS = WT_WAVES * 32;
 
 template <int NP>
 struct WeightsLds {
-  uint16_t q[2][NP][WT_ROWS * K_STRIDE];
+  alignas(16) uint16_t q[2][NP][WT_ROWS * K_STRIDE];
   float2 stats[2][WT_ROWS];
-  int32_t pos[WT_KEYS];
+  alignas(16) int32_t pos[WT_KEYS];
 };
 
 template <int DT>
-__global__ __launch_bounds__(64 * WT_WAVES, 2) void rows_weights_kernel(const QuantAttendArgs a, const int shares) {
+__global__ __launch_bounds__(64 * WT_WAVES, DT == CKV_F32 ? 2 : 4) void rows_weights_kernel(const QuantAttendArgs a,
+                                                                                          const int shares) {
   constexpr int NP = pieces(DT);
-  __shared__ WeightsLds<NP> lds;
+  __shared__ __align__(16) WeightsLds<NP> lds;
   const ckv_quant_cache& c = a.cache;
   const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int half = lane >> 5;
   const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
-  const int64_t tile0 = (int64_t)blockIdx.y * WT_WAVES, tile = tile0 + wave;
-  if (tile0 * KEYS >= n) return;
+  const int64_t first_row = (int64_t)blockIdx.y * WT_KEYS;
+  if (first_row >= n) return;
   const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
-  const int live_tiles = (n + KEYS - 1) / KEYS;
+  const int live_tiles = (n + KEYS - 1) / KEYS, tile0 = (int)(first_row / KEYS);
   const QuantHead q = quant_head(c, b, h);
   const int block_log2 = 31 - __clz(c.block);
-  const int row0 = (int)tile * KEYS;
-  const bool live = tile < live_tiles;
-  // least and largest position of this wave's rows, and of the workgroup's
+  const int row0 = (int)first_row + 32 * wave;
+  const bool full = row0 + 32 <= n;
+  // least and largest position of the tile that this wave's rows lie in, and of the workgroup's
   int2 range{0x7fffffff, -1}, all{0x7fffffff, -1};
 #pragma unroll
-  for (int w = 0; w < WT_WAVES; ++w) {
-    if (tile0 + w >= live_tiles) break;
-    const int2 r = a.ranges[(int64_t)bh * tiles + tile0 + w];
-    if (w == wave) range = r;
+  for (int t = 0; t < WT_KEYS / KEYS; ++t) {
+    if (tile0 + t >= live_tiles) break;
+    const int2 r = a.ranges[(int64_t)bh * tiles + tile0 + t];
+    if (t == wave >> 1) range = r;
     all.x = min(all.x, r.x);
     all.y = max(all.y, r.y);
   }
-  {
-    const int64_t r = tile0 * KEYS + tid;
+  if (tid < WT_KEYS) {
+    const int64_t r = first_row + tid;
     lds.pos[tid] = r < n ? gload_i32(q.positions + r) : 0x7fffffff;  // nobody sees rows past the last
   }
-  uint4 kop[2][8];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = min(row0 + 32 * i + (lane & 31), n - 1);
+  uint4 kop[8];
+  {
+    const int r = min(row0 + (lane & 31), n - 1);
     const float scale = gload_f32(q.key_scales + (r >> block_log2));
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
       const uint2 w = *reinterpret_cast<const uint2*>(q.key_codes + (int64_t)r * D + 16 * s + 8 * half);
-      kop[i][s] = scaled_codes8(w.x, w.y, scale);
+      kop[s] = scaled_codes8(w.x, w.y, scale);
     }
   }
-  // steps whose queries t see any of some rows: seen - count + t >= least position, and > largest - window
-  const int64_t first_at = (int64_t)seen - count;
+  // steps whose queries t see any of the rows: seen - count + t >= least position, and > largest - window
   const int steps = (a.rows + WT_ROWS - 1) / WT_ROWS;
-  auto steps_of = [&](int2 r, int* lo, int* hi) {
-    const int64_t t_lo = max((int64_t)r.x - first_at, (int64_t)0);
-    int64_t t_hi = (int64_t)count - 1;
-    if (a.window > 0) t_hi = min(t_hi, (int64_t)r.y + a.window - 1 - first_at);
-    *lo = (int)min(t_lo * a.group / WT_ROWS, (int64_t)steps);
-    *hi = t_hi < 0 ? 0 : (int)min((t_hi * a.group + a.group - 1) / WT_ROWS + 1, (int64_t)steps);
-  };
-  int step_lo, step_hi, my_lo, my_hi;
-  steps_of(all, &step_lo, &step_hi);
-  steps_of(range, &my_lo, &my_hi);
-  if (!live) my_hi = 0;
+  const int64_t first_at = (int64_t)seen - count;
+  const int64_t t_lo = max((int64_t)all.x - first_at, (int64_t)0);
+  int64_t t_hi = (int64_t)count - 1;
+  if (a.window > 0) t_hi = min(t_hi, (int64_t)all.y + a.window - 1 - first_at);
+  const int step_lo = (int)min(t_lo * a.group / WT_ROWS, (int64_t)steps);
+  const int step_hi = t_hi < 0 ? 0 : (int)min((t_hi * a.group + a.group - 1) / WT_ROWS + 1, (int64_t)steps);
   const float sl2 = a.scale_log2;
   const float2* stats = a.stats + (int64_t)bh * a.row_pad;
-  // a thread stages 16 dims of the query rows tid / 8 and tid / 8 + 32 of a step, as they are in memory
-  const int qd = 16 * (tid & 7);
+  // a thread stages 16 dims of query row tid / 8 of a step, as they are in memory
+  const int qd = 16 * (tid & 7), qr = tid >> 3;
   constexpr int RAW = DT == CKV_F32 ? 4 : 2;  // 16-byte pieces
-  uint4 raw[2][RAW];
+  uint4 raw[RAW];
   float2 next_st{0.0f, 0.0f};
   auto load = [&](int step) __attribute__((always_inline)) {
+    const int row = min(step * WT_ROWS + qr, a.rows - 1);
+    const int t = token_of(a, row), g = row - t * a.group;
+    const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
+                         (int64_t)t * a.query.token_stride + qd;
+    const char* from = reinterpret_cast<const char*>(a.query.data) + base * (DT == CKV_F32 ? 4 : 2);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int row = min(step * WT_ROWS + (tid >> 3) + 32 * x, a.rows - 1);
-      const int t = row / a.group, g = row - t * a.group;
-      const int64_t base = (int64_t)b * a.query.batch_stride + (int64_t)(h * a.group + g) * a.query.head_stride +
-                           (int64_t)t * a.query.token_stride + qd;
-      const char* from = reinterpret_cast<const char*>(a.query.data) + base * (DT == CKV_F32 ? 4 : 2);
-#pragma unroll
-      for (int i = 0; i < RAW; ++i) raw[x][i] = gload16(from + 16 * i);
-    }
+    for (int i = 0; i < RAW; ++i) raw[i] = gload16(from + 16 * i);
     if (tid < WT_ROWS) {
       const int r = step * WT_ROWS + tid;
-      next_st = r < a.rows ? stats[r] : float2{0.0f, 0.0f};  // a row past the last gives nothing
+      next_st = r < a.rows ? stats[r] : float2{0.0f, 0.0f};
     }
   };
   auto store = [&](int stage) __attribute__((always_inline)) {
+    uint4* to = reinterpret_cast<uint4*>(&lds.q[stage][0][qr * K_STRIDE + qd]);
+    if constexpr (DT == CKV_BF16) {
+      to[0] = raw[0];
+      to[1] = raw[1];
+    } else {
+      uint32_t w[NP * 8];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int qr = (tid >> 3) + 32 * x;
-      if constexpr (DT == CKV_BF16) {
-        uint4* to = reinterpret_cast<uint4*>(&lds.q[stage][0][qr * K_STRIDE + qd]);
-        to[0] = raw[x][0];
-        to[1] = raw[x][1];
-      } else {
-        uint32_t w[NP * 8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t* r = reinterpret_cast<const uint32_t*>(&raw[x][0]);
-          float lo, hi;
-          if constexpr (DT == CKV_F16) {
-            lo = (float)__builtin_bit_cast(_Float16, (uint16_t)(r[i] & 0xffffu));
-            hi = (float)__builtin_bit_cast(_Float16, (uint16_t)(r[i] >> 16));
-          } else {
-            lo = ckv_u2f(r[2 * i]);
-            hi = ckv_u2f(r[2 * i + 1]);
-          }
-          split_pair<NP>(lo, hi, w + i, 8);
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t* r = reinterpret_cast<const uint32_t*>(&raw[0]);
+        float lo, hi;
+        if constexpr (DT == CKV_F16) {
+          lo = (float)__builtin_bit_cast(_Float16, (uint16_t)(r[i] & 0xffffu));
+          hi = (float)__builtin_bit_cast(_Float16, (uint16_t)(r[i] >> 16));
+        } else {
+          lo = ckv_u2f(r[2 * i]);
+          hi = ckv_u2f(r[2 * i + 1]);
         }
+        split_pair<NP>(lo, hi, w + i, 8);
+      }
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          uint4* to = reinterpret_cast<uint4*>(&lds.q[stage][p][qr * K_STRIDE + qd]);
-          to[0] = uint4{w[8 * p], w[8 * p + 1], w[8 * p + 2], w[8 * p + 3]};
-          to[1] = uint4{w[8 * p + 4], w[8 * p + 5], w[8 * p + 6], w[8 * p + 7]};
-        }
+      for (int p = 0; p < NP; ++p) {
+        uint4* piece = to + p * (WT_ROWS * K_STRIDE / 8);
+        piece[0] = uint4{w[8 * p], w[8 * p + 1], w[8 * p + 2], w[8 * p + 3]};
+        piece[1] = uint4{w[8 * p + 4], w[8 * p + 5], w[8 * p + 6], w[8 * p + 7]};
       }
     }
     if (tid < WT_ROWS) lds.stats[stage][tid] = next_st;
   };
-  f32x16_t got[2] = {f32x16_t{}, f32x16_t{}};
+  f32x16_t got = {};
   int stage = 0;
   const int first = step_lo + (int)blockIdx.z;
   if (first < step_hi) {
@@ -651,82 +642,73 @@ __global__ __launch_bounds__(64 * WT_WAVES, 2) void rows_weights_kernel(const Qu
   }
   __syncthreads();
   for (int step = first; step < step_hi; step += shares) {
-    const bool more = step + shares < step_hi;
-    if (more) load(step + shares);
-    if (step >= my_lo && step < my_hi) {
+    load(min(step + shares, step_hi - 1));
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int qrow = 32 * x + (lane & 31);
-        f32x16_t acc[2] = {f32x16_t{}, f32x16_t{}};
+    for (int x = 0; x < 2; ++x) {
+      const int qrow = 32 * x + (lane & 31);
+      f32x16_t acc = {};
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
+      for (int s = 0; s < 8; ++s) {
 #pragma unroll
-          for (int p = 0; p < NP; ++p) {
-            const uint4 qop = *reinterpret_cast<const uint4*>(&lds.q[stage][p][qrow * K_STRIDE + 16 * s + 8 * half]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) acc[i] = mfma32(kop[i][s], qop, acc[i]);
-          }
-        }
-        const float2 st = lds.stats[stage][qrow];
+        for (int p = 0; p < NP; ++p)
+          acc = mfma32(kop[s], *reinterpret_cast<const uint4*>(&lds.q[stage][p][qrow * K_STRIDE + 16 * s + 8 * half]),
+                       acc);
+      }
+      const float2 st = lds.stats[stage][qrow];
+      // the 32 query rows together first, on the scalar unit: all there and all seeing all of the wave's rows
+      const int row = step * WT_ROWS + 32 * x, last = row + 31;
+      bool clear = full && last < a.rows;
+      if (clear) {
+        const int t0 = token_of(a, row), t1 = token_of(a, last);
+        int lo, hi, unused;
+        query_range(a, t0 * a.group, count, seen, &unused, &hi);
+        query_range(a, t1 * a.group, count, seen, &lo, &unused);
+        clear = t1 < count && range.x >= lo && range.y <= hi;
+      }
+      if (!clear) {
+        asm volatile("");
         int lo, hi;
         query_range(a, step * WT_ROWS + qrow, count, seen, &lo, &hi);
-        if (row0 + KEYS > n || __ballot(range.x < lo || range.y > hi) != 0) {
-          asm volatile("");
-          const Seen see(lo, hi);
+        const Seen see(lo, hi);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+        for (int g = 0; g < 4; ++g) {
+          const int4 p = *reinterpret_cast<const int4*>(&lds.pos[32 * wave + 8 * g + 4 * half]);
+          const int at[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int4 p = *reinterpret_cast<const int4*>(&lds.pos[KEYS * wave + 32 * i + 8 * g + 4 * half]);
-              const int at[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float y = acc[i][4 * g + e];
-                see.mask(y, at[e]);
-                acc[i][4 * g + e] = y;
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][v], sl2, -st.x));
-            got[i][v] = __builtin_fmaf(p, st.y, got[i][v]);
+          for (int e = 0; e < 4; ++e) {
+            float y = acc[4 * g + e];
+            see.mask(y, at[e]);
+            acc[4 * g + e] = y;
           }
         }
       }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], sl2, -st.x));
+        got[v] = __builtin_fmaf(p, st.y, got[v]);
+      }
     }
-    if (more) store(stage ^ 1);
+    store(stage ^ 1);
     __syncthreads();
     stage ^= 1;
   }
-  if (!live) return;
+  // lane 4 g + e of each half writes its row 8 g + 4 half + e
+  float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-#pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      float x = got[i][v];
-      x = add_xor_f32<1>(x);
-      x = add_xor_f32<2>(x);
-      x = add_xor_f32<4>(x);
-      x = x + xor_f32<8>(x);
-      got[i][v] = add_xor16(x);
-    }
+  for (int v = 0; v < 16; ++v) {
+    float x = got[v];
+    x = add_xor_f32<1>(x);
+    x = add_xor_f32<2>(x);
+    x = add_xor_f32<4>(x);
+    x = x + xor_f32<8>(x);
+    x = add_xor16(x);
+    sum = (lane & 15) == v ? x : sum;
   }
-  // lane 4 g + e of each half writes its rows 8 g + 4 half + e
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float x = got[i][0];
-#pragma unroll
-    for (int v = 1; v < 16; ++v) x = (lane & 15) == v ? got[i][v] : x;
-    const int v = lane & 15;
-    const int r = row0 + 32 * i + 8 * (v >> 2) + 4 * half + (v & 3);
-    if ((lane & 16) == 0 && r < n) {
-      if (shares == 1) q.weights[r] += x;
-      else a.sums[((int64_t)blockIdx.z * gridDim.x + bh) * c.capacity + r] = x;
-    }
+  const int v = lane & 15;
+  const int r = row0 + 8 * (v >> 2) + 4 * half + (v & 3);
+  if ((lane & 16) == 0 && r < n) {
+    if (shares == 1) q.weights[r] += sum;
+    else a.sums[((int64_t)blockIdx.z * gridDim.x + bh) * c.capacity + r] = sum;
   }
 }
 
