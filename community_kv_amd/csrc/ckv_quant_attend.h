@@ -22,14 +22,15 @@ struct QuantAttendArgs {
   const int32_t* counts;
   void* out;
   float* lse;
-  float* part_max;   // [batch][kv_heads][row_pad][splits], log2
+  float* part_max;   // [kv_heads][row_pad][parts], log2
   float* part_sum;
-  float* part_acc;   // [batch][kv_heads][splits][row_pad][128]
+  float* part_acc;   // [kv_heads][parts][row_pad][128]
   float2* stats;     // [batch][kv_heads][row_pad]: log2 maximum and 1 / sum (0, 0 without a row), or null
   int2* ranges;      // [batch][kv_heads][tiles]: least and largest position of every RANGE_TILE rows, or null
+  float* scores;     // [batch][kv_heads][rows][capacity] masked scores, log2, or null
   float* sums;       // [shares][batch][kv_heads][capacity] received weights, or null
   float scale_log2;  // softmax_scale * log2 e
-  int32_t tokens, group, rows, row_pad, window, splits;
+  int32_t tokens, group, rows, row_pad, window, parts;
   uint32_t group_magic;  // ceil(2^32 / group), 0 for a group of one
 };
 
@@ -84,9 +85,54 @@ __device__ inline int new_count(const QuantAttendArgs& a, int b) {
   return a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
 }
 
-// The rows [lo, hi) of part `split`: equal parts of whole units.
-__host__ __device__ inline int part_rows(int n, int splits) {
-  return ((n + splits - 1) / splits + PART_UNIT - 1) / PART_UNIT * PART_UNIT;
+// The cache rows of all sequences in `parts` parts of nearly equal size, so that
+// every workgroup of a ragged batch has the same work: part size = the rows of
+// the batch over parts - batch (whole units), a sequence of n rows has
+// max(1, ceil(n / size)) parts, which together are at most `parts`.  With as
+// many parts as sequences each sequence is one part.  Every wave works this out
+// for itself, 64 sequences at a time.
+struct Part {
+  int sequence;    // -1: none
+  int index;       // within the sequence
+  int first;       // number of the sequence's first part
+  int count;       // the sequence's parts
+  int rows;        // rows of a part
+};
+
+__device__ inline int part_size(const ckv_quant_cache& c, int parts) {
+  if (parts <= c.batch) return 0x7fffff80;
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0;
+  for (int b0 = 0; b0 < c.batch; b0 += 64) total += b0 + lane < c.batch ? quant_length(c, b0 + lane) : 0;
+  for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
+  const int64_t spare = parts - c.batch;
+  const int64_t units = ((total + spare - 1) / spare + PART_UNIT - 1) / PART_UNIT;
+  return (int)min(max(units, (int64_t)1) * PART_UNIT, (int64_t)0x7fffff80);
+}
+
+__device__ inline int parts_of_sequence(int n, int size) { return n > size ? (n - 1) / size + 1 : 1; }
+
+// Part number `part` (wanted < 0), or sequence `wanted`'s first part.
+__device__ inline Part find_part(const ckv_quant_cache& c, int parts, int part, int wanted) {
+  const int size = part_size(c, parts);
+  if (parts <= c.batch) {
+    const int b = wanted < 0 ? part : wanted;
+    return Part{b, 0, b, 1, size};
+  }
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int b0 = 0; b0 < c.batch; b0 += 64) {
+    const int mine = b0 + lane < c.batch ? parts_of_sequence(quant_length(c, b0 + lane), size) : 0;
+    const int end = before + wave_inclusive_scan(mine);  // parts up to and with this lane's sequence
+    const uint64_t hit = wanted < 0 ? __ballot(mine > 0 && part < end) : __ballot(b0 + lane == wanted);
+    if (hit) {
+      const int at = __ffsll((unsigned long long)hit) - 1;
+      const int count = __builtin_amdgcn_readlane(mine, at), first = __builtin_amdgcn_readlane(end, at) - count;
+      return Part{b0 + at, part - first, first, count, size};
+    }
+    before = __builtin_amdgcn_readlane(end, 63);
+  }
+  return Part{-1, 0, 0, 0, size};
 }
 
 // row / group without a division: exact while row * group < 2^32 (rows are below 2^22, groups at most 16).

@@ -20,6 +20,8 @@ using namespace ckv;
 
 constexpr int STEP = 32;  // cache rows a wave takes at a time
 constexpr int WAVES = 4;
+constexpr int FEW_WORKGROUPS = 512;  // workgroups that split the cache rows: two a compute unit, all at once
+constexpr int MAX_PARTS = FEW_WORKGROUPS;  // of one sequence
 static_assert(PART_UNIT % (WAVES * STEP) == 0, "parts are whole rounds of the waves");
 
 int fail(int code, const char* message) { return ckv_internal::set_error(code, message); }
@@ -187,10 +189,10 @@ __device__ inline void add_step(const float* sc, float vs, const uint4* vop, boo
 #pragma unroll
   for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[i]);
   if (__ballot(top > r.m + RESCALE) != 0) {
-    float t = fmaxf(r.m, top);
-    t = fmaxf(t, xor_f32<16>(t));
+    float t = fmaxf(top, xor_f32<16>(top));
     t = fmaxf(t, xor_f32<32>(t));
-    const float corr = r.m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(r.m - t);
+    t = t > r.m + RESCALE ? t : r.m;  // a query's own scores alone decide
+    const float corr = r.m == t ? 1.0f : __builtin_amdgcn_exp2f(r.m - t);
     const int L = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -243,19 +245,24 @@ __device__ inline void add_step(const float* sc, float vs, const uint4* vop, boo
 
 // One workgroup of four waves takes a part of the cache rows of a (sequence,
 // head) for NR * 16 query rows; its waves take steps in turn and join in LDS.
+// Bound by memory: eight sequences of 16k-131k rows (32/8 heads, one query,
+// bf16) read 1.69 GB in 283 us, 6.0 TB/s.  512 workgroups, all resident, two
+// waves a SIMD: 1,024 and 2,048 workgroups take 3 and 8 % longer there and 9 and
+// 20 % at one sequence of 131k; three waves a SIMD (168 registers) the same or
+// longer, reading a step ahead into a second set of registers the same.
 template <int DT, int NR>
-__global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const QuantAttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES, NR == 1 ? 2 : 1) void attend_split_kernel(const QuantAttendArgs a) {
   __shared__ float m_s[WAVES][16];
   __shared__ float l_s[WAVES][16];
   __shared__ float o_s[WAVES][16 * D];
   const ckv_quant_cache& c = a.cache;
-  const int b = blockIdx.z / c.kv_heads, h = blockIdx.z % c.kv_heads;
-  const int row0 = blockIdx.x * (16 * NR), split = blockIdx.y;
+  const int h = blockIdx.x % c.kv_heads, number = blockIdx.x / c.kv_heads, row0 = blockIdx.y * (16 * NR);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, L = lane >> 4, col = lane & 15;
+  const Part part = find_part(c, a.parts, number, -1);
+  const int b = part.sequence;
+  if (b < 0) return;  // the join knows how many parts there are
   const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
-  const int per = part_rows(n, a.splits);
-  const int lo_row = (int)min((int64_t)split * per, (int64_t)n), hi_row = min(lo_row + per, n);
-  if (split > 0 && lo_row >= n) return;  // the join knows how many parts there are
+  const int lo_row = part.index * part.rows, hi_row = (int)min((int64_t)lo_row + part.rows, (int64_t)n);
   const QuantHead q = quant_head(c, b, h);
   const int block_log2 = 31 - __clz(c.block);
   QueryTile<DT> query[NR];
@@ -297,6 +304,12 @@ __global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const QuantAtt
       float sc[8];
       step_scores<DT>(cur, query[r], a.scale_log2, sc);
       if (tail || by_position) mask_step(by_position ? q.positions : nullptr, t0, n, lo[r], hi[r], sc);
+      if (NR == 1 && a.scores && col < a.rows && t0 + 8 * L < n) {
+        float4* p = reinterpret_cast<float4*>(
+            a.scores + (((int64_t)b * c.kv_heads + h) * a.rows + col) * c.capacity + t0 + 8 * L);
+        p[0] = float4{sc[0], sc[1], sc[2], sc[3]};
+        p[1] = float4{sc[4], sc[5], sc[6], sc[7]};
+      }
       add_step<DT>(sc, cur.vs, vop, fix_nan, raw, run[r]);
     }
   }
@@ -333,7 +346,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const QuantAtt
         acc += o_s[w][x] * f;
       }
       const int64_t bh = (int64_t)b * c.kv_heads + h;
-      if (a.splits == 1) {
+      if (a.parts == c.batch) {
         int64_t at_out, at_lse;
         output_index(a, b, h, row, &at_out, &at_lse);
         store_out<DT>(a.out, at_out + d, sum == 0.0f ? 0.0f : acc / sum);
@@ -342,43 +355,98 @@ __global__ __launch_bounds__(64 * WAVES) void attend_split_kernel(const QuantAtt
           if (a.stats) a.stats[bh * a.row_pad + row] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
         }
       } else {
-        a.part_acc[((bh * a.splits + split) * a.row_pad + row) * D + d] = acc;
+        a.part_acc[(((int64_t)h * a.parts + number) * a.row_pad + row) * D + d] = acc;
         if (d == 0) {
-          a.part_max[(bh * a.row_pad + row) * a.splits + split] = m;
-          a.part_sum[(bh * a.row_pad + row) * a.splits + split] = sum;
+          a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m;
+          a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
         }
       }
     }
   }
 }
 
-// Joins the parts of one query row (a workgroup of 128 threads, a dim each).
+// Joins the parts of one query row: a workgroup of 256 threads, a part each for
+// the maximum and the sum, then four dims and every eighth part each.
+constexpr int JOIN_THREADS = 256;
+
 template <int DT>
-__global__ __launch_bounds__(D) void attend_join_kernel(const QuantAttendArgs a) {
+__global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(const QuantAttendArgs a) {
+  __shared__ float factor[MAX_PARTS];
+  __shared__ float scratch[4];
+  __shared__ float4 acc_s[JOIN_THREADS];
   const ckv_quant_cache& c = a.cache;
-  const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, d = threadIdx.x;
-  const int n = quant_length(c, b);
-  const int per = part_rows(n, a.splits);
-  const int parts = n > 0 ? (n + per - 1) / per : 1;
-  const int64_t bh = (int64_t)b * c.kv_heads + h;
-  const float* pm = a.part_max + (bh * a.row_pad + row) * a.splits;
-  const float* pl = a.part_sum + (bh * a.row_pad + row) * a.splits;
+  const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const Part part = find_part(c, a.parts, 0, b);
+  const float* pm = a.part_max + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
+  const float* pl = a.part_sum + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
   float m = NEG_INF;
-  for (int s = 0; s < parts; ++s) m = fmaxf(m, pm[s]);
+  for (int s = tid; s < part.count; s += JOIN_THREADS) m = fmaxf(m, pm[s]);
+  m = block_max256(m, scratch);
   const float at = m == NEG_INF ? 0.0f : m;
-  float sum = 0.0f, acc = 0.0f;
-  for (int s = 0; s < parts; ++s) {
+  float sum = 0.0f;
+  for (int s = tid; s < part.count; s += JOIN_THREADS) {
     const float f = __builtin_amdgcn_exp2f(pm[s] - at);
+    factor[s] = f;
     sum += pl[s] * f;
-    acc += a.part_acc[((bh * a.splits + s) * a.row_pad + row) * D + d] * f;
   }
+  sum = wave_sum_tree(sum);
+  __syncthreads();  // scratch is read
+  if ((tid & 63) == 0) scratch[tid >> 6] = sum;
+  __syncthreads();
+  sum = (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
+  const int dim = 4 * (tid & 31);
+  float4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.first) * a.row_pad + row) * D + dim;
+#pragma unroll 4
+  for (int s = tid >> 5; s < part.count; s += JOIN_THREADS / 32) {
+    const float4 x = *reinterpret_cast<const float4*>(pa + (int64_t)s * a.row_pad * D);
+    const float f = factor[s];
+    acc.x += x.x * f;
+    acc.y += x.y * f;
+    acc.z += x.z * f;
+    acc.w += x.w * f;
+  }
+  acc_s[tid] = acc;
+  __syncthreads();
   int64_t at_out, at_lse;
   output_index(a, b, h, row, &at_out, &at_lse);
-  store_out<DT>(a.out, at_out + d, sum == 0.0f ? 0.0f : acc / sum);
-  if (d == 0) {
-    a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + __log2f(sum)) * LN2;
-    if (a.stats) a.stats[bh * a.row_pad + row] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
+  if (tid < D) {
+    float x = 0.0f;
+#pragma unroll
+    for (int g = 0; g < JOIN_THREADS / 32; ++g) x += reinterpret_cast<const float*>(acc_s)[g * D + tid];
+    store_out<DT>(a.out, at_out + tid, sum == 0.0f ? 0.0f : x / sum);
   }
+  if (tid == 0) {
+    a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + __log2f(sum)) * LN2;
+    if (a.stats)
+      a.stats[((int64_t)b * c.kv_heads + h) * a.row_pad + row] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
+  }
+}
+
+// Received weight from the scores that the split kernel left (at most 16 query
+// rows a head): a thread adds up four cache rows over the query rows.  Writing
+// and reading 4 bytes a row and query costs less than the keys again.
+__global__ __launch_bounds__(256) void weights_of_scores_kernel(const QuantAttendArgs a) {
+  const ckv_quant_cache& c = a.cache;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int n = quant_length(c, b);
+  const int64_t r = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (r >= n) return;
+  const int64_t bh = (int64_t)b * c.kv_heads + h;
+  const float* from = a.scores + bh * a.rows * c.capacity + r;
+  const float2* stats = a.stats + bh * a.row_pad;
+  float got[4] = {};
+  for (int row = 0; row < a.rows; ++row) {
+    const float4 s = *reinterpret_cast<const float4*>(from + (int64_t)row * c.capacity);
+    const float2 st = stats[row];
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) got[i] += v[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(v[i] - st.x) * st.y;
+  }
+  float* to = quant_head(c, b, h).weights + r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (r + i < n) to[i] += got[i];
 }
 
 // Received weight: a wave owns 32 cache rows of a (sequence, head), goes over
@@ -428,29 +496,27 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendAr
 template <int DT>
 int row_tiles(int rows) { return rows > 16 && DT == CKV_BF16 ? 2 : 1; }
 
-// Parts that the rows of a (sequence, head) are split into: enough workgroups
-// to fill the chip (1,024 of the few-row kernel's, four a compute unit; 256 of
-// the many-row kernel's, which has a compute unit to itself).
-int parts_of(const ckv_quant_cache* c, int64_t row_blocks, int64_t workgroups) {
-  const int64_t heads = (int64_t)c->batch * c->kv_heads * row_blocks;
-  const int64_t most = ((int64_t)c->capacity + PART_UNIT - 1) / PART_UNIT;
-  int64_t want = (workgroups + heads - 1) / heads;
-  if (want > 64) want = 64;
-  if (want > most) want = most;
-  return (int)(want < 1 ? 1 : want);
+// Parts that the cache rows of the batch are split into: enough workgroups to
+// fill the chip (`workgroups`), no more than there are units.
+int parts_for(const ckv_quant_cache* c, int64_t row_blocks, int64_t workgroups) {
+  const int64_t units = ((int64_t)c->capacity + PART_UNIT - 1) / PART_UNIT;
+  const int64_t want = workgroups / ((int64_t)c->kv_heads * row_blocks);
+  if (want <= c->batch) return c->batch;
+  return (int)(want < c->batch * units ? want : c->batch * units);
 }
 
-constexpr int64_t MAX_ROWS = 1 << 22;  // query rows of a head: the grids' second dimension holds their blocks
+constexpr int64_t MAX_ROWS = 1 << 21;  // query rows of a head: the grids' second dimension holds their blocks
 
 struct AttendLayout {
-  int splits, row_pad;
-  bool many;
-  size_t stats, ranges, sums, max, sum, acc, bytes;
+  int parts, row_pad;
+  bool many, keep_scores;
+  size_t stats, ranges, scores, sums, max, sum, acc, bytes;
   AttendLayout(const ckv_quant_cache* c, int rows, int dtype, bool accumulate) {
     row_pad = (rows + 15) / 16 * 16;
     many = rows > FEW_ROWS;
     const int64_t block = many ? many_row_block(dtype) : 16;
-    splits = parts_of(c, (rows + block - 1) / block, many ? 256 : 1024);
+    parts = parts_for(c, (rows + block - 1) / block, many ? 256 : FEW_WORKGROUPS);
+    keep_scores = accumulate && rows <= 16;
     const size_t heads = (size_t)c->batch * c->kv_heads;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -462,17 +528,18 @@ struct AttendLayout {
     ranges = take(many ? heads * ((c->capacity + RANGE_TILE - 1) / RANGE_TILE) * sizeof(int2) : 0);
     const int shares = many && accumulate ? many_row_shares(c, rows) : 1;
     sums = take(shares > 1 ? heads * c->capacity * shares * sizeof(float) : 0);
-    const size_t parts = splits > 1 ? heads * row_pad * splits * sizeof(float) : 0;
-    max = take(parts);
-    sum = take(parts);
-    acc = take(parts * D);
+    scores = take(keep_scores ? heads * rows * c->capacity * sizeof(float) : 0);
+    const size_t each = parts > c->batch ? (size_t)c->kv_heads * row_pad * parts * sizeof(float) : 0;
+    max = take(each);
+    sum = take(each);
+    acc = take(each * D);
     bytes = at;
   }
 };
 
 template <int DT, int NR>
 void launch_split(const QuantAttendArgs& a, hipStream_t s) {
-  const dim3 grid((a.rows + 16 * NR - 1) / (16 * NR), a.splits, a.cache.batch * a.cache.kv_heads);
+  const dim3 grid(a.parts * a.cache.kv_heads, (a.rows + 16 * NR - 1) / (16 * NR));
   attend_split_kernel<DT, NR><<<grid, 64 * WAVES, 0, s>>>(a);
 }
 
@@ -486,12 +553,17 @@ int launch_attend(const QuantAttendArgs& a, bool many, bool accumulate, hipStrea
     else launch_split<DT, 1>(a, s);
     rc = launched("ckv_quant_attention");
   }
-  if (!rc && a.splits > 1) {
-    attend_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), D, 0, s>>>(a);
+  if (!rc && a.parts > a.cache.batch) {
+    attend_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
     rc = launched("ckv_quant_attention");
   }
   if (!rc && accumulate) {
     if (many) return launch_many_rows_weights(a, DT, s);
+    if (a.scores) {
+      const dim3 grid((a.cache.capacity + 1023) / 1024, a.cache.kv_heads, a.cache.batch);
+      weights_of_scores_kernel<<<grid, 256, 0, s>>>(a);
+      return launched("ckv_quant_attention");
+    }
     const dim3 grid((a.cache.capacity + WAVES * STEP - 1) / (WAVES * STEP), a.cache.kv_heads, a.cache.batch);
     weights_kernel<DT><<<grid, 64 * WAVES, 0, s>>>(a);
     rc = launched("ckv_quant_attention");
@@ -526,7 +598,7 @@ extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant
   if (group > CKV_MAX_GROUP) return fail(CKV_E_LIMIT, "ckv_quant_attention: group size exceeds 16");
   if (tokens <= 0 || window < 0) return fail(CKV_E_INVALID, "ckv_quant_attention: tokens must be positive, window not negative");
   if ((int64_t)tokens * group > MAX_ROWS)
-    return fail(CKV_E_LIMIT, "ckv_quant_attention: more than 2^22 query rows a head");
+    return fail(CKV_E_LIMIT, "ckv_quant_attention: more than 2^21 query rows a head");
   if (!(softmax_scale > 0.0f) || softmax_scale > 1e30f)
     return fail(CKV_E_INVALID, "ckv_quant_attention: softmax_scale must be positive");
   const int unit = dtype == CKV_F32 ? 4 : 8;
@@ -551,6 +623,7 @@ extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant
   a.part_acc = reinterpret_cast<float*>(ws + lay.acc);
   a.stats = accumulate ? reinterpret_cast<float2*>(ws + lay.stats) : nullptr;
   a.ranges = lay.many ? reinterpret_cast<int2*>(ws + lay.ranges) : nullptr;
+  a.scores = lay.keep_scores ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
   a.sums = reinterpret_cast<float*>(ws + lay.sums);
   a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
   a.tokens = tokens;
@@ -559,7 +632,7 @@ extern "C" int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant
   a.rows = tokens * group;
   a.row_pad = lay.row_pad;
   a.window = window;
-  a.splits = lay.splits;
+  a.parts = lay.parts;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == CKV_BF16) return launch_attend<CKV_BF16>(a, lay.many, accumulate != 0, s);
   if (dtype == CKV_F16) return launch_attend<CKV_F16>(a, lay.many, accumulate != 0, s);

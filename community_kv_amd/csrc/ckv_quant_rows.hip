@@ -177,15 +177,17 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   extern __shared__ __align__(16) unsigned char lds_raw[];
   RowsLds& lds = *reinterpret_cast<RowsLds*>(lds_raw);
   const ckv_quant_cache& c = a.cache;
-  const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
+  // workgroups that follow one another go to different XCDs: one head's to one, where they share its L2
+  const int h = blockIdx.x, number = blockIdx.z;
   // the blocks of the newest rows see the most: they go first
   const int block0 = (int)(gridDim.y - 1 - blockIdx.y) * 32 * W;
-  const int split = blockIdx.z;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
+  const Part part = find_part(c, a.parts, number, -1);
+  const int b = part.sequence;
+  if (b < 0) return;
+  const int64_t bh = (int64_t)b * c.kv_heads + h;
   const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
-  const int per = part_rows(n, a.splits);
-  const int lo_row = (int)min((int64_t)split * per, (int64_t)n), hi_row = min(lo_row + per, n);
-  if (split > 0 && lo_row >= n) return;
+  const int lo_row = part.index * part.rows, hi_row = (int)min((int64_t)lo_row + part.rows, (int64_t)n);
   const QuantHead q = quant_head(c, b, h);
   const int block_log2 = 31 - __clz(c.block);
   const int row = block0 + 32 * wave + (lane & 31);
@@ -361,8 +363,8 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
     top = max3(top, cur[1][15], cur[1][15]);
     top = max_xor32(top);
     if (__ballot(top > m + grow_by) != 0) {
-      const float t = fmaxf(m, top);
-      const float f = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((m - t) * sl2);
+      const float t = top > m + grow_by ? top : m;  // a query's own scores alone decide
+      const float f = m == t ? 1.0f : __builtin_amdgcn_exp2f((m - t) * sl2);
       m = t;
       l *= f;
 #pragma unroll
@@ -439,8 +441,8 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   if (row >= a.rows) return;
   const float sum = hi < 0 ? 0.0f : add_xor32(l);
   const float top = m == NEG_INF ? 0.0f : m * sl2;
-  if (a.splits > 1) {
-    float* acc = a.part_acc + (((int64_t)bh * a.splits + split) * a.row_pad + row) * D;
+  if (a.parts > c.batch) {
+    float* acc = a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + row) * D;
 #pragma unroll
     for (int db = 0; db < 4; ++db) {
 #pragma unroll
@@ -450,8 +452,8 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
                    : float4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
     }
     if (half == 0) {
-      a.part_max[((int64_t)bh * a.row_pad + row) * a.splits + split] = m == NEG_INF || hi < 0 ? NEG_INF : top;
-      a.part_sum[((int64_t)bh * a.row_pad + row) * a.splits + split] = sum;
+      a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m == NEG_INF || hi < 0 ? NEG_INF : top;
+      a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
     }
     return;
   }
@@ -507,7 +509,7 @@ int launch_rows(const QuantAttendArgs& a, hipStream_t s) {
     }
     if (device >= 0 && device < 64) ready[device] = true;
   }
-  const dim3 grid(c.batch * c.kv_heads, (a.rows + 32 * W - 1) / (32 * W), a.splits);
+  const dim3 grid(c.kv_heads, (a.rows + 32 * W - 1) / (32 * W), a.parts);
   kernel<<<grid, 64 * W, sizeof(RowsLds), s>>>(a);
   return launched("ckv_quant_attention");
 }

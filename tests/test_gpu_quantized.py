@@ -220,6 +220,37 @@ def test_attend_long_prompt_rows(device, dtype):
     _attend_case(device, gen, cache, group=4, tokens=211, dtype=dtype, accumulate=True, window=64)
 
 
+def test_attend_many_sequences(device):
+    """More sequences than lanes of a wave, lengths from none to several parts, one KV head."""
+    gen = torch.Generator().manual_seed(15)
+    lengths = torch.randint(0, 700, (70,), generator=gen).tolist()
+    lengths[0], lengths[64], lengths[69] = 0, 0, 704
+    cache = _fill(device, gen, batch=70, heads=1, capacity=704, block=32, lengths=lengths)
+    _attend_case(device, gen, cache, group=2, tokens=1, dtype=torch.bfloat16, accumulate=True)
+    counts = [min(3, n) for n in lengths]
+    _attend_case(device, gen, cache, group=2, tokens=3, dtype=torch.float16, accumulate=True, counts=counts)
+
+
+@pytest.mark.parametrize("group,tokens,dtype", [(2, 3, torch.bfloat16), (4, 12, torch.bfloat16), (5, 40, torch.bfloat16),
+                                                (4, 20, torch.float32)])
+def test_attend_padded_queries_hold_anything(device, group, tokens, dtype):
+    """Queries past a sequence's count, NaN here, touch neither the others' outputs nor the received weights."""
+    gen = torch.Generator().manual_seed(16)
+    cache = _fill(device, gen, batch=2, heads=2, capacity=320, block=64, lengths=[300, 129])
+    query = _rows(gen, 2, 2 * group, tokens, dtype=dtype)
+    counts = [tokens - 1, tokens // 2]
+    weights = cache.weights.clone()
+    clean = quantized_attention(query.to(device), cache, softmax_scale=SCALE, counts=_i32(counts, device), accumulate=True)
+    clean += (cache.weights.clone(),)
+    cache.weights.copy_(weights)
+    for b in range(2):
+        query[b, :, counts[b]:] = float("nan")
+    got = quantized_attention(query.to(device), cache, softmax_scale=SCALE, counts=_i32(counts, device), accumulate=True)
+    torch.cuda.synchronize()
+    for a, b in zip(clean, got + (cache.weights,)):
+        assert torch.equal(a, b) and not b.isnan().any()
+
+
 def test_attend_window_leaves_rows_empty(device):
     """Rows whose window holds no cached position: zeros and -inf, no NaN, no weight."""
     gen = torch.Generator().manual_seed(9)
