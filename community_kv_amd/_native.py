@@ -53,6 +53,7 @@ MAX_SELECT_ROWS = 8192
 MAX_DESCRIPTORS = 4096
 MAX_SINKS = 256
 MAX_WINDOW = 1024
+QUANT_COUNTERS = 32
 
 EXPORTED_SYMBOLS = (
     "ckv_score_select",

@@ -73,9 +73,9 @@ class QuantizedKVCache:
                 raise ValueError(f"{name} must be contiguous")
             if tensor.device != codes.device:
                 raise ValueError("all tensors of a cache must share one device")
-        if codes.data_ptr() % 16 or self.value_codes.data_ptr() % 16:
-            raise ValueError("codes must be 16-byte aligned")
-        counters = torch.zeros(batch * (heads + 1), dtype=torch.int32, device=codes.device)
+        if any(t.data_ptr() % 16 for t in (codes, self.value_codes, self.positions, self.weights) if t is not None):
+            raise ValueError("codes, positions and weights must be 16-byte aligned")
+        counters = torch.zeros(batch * nat.QUANT_COUNTERS, dtype=torch.int32, device=codes.device)
         object.__setattr__(self, "_counters", counters)
         object.__setattr__(self, "_struct", nat.QuantCache(
             codes.data_ptr(), self.value_codes.data_ptr(), self.key_scales.data_ptr(), self.value_scales.data_ptr(),

@@ -1,12 +1,11 @@
 // Writing into the 8-bit KV cache, and eviction from it (gfx950).
 //
-// append_kernel: a workgroup of 256 threads owns one block of rows of one
-// sequence, head and tensor (key or value): 16 threads a row, 8 values each.
-// It reads its new rows once into registers, takes the block's largest
-// magnitude, settles the scale, and writes codes of 8 bytes a thread (a row of
-// 128 bytes by 16 neighbouring threads).  Earlier rows of the block are touched
-// only when the scale grows.  The last workgroup of a sequence moves its
-// cursors: every workgroup has read them by then.
+// append_kernel: a workgroup of 512 threads owns one block of rows of one
+// sequence and head, keys in its first half and values in its second: 16
+// threads a row, 8 values each.  It reads its new rows once into registers,
+// takes the block's largest magnitude, settles the scale, and writes codes of 8
+// bytes a thread (a row of 128 bytes by 16 neighbouring threads).  Earlier rows
+// of the block are touched only when the scale grows.
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
@@ -31,8 +30,8 @@ int validate_quant_cache(const ckv_quant_cache* c, const char* what) {
   if (c->capacity % c->block) return fail(CKV_E_INVALID, "capacity must be a multiple of block");
   if (c->capacity > (1 << 30)) return fail(CKV_E_LIMIT, "capacity above 2^30 rows");
   if (c->batch > 32767 || c->kv_heads > 32767) return fail(CKV_E_LIMIT, "batch or kv_heads above 32767");
-  if (((uintptr_t)c->key_codes | (uintptr_t)c->value_codes) & 15)
-    return fail(CKV_E_INVALID, "codes must be 16-byte aligned");
+  if (((uintptr_t)c->key_codes | (uintptr_t)c->value_codes | (uintptr_t)c->positions | (uintptr_t)c->weights) & 15)
+    return fail(CKV_E_INVALID, "codes, positions and weights must be 16-byte aligned");
   return CKV_OK;
 }
 
@@ -42,6 +41,7 @@ namespace {
 using namespace ckv;
 
 constexpr int THREADS = 256;
+constexpr int COUNTER_STRIDE = CKV_QUANT_COUNTERS;  // words between two sequences' counters: a cache line each
 
 int fail(int code, const char* message) { return ckv_internal::set_error(code, message); }
 
@@ -70,8 +70,8 @@ __device__ inline void load_new8(const void* base, int64_t index, float* out) {
 
 // Multiplies the codes of the block's rows [row0, row0 + rows) by `ratio`.
 __device__ inline void rescale_rows(uint8_t* codes, int64_t row0, int rows, float ratio) {
-  const int col = (threadIdx.x & 15) * 8;
-  for (int r = threadIdx.x >> 4; r < rows; r += THREADS / 16) {
+  const int tid = threadIdx.x & (THREADS - 1), col = (tid & 15) * 8;
+  for (int r = tid >> 4; r < rows; r += THREADS / 16) {
     uint2* p = reinterpret_cast<uint2*>(codes + (row0 + r) * D + col);
     const uint2 w = *p;
     float v[8];
@@ -90,24 +90,42 @@ struct AppendArgs {
   int32_t tokens;
 };
 
+// The cursors of a sequence move when every workgroup has read them.  With few
+// workgroups a sequence (`ticket`) the last to finish moves them; the tickets of
+// many would queue at one address (12 ns each: the 8,192 workgroups of a 32k
+// prompt took 107 us with tickets, 51 with advance_kernel behind them, where a
+// second launch costs a single token's append 1.9 us more than its 8 tickets).
+__device__ inline void advance(const ckv_quant_cache& c, int b, int start, int seen, int count) {
+  const int end = (int)min((int64_t)start + count, (int64_t)c.capacity);
+  c.cursors[b] = end;
+  c.cursors[c.batch + b] = seen + (end - start);
+  if ((int64_t)start + count > c.capacity) c.cursors[2 * c.batch + b] = 1;
+}
+
+__device__ inline int append_count(const AppendArgs& a, int b) {
+  return a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
+}
+
 template <int DT, int SWEEPS>
-__global__ __launch_bounds__(THREADS) void append_kernel(const AppendArgs a) {
+__global__ __launch_bounds__(2 * THREADS) void append_kernel(const AppendArgs a, const bool ticket) {
   constexpr int BLOCK = 16 * SWEEPS;
-  __shared__ float scratch[4];
+  __shared__ float scratch[2][4];
   const ckv_quant_cache& c = a.cache;
-  const int b = blockIdx.z >> 1, tensor = blockIdx.z & 1, h = blockIdx.y;
+  const int b = blockIdx.z, h = blockIdx.y, tensor = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int tid = threadIdx.x & (THREADS - 1);
   const int start = quant_length(c, b), seen = c.cursors[c.batch + b];
-  const int count = a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
+  const int count = append_count(a, b);
   const int end = (int)min((int64_t)start + count, (int64_t)c.capacity);
   const int64_t blk = start / BLOCK + (int64_t)blockIdx.x;
   const int64_t row0 = blk * BLOCK;
   const int lo = (int)max((int64_t)start, row0), hi = (int)min((int64_t)end, row0 + BLOCK);
-  if (lo < hi && row0 < c.capacity) {
+  if (lo < hi) {  // the same for the whole workgroup
     const QuantHead q = quant_head(c, b, h);
     const ckv_quant_rows in = tensor ? a.value : a.key;
     const int64_t base = (int64_t)b * in.batch_stride + (int64_t)h * in.head_stride;
-    const int tid = threadIdx.x, col = (tid & 15) * 8;
+    const int col = (tid & 15) * 8;
     float v[SWEEPS][8];
+    const float old = row0 < start ? q.scales(tensor)[blk] : 0.0f;
     float amax = 0.0f;
 #pragma unroll
     for (int s = 0; s < SWEEPS; ++s) {
@@ -122,8 +140,11 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendArgs a) {
         for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(v[s][i]));
       }
     }
-    amax = block_max256(amax, scratch);
-    const float old = row0 < start ? q.scales(tensor)[blk] : 0.0f;
+    wait_vm();  // the old scale has arrived before another wave may write the new one
+    amax = wave_max(amax);
+    if ((tid & 63) == 0) scratch[tensor][tid >> 6] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(scratch[tensor][0], scratch[tensor][1]), fmaxf(scratch[tensor][2], scratch[tensor][3]));
     const float scale = fmaxf(old, block_scale(amax));
     const float inv = inverse_scale(scale);
 #pragma unroll
@@ -144,56 +165,75 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendArgs a) {
         if (q.weights) q.weights[row] = 0.0f;
       }
     }
-    __syncthreads();  // every wave has read the old scale
     if (tid == 0 && scale != old) q.scales(tensor)[blk] = scale;
-  } else {
-    __syncthreads();
   }
-  // Two counters in a row, so that a long prompt's workgroups do not all meet
-  // at one address.
+  if (!ticket) return;
+  __syncthreads();  // every wave has read the cursors
   if (threadIdx.x == 0) {
-    uint32_t* head = c.counters + (int64_t)b * (c.kv_heads + 1) + h;
-    uint32_t* sequence = c.counters + (int64_t)b * (c.kv_heads + 1) + c.kv_heads;
-    if (atomicAdd(head, 1u) == 2 * gridDim.x - 1) {
-      st_agent_u32(head, 0u);
-      if (atomicAdd(sequence, 1u) == (uint32_t)c.kv_heads - 1) {
-        st_agent_u32(sequence, 0u);
-        c.cursors[b] = end;
-        c.cursors[c.batch + b] = seen + (end - start);
-        if ((int64_t)start + count > c.capacity) c.cursors[2 * c.batch + b] = 1;
-      }
+    uint32_t* counter = c.counters + (int64_t)b * COUNTER_STRIDE;
+    if (atomicAdd(counter, 1u) == gridDim.x * gridDim.y - 1) {
+      st_agent_u32(counter, 0u);
+      advance(c, b, start, seen, count);
     }
   }
+}
+
+__global__ __launch_bounds__(THREADS) void advance_kernel(const AppendArgs a) {
+  const ckv_quant_cache& c = a.cache;
+  const int b = blockIdx.x * THREADS + threadIdx.x;
+  if (b < c.batch) advance(c, b, quant_length(c, b), c.cursors[c.batch + b], append_count(a, b));
 }
 
 template <int DT>
 int launch_append(const AppendArgs& a, hipStream_t stream) {
   const int block = a.cache.block;
-  // a count of `tokens` rows from any start touches at most this many blocks
-  const int64_t blocks = min((int64_t)(a.tokens - 1) / block + 2, (int64_t)a.cache.capacity / block);
-  const dim3 grid((uint32_t)blocks, a.cache.kv_heads, 2 * a.cache.batch);
-  if (block == 16) append_kernel<DT, 1><<<grid, THREADS, 0, stream>>>(a);
-  else if (block == 32) append_kernel<DT, 2><<<grid, THREADS, 0, stream>>>(a);
-  else if (block == 64) append_kernel<DT, 4><<<grid, THREADS, 0, stream>>>(a);
-  else append_kernel<DT, 8><<<grid, THREADS, 0, stream>>>(a);
-  return launched("ckv_quant_append");
+  // tokens rows from any start touch at most this many blocks
+  const int64_t blocks = min((int64_t)(a.tokens + block - 2) / block + 1, (int64_t)a.cache.capacity / block);
+  const dim3 grid((uint32_t)blocks, a.cache.kv_heads, a.cache.batch);
+  const bool ticket = blocks * a.cache.kv_heads <= 64;
+  if (block == 16) append_kernel<DT, 1><<<grid, 2 * THREADS, 0, stream>>>(a, ticket);
+  else if (block == 32) append_kernel<DT, 2><<<grid, 2 * THREADS, 0, stream>>>(a, ticket);
+  else if (block == 64) append_kernel<DT, 4><<<grid, 2 * THREADS, 0, stream>>>(a, ticket);
+  else append_kernel<DT, 8><<<grid, 2 * THREADS, 0, stream>>>(a, ticket);
+  int rc = launched("ckv_quant_append");
+  if (!rc && !ticket) {
+    advance_kernel<<<(a.cache.batch + THREADS - 1) / THREADS, THREADS, 0, stream>>>(a);
+    rc = launched("ckv_quant_append");
+  }
+  return rc;
 }
 
 // ---------------------------------------------------------------------------
 // Eviction
 // ---------------------------------------------------------------------------
 
+// Rows of one workgroup of the selection by several workgroups.
+constexpr int CHUNK_THREADS = 256;
+constexpr int CHUNK_KEYS = 16;  // keys of a thread
+constexpr int CHUNK = CHUNK_THREADS * CHUNK_KEYS;
+// The keys' digits: 11, 11 and 10 bits.
+constexpr int DIGITS = 3;
+__host__ __device__ constexpr int digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
+__host__ __device__ constexpr int digit_bins(int d) { return d == 2 ? 1024 : 2048; }
+__host__ __device__ constexpr int digit_bin0(int d) { return 2048 * d; }
+constexpr int ALL_BINS = 2048 + 2048 + 1024;
+
 // Workspace of one (sequence, head), in 32-bit words: two saved scales of the
-// block that holds row `keep`, then the row count before, then the keys of
-// every row, the kept rows from `keep` on (ascending), and for every 32 rows
-// below `keep` the mask of freed rows and their number before.
+// block that holds row `keep`, the row count before, then what the digits found
+// so far (prefix and rows wanted of it, a pair a digit), the digits' histograms,
+// four counts a chunk, the keys of every row, the kept rows from `keep` on
+// (ascending), and for every 32 rows below `keep` the mask of freed rows and
+// their number before.
 struct EvictLayout {
-  int64_t keys, movers, holes, base, words;
+  int64_t found, hist, counts, keys, movers, holes, base, words;
   __host__ __device__ EvictLayout(int64_t capacity, int64_t keep) {
-    const int64_t groups = (keep + 31) / 32;
-    keys = 4;
+    const int64_t groups = (keep + 31) / 32, chunks = (capacity + CHUNK - 1) / CHUNK;
+    found = 4;
+    hist = found + 2 * DIGITS + 2;
+    counts = hist + ALL_BINS;
+    keys = counts + 4 * chunks;
     movers = keys + capacity;
-    holes = movers + keep;
+    holes = movers + ((keep + 3) & ~(int64_t)3);
     base = holes + groups;
     words = (base + groups + 3) & ~(int64_t)3;
   }
@@ -212,6 +252,9 @@ __device__ inline uint32_t evict_key(float w, bool is_protected) {
   if (w != w) return 0xfffffffeu;
   return ordered_f32(w + 0.0f);
 }
+
+// Capacities up to this are selected by one workgroup a (sequence, head).
+constexpr int SELECT_ALONE = 8192;
 
 constexpr int SEL_THREADS = 1024;
 constexpr int SEL_WAVES = SEL_THREADS / 64;
@@ -306,6 +349,271 @@ __global__ __launch_bounds__(SEL_THREADS) void evict_select_kernel(const EvictAr
   }
 }
 
+// The same by several workgroups a (sequence, head), for long sequences, in
+// launches that follow one another: keys and the histogram of their first digit;
+// the second digit's and the third's among the rows that match so far; counts of
+// kept and tied rows a chunk, below row `keep` and from it on; the lists, each
+// chunk behind those before it.
+struct ChunkPlace {
+  uint32_t* ws;
+  int n, seen;
+  int64_t first;  // row of this thread's first key
+};
+
+__device__ inline bool chunk_place(const EvictArgs& a, const EvictLayout& lay, ChunkPlace* p) {
+  const ckv_quant_cache& c = a.from;
+  const int b = blockIdx.z, h = blockIdx.y;
+  p->ws = a.workspace + ((int64_t)b * c.kv_heads + h) * lay.words;
+  p->n = quant_length(c, b);
+  p->seen = c.cursors[c.batch + b];
+  p->first = (int64_t)blockIdx.x * CHUNK + (int64_t)threadIdx.x * CHUNK_KEYS;
+  return p->n > a.keep && (int64_t)blockIdx.x * CHUNK < p->n;
+}
+
+__device__ inline void load_keys(const uint32_t* keys, uint32_t* k) {
+#pragma unroll
+  for (int i = 0; i < CHUNK_KEYS / 4; ++i) {
+    const uint4 w = gload16(keys + 4 * i);
+    k[4 * i] = w.x;
+    k[4 * i + 1] = w.y;
+    k[4 * i + 2] = w.z;
+    k[4 * i + 3] = w.w;
+  }
+}
+
+// Adds the bins of this thread's keys that match (`in`) to the histogram in LDS,
+// a whole wave at once where its lanes agree (equal weights are common).
+__device__ inline void count_bin(int* hist, bool in, uint32_t bin) {
+  const uint64_t lanes = __ballot(in);
+  if (lanes == 0) return;
+  const int leader = __ffsll((unsigned long long)lanes) - 1;
+  const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, leader);
+  if (__ballot(in && bin != first) == 0) {
+    if ((int)(threadIdx.x & 63) == leader) atomicAdd(&hist[first], __popcll(lanes));
+  } else if (in) {
+    atomicAdd(&hist[bin], 1);
+  }
+}
+
+// The bin of digit d where the rows counted from the highest bin reach `target`,
+// and how many are still wanted of that bin.  Every thread of the workgroup.
+__device__ inline void find_digit(const uint32_t* hist, int bins, int target, int* scratch, int* bin, int* left) {
+  const int each = bins / CHUNK_THREADS, top = bins - 1 - (int)threadIdx.x * each;
+  int mine[8], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    mine[i] = i < each ? (int)hist[top - i] : 0;
+    sum += mine[i];
+  }
+  int before = wave_inclusive_scan(sum);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = before;
+  __syncthreads();
+  before -= sum;
+  for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) before += scratch[w];
+  __syncthreads();
+  if (before < target && before + sum >= target) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (before < target && before + mine[i] >= target) {
+        scratch[0] = top - i;
+        scratch[1] = target - before;
+      }
+      before += mine[i];
+    }
+  }
+  __syncthreads();
+  *bin = scratch[0];
+  *left = scratch[1];
+}
+
+__global__ __launch_bounds__(256) void evict_clear_kernel(const EvictArgs a) {
+  const EvictLayout lay(a.from.capacity, a.keep);
+  uint32_t* hist = a.workspace + (int64_t)blockIdx.x * lay.words + lay.hist;
+  for (int i = threadIdx.x; i < ALL_BINS; i += 256) hist[i] = 0;
+}
+
+template <int DIGIT>
+__global__ __launch_bounds__(CHUNK_THREADS) void evict_digit_kernel(const EvictArgs a) {
+  constexpr int BINS = digit_bins(DIGIT), SHIFT = digit_shift(DIGIT);
+  __shared__ int hist[BINS];
+  __shared__ int scratch[4];
+  const EvictLayout lay(a.from.capacity, a.keep);
+  ChunkPlace at;
+  const bool work = chunk_place(a, lay, &at);
+  if (DIGIT == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
+    const ckv_quant_cache& c = a.from;
+    const QuantHead q = quant_head(c, blockIdx.z, blockIdx.y);
+    const int64_t blk = a.keep / c.block;
+    at.ws[0] = a.keep < c.capacity ? __float_as_uint(q.key_scales[blk]) : 0u;
+    at.ws[1] = a.keep < c.capacity ? __float_as_uint(q.value_scales[blk]) : 0u;
+    at.ws[2] = (uint32_t)at.n;
+  }
+  if (!work) return;
+  uint32_t prefix = 0;
+  if constexpr (DIGIT > 0) {
+    // the digit before, from its histogram
+    const uint32_t* found = at.ws + lay.found + 2 * (DIGIT - 1);
+    const uint32_t known = DIGIT > 1 ? found[-2] : 0u;
+    const int target = DIGIT > 1 ? (int)found[-1] : a.keep;
+    int bin, left;
+    find_digit(at.ws + lay.hist + digit_bin0(DIGIT - 1), digit_bins(DIGIT - 1), target, scratch, &bin, &left);
+    prefix = known | ((uint32_t)bin << digit_shift(DIGIT - 1));
+    if (blockIdx.x == 0 && threadIdx.x == 0) {  // for the launches to come
+      at.ws[lay.found + 2 * (DIGIT - 1)] = prefix;
+      at.ws[lay.found + 2 * (DIGIT - 1) + 1] = (uint32_t)left;
+    }
+  }
+  for (int i = threadIdx.x; i < BINS; i += CHUNK_THREADS) hist[i] = 0;
+  __syncthreads();
+  uint32_t k[CHUNK_KEYS];
+  uint32_t* keys = at.ws + lay.keys + at.first;
+  if constexpr (DIGIT == 0) {
+    const QuantHead q = quant_head(a.from, blockIdx.z, blockIdx.y);
+    const int64_t newest = (int64_t)at.seen - a.recent;
+#pragma unroll
+    for (int i = 0; i < CHUNK_KEYS / 4; ++i) {
+      const int64_t r = at.first + 4 * i;
+      if (r < at.n) {  // capacity is a multiple of 16: four rows at once stay inside
+        const float4 w = *reinterpret_cast<const float4*>(q.weights + r);
+        const int4 p = *reinterpret_cast<const int4*>(q.positions + r);
+        k[4 * i] = evict_key(w.x, p.x < a.num_sink || p.x >= newest);
+        k[4 * i + 1] = evict_key(w.y, p.y < a.num_sink || p.y >= newest);
+        k[4 * i + 2] = evict_key(w.z, p.z < a.num_sink || p.z >= newest);
+        k[4 * i + 3] = evict_key(w.w, p.w < a.num_sink || p.w >= newest);
+        *reinterpret_cast<uint4*>(keys + 4 * i) = uint4{k[4 * i], k[4 * i + 1], k[4 * i + 2], k[4 * i + 3]};
+      }
+    }
+  } else if (at.first < at.n) {
+    load_keys(keys, k);
+  }
+#pragma unroll
+  for (int i = 0; i < CHUNK_KEYS; ++i) {
+    const bool in = at.first + i < at.n && (DIGIT == 0 || (k[i] >> digit_shift(DIGIT - 1)) == (prefix >> digit_shift(DIGIT - 1)));
+    count_bin(hist, in, in ? (k[i] >> SHIFT) & (BINS - 1) : 0u);
+  }
+  __syncthreads();
+  uint32_t* all = at.ws + lay.hist + digit_bin0(DIGIT);
+  for (int i = threadIdx.x; i < BINS; i += CHUNK_THREADS) {
+    const int x = hist[i];
+    if (x) atomicAdd(&all[i], (uint32_t)x);
+  }
+}
+
+// The threshold key and how many of the rows that equal it are kept.
+__device__ inline void threshold(const EvictArgs& a, const EvictLayout& lay, const uint32_t* ws, int* scratch,
+                                 uint32_t* key, int* ties) {
+  const uint32_t* found = ws + lay.found + 2 * (DIGITS - 2);
+  int bin;
+  find_digit(ws + lay.hist + digit_bin0(DIGITS - 1), digit_bins(DIGITS - 1), (int)found[1], scratch, &bin, ties);
+  *key = found[0] | (uint32_t)bin;
+}
+
+__device__ inline int block_sum256(int x, int* scratch) {
+  const int s = wave_inclusive_scan(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = s;
+  __syncthreads();
+  return (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
+}
+
+__global__ __launch_bounds__(CHUNK_THREADS) void evict_count_kernel(const EvictArgs a) {
+  __shared__ int scratch[4];
+  const EvictLayout lay(a.from.capacity, a.keep);
+  ChunkPlace at;
+  if (!chunk_place(a, lay, &at)) return;
+  uint32_t key;
+  int ties;
+  threshold(a, lay, at.ws, scratch, &key, &ties);
+  uint32_t k[CHUNK_KEYS];
+  int above[2] = {0, 0}, equal[2] = {0, 0};  // below row `keep`, from it on
+  if (at.first < at.n) {
+    load_keys(at.ws + lay.keys + at.first, k);
+#pragma unroll
+    for (int i = 0; i < CHUNK_KEYS; ++i) {
+      const bool in = at.first + i < at.n, high = at.first + i >= a.keep;
+      above[0] += in && !high && k[i] > key;
+      above[1] += in && high && k[i] > key;
+      equal[0] += in && !high && k[i] == key;
+      equal[1] += in && high && k[i] == key;
+    }
+  }
+  const int low = block_sum256(above[0] | (equal[0] << 16), scratch);
+  const int high = block_sum256(above[1] | (equal[1] << 16), scratch);
+  if (threadIdx.x == 0) {
+    uint32_t* counts = at.ws + lay.counts + 4 * blockIdx.x;
+    counts[0] = (uint32_t)low & 0xffffu;
+    counts[1] = (uint32_t)low >> 16;
+    counts[2] = (uint32_t)high & 0xffffu;
+    counts[3] = (uint32_t)high >> 16;
+  }
+}
+
+__global__ __launch_bounds__(CHUNK_THREADS) void evict_list_kernel(const EvictArgs a) {
+  __shared__ int scratch[4];
+  const EvictLayout lay(a.from.capacity, a.keep);
+  ChunkPlace at;
+  if (!chunk_place(a, lay, &at)) return;
+  uint32_t key;
+  int ties;
+  threshold(a, lay, at.ws, scratch, &key, &ties);
+  auto scan = [&](int x) {
+    const int incl = wave_inclusive_scan(x);
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) scratch[wave] = incl;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < wave; ++w) before += scratch[w];
+    return before + incl - x;
+  };
+  // of the chunks before, one a thread: tied rows, kept rows from `keep` on, kept rows below it
+  int tied = 0, moved = 0, kept_low = 0;
+  for (int c0 = 0; c0 < (int)blockIdx.x; c0 += CHUNK_THREADS) {
+    const int c = c0 + (int)threadIdx.x;
+    uint4 n{0u, 0u, 0u, 0u};
+    if (c < (int)blockIdx.x) n = *reinterpret_cast<const uint4*>(at.ws + lay.counts + 4 * (int64_t)c);
+    const int earlier = tied + scan((int)(n.y + n.w));
+    const int take_low = min(max(ties - earlier, 0), (int)n.y);
+    const int take_high = min(max(ties - earlier - (int)n.y, 0), (int)n.w);
+    tied += block_sum256((int)(n.y + n.w), scratch);
+    moved += block_sum256((int)n.z + take_high, scratch);
+    kept_low += block_sum256((int)n.x + take_low, scratch);
+  }
+  const int64_t chunk0 = (int64_t)blockIdx.x * CHUNK;
+  int freed = (int)min(chunk0, (int64_t)a.keep) - kept_low;
+  uint32_t k[CHUNK_KEYS];
+#pragma unroll
+  for (int i = 0; i < CHUNK_KEYS; ++i) k[i] = 0;
+  if (at.first < at.n) load_keys(at.ws + lay.keys + at.first, k);
+  int equal = 0;
+#pragma unroll
+  for (int i = 0; i < CHUNK_KEYS; ++i) equal += at.first + i < at.n && k[i] == key;
+  int rank = tied + scan(equal);
+  uint32_t kept = 0;  // bit i: row first + i
+#pragma unroll
+  for (int i = 0; i < CHUNK_KEYS; ++i) {
+    const bool in = at.first + i < at.n, tie = in && k[i] == key;
+    if (in && (k[i] > key || (tie && rank < ties))) kept |= 1u << i;
+    rank += tie;
+  }
+  // rows of this thread below `keep` and in use, from `keep` on
+  const int low_rows = (int)min(max((int64_t)a.keep - at.first, (int64_t)0), (int64_t)CHUNK_KEYS);
+  const uint32_t low_mask = low_rows >= 32 ? 0xffffffffu : (1u << low_rows) - 1u;
+  const uint32_t holes = ~kept & low_mask, movers = kept & ~low_mask;
+  const int before = scan(__popc(holes) | (__popc(movers) << 16));
+  freed += before & 0xffff;
+  moved += before >> 16;
+  uint32_t* list = at.ws + lay.movers;
+  for (uint32_t m = movers; m; m &= m - 1) list[moved++] = (uint32_t)(at.first + __ffs((int)m) - 1);
+  // two threads' sixteen rows make a word of the mask
+  const uint32_t other = (uint32_t)__shfl_xor((int)holes, 1);
+  if ((threadIdx.x & 1) == 0 && at.first < a.keep) {
+    at.ws[lay.holes + (at.first >> 5)] = holes | (other << 16);
+    at.ws[lay.base + (at.first >> 5)] = (uint32_t)freed;
+  }
+}
+
 // A workgroup writes one block of rows of the result: rows that stay (copied
 // only when the result is another cache) and rows moved in from `keep` on.  No
 // row is both read as a source and written: sources are at or past `keep`.
@@ -380,6 +688,7 @@ __global__ __launch_bounds__(THREADS) void evict_move_kernel(const EvictArgs a, 
       for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(v[i] * scale_of[s]));
     }
   }
+  wait_vm();  // the old scale has arrived before another wave may write the new one
   amax = block_max256(amax, scratch);
   const float scale = any ? fmaxf(old, block_scale(amax)) : old;
   const float inv = inverse_scale(scale);
@@ -410,7 +719,6 @@ __global__ __launch_bounds__(THREADS) void evict_move_kernel(const EvictArgs a, 
       if (dst.weights) dst.weights[row] = src.weights[from[s]];
     }
   }
-  __syncthreads();  // every wave has read the old scale
   if (tid == 0 && (!in_place || scale != old)) dst.scales(tensor)[blk] = scale;
 }
 
@@ -475,7 +783,17 @@ extern "C" int ckv_quant_evict(const ckv_quant_cache* cache, const ckv_quant_cac
   }
   const EvictArgs a{*cache, into ? *into : *cache, reinterpret_cast<uint32_t*>(workspace), most, num_sink, recent};
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  evict_select_kernel<<<dim3(cache->kv_heads, cache->batch), SEL_THREADS, 0, s>>>(a);
+  if (cache->capacity <= SELECT_ALONE) {
+    evict_select_kernel<<<dim3(cache->kv_heads, cache->batch), SEL_THREADS, 0, s>>>(a);
+  } else {
+    const dim3 chunks((cache->capacity + CHUNK - 1) / CHUNK, cache->kv_heads, cache->batch);
+    evict_clear_kernel<<<cache->batch * cache->kv_heads, 256, 0, s>>>(a);
+    evict_digit_kernel<0><<<chunks, CHUNK_THREADS, 0, s>>>(a);
+    evict_digit_kernel<1><<<chunks, CHUNK_THREADS, 0, s>>>(a);
+    evict_digit_kernel<2><<<chunks, CHUNK_THREADS, 0, s>>>(a);
+    evict_count_kernel<<<chunks, CHUNK_THREADS, 0, s>>>(a);
+    evict_list_kernel<<<chunks, CHUNK_THREADS, 0, s>>>(a);
+  }
   rc = launched("ckv_quant_evict");
   if (rc) return rc;
   const dim3 grid((most + cache->block - 1) / cache->block, cache->kv_heads, 2 * cache->batch);

@@ -66,6 +66,7 @@ extern "C" {
 #define CKV_MAX_DESCRIPTORS 4096
 #define CKV_MAX_SINKS 256
 #define CKV_MAX_WINDOW 1024
+#define CKV_QUANT_COUNTERS 32       /* counter words of a sequence of an 8-bit cache */
 
 enum ckv_status {
   CKV_OK = 0,
@@ -581,7 +582,7 @@ typedef struct ckv_quant_cache {
   int32_t* positions;      /* [batch][kv_heads][capacity] */
   float* weights;          /* [batch][kv_heads][capacity] attention received, or null */
   int32_t* cursors;        /* [3][batch]: rows in use, tokens ever appended, overflow (1: tokens were dropped) */
-  uint32_t* counters;      /* [batch][kv_heads + 1], zero before first use; the kernels leave it zero */
+  uint32_t* counters;      /* [batch][CKV_QUANT_COUNTERS], zero before first use; the kernels leave it zero */
   int32_t capacity;        /* rows, a multiple of block */
   int32_t batch;
   int32_t kv_heads;

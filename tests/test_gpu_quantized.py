@@ -384,6 +384,24 @@ def test_evict_orders_special_weights(device):
         _same(cache, oracle, f"keep {keep}")
 
 
+@pytest.mark.parametrize("keep,num_sink,recent", [(5000, 10, 64), (1, 0, 0), (4096, 0, 4096), (12_287, 3, 5),
+                                                  (8193, 100, 0)])
+def test_evict_several_workgroups(device, keep, num_sink, recent):
+    """Sequences long enough for several workgroups: special weights, many ties, lengths at and around the chunks."""
+    gen = torch.Generator().manual_seed(keep)
+    lengths = [12_288, 4096, 9001, 4097]
+    cache = _fill(device, gen, batch=4, heads=2, capacity=12_288, block=64, lengths=lengths)
+    special = torch.tensor([0.0, -0.0, 1.0, 1.0, float("inf"), -float("inf"), float("nan"), -3.0, 1e-45, 7.25])
+    pick = torch.randint(0, 10, cache.weights.shape, generator=gen)
+    cache.weights.copy_(torch.where(torch.rand(cache.weights.shape, generator=gen) < 0.7, special[pick],
+                                    torch.rand(cache.weights.shape, generator=gen) ** 8))
+    oracle = oq.Cache.of(cache)
+    evict(cache, keep=keep, num_sink=num_sink, recent=recent)
+    torch.cuda.synchronize()
+    oracle.evict(keep=keep, num_sink=num_sink, recent=recent)
+    _same(cache, oracle)
+
+
 def test_evict_moves_between_scales(device):
     """Rows of very different size meet in one block; NaN codes move as they are."""
     gen = torch.Generator().manual_seed(21)
