@@ -356,7 +356,8 @@ def ptr(tensor: torch.Tensor | None) -> int | None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of ``device`` (0.1 us; 2 us through a Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def require_device(*tensors: torch.Tensor) -> torch.device:

@@ -47,6 +47,8 @@ class QuantizedKVCache:
     weights: torch.Tensor | None = None  # [batch, kv_heads, capacity] float32: attention received
     _counters: torch.Tensor = field(init=False, repr=False)
     _struct: nat.QuantCache = field(init=False, repr=False)
+    _ref: object = field(init=False, repr=False)  # the struct by reference, made once: a call costs microseconds
+    _sizes: dict = field(init=False, repr=False)  # workspace bytes by call shape
 
     def __post_init__(self) -> None:
         codes = self.key_codes
@@ -76,11 +78,12 @@ class QuantizedKVCache:
         if any(t.data_ptr() % 16 for t in (codes, self.value_codes, self.positions, self.weights) if t is not None):
             raise ValueError("codes, positions and weights must be 16-byte aligned")
         counters = torch.zeros(batch * nat.QUANT_COUNTERS, dtype=torch.int32, device=codes.device)
-        object.__setattr__(self, "_counters", counters)
-        object.__setattr__(self, "_struct", nat.QuantCache(
+        struct = nat.QuantCache(
             codes.data_ptr(), self.value_codes.data_ptr(), self.key_scales.data_ptr(), self.value_scales.data_ptr(),
             self.positions.data_ptr(), nat.ptr(self.weights), self.cursors.data_ptr(), counters.data_ptr(), capacity,
-            batch, heads, self.block))
+            batch, heads, self.block)
+        for name, value in (("_counters", counters), ("_struct", struct), ("_ref", ctypes.byref(struct)), ("_sizes", {})):
+            object.__setattr__(self, name, value)
 
     @classmethod
     def allocate(cls, *, batch: int = 1, kv_heads: int, capacity: int, block: int = 64, track_weights: bool = False,
@@ -166,19 +169,25 @@ class QuantizedKVCache:
 def _rows(tensor: torch.Tensor) -> tuple[nat.QuantRows, torch.Tensor]:
     """The C view of [batch, heads, tokens, 128] and the tensor it points to
     (a copy where the strides or the address do not suit 16-byte loads)."""
-    unit = 4 if tensor.dtype == torch.float32 else 8
-    strides = [0 if size == 1 else stride for size, stride in zip(tensor.shape[:3], tensor.stride())]
-    if tensor.stride(3) != 1 or tensor.data_ptr() % 16 or any(s % unit for s in strides):
-        tensor = tensor.contiguous()
-        if tensor.data_ptr() % 16:
-            tensor = tensor.clone()
-        strides = tensor.stride()[:3]
-    return nat.QuantRows(tensor.data_ptr(), *strides), tensor
+    unit = 4 if tensor.dtype is torch.float32 else 8
+    b, h, t, d = tensor.stride()
+    address = tensor.data_ptr()
+    if d != 1 or address % 16 or (b | h | t) % unit:
+        b, h, t = (0 if size == 1 else stride for size, stride in zip(tensor.shape, (b, h, t)))
+        if d != 1 or address % 16 or (b | h | t) % unit:
+            tensor = tensor.contiguous() if d != 1 or address % 16 == 0 else tensor.clone(
+                memory_format=torch.contiguous_format)
+            if tensor.data_ptr() % 16:
+                tensor = tensor.clone()
+            b, h, t, d = tensor.stride()
+            address = tensor.data_ptr()
+    return nat.QuantRows(address, b, h, t), tensor
 
 
 def _check_rows(cache: QuantizedKVCache, name: str, tensor: torch.Tensor) -> None:
-    if tensor.ndim != 4 or tensor.shape[0] != cache.batch or tensor.shape[-1] != HEAD_DIM:
-        raise ValueError(f"{name} must have shape [{cache.batch}, heads, tokens, {HEAD_DIM}], not {tuple(tensor.shape)}")
+    shape = tensor.shape
+    if len(shape) != 4 or shape[0] != cache._struct.batch or shape[3] != HEAD_DIM:
+        raise ValueError(f"{name} must have shape [{cache.batch}, heads, tokens, {HEAD_DIM}], not {tuple(shape)}")
     if tensor.dtype not in _DTYPES:
         raise TypeError(f"{name} must use bfloat16, float16 or float32, not {tensor.dtype}")
     if tensor.requires_grad and torch.is_grad_enabled():
@@ -195,11 +204,13 @@ def _check_counts(cache: QuantizedKVCache, counts: torch.Tensor | None) -> torch
 
 def _call(device: torch.device, function, *args) -> None:
     """Calls a C entry on the current stream of ``device``."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        nat.check(function(*args, nat.stream_handle(device)))
-        return
-    with torch.cuda.device(device):
-        nat.check(function(*args, nat.stream_handle(device)))
+    if device.index == torch.cuda.current_device():
+        rc = function(*args, nat.stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, nat.stream_handle(device))
+    if rc:
+        nat.check(rc)
 
 
 def quantized_append(cache: QuantizedKVCache, key: torch.Tensor, value: torch.Tensor, *,
@@ -212,7 +223,7 @@ def quantized_append(cache: QuantizedKVCache, key: torch.Tensor, value: torch.Te
     (``assert_no_overflow``).  A value that is not finite is stored as NaN."""
     _check_rows(cache, "key", key)
     _check_rows(cache, "value", value)
-    if key.shape[1] != cache.kv_heads or value.shape != key.shape:
+    if key.shape[1] != cache._struct.kv_heads or value.shape != key.shape:
         raise ValueError(f"key and value must both have {cache.kv_heads} heads and the same tokens")
     if value.dtype != key.dtype:
         raise TypeError("key and value must share a dtype")
@@ -223,7 +234,7 @@ def quantized_append(cache: QuantizedKVCache, key: torch.Tensor, value: torch.Te
         return
     key_rows, key = _rows(key)
     value_rows, value = _rows(value)
-    _call(device, nat.lib().ckv_quant_append, ctypes.byref(cache._struct), ctypes.byref(key_rows),
+    _call(device, nat.lib().ckv_quant_append, cache._ref, ctypes.byref(key_rows),
           ctypes.byref(value_rows), tokens, nat.ptr(counts), _DTYPES[key.dtype])
 
 
@@ -261,13 +272,15 @@ def quantized_attention(query: torch.Tensor, cache: QuantizedKVCache, *, softmax
     if tokens == 0:
         return out, lse
     lib = nat.lib()
-    struct = ctypes.byref(cache._struct)
-    size = lib.ckv_quant_attention_workspace_bytes(struct, heads, tokens, _DTYPES[query.dtype], accumulate)
+    dtype = _DTYPES[query.dtype]
+    call = (heads, tokens, dtype, accumulate)
+    size = cache._sizes.get(call)
+    if size is None:
+        size = cache._sizes[call] = lib.ckv_quant_attention_workspace_bytes(cache._ref, heads, tokens, dtype, accumulate)
     workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     rows, query = _rows(query)
-    _call(device, lib.ckv_quant_attention, struct, ctypes.byref(rows), heads, tokens, nat.ptr(counts),
-          _DTYPES[query.dtype], softmax_scale, min(window, 2**31 - 1), accumulate, out.data_ptr(), lse.data_ptr(),
-          nat.ptr(workspace))
+    _call(device, lib.ckv_quant_attention, cache._ref, ctypes.byref(rows), heads, tokens, nat.ptr(counts), dtype,
+          softmax_scale, min(window, 2**31 - 1), accumulate, out.data_ptr(), lse.data_ptr(), nat.ptr(workspace))
     return out, lse
 
 
@@ -301,11 +314,10 @@ def evict(cache: QuantizedKVCache, *, keep: int, num_sink: int = 0, recent: int 
     keep = min(keep, cache.capacity)
     num_sink, recent = min(num_sink, keep), min(recent, keep)
     lib = nat.lib()
-    struct = ctypes.byref(cache._struct)
-    size = lib.ckv_quant_evict_workspace_bytes(struct, keep)
+    size = lib.ckv_quant_evict_workspace_bytes(cache._ref, keep)
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    _call(device, lib.ckv_quant_evict, struct, None if into is None else ctypes.byref(into._struct), keep, num_sink,
-          recent, workspace.data_ptr())
+    _call(device, lib.ckv_quant_evict, cache._ref, None if into is None else into._ref, keep, num_sink, recent,
+          workspace.data_ptr())
 
 
 __all__ = ["QuantizedKVCache", "evict", "quantized_append", "quantized_attention"]

@@ -253,14 +253,14 @@ __device__ inline uint32_t evict_key(float w, bool is_protected) {
   return ordered_f32(w + 0.0f);
 }
 
-// Capacities up to this are selected by one workgroup a (sequence, head).
-constexpr int SELECT_ALONE = 8192;
+// One workgroup a (sequence, head) selects where its threads hold all keys, SEL_KEYS
+// each: 256 threads up to 2,048 rows (their barriers cost less), 1,024 up to 8,192.
+constexpr int SEL_KEYS = 8;
+constexpr int SELECT_FEW = 256, SELECT_MANY = 1024;
 
-constexpr int SEL_THREADS = 1024;
-constexpr int SEL_WAVES = SEL_THREADS / 64;
-
-// Exclusive scan of x over the workgroup, and its total.
-__device__ inline int scan1024(int x, int* total, int* scratch) {
+// Exclusive scan of x over a workgroup of T threads, and its total.
+template <int T>
+__device__ inline int block_scan(int x, int* total, int* scratch) {
   const int incl = wave_inclusive_scan(x);
   const int wave = threadIdx.x >> 6;
   __syncthreads();
@@ -268,7 +268,7 @@ __device__ inline int scan1024(int x, int* total, int* scratch) {
   __syncthreads();
   int before = 0, sum = 0;
 #pragma unroll
-  for (int w = 0; w < SEL_WAVES; ++w) {
+  for (int w = 0; w < T / 64; ++w) {
     const int v = scratch[w];
     if (w < wave) before += v;
     sum += v;
@@ -277,76 +277,159 @@ __device__ inline int scan1024(int x, int* total, int* scratch) {
   return before + incl - x;
 }
 
-// One workgroup a (sequence, head): the keys once, then the `keep`-th largest
-// by four passes over their bytes, then one pass in row order that takes ties
-// by the lower row and lists the freed rows below `keep` and the kept ones above.
-__global__ __launch_bounds__(SEL_THREADS) void evict_select_kernel(const EvictArgs a) {
-  __shared__ int hist[256];
-  __shared__ int scratch[SEL_WAVES];
-  __shared__ int found[2];
+// Adds this lane's bin (where `in`) to the histogram in LDS, a whole wave at once
+// where its lanes agree (equal weights are common).
+__device__ inline void count_bin(int* hist, bool in, uint32_t bin) {
+  const uint64_t lanes = __ballot(in);
+  if (lanes == 0) return;
+  const int leader = __ffsll((unsigned long long)lanes) - 1;
+  const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, leader);
+  if (__ballot(in && bin != first) == 0) {
+    if ((int)(threadIdx.x & 63) == leader) atomicAdd(&hist[first], __popcll(lanes));
+  } else if (in) {
+    atomicAdd(&hist[bin], 1);
+  }
+}
+
+// The bin where the rows counted from the highest bin reach `target`, and how
+// many are still wanted of that bin.  Every thread of the workgroup of T; scratch
+// holds T / 64 + 2 words.
+template <int T>
+__device__ inline void find_digit(const int* hist, int bins, int target, int* scratch, int* bin, int* left) {
+  constexpr int MOST = 2048 / T;
+  const int each = bins / T, top = bins - 1 - (int)threadIdx.x * each;
+  int mine[MOST], sum = 0;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    mine[i] = i < each ? hist[top - i] : 0;
+    sum += mine[i];
+  }
+  int total;
+  int before = block_scan<T>(sum, &total, scratch);
+  if (before < target && before + sum >= target) {
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      if (before < target && before + mine[i] >= target) {
+        scratch[T / 64] = top - i;
+        scratch[T / 64 + 1] = target - before;
+      }
+      before += mine[i];
+    }
+  }
+  __syncthreads();
+  *bin = scratch[T / 64];
+  *left = scratch[T / 64 + 1];
+}
+
+// Which of this thread's K rows from `first` on are kept: those above `key`, and
+// of those that equal it the first `ties` of all, `rank` of which come before.
+template <int K>
+__device__ inline uint32_t kept_rows(const uint32_t* k, int64_t first, int n, uint32_t key, int ties, int rank) {
+  uint32_t kept = 0;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const bool in = first + i < n, tie = in && k[i] == key;
+    if (in && (k[i] > key || (tie && rank < ties))) kept |= 1u << i;
+    rank += tie;
+  }
+  return kept;
+}
+
+__device__ inline uint32_t low_rows(int64_t first, int keep, int rows) {
+  return (1u << (int)min(max((int64_t)keep - first, (int64_t)0), (int64_t)rows)) - 1u;  // rows <= 16
+}
+
+// Writes this thread's lists: `kept` of K rows from `first` on, `before` packs the
+// freed rows below `keep` (low half) and the kept ones from it on before them in the
+// workgroup, freed0 and moved0 those before the workgroup.
+template <int K>
+__device__ inline void write_lists(uint32_t* ws, const EvictLayout& lay, int64_t first, int keep, uint32_t kept,
+                                   int before, int freed0, int moved0) {
+  const uint32_t low = low_rows(first, keep, K);
+  int moved = moved0 + (before >> 16);
+  for (uint32_t m = kept & ~low; m; m &= m - 1) ws[lay.movers + moved++] = (uint32_t)(first + __ffs((int)m) - 1);
+  // 32 / K threads' rows make a word of the mask
+  uint32_t holes = (~kept & low) << (first & 31);
+#pragma unroll
+  for (int o = 1; o < 32 / K; o <<= 1) holes |= (uint32_t)__shfl_xor((int)holes, o);
+  if ((first & 31) == 0 && first < keep) {
+    ws[lay.holes + (first >> 5)] = holes;
+    ws[lay.base + (first >> 5)] = (uint32_t)(freed0 + (before & 0xffff));
+  }
+}
+
+// Loads this thread's keys from the weights and positions, four rows at once (the
+// capacity is a multiple of 16).
+template <int K>
+__device__ inline void make_keys(const EvictArgs& a, const QuantHead& q, int64_t first, int n, int seen, uint32_t* k) {
+  const int64_t newest = (int64_t)seen - a.recent;
+#pragma unroll
+  for (int i = 0; i < K; i += 4) {
+    if (first + i < n) {
+      const float4 w = *reinterpret_cast<const float4*>(q.weights + first + i);
+      const int4 p = *reinterpret_cast<const int4*>(q.positions + first + i);
+      k[i] = evict_key(w.x, p.x < a.num_sink || p.x >= newest);
+      k[i + 1] = evict_key(w.y, p.y < a.num_sink || p.y >= newest);
+      k[i + 2] = evict_key(w.z, p.z < a.num_sink || p.z >= newest);
+      k[i + 3] = evict_key(w.w, p.w < a.num_sink || p.w >= newest);
+    } else {
+      k[i] = k[i + 1] = k[i + 2] = k[i + 3] = 0;
+    }
+  }
+}
+
+__device__ inline void write_header(const EvictArgs& a, const QuantHead& q, uint32_t* ws, int n) {
+  const int64_t blk = a.keep / a.from.block;
+  const bool inside = a.keep < a.from.capacity;
+  ws[0] = inside ? __float_as_uint(q.key_scales[blk]) : 0u;
+  ws[1] = inside ? __float_as_uint(q.value_scales[blk]) : 0u;
+  ws[2] = (uint32_t)n;
+}
+
+// One workgroup a (sequence, head), a thread's keys (eight rows in order) in
+// registers: the `keep`-th largest by its three digits from the highest, then two
+// scans in row order, for the ties (taken by the lower row) and for the lists of
+// freed rows below `keep` and kept ones from it on.
+template <int T>
+__global__ __launch_bounds__(T) void evict_select_kernel(const EvictArgs a) {
+  __shared__ int hist[2048];
+  __shared__ int scratch[T / 64 + 2];
   const ckv_quant_cache& c = a.from;
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int n = quant_length(c, b), seen = c.cursors[c.batch + b];
   const QuantHead q = quant_head(c, b, h);
   const EvictLayout lay(c.capacity, a.keep);
   uint32_t* ws = a.workspace + ((int64_t)b * c.kv_heads + h) * lay.words;
-  if (tid == 0) {
-    const int64_t blk = a.keep / c.block;
-    const bool inside = a.keep < c.capacity;
-    ws[0] = inside ? __float_as_uint(q.key_scales[blk]) : 0u;
-    ws[1] = inside ? __float_as_uint(q.value_scales[blk]) : 0u;
-    ws[2] = (uint32_t)n;
-  }
+  if (tid == 0) write_header(a, q, ws, n);
   if (n <= a.keep) return;
-  uint32_t* keys = ws + lay.keys;
-  const int64_t newest = (int64_t)seen - a.recent;
-  for (int i = tid; i < n; i += SEL_THREADS) {
-    const int p = q.positions[i];
-    keys[i] = evict_key(q.weights[i], p < a.num_sink || p >= newest);
-  }
-  __syncthreads();
-  uint32_t prefix = 0, mask = 0;
+  uint32_t k[SEL_KEYS];
+  const int first = tid * SEL_KEYS;
+  make_keys<SEL_KEYS>(a, q, first, n, seen, k);
+  uint32_t prefix = 0;
   int target = a.keep;  // how many of the rows that match the prefix are kept
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+#pragma unroll
+  for (int d = 0; d < DIGITS; ++d) {
+    const int bins = digit_bins(d), shift = digit_shift(d);
+    for (int i = tid; i < bins; i += T) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += SEL_THREADS) {
-      const uint32_t k = keys[i];
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+#pragma unroll
+    for (int i = 0; i < SEL_KEYS; ++i) {
+      const bool in = first + i < n && (d == 0 || (k[i] >> digit_shift(d - 1)) == (prefix >> digit_shift(d - 1)));
+      count_bin(hist, in, (k[i] >> shift) & (bins - 1));
     }
     __syncthreads();
-    if (tid < 64) find_threshold_bin(hist, target, &found[0], &found[1]);
-    __syncthreads();
-    prefix |= (uint32_t)found[0] << shift;
-    mask |= 255u << shift;
-    target -= found[1];
-    __syncthreads();
+    int bin;
+    find_digit<T>(hist, bins, target, scratch, &bin, &target);
+    prefix |= (uint32_t)bin << shift;
   }
-  // in row order: `ties` of the rows at the threshold so far, `above` kept rows from keep on, `freed` rows below it
-  uint32_t* movers = ws + lay.movers;
-  uint32_t* holes = ws + lay.holes;
-  uint32_t* base = ws + lay.base;
-  int ties = 0, above = 0, freed = 0;
-  for (int64_t i0 = 0; i0 < n; i0 += SEL_THREADS) {
-    const int64_t i = i0 + tid;
-    const uint32_t k = i < n ? keys[i] : 0u;
-    const bool tie = i < n && k == prefix;
-    int total;
-    const int rank = scan1024(tie, &total, scratch);
-    const bool kept = i < n && (k > prefix || (tie && ties + rank < target));
-    ties += total;
-    const bool hole = i < a.keep && !kept;
-    const bool mover = i >= a.keep && kept;
-    const int at = scan1024((mover ? 1 << 16 : 0) | (hole ? 1 : 0), &total, scratch);
-    if (mover) movers[above + (at >> 16)] = (uint32_t)i;
-    const uint64_t ballot = __ballot(hole);
-    if ((tid & 31) == 0 && i < a.keep) {
-      holes[i >> 5] = (uint32_t)(ballot >> (tid & 32));
-      base[i >> 5] = (uint32_t)(freed + (at & 0xffff));
-    }
-    above += total >> 16;
-    freed += total & 0xffff;
-  }
+  int equal = 0, total;
+#pragma unroll
+  for (int i = 0; i < SEL_KEYS; ++i) equal += first + i < n && k[i] == prefix;
+  const int rank = block_scan<T>(equal, &total, scratch);
+  const uint32_t kept = kept_rows<SEL_KEYS>(k, first, n, prefix, target, rank);
+  const uint32_t low = low_rows(first, a.keep, SEL_KEYS);
+  const int before = block_scan<T>(__popc(~kept & low) | (__popc(kept & ~low) << 16), &total, scratch);
+  write_lists<SEL_KEYS>(ws, lay, first, a.keep, kept, before, 0, 0);
 }
 
 // The same by several workgroups a (sequence, head), for long sequences, in
@@ -381,52 +464,6 @@ __device__ inline void load_keys(const uint32_t* keys, uint32_t* k) {
   }
 }
 
-// Adds the bins of this thread's keys that match (`in`) to the histogram in LDS,
-// a whole wave at once where its lanes agree (equal weights are common).
-__device__ inline void count_bin(int* hist, bool in, uint32_t bin) {
-  const uint64_t lanes = __ballot(in);
-  if (lanes == 0) return;
-  const int leader = __ffsll((unsigned long long)lanes) - 1;
-  const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, leader);
-  if (__ballot(in && bin != first) == 0) {
-    if ((int)(threadIdx.x & 63) == leader) atomicAdd(&hist[first], __popcll(lanes));
-  } else if (in) {
-    atomicAdd(&hist[bin], 1);
-  }
-}
-
-// The bin of digit d where the rows counted from the highest bin reach `target`,
-// and how many are still wanted of that bin.  Every thread of the workgroup.
-__device__ inline void find_digit(const uint32_t* hist, int bins, int target, int* scratch, int* bin, int* left) {
-  const int each = bins / CHUNK_THREADS, top = bins - 1 - (int)threadIdx.x * each;
-  int mine[8], sum = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    mine[i] = i < each ? (int)hist[top - i] : 0;
-    sum += mine[i];
-  }
-  int before = wave_inclusive_scan(sum);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = before;
-  __syncthreads();
-  before -= sum;
-  for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) before += scratch[w];
-  __syncthreads();
-  if (before < target && before + sum >= target) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (before < target && before + mine[i] >= target) {
-        scratch[0] = top - i;
-        scratch[1] = target - before;
-      }
-      before += mine[i];
-    }
-  }
-  __syncthreads();
-  *bin = scratch[0];
-  *left = scratch[1];
-}
-
 __global__ __launch_bounds__(256) void evict_clear_kernel(const EvictArgs a) {
   const EvictLayout lay(a.from.capacity, a.keep);
   uint32_t* hist = a.workspace + (int64_t)blockIdx.x * lay.words + lay.hist;
@@ -437,18 +474,12 @@ template <int DIGIT>
 __global__ __launch_bounds__(CHUNK_THREADS) void evict_digit_kernel(const EvictArgs a) {
   constexpr int BINS = digit_bins(DIGIT), SHIFT = digit_shift(DIGIT);
   __shared__ int hist[BINS];
-  __shared__ int scratch[4];
+  __shared__ int scratch[CHUNK_THREADS / 64 + 2];
   const EvictLayout lay(a.from.capacity, a.keep);
   ChunkPlace at;
   const bool work = chunk_place(a, lay, &at);
-  if (DIGIT == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
-    const ckv_quant_cache& c = a.from;
-    const QuantHead q = quant_head(c, blockIdx.z, blockIdx.y);
-    const int64_t blk = a.keep / c.block;
-    at.ws[0] = a.keep < c.capacity ? __float_as_uint(q.key_scales[blk]) : 0u;
-    at.ws[1] = a.keep < c.capacity ? __float_as_uint(q.value_scales[blk]) : 0u;
-    at.ws[2] = (uint32_t)at.n;
-  }
+  const QuantHead q = quant_head(a.from, blockIdx.z, blockIdx.y);
+  if (DIGIT == 0 && blockIdx.x == 0 && threadIdx.x == 0) write_header(a, q, at.ws, at.n);
   if (!work) return;
   uint32_t prefix = 0;
   if constexpr (DIGIT > 0) {
@@ -457,7 +488,8 @@ __global__ __launch_bounds__(CHUNK_THREADS) void evict_digit_kernel(const EvictA
     const uint32_t known = DIGIT > 1 ? found[-2] : 0u;
     const int target = DIGIT > 1 ? (int)found[-1] : a.keep;
     int bin, left;
-    find_digit(at.ws + lay.hist + digit_bin0(DIGIT - 1), digit_bins(DIGIT - 1), target, scratch, &bin, &left);
+    find_digit<CHUNK_THREADS>(reinterpret_cast<const int*>(at.ws) + lay.hist + digit_bin0(DIGIT - 1),
+                              digit_bins(DIGIT - 1), target, scratch, &bin, &left);
     prefix = known | ((uint32_t)bin << digit_shift(DIGIT - 1));
     if (blockIdx.x == 0 && threadIdx.x == 0) {  // for the launches to come
       at.ws[lay.found + 2 * (DIGIT - 1)] = prefix;
@@ -469,20 +501,10 @@ __global__ __launch_bounds__(CHUNK_THREADS) void evict_digit_kernel(const EvictA
   uint32_t k[CHUNK_KEYS];
   uint32_t* keys = at.ws + lay.keys + at.first;
   if constexpr (DIGIT == 0) {
-    const QuantHead q = quant_head(a.from, blockIdx.z, blockIdx.y);
-    const int64_t newest = (int64_t)at.seen - a.recent;
+    make_keys<CHUNK_KEYS>(a, q, at.first, at.n, at.seen, k);
 #pragma unroll
-    for (int i = 0; i < CHUNK_KEYS / 4; ++i) {
-      const int64_t r = at.first + 4 * i;
-      if (r < at.n) {  // capacity is a multiple of 16: four rows at once stay inside
-        const float4 w = *reinterpret_cast<const float4*>(q.weights + r);
-        const int4 p = *reinterpret_cast<const int4*>(q.positions + r);
-        k[4 * i] = evict_key(w.x, p.x < a.num_sink || p.x >= newest);
-        k[4 * i + 1] = evict_key(w.y, p.y < a.num_sink || p.y >= newest);
-        k[4 * i + 2] = evict_key(w.z, p.z < a.num_sink || p.z >= newest);
-        k[4 * i + 3] = evict_key(w.w, p.w < a.num_sink || p.w >= newest);
-        *reinterpret_cast<uint4*>(keys + 4 * i) = uint4{k[4 * i], k[4 * i + 1], k[4 * i + 2], k[4 * i + 3]};
-      }
+    for (int i = 0; i < CHUNK_KEYS; i += 4) {
+      if (at.first + i < at.n) *reinterpret_cast<uint4*>(keys + i) = uint4{k[i], k[i + 1], k[i + 2], k[i + 3]};
     }
   } else if (at.first < at.n) {
     load_keys(keys, k);
@@ -505,20 +527,13 @@ __device__ inline void threshold(const EvictArgs& a, const EvictLayout& lay, con
                                  uint32_t* key, int* ties) {
   const uint32_t* found = ws + lay.found + 2 * (DIGITS - 2);
   int bin;
-  find_digit(ws + lay.hist + digit_bin0(DIGITS - 1), digit_bins(DIGITS - 1), (int)found[1], scratch, &bin, ties);
+  find_digit<CHUNK_THREADS>(reinterpret_cast<const int*>(ws) + lay.hist + digit_bin0(DIGITS - 1),
+                            digit_bins(DIGITS - 1), (int)found[1], scratch, &bin, ties);
   *key = found[0] | (uint32_t)bin;
 }
 
-__device__ inline int block_sum256(int x, int* scratch) {
-  const int s = wave_inclusive_scan(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = s;
-  __syncthreads();
-  return (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
-}
-
 __global__ __launch_bounds__(CHUNK_THREADS) void evict_count_kernel(const EvictArgs a) {
-  __shared__ int scratch[4];
+  __shared__ int scratch[CHUNK_THREADS / 64 + 2];
   const EvictLayout lay(a.from.capacity, a.keep);
   ChunkPlace at;
   if (!chunk_place(a, lay, &at)) return;
@@ -538,8 +553,9 @@ __global__ __launch_bounds__(CHUNK_THREADS) void evict_count_kernel(const EvictA
       equal[1] += in && high && k[i] == key;
     }
   }
-  const int low = block_sum256(above[0] | (equal[0] << 16), scratch);
-  const int high = block_sum256(above[1] | (equal[1] << 16), scratch);
+  int low, high;
+  block_scan<CHUNK_THREADS>(above[0] | (equal[0] << 16), &low, scratch);
+  block_scan<CHUNK_THREADS>(above[1] | (equal[1] << 16), &high, scratch);
   if (threadIdx.x == 0) {
     uint32_t* counts = at.ws + lay.counts + 4 * blockIdx.x;
     counts[0] = (uint32_t)low & 0xffffu;
@@ -550,71 +566,48 @@ __global__ __launch_bounds__(CHUNK_THREADS) void evict_count_kernel(const EvictA
 }
 
 __global__ __launch_bounds__(CHUNK_THREADS) void evict_list_kernel(const EvictArgs a) {
-  __shared__ int scratch[4];
+  __shared__ int scratch[CHUNK_THREADS / 64 + 2];
   const EvictLayout lay(a.from.capacity, a.keep);
   ChunkPlace at;
   if (!chunk_place(a, lay, &at)) return;
   uint32_t key;
   int ties;
   threshold(a, lay, at.ws, scratch, &key, &ties);
-  auto scan = [&](int x) {
-    const int incl = wave_inclusive_scan(x);
-    const int wave = threadIdx.x >> 6;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63) scratch[wave] = incl;
-    __syncthreads();
-    int before = 0;
-    for (int w = 0; w < wave; ++w) before += scratch[w];
-    return before + incl - x;
-  };
   // of the chunks before, one a thread: tied rows, kept rows from `keep` on, kept rows below it
   int tied = 0, moved = 0, kept_low = 0;
   for (int c0 = 0; c0 < (int)blockIdx.x; c0 += CHUNK_THREADS) {
     const int c = c0 + (int)threadIdx.x;
     uint4 n{0u, 0u, 0u, 0u};
     if (c < (int)blockIdx.x) n = *reinterpret_cast<const uint4*>(at.ws + lay.counts + 4 * (int64_t)c);
-    const int earlier = tied + scan((int)(n.y + n.w));
+    int sum_tied, sum_moved, sum_kept;
+    const int earlier = tied + block_scan<CHUNK_THREADS>((int)(n.y + n.w), &sum_tied, scratch);
     const int take_low = min(max(ties - earlier, 0), (int)n.y);
     const int take_high = min(max(ties - earlier - (int)n.y, 0), (int)n.w);
-    tied += block_sum256((int)(n.y + n.w), scratch);
-    moved += block_sum256((int)n.z + take_high, scratch);
-    kept_low += block_sum256((int)n.x + take_low, scratch);
+    block_scan<CHUNK_THREADS>((int)n.z + take_high, &sum_moved, scratch);
+    block_scan<CHUNK_THREADS>((int)n.x + take_low, &sum_kept, scratch);
+    tied += sum_tied;
+    moved += sum_moved;
+    kept_low += sum_kept;
   }
   const int64_t chunk0 = (int64_t)blockIdx.x * CHUNK;
-  int freed = (int)min(chunk0, (int64_t)a.keep) - kept_low;
+  const int freed = (int)min(chunk0, (int64_t)a.keep) - kept_low;
   uint32_t k[CHUNK_KEYS];
 #pragma unroll
   for (int i = 0; i < CHUNK_KEYS; ++i) k[i] = 0;
   if (at.first < at.n) load_keys(at.ws + lay.keys + at.first, k);
-  int equal = 0;
+  int equal = 0, total;
 #pragma unroll
   for (int i = 0; i < CHUNK_KEYS; ++i) equal += at.first + i < at.n && k[i] == key;
-  int rank = tied + scan(equal);
-  uint32_t kept = 0;  // bit i: row first + i
-#pragma unroll
-  for (int i = 0; i < CHUNK_KEYS; ++i) {
-    const bool in = at.first + i < at.n, tie = in && k[i] == key;
-    if (in && (k[i] > key || (tie && rank < ties))) kept |= 1u << i;
-    rank += tie;
-  }
-  // rows of this thread below `keep` and in use, from `keep` on
-  const int low_rows = (int)min(max((int64_t)a.keep - at.first, (int64_t)0), (int64_t)CHUNK_KEYS);
-  const uint32_t low_mask = low_rows >= 32 ? 0xffffffffu : (1u << low_rows) - 1u;
-  const uint32_t holes = ~kept & low_mask, movers = kept & ~low_mask;
-  const int before = scan(__popc(holes) | (__popc(movers) << 16));
-  freed += before & 0xffff;
-  moved += before >> 16;
-  uint32_t* list = at.ws + lay.movers;
-  for (uint32_t m = movers; m; m &= m - 1) list[moved++] = (uint32_t)(at.first + __ffs((int)m) - 1);
-  // two threads' sixteen rows make a word of the mask
-  const uint32_t other = (uint32_t)__shfl_xor((int)holes, 1);
-  if ((threadIdx.x & 1) == 0 && at.first < a.keep) {
-    at.ws[lay.holes + (at.first >> 5)] = holes | (other << 16);
-    at.ws[lay.base + (at.first >> 5)] = (uint32_t)freed;
-  }
+  const int rank = tied + block_scan<CHUNK_THREADS>(equal, &total, scratch);
+  const uint32_t kept = kept_rows<CHUNK_KEYS>(k, at.first, at.n, key, ties, rank);
+  const uint32_t low = low_rows(at.first, a.keep, CHUNK_KEYS);
+  const int before =
+      block_scan<CHUNK_THREADS>(__popc(~kept & low) | (__popc(kept & ~low) << 16), &total, scratch);
+  write_lists<CHUNK_KEYS>(at.ws, lay, at.first, a.keep, kept, before, freed, moved);
 }
 
-// A workgroup writes one block of rows of the result: rows that stay (copied
+// A workgroup of 256 threads writes one block of rows of the result, keys in its
+// first half and values in its second, 16 codes a thread: rows that stay (copied
 // only when the result is another cache) and rows moved in from `keep` on.  No
 // row is both read as a source and written: sources are at or past `keep`.
 template <int SWEEPS>
@@ -622,12 +615,13 @@ __global__ __launch_bounds__(THREADS) void evict_move_kernel(const EvictArgs a, 
   constexpr int BLOCK = 16 * SWEEPS;
   __shared__ float scratch[4];
   const ckv_quant_cache& c = a.from;
-  const int b = blockIdx.z >> 1, tensor = blockIdx.z & 1, h = blockIdx.y, tid = threadIdx.x;
+  const int b = blockIdx.z, h = blockIdx.y, tensor = __builtin_amdgcn_readfirstlane(threadIdx.x >> 7);
+  const int tid = threadIdx.x & 127;
   const EvictLayout lay(c.capacity, a.keep);
   const uint32_t* ws = a.workspace + ((int64_t)b * c.kv_heads + h) * lay.words;
   const int n = (int)ws[2];
   const int left = min(n, a.keep);
-  if (blockIdx.x == 0 && h == 0 && tensor == 0 && tid == 0) {
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) {
     // the selection read the cursors; nothing of this launch does, but from a cache that stays as it is
     if (!in_place) {
       a.to.cursors[a.to.batch + b] = c.cursors[c.batch + b];
@@ -638,82 +632,93 @@ __global__ __launch_bounds__(THREADS) void evict_move_kernel(const EvictArgs a, 
   const bool moves = n > a.keep;
   const int row0 = blockIdx.x * BLOCK;
   if (row0 >= left || (in_place && !moves)) return;
+  // freed rows of this block and their number before, a word for 32 rows (a block of 16 takes half of one)
+  constexpr int WORDS = (BLOCK + 31) / 32;
+  uint32_t mask[WORDS], base[WORDS];
+  uint32_t any = 0;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int word = (row0 >> 5) + w;
+    const bool in = moves && 32 * word < left;
+    mask[w] = in ? ws[lay.holes + word] : 0u;
+    base[w] = in ? ws[lay.base + word] : 0u;
+    any |= BLOCK < 32 ? (mask[w] >> (row0 & 31)) & 0xffffu : mask[w];
+  }
+  if (in_place && !any) return;
   const QuantHead src = quant_head(c, b, h), dst = quant_head(a.to, b, h);
-  const int col = (tid & 15) * 8;
   const uint32_t* movers = ws + lay.movers;
+  const int col = (tid & 7) * 16;
   // the row that each of this thread's rows takes its content from (-1: none)
   int from[SWEEPS];
   bool hole[SWEEPS];
-  bool any = false;
 #pragma unroll
   for (int s = 0; s < SWEEPS; ++s) {
-    const int row = row0 + 16 * s + (tid >> 4);
-    from[s] = row < left ? row : -1;
-    hole[s] = false;
-    if (moves && row < left) {
-      const uint32_t m = ws[lay.holes + (row >> 5)];
-      if ((m >> (row & 31)) & 1u) {
-        hole[s] = true;
-        any = true;
-        from[s] = (int)movers[ws[lay.base + (row >> 5)] + __popc(m & ((1u << (row & 31)) - 1u))];
-      }
-    }
+    const int row = row0 + 16 * s + (tid >> 3);
+    const uint32_t m = mask[s >> 1];
+    hole[s] = row < left && ((m >> (row & 31)) & 1u);
+    from[s] = row >= left ? -1 : hole[s] ? (int)movers[base[s >> 1] + __popc(m & ((1u << (row & 31)) - 1u))] : row;
   }
-  any = __syncthreads_or(any);
-  if (in_place && !any) return;
-  uint2 w[SWEEPS];
+  uint4 w[SWEEPS];
   float scale_of[SWEEPS];
-  const int straddle = a.keep / BLOCK;
+  const int straddle = a.keep / BLOCK, blk = row0 / BLOCK;
+  // in place, the block around row `keep` is a source and a target: its scale was saved
+  auto scale_at = [&](int block) {
+    return in_place && block == straddle ? __uint_as_float(ws[tensor]) : gload_f32(src.scales(tensor) + block);
+  };
 #pragma unroll
   for (int s = 0; s < SWEEPS; ++s) {
-    w[s] = uint2{0u, 0u};
+    w[s] = uint4{0u, 0u, 0u, 0u};
     scale_of[s] = 1.0f;
     if (from[s] >= 0 && (hole[s] || !in_place)) {
-      w[s] = *reinterpret_cast<const uint2*>(src.codes(tensor) + (int64_t)from[s] * D + col);
-      // in place, the block around row `keep` is a target too: its scale was saved
-      scale_of[s] = in_place && from[s] / BLOCK == straddle ? __uint_as_float(ws[tensor])
-                                                           : src.scales(tensor)[from[s] / BLOCK];
+      w[s] = gload16(src.codes(tensor) + (int64_t)from[s] * D + col);
+      scale_of[s] = scale_at(from[s] / BLOCK);
     }
   }
-  const int blk = row0 / BLOCK;
-  const float old = in_place && blk == straddle ? __uint_as_float(ws[tensor]) : src.scales(tensor)[blk];
+  const float old = scale_at(blk);
   float amax = 0.0f;
 #pragma unroll
   for (int s = 0; s < SWEEPS; ++s) {
     if (hole[s]) {
-      float v[8];
+      float v[16];
       decode4(w[s].x, v);
       decode4(w[s].y, v + 4);
+      decode4(w[s].z, v + 8);
+      decode4(w[s].w, v + 12);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(v[i] * scale_of[s]));
+      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, finite_abs(v[i] * scale_of[s]));
     }
   }
   wait_vm();  // the old scale has arrived before another wave may write the new one
-  amax = block_max256(amax, scratch);
+  amax = wave_max(amax);
+  if ((tid & 63) == 0) scratch[threadIdx.x >> 6] = amax;
+  __syncthreads();
+  amax = fmaxf(scratch[2 * tensor], scratch[2 * tensor + 1]);
   const float scale = any ? fmaxf(old, block_scale(amax)) : old;
-  const float inv = inverse_scale(scale);
-  const float ratio = old * inv;
+  const float inv = inverse_scale(scale), ratio = old * inv;
 #pragma unroll
   for (int s = 0; s < SWEEPS; ++s) {
-    const int row = row0 + 16 * s + (tid >> 4);
+    const int row = row0 + 16 * s + (tid >> 3);
     if (from[s] < 0) continue;
-    uint2* p = reinterpret_cast<uint2*>(dst.codes(tensor) + (int64_t)row * D + col);
-    if (!hole[s] && scale == old) {
-      if (!in_place) *p = w[s];
+    uint4* p = reinterpret_cast<uint4*>(dst.codes(tensor) + (int64_t)row * D + col);
+    const float factor = hole[s] ? scale_of[s] * inv : ratio;
+    if (factor == 1.0f) {  // the codes as they are
+      if (hole[s] || !in_place) *p = w[s];
       continue;
     }
     if (!hole[s] && in_place) w[s] = *p;
-    float v[8];
-    decode4(w[s].x, v);
-    decode4(w[s].y, v + 4);
+    uint32_t x[4] = {w[s].x, w[s].y, w[s].z, w[s].w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= hole[s] ? scale_of[s] * inv : ratio;
-    *p = uint2{encode4(v[0], v[1], v[2], v[3]), encode4(v[4], v[5], v[6], v[7])};
+    for (int i = 0; i < 4; ++i) {
+      float v[4];
+      decode4(x[i], v);
+      x[i] = encode4(v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor);
+    }
+    *p = uint4{x[0], x[1], x[2], x[3]};
   }
-  if (tensor == 0 && (tid & 15) == 0) {
+  if (tensor == 0 && (tid & 7) == 0) {
 #pragma unroll
     for (int s = 0; s < SWEEPS; ++s) {
-      const int row = row0 + 16 * s + (tid >> 4);
+      const int row = row0 + 16 * s + (tid >> 3);
       if (from[s] < 0 || (in_place && !hole[s])) continue;
       dst.positions[row] = src.positions[from[s]];
       if (dst.weights) dst.weights[row] = src.weights[from[s]];
@@ -783,8 +788,11 @@ extern "C" int ckv_quant_evict(const ckv_quant_cache* cache, const ckv_quant_cac
   }
   const EvictArgs a{*cache, into ? *into : *cache, reinterpret_cast<uint32_t*>(workspace), most, num_sink, recent};
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (cache->capacity <= SELECT_ALONE) {
-    evict_select_kernel<<<dim3(cache->kv_heads, cache->batch), SEL_THREADS, 0, s>>>(a);
+  const dim3 heads(cache->kv_heads, cache->batch);
+  if (cache->capacity <= SELECT_FEW * SEL_KEYS) {
+    evict_select_kernel<SELECT_FEW><<<heads, SELECT_FEW, 0, s>>>(a);
+  } else if (cache->capacity <= SELECT_MANY * SEL_KEYS) {
+    evict_select_kernel<SELECT_MANY><<<heads, SELECT_MANY, 0, s>>>(a);
   } else {
     const dim3 chunks((cache->capacity + CHUNK - 1) / CHUNK, cache->kv_heads, cache->batch);
     evict_clear_kernel<<<cache->batch * cache->kv_heads, 256, 0, s>>>(a);
@@ -796,7 +804,7 @@ extern "C" int ckv_quant_evict(const ckv_quant_cache* cache, const ckv_quant_cac
   }
   rc = launched("ckv_quant_evict");
   if (rc) return rc;
-  const dim3 grid((most + cache->block - 1) / cache->block, cache->kv_heads, 2 * cache->batch);
+  const dim3 grid((most + cache->block - 1) / cache->block, cache->kv_heads, cache->batch);
   const bool in_place = !into;
   if (cache->block == 16) evict_move_kernel<1><<<grid, THREADS, 0, s>>>(a, in_place);
   else if (cache->block == 32) evict_move_kernel<2><<<grid, THREADS, 0, s>>>(a, in_place);

@@ -74,12 +74,13 @@ struct StepCodes {
   uint4 k[2][2];
   uint2 v[8];
   float ks, vs;
+  int4 pos[2];  // positions of the rows 8 L .. 8 L + 7, where masks need them
 };
 
 __device__ inline int step_row(int j, int m) { return 8 * (m >> 2) + 4 * j + (m & 3); }
 
 template <bool WITH_V = true>
-__device__ inline void load_step(const QuantHead& q, int t0, int last, int block_log2, StepCodes& s) {
+__device__ inline void load_step(const QuantHead& q, int t0, int last, int block_log2, bool positions, StepCodes& s) {
   const int lane = threadIdx.x & 63, L = lane >> 4, c = lane & 15;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -89,6 +90,12 @@ __device__ inline void load_step(const QuantHead& q, int t0, int last, int block
   }
   const int blk = min(t0 + 8 * L, last) >> block_log2;
   s.ks = gload_f32(q.key_scales + blk);
+  if (positions) {
+    // eight rows at once: the capacity is a multiple of 16
+    const int32_t* p = q.positions + (min(t0 + 8 * L, last) & ~7);
+    s.pos[0] = __builtin_bit_cast(int4, gload16(p));
+    s.pos[1] = __builtin_bit_cast(int4, gload16(p + 4));
+  }
   if constexpr (WITH_V) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -122,18 +129,14 @@ __device__ inline void step_scores(const StepCodes& s, const QueryTile<DT>& q, f
   }
 }
 
-// Masks the scores of the step from t0 on: n rows in use; `positions` null where
-// every row in use is seen by every query.
-__device__ inline void mask_step(const int32_t* positions, int t0, int n, int lo, int hi, float* sc) {
+// Masks the scores of the step from t0 on: n rows in use; by_position: only
+// positions in [lo, hi] are seen, otherwise all rows in use are.
+__device__ inline void mask_step(const StepCodes& s, bool by_position, int t0, int n, int lo, int hi, float* sc) {
   const int L = (threadIdx.x & 63) >> 4;
+  const int p[8] = {s.pos[0].x, s.pos[0].y, s.pos[0].z, s.pos[0].w, s.pos[1].x, s.pos[1].y, s.pos[1].z, s.pos[1].w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = t0 + 8 * L + i;
-    bool ok = r < n;
-    if (positions) {
-      const int p = gload_i32(positions + min(r, n - 1));
-      ok = ok && p >= lo && p <= hi;
-    }
+    const bool ok = t0 + 8 * L + i < n && (!by_position || (p[i] >= lo && p[i] <= hi));
     sc[i] = ok ? sc[i] : NEG_INF;
   }
 }
@@ -244,19 +247,19 @@ __device__ inline void add_step(const float* sc, float vs, const uint4* vop, boo
 }
 
 // One workgroup of four waves takes a part of the cache rows of a (sequence,
-// head) for NR * 16 query rows; its waves take steps in turn and join in LDS.
+// head) for 16 query rows; its waves take steps in turn and join in LDS.
 // Bound by memory: eight sequences of 16k-131k rows (32/8 heads, one query,
 // bf16) read 1.69 GB in 283 us, 6.0 TB/s.  512 workgroups, all resident, two
 // waves a SIMD: 1,024 and 2,048 workgroups take 3 and 8 % longer there and 9 and
 // 20 % at one sequence of 131k; three waves a SIMD (168 registers) the same or
 // longer, reading a step ahead into a second set of registers the same.
-template <int DT, int NR>
-__global__ __launch_bounds__(64 * WAVES, NR == 1 ? 2 : 1) void attend_split_kernel(const QuantAttendArgs a) {
+template <int DT>
+__global__ __launch_bounds__(64 * WAVES, 2) void attend_split_kernel(const QuantAttendArgs a) {
   __shared__ float m_s[WAVES][16];
   __shared__ float l_s[WAVES][16];
   __shared__ float o_s[WAVES][16 * D];
   const ckv_quant_cache& c = a.cache;
-  const int h = blockIdx.x % c.kv_heads, number = blockIdx.x / c.kv_heads, row0 = blockIdx.y * (16 * NR);
+  const int h = blockIdx.x % c.kv_heads, number = blockIdx.x / c.kv_heads, row0 = 16 * blockIdx.y;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, L = lane >> 4, col = lane & 15;
   const Part part = find_part(c, a.parts, number, -1);
   const int b = part.sequence;
@@ -265,23 +268,20 @@ __global__ __launch_bounds__(64 * WAVES, NR == 1 ? 2 : 1) void attend_split_kern
   const int lo_row = part.index * part.rows, hi_row = (int)min((int64_t)lo_row + part.rows, (int64_t)n);
   const QuantHead q = quant_head(c, b, h);
   const int block_log2 = 31 - __clz(c.block);
-  QueryTile<DT> query[NR];
-  Running run[NR];
-  int lo[NR], hi[NR];
+  QueryTile<DT> query;
+  Running run;
+  int lo, hi;
+  load_query_tile<DT>(a, b, h, row0, query);
+  query_range(a, row0 + col, count, seen, &lo, &hi);
+  run.m = NEG_INF;
+  run.l = 0.0f;
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    load_query_tile<DT>(a, b, h, row0 + 16 * r, query[r]);
-    query_range(a, row0 + 16 * r + col, count, seen, &lo[r], &hi[r]);
-    run[r].m = NEG_INF;
-    run[r].l = 0.0f;
-#pragma unroll
-    for (int nb = 0; nb < 8; ++nb) run[r].o[nb] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int nb = 0; nb < 8; ++nb) run.o[nb] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   // with one new token and no window every row in use is at or before it
   const bool by_position = a.window > 0 || a.tokens > 1 || count < a.tokens;
   StepCodes cur;
   for (int t0 = lo_row + wave * STEP; t0 < hi_row; t0 += WAVES * STEP) {
-    load_step(q, t0, n - 1, block_log2, cur);
+    load_step(q, t0, n - 1, block_log2, by_position, cur);
     const bool tail = t0 + STEP > n;
     bool fix_nan = false;
     uint2 raw[8];
@@ -299,39 +299,35 @@ __global__ __launch_bounds__(64 * WAVES, NR == 1 ? 2 : 1) void attend_split_kern
     }
     uint4 vop[8];
     value_operands(cur.v, vop);
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      float sc[8];
-      step_scores<DT>(cur, query[r], a.scale_log2, sc);
-      if (tail || by_position) mask_step(by_position ? q.positions : nullptr, t0, n, lo[r], hi[r], sc);
-      if (NR == 1 && a.scores && col < a.rows && t0 + 8 * L < n) {
-        float4* p = reinterpret_cast<float4*>(
-            a.scores + (((int64_t)b * c.kv_heads + h) * a.rows + col) * c.capacity + t0 + 8 * L);
-        p[0] = float4{sc[0], sc[1], sc[2], sc[3]};
-        p[1] = float4{sc[4], sc[5], sc[6], sc[7]};
-      }
-      add_step<DT>(sc, cur.vs, vop, fix_nan, raw, run[r]);
+    float sc[8];
+    step_scores<DT>(cur, query, a.scale_log2, sc);
+    if (tail || by_position) mask_step(cur, by_position, t0, n, lo, hi, sc);
+    if (a.scores && col < a.rows && t0 + 8 * L < n) {
+      float4* p = reinterpret_cast<float4*>(
+          a.scores + (((int64_t)b * c.kv_heads + h) * a.rows + col) * c.capacity + t0 + 8 * L);
+      p[0] = float4{sc[0], sc[1], sc[2], sc[3]};
+      p[1] = float4{sc[4], sc[5], sc[6], sc[7]};
     }
+    add_step<DT>(sc, cur.vs, vop, fix_nan, raw, run);
   }
-  // join the waves, one tile of 16 query rows after the other
-#pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    float l = add_xor16(run[r].l);
+  // join the waves
+  {
+    float l = add_xor16(run.l);
     l = add_xor32(l);
     __syncthreads();
     if (L == 0) {
-      m_s[wave][col] = run[r].m;
+      m_s[wave][col] = run.m;
       l_s[wave][col] = l;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float4* p = reinterpret_cast<float4*>(&o_s[wave][(4 * L + i) * D + 8 * col]);
-      p[0] = float4{run[r].o[0][i], run[r].o[1][i], run[r].o[2][i], run[r].o[3][i]};
-      p[1] = float4{run[r].o[4][i], run[r].o[5][i], run[r].o[6][i], run[r].o[7][i]};
+      p[0] = float4{run.o[0][i], run.o[1][i], run.o[2][i], run.o[3][i]};
+      p[1] = float4{run.o[4][i], run.o[5][i], run.o[6][i], run.o[7][i]};
     }
     __syncthreads();
     for (int x = tid; x < 16 * D; x += 64 * WAVES) {
-      const int i = x >> 7, d = x & (D - 1), row = row0 + 16 * r + i;
+      const int i = x >> 7, d = x & (D - 1), row = row0 + i;
       if (row >= a.rows) continue;
       float m = m_s[0][i];
 #pragma unroll
@@ -464,7 +460,7 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendAr
   const QuantHead q = quant_head(c, b, h);
   const bool by_position = a.window > 0 || a.tokens > 1 || count < a.tokens;
   StepCodes s;
-  load_step<false>(q, t0, n - 1, 31 - __clz(c.block), s);
+  load_step<false>(q, t0, n - 1, 31 - __clz(c.block), by_position, s);
   const float2* stats = a.stats + ((int64_t)b * c.kv_heads + h) * a.row_pad;
   float got[8] = {};
   for (int row0 = 0; row0 < a.rows; row0 += 16) {
@@ -475,7 +471,7 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendAr
     const float2 st = row0 + col < a.rows ? stats[row0 + col] : float2{0.0f, 0.0f};
     float sc[8];
     step_scores<DT>(s, query, a.scale_log2, sc);
-    mask_step(by_position ? q.positions : nullptr, t0, n, lo, hi, sc);
+    mask_step(s, by_position, t0, n, lo, hi, sc);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       got[i] += sc[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(sc[i] - st.x) * st.y;
@@ -492,16 +488,18 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendAr
   }
 }
 
-// Query rows a workgroup: 16 while that holds all of them, else 32.
-template <int DT>
-int row_tiles(int rows) { return rows > 16 && DT == CKV_BF16 ? 2 : 1; }
-
 // Parts that the cache rows of the batch are split into: enough workgroups to
-// fill the chip (`workgroups`), no more than there are units.
-int parts_for(const ckv_quant_cache* c, int64_t row_blocks, int64_t workgroups) {
+// fill the chip (`workgroups`), no more than there are units.  A few units are
+// left in one part, which needs no join: with one query a sequence and up to
+// eight units (1,024 rows) one part takes 5.5, 6.8 and 9.6 us at 256, 512 and
+// 1,024 rows where parts and their join take 10.2 to 10.4 (2,048 rows: 15.1 and
+// 10.4; replayed, 8 heads over 2).
+constexpr int ONE_PART_UNITS = 8;
+
+int parts_for(const ckv_quant_cache* c, int64_t row_blocks, int64_t workgroups, int64_t alone) {
   const int64_t units = ((int64_t)c->capacity + PART_UNIT - 1) / PART_UNIT;
   const int64_t want = workgroups / ((int64_t)c->kv_heads * row_blocks);
-  if (want <= c->batch) return c->batch;
+  if (want <= c->batch || units <= alone) return c->batch;
   return (int)(want < c->batch * units ? want : c->batch * units);
 }
 
@@ -515,7 +513,7 @@ struct AttendLayout {
     row_pad = (rows + 15) / 16 * 16;
     many = rows > FEW_ROWS;
     const int64_t block = many ? many_row_block(dtype) : 16;
-    parts = parts_for(c, (rows + block - 1) / block, many ? 256 : FEW_WORKGROUPS);
+    parts = parts_for(c, (rows + block - 1) / block, many ? 256 : FEW_WORKGROUPS, many ? 1 : ONE_PART_UNITS);
     keep_scores = accumulate && rows <= 16;
     const size_t heads = (size_t)c->batch * c->kv_heads;
     size_t at = 0;
@@ -537,20 +535,14 @@ struct AttendLayout {
   }
 };
 
-template <int DT, int NR>
-void launch_split(const QuantAttendArgs& a, hipStream_t s) {
-  const dim3 grid(a.parts * a.cache.kv_heads, (a.rows + 16 * NR - 1) / (16 * NR));
-  attend_split_kernel<DT, NR><<<grid, 64 * WAVES, 0, s>>>(a);
-}
-
 template <int DT>
 int launch_attend(const QuantAttendArgs& a, bool many, bool accumulate, hipStream_t s) {
   int rc;
   if (many) {
     rc = launch_many_rows(a, DT, s);
   } else {
-    if (row_tiles<DT>(a.rows) == 2) launch_split<DT, 2>(a, s);
-    else launch_split<DT, 1>(a, s);
+    const dim3 grid(a.parts * a.cache.kv_heads, (a.rows + 15) / 16);
+    attend_split_kernel<DT><<<grid, 64 * WAVES, 0, s>>>(a);
     rc = launched("ckv_quant_attention");
   }
   if (!rc && a.parts > a.cache.batch) {
