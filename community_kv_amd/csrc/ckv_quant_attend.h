@@ -107,7 +107,8 @@ __device__ inline int part_size(const ckv_quant_cache& c, int parts) {
   for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
   const int64_t spare = parts - c.batch;
   const int64_t units = ((total + spare - 1) / spare + PART_UNIT - 1) / PART_UNIT;
-  return (int)min(max(units, (int64_t)1) * PART_UNIT, (int64_t)0x7fffff80);
+  // the same on every lane, and said so: what follows from it stays on the scalar unit
+  return __builtin_amdgcn_readfirstlane((int)min(max(units, (int64_t)1) * PART_UNIT, (int64_t)0x7fffff80));
 }
 
 __device__ inline int parts_of_sequence(int n, int size) { return n > size ? (n - 1) / size + 1 : 1; }

@@ -234,51 +234,34 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   const float grow_by = RESCALE / sl2;
   float m = NEG_INF;  // running maximum of the unscaled scores, shared by a row's two lanes
   float l = 0.0f;     // this lane's share of the sum
+  // S^T of a tile: accumulator i holds cache rows 32 i + 8 (v / 4) + 4 half + v % 4 of the lane's query
   f32x16_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = f32x16_t{};
 
-  // Scores of the tile staged in `stage`: accumulator i holds cache rows
-  // 32 i + 8 (v / 4) + 4 half + v % 4.
-  auto qk_tile = [&](int stage, f32x16_t (&acc)[2]) __attribute__((always_inline)) {
-    const uint16_t* k_s = lds.k[stage];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) acc[i] = f32x16_t{};
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 kf = *reinterpret_cast<const uint4*>(k_s + (32 * i + (lane & 31)) * K_STRIDE + 16 * s + 8 * half);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) acc[i] = mfma32(kf, qreg[p][s], acc[i]);
-      }
-    }
-  };
   auto is_masked = [&](const TileRef& t, int all_lo, int all_hi) __attribute__((always_inline)) {
     return t.lo < all_lo || t.hi > all_hi || (t.tile + 1) * KEYS > n;
   };
   TileCodes<W> kc, vc;
-  // Values of a tile to LDS.  Where some query does not see some row, NaN codes
-  // become zeros (a masked row's zero probability times NaN would spread it) and
-  // are made up for afterwards, and the positions are staged too.
-  auto stage_values = [&](const TileRef& t, int stage) __attribute__((always_inline)) {
-    if (is_masked(t, group_lo, group_hi)) {
-      asm volatile("");
-      bool nan = false;
+  // Before a tile's values go to LDS: where some query does not see some row, NaN
+  // codes become zeros (a masked row's zero probability times NaN would spread it)
+  // and are made up for afterwards, and the positions are staged.
+  auto prepare_values = [&](const TileRef& t, int stage) __attribute__((always_inline)) {
+    if (!is_masked(t, group_lo, group_hi)) return;
+    asm volatile("");
+    bool nan = false;
 #pragma unroll
-      for (int i = 0; i < TileCodes<W>::C; ++i) {
-        nan |= drop_nan_codes(vc.w[i].x);
-        nan |= drop_nan_codes(vc.w[i].y);
-        nan |= drop_nan_codes(vc.w[i].z);
-        nan |= drop_nan_codes(vc.w[i].w);
-      }
-      if (nan) lds.nan[stage] = t.tile;
-      if (tid < KEYS) {
-        const int r = t.tile * KEYS + tid;
-        lds.pos[stage][tid] = r < n ? gload_i32(q.positions + r) : 0x7fffffff;
-      }
+    for (int i = 0; i < TileCodes<W>::C; ++i) {
+      nan |= drop_nan_codes(vc.w[i].x);
+      nan |= drop_nan_codes(vc.w[i].y);
+      nan |= drop_nan_codes(vc.w[i].z);
+      nan |= drop_nan_codes(vc.w[i].w);
     }
-    store_codes<W>(vc, lds.v[stage], V_STRIDE);
+    if (nan) lds.nan[stage] = t.tile;
+    if (tid < KEYS) {
+      const int r = t.tile * KEYS + tid;
+      lds.pos[stage][tid] = r < n ? gload_i32(q.positions + r) : 0x7fffffff;
+    }
   };
   auto load_keys = [&](const TileRef& t) __attribute__((always_inline)) {
     load_codes<W>(q.key_codes, q.key_scales, t.tile, n, block_log2, kc);
@@ -287,81 +270,87 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
     load_codes<W>(q.value_codes, q.value_scales, t.tile, n, block_log2, vc);
   };
 
-  // One bf16 piece: the next tile's scores are computed beside this tile's
-  // exponentials, so keys are staged a tile ahead of values.  Past the last
-  // tile the pipeline stages that tile again, unused.
-  constexpr bool AHEAD = NP == 1;
+  // Two groups of four waves, one of each on a SIMD, take turns: while one has
+  // the matrix cores (M_i: O += V P of its tile i and the scores of tile i + 1) the
+  // other has the vector ALUs (V_i: the softmax of its tile), and a barrier changes
+  // them over.  The first group does V_i in slot 2 i and M_i in slot 2 i + 1, the
+  // second each a slot later.  M_i reads X_i = {values of tile i, keys of tile
+  // i + 1} from LDS and between its products stores X_(i + 1), which takes the
+  // place of X_(i - 1), last read in slot 2 i.  (The positions that masks need
+  // are staged by the first group, a slot before it needs them.)  One group alone
+  // (four waves) does V_i, M_i and a barrier.  Past the last tile the pipeline
+  // stages that tile again, unused.  2,048 queries over 32k rows (32/8 heads,
+  // bf16): 1.00 to 1.06 ms, 1,010 to 1,070 TFLOP/s; without turns 1.03 to 1.12.
+  // What is left is the matrix cores' own rate: with neither staging nor
+  // exponentials the loop takes 0.92 ms, and a large library product runs at
+  // 1,300 TFLOP/s on this card.
+  constexpr bool TURNS = W == 8;
+  const bool second = TURNS && wave >= 4;
   const int64_t tiles = (c.capacity + KEYS - 1) / KEYS;
-  TileWalk walk(a.ranges + (int64_t)bh * tiles, lo_row / KEYS, (hi_row + KEYS - 1) / KEYS, walk_lo, walk_hi);
-  int left = 0;  // of here, next, third: tiles that there are
-  TileRef here, next, third;
+  TileWalk walk(a.ranges + bh * tiles, lo_row / KEYS, (int)(((int64_t)hi_row + KEYS - 1) / KEYS), walk_lo, walk_hi);
+  int left = 0;  // of t0, t1, t2, t3: tiles that there are
   auto advance = [&](const TileRef& after) __attribute__((always_inline)) {
     const TileRef t = walk.next();
     if (t.tile < 0) return after;
     ++left;
     return t;
   };
-  here = advance(TileRef{-1, 0, 0});
-  next = advance(here);
-  third = advance(next);
-  int kstage = 0, vstage = 0;
-  f32x16_t sa[2], sb[2];
+  TileRef t0 = advance(TileRef{-1, 0, 0});
+  TileRef t1 = advance(t0), t2 = advance(t1);
+  int stage = 0;  // X_i has its values in v[i & 1], its keys in k[(i + 1) & 1]
+  f32x16_t sc[2];
   if (tid < 2) lds.nan[tid] = -1;
   __syncthreads();
   if (left > 0) {
-    load_keys(here);
-    load_values(here);
+    load_keys(t0);
     store_codes<W>(kc, lds.k[0], K_STRIDE);
-    stage_values(here, 0);
-    load_keys(next);
-    load_values(next);
-    if (AHEAD) {
-      store_codes<W>(kc, lds.k[1], K_STRIDE);
-      load_keys(third);
-    }
+    load_values(t0);
+    load_keys(t1);
+    prepare_values(t0, 0);
+    store_codes<W>(vc, lds.v[0], V_STRIDE);
+    store_codes<W>(kc, lds.k[1], K_STRIDE);
+    load_values(t1);
+    load_keys(t2);
     __syncthreads();
-    if (AHEAD) {
-      qk_tile(0, sa);
-      __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int i = k & 1, x = k >> 1;
+      const uint4 kf = *reinterpret_cast<const uint4*>(&lds.k[0][(32 * i + (lane & 31)) * K_STRIDE + 16 * x + 8 * half]);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) sc[i] = mfma32(kf, qreg[p][x], x == 0 && p == 0 ? f32x16_t{} : sc[i]);
     }
+    __syncthreads();  // k[0] is free
+    if (second) __syncthreads();
   }
 
-  // One tile.  AHEAD: `cur` holds its scores, its values are in v[vstage], the
-  // next tile's keys in k[kstage ^ 1]; kc holds the third tile's keys, vc the
-  // next tile's values.  Otherwise its keys are in k[kstage] and kc holds the
-  // next tile's.
-  auto tile_step = [&](f32x16_t (&cur)[2], f32x16_t (&nxt)[2]) __attribute__((always_inline)) {
-    const TileRef fourth = advance(third);
-    // the stages that the last tile used are free: fill them
-    stage_values(next, vstage ^ 1);
-    store_codes<W>(kc, lds.k[AHEAD ? kstage : kstage ^ 1], K_STRIDE);
-    load_keys(AHEAD ? fourth : third);
-    load_values(third);
-    if (!AHEAD) qk_tile(kstage, cur);
-    if (is_masked(here, wave_lo, wave_hi)) {
+  uint32_t pb[NP][2][8];
+  while (left > 0) {
+    // ---- V_i: the vector ALUs ----
+    if (is_masked(t0, wave_lo, wave_hi)) {
       asm volatile("");  // a branch, not selects on every tile
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int4 p = *reinterpret_cast<const int4*>(&lds.pos[vstage][32 * i + 8 * g + 4 * half]);
+          const int4 p = *reinterpret_cast<const int4*>(&lds.pos[stage][32 * i + 8 * g + 4 * half]);
           const int at[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x = cur[i][4 * g + e];
+            float x = sc[i][4 * g + e];
             see.mask(x, at[e]);
-            cur[i][4 * g + e] = x;
+            sc[i][4 * g + e] = x;
           }
         }
       }
     }
-    float top = max3(cur[0][0], cur[0][1], cur[1][0]);
+    float tops[4];
 #pragma unroll
-    for (int v = 2; v < 16; v += 2) top = max3(top, cur[0][v], cur[0][v + 1]);
-#pragma unroll
-    for (int v = 1; v < 15; v += 2) top = max3(top, cur[1][v], cur[1][v + 1]);
-    top = max3(top, cur[1][15], cur[1][15]);
-    top = max_xor32(top);
+    for (int x = 0; x < 4; ++x) {
+      const f32x16_t& v = sc[x >> 1];
+      const int e = 8 * (x & 1);
+      tops[x] = max3(max3(v[e], v[e + 1], v[e + 2]), max3(v[e + 3], v[e + 4], v[e + 5]), max3(v[e + 6], v[e + 7], v[e + 7]));
+    }
+    const float top = max_xor32(max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]));
     if (__ballot(top > m + grow_by) != 0) {
       const float t = top > m + grow_by ? top : m;  // a query's own scores alone decide
       const float f = m == t ? 1.0f : __builtin_amdgcn_exp2f((m - t) * sl2);
@@ -371,43 +360,74 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
       for (int i = 0; i < 4; ++i) o[i] *= f;
     }
     const float mc = m == NEG_INF ? 0.0f : m * sl2;
-    if (AHEAD) qk_tile(kstage ^ 1, nxt);  // on the last tile: unused
-    uint32_t pb[NP][2][8];
+    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int v = 0; v < 16; v += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v], sl2, -mc));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[i][v + 1], sl2, -mc));
-        l += p0;
-        l += p1;
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][v], sl2, -mc));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][v + 1], sl2, -mc));
+        sums[v & 2] += p0;
+        sums[(v & 2) + 1] += p1;
         split_pair<NP>(p0, p1, &pb[0][i][v >> 1], 16);
+        // in this slot: the compiler moves the exponentials behind the barrier otherwise
+#pragma unroll
+        for (int p = 0; TURNS && p < NP; ++p) asm volatile("" : "+v"(pb[p][i][v >> 1]));
       }
     }
-    const uint16_t* v_s = lds.v[vstage];
+    l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    if (TURNS) __syncthreads();
+    // ---- M_i: the matrix cores, and the staging of X_(i + 1) between the products ----
+    if (TURNS) __builtin_amdgcn_s_setprio(1);
+    const TileRef t3 = advance(t2);
+    // Operands from LDS are read AHEAD products before they are used: 16 of
+    // values (rows 16 (k / 4) of the tile, dims 32 (k % 4)), then 16 of keys.
+    const uint16_t* v_at = lds.v[stage] + (4 * half + ((lane & 15) >> 2)) * V_STRIDE + 16 * ((lane >> 4) & 1) +
+                           4 * (lane & 3);
+    const uint16_t* k_at = lds.k[stage ^ 1] + (lane & 31) * K_STRIDE + 8 * half;
+    auto operand = [&](int k) __attribute__((always_inline)) {
+      if (k < 16) {
+        const uint16_t* p = v_at + 16 * (k >> 2) * V_STRIDE + 32 * (k & 3);
+        const uint2 x = lds_read_tr16(p), y = lds_read_tr16(p + 8 * V_STRIDE);
+        return uint4{x.x, x.y, y.x, y.y};
+      }
+      return *reinterpret_cast<const uint4*>(k_at + 32 * (k & 1) * K_STRIDE + 16 * ((k - 16) >> 1));
+    };
+    constexpr int AHEAD = 6;
+    uint4 op[AHEAD];
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const int i = kk >> 1, vb = 4 * (kk & 1);
-      const uint16_t* vrow = v_s + (16 * kk + 4 * half + ((lane & 15) >> 2)) * V_STRIDE + 16 * ((lane >> 4) & 1) +
-                             4 * (lane & 3);
+    for (int k = 0; k < AHEAD; ++k) op[k] = operand(k);
+    prepare_values(t1, stage ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int db = 0; db < 4; ++db) {
-        const uint2 x = lds_read_tr16(vrow + 32 * db);
-        const uint2 y = lds_read_tr16(vrow + 8 * V_STRIDE + 32 * db);
+    for (int k = 0; k < 32; ++k) {
+      const uint4 now = op[k % AHEAD];
+      if (k < 16) {
+        const int i = k >> 3, vb = 4 * ((k >> 2) & 1), db = k & 3;
 #pragma unroll
         for (int p = 0; p < NP; ++p)
-          o[db] = mfma32(uint4{x.x, x.y, y.x, y.y},
-                         uint4{pb[p][i][vb], pb[p][i][vb + 1], pb[p][i][vb + 2], pb[p][i][vb + 3]}, o[db]);
+          o[db] = mfma32(now, uint4{pb[p][i][vb], pb[p][i][vb + 1], pb[p][i][vb + 2], pb[p][i][vb + 3]}, o[db]);
+      } else {
+        const int i = k & 1, x = (k - 16) >> 1;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) sc[i] = mfma32(now, qreg[p][x], k < 18 && p == 0 ? f32x16_t{} : sc[i]);
       }
+      if (k + AHEAD < 32) op[k % AHEAD] = operand(k + AHEAD);
+      if (k == 4) store_codes<W>(vc, lds.v[stage ^ 1], V_STRIDE);
+      if (k == 10) store_codes<W>(kc, lds.k[stage], K_STRIDE);
+      if (k == 14) load_values(t2);
+      if (k == 18) load_keys(t3);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (is_masked(here, group_lo, group_hi) && lds.nan[vstage] == here.tile) {
+    if (TURNS) __builtin_amdgcn_s_setprio(0);
+    if (is_masked(t0, group_lo, group_hi) && lds.nan[stage] == t0.tile) {
       asm volatile("");
       // NaN codes that were staged as zeros: NaN where a query sees their row
 #pragma nounroll
       for (int r = 0; r < KEYS; ++r) {
-        if (here.tile * KEYS + r >= n) break;
-        const bool sees = (uint32_t)(lds.pos[vstage][r] - see.lo) <= see.span;
-        const uint8_t* code = q.value_codes + (int64_t)(here.tile * KEYS + r) * D + 4 * half;
+        if (t0.tile * KEYS + r >= n) break;
+        const bool sees = (uint32_t)(lds.pos[stage][r] - see.lo) <= see.span;
+        const uint8_t* code = q.value_codes + (int64_t)(t0.tile * KEYS + r) * D + 4 * half;
 #pragma unroll
         for (int db = 0; db < 4; ++db) {
 #pragma unroll
@@ -421,21 +441,12 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
       }
     }
     __syncthreads();
-    kstage ^= 1;
-    vstage ^= 1;
-    here = next;
-    next = third;
-    third = fourth;
+    stage ^= 1;
+    t0 = t1;
+    t1 = t2;
+    t2 = t3;
     --left;
-  };
-  while (left > 0) {
-    if constexpr (AHEAD) {
-      tile_step(sa, sb);
-      if (left == 0) break;
-      tile_step(sb, sa);
-    } else {
-      tile_step(sa, sa);
-    }
+    if (TURNS && !second && left == 0) __syncthreads();  // the second group's last slot
   }
 
   if (row >= a.rows) return;
