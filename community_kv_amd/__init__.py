@@ -21,6 +21,7 @@ from community_kv_amd.attention.quantized import (  # noqa: F401
     quantized_append,
     quantized_attention,
 )
+from community_kv_amd.attention.quantized_cache import QuantizedCache, QuantizedCacheAttention  # noqa: F401
 
 __all__ = [
     "ATTENTION_IMPLEMENTATION",

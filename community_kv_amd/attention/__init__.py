@@ -6,6 +6,7 @@ from community_kv_amd.attention.decode import DecodeLayerWorkspace, decode_layer
 from community_kv_amd.attention.flash_attention import prefill_attention_topk
 from community_kv_amd.attention.kernels.packed_segments import PackedSegments
 from community_kv_amd.attention.quantized import QuantizedKVCache, evict, quantized_append, quantized_attention
+from community_kv_amd.attention.quantized_cache import QuantizedCache, QuantizedCacheAttention, QuantizedCacheLayer
 
 __all__ = [
     "ATTENTION_IMPLEMENTATION",
@@ -13,6 +14,9 @@ __all__ = [
     "DecodeLayerWorkspace",
     "HuggingFaceAttention",
     "PackedSegments",
+    "QuantizedCache",
+    "QuantizedCacheAttention",
+    "QuantizedCacheLayer",
     "QuantizedKVCache",
     "StaticCache",
     "StaticCacheLayer",

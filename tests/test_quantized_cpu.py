@@ -215,3 +215,60 @@ def test_oracle_block_scale_and_growth():
     got, want = cache.value(0, 0, 0, np.arange(40)), x[0, 0]
     step = np.maximum(np.abs(want) * 2.0 ** -4, whole.scales[0][0, 0, np.arange(40) // 32][:, None] * 2.0 ** -9)
     assert (np.abs(got - want) <= step).all()  # half a step, and another half among the subnormals
+
+
+# ------------------------------------------------------------------------------------------ Hugging Face cache
+
+@pytest.mark.parametrize("change", [dict(max_cache_len=0), dict(budget=-1), dict(budget=64, num_sink=10, recent=60),
+                                    dict(budget=64, slack=64), dict(slack=-1)])
+def test_cache_layer_refuses(change):
+    from community_kv_amd.attention import QuantizedCacheLayer
+
+    with pytest.raises(ValueError):
+        QuantizedCacheLayer(**(dict(max_cache_len=128, num_sink=4, recent=16) | change))
+
+
+def test_cache_layer_protocol():
+    from community_kv_amd import QuantizedCache
+
+    cache = QuantizedCache(num_hidden_layers=2, max_cache_len=100)
+    layer = cache.layer(1)
+    assert cache.get_seq_length() == 0 and layer.get_max_length() == 100 and not layer.is_initialized
+    x = torch.zeros(1, 2, 101, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="capacity"):
+        cache.update(x, x, 1)
+    with pytest.raises(ValueError, match="one sequence"):
+        cache.update(x.expand(2, 2, 101, 128)[:, :, :3], x.expand(2, 2, 101, 128)[:, :, :3], 1)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        cache.update(x[:, :, :3], x[:, :, :3], 1)
+    assert layer.seen == 0 and layer.rows == 0
+    with pytest.raises(RuntimeError, match="in the cache first"):
+        layer.attend(x[:, :, :1], 1.0)
+    with pytest.raises(NotImplementedError):
+        layer.reorder_cache(torch.zeros(1, dtype=torch.long))
+    with pytest.raises(NotImplementedError):
+        layer.offload()
+    layer.rows, layer.seen = 40, 40
+    layer.store.cursors[:2] = 40
+    layer.crop(38)
+    layer.crop(-3)
+    layer.crop(99)
+    assert layer.rows == layer.seen == 35 and layer.store.cursors.tolist() == [[35], [35], [0]]
+    layer.budget, layer.seen = 30, 60
+    with pytest.raises(ValueError, match="evicted"):
+        layer.crop(50)
+    layer.reset()
+    assert layer.seen == 0 and not layer.store.cursors.any()
+
+
+def test_attention_function_refuses_what_it_does_not_do():
+    from community_kv_amd import QuantizedCache, QuantizedCacheAttention
+
+    attention = QuantizedCacheAttention(QuantizedCache(num_hidden_layers=1, max_cache_len=64))
+    module = torch.nn.Module()
+    module.layer_idx = 0
+    x = torch.zeros(1, 2, 1, 128)
+    for extra in (dict(dropout=0.1), dict(softcap=30.0), dict(s_aux=torch.zeros(2)), dict(is_causal=False),
+                  dict(attention_mask=torch.zeros(1, 1, 1, 1))):
+        with pytest.raises(ValueError):
+            attention.forward(module, x, x, x, **(dict(attention_mask=None, scaling=1.0) | extra))
