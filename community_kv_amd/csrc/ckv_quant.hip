@@ -92,9 +92,11 @@ struct AppendArgs {
 
 // The cursors of a sequence move when every workgroup has read them.  With few
 // workgroups a sequence (`ticket`) the last to finish moves them; the tickets of
-// many would queue at one address (12 ns each: the 8,192 workgroups of a 32k
-// prompt took 107 us with tickets, 51 with advance_kernel behind them, where a
-// second launch costs a single token's append 1.9 us more than its 8 tickets).
+// many queue at one address (12 ns each), and advance_kernel behind the append is
+// quicker.  Both in a graph, 8 heads in blocks of 64: one token of 8 sequences 5.4 us
+// with tickets and 6.2 with advance_kernel; of one sequence, 449 tokens (64
+// workgroups) 7.5 and 7.9, 960 tokens (128) 8.1 and 8.0, 4,096 (520) 14.4 and 10.8,
+// 32,768 into an empty cache 61 and 41.
 __device__ inline void advance(const ckv_quant_cache& c, int b, int start, int seen, int count) {
   const int end = (int)min((int64_t)start + count, (int64_t)c.capacity);
   c.cursors[b] = end;
@@ -253,10 +255,14 @@ __device__ inline uint32_t evict_key(float w, bool is_protected) {
   return ordered_f32(w + 0.0f);
 }
 
-// One workgroup a (sequence, head) selects where its threads hold all keys, SEL_KEYS
-// each: 256 threads up to 2,048 rows (their barriers cost less), 1,024 up to 8,192.
-constexpr int SEL_KEYS = 8;
+// One workgroup a (sequence, head) selects where its threads hold all keys, and
+// several where they do not.  A whole eviction of 8 heads, half the rows kept, in a
+// graph: capacity 1,000 13.6 us with 256 threads of 8 keys, 14.4 with 1,024 (their
+// barriers), 28.5 with several workgroups (the launches); 8,000 17.3 with 1,024
+// threads of 8 keys, 32.6; 12,000 24.0 with 1,024 of 16, 35.7; 16,300 27.9, 38.3;
+// 32 keys a thread, 32,000 48.9, 43.4.
 constexpr int SELECT_FEW = 256, SELECT_MANY = 1024;
+constexpr int KEYS_FEW = 8, KEYS_MANY = 16;
 
 // Exclusive scan of x over a workgroup of T threads, and its total.
 template <int T>
@@ -336,7 +342,7 @@ __device__ inline uint32_t kept_rows(const uint32_t* k, int64_t first, int n, ui
 }
 
 __device__ inline uint32_t low_rows(int64_t first, int keep, int rows) {
-  return (1u << (int)min(max((int64_t)keep - first, (int64_t)0), (int64_t)rows)) - 1u;  // rows <= 16
+  return (uint32_t)((1ull << (int)min(max((int64_t)keep - first, (int64_t)0), (int64_t)rows)) - 1ull);  // rows <= 32
 }
 
 // Writes this thread's lists: `kept` of K rows from `first` on, `before` packs the
@@ -386,11 +392,11 @@ __device__ inline void write_header(const EvictArgs& a, const QuantHead& q, uint
   ws[2] = (uint32_t)n;
 }
 
-// One workgroup a (sequence, head), a thread's keys (eight rows in order) in
+// One workgroup a (sequence, head), a thread's KEYS rows in order in
 // registers: the `keep`-th largest by its three digits from the highest, then two
 // scans in row order, for the ties (taken by the lower row) and for the lists of
 // freed rows below `keep` and kept ones from it on.
-template <int T>
+template <int T, int KEYS>
 __global__ __launch_bounds__(T) void evict_select_kernel(const EvictArgs a) {
   __shared__ int hist[2048];
   __shared__ int scratch[T / 64 + 2];
@@ -402,9 +408,9 @@ __global__ __launch_bounds__(T) void evict_select_kernel(const EvictArgs a) {
   uint32_t* ws = a.workspace + ((int64_t)b * c.kv_heads + h) * lay.words;
   if (tid == 0) write_header(a, q, ws, n);
   if (n <= a.keep) return;
-  uint32_t k[SEL_KEYS];
-  const int first = tid * SEL_KEYS;
-  make_keys<SEL_KEYS>(a, q, first, n, seen, k);
+  uint32_t k[KEYS];
+  const int first = tid * KEYS;
+  make_keys<KEYS>(a, q, first, n, seen, k);
   uint32_t prefix = 0;
   int target = a.keep;  // how many of the rows that match the prefix are kept
 #pragma unroll
@@ -413,7 +419,7 @@ __global__ __launch_bounds__(T) void evict_select_kernel(const EvictArgs a) {
     for (int i = tid; i < bins; i += T) hist[i] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < SEL_KEYS; ++i) {
+    for (int i = 0; i < KEYS; ++i) {
       const bool in = first + i < n && (d == 0 || (k[i] >> digit_shift(d - 1)) == (prefix >> digit_shift(d - 1)));
       count_bin(hist, in, (k[i] >> shift) & (bins - 1));
     }
@@ -424,12 +430,12 @@ __global__ __launch_bounds__(T) void evict_select_kernel(const EvictArgs a) {
   }
   int equal = 0, total;
 #pragma unroll
-  for (int i = 0; i < SEL_KEYS; ++i) equal += first + i < n && k[i] == prefix;
+  for (int i = 0; i < KEYS; ++i) equal += first + i < n && k[i] == prefix;
   const int rank = block_scan<T>(equal, &total, scratch);
-  const uint32_t kept = kept_rows<SEL_KEYS>(k, first, n, prefix, target, rank);
-  const uint32_t low = low_rows(first, a.keep, SEL_KEYS);
+  const uint32_t kept = kept_rows<KEYS>(k, first, n, prefix, target, rank);
+  const uint32_t low = low_rows(first, a.keep, KEYS);
   const int before = block_scan<T>(__popc(~kept & low) | (__popc(kept & ~low) << 16), &total, scratch);
-  write_lists<SEL_KEYS>(ws, lay, first, a.keep, kept, before, 0, 0);
+  write_lists<KEYS>(ws, lay, first, a.keep, kept, before, 0, 0);
 }
 
 // The same by several workgroups a (sequence, head), for long sequences, in
@@ -789,10 +795,12 @@ extern "C" int ckv_quant_evict(const ckv_quant_cache* cache, const ckv_quant_cac
   const EvictArgs a{*cache, into ? *into : *cache, reinterpret_cast<uint32_t*>(workspace), most, num_sink, recent};
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 heads(cache->kv_heads, cache->batch);
-  if (cache->capacity <= SELECT_FEW * SEL_KEYS) {
-    evict_select_kernel<SELECT_FEW><<<heads, SELECT_FEW, 0, s>>>(a);
-  } else if (cache->capacity <= SELECT_MANY * SEL_KEYS) {
-    evict_select_kernel<SELECT_MANY><<<heads, SELECT_MANY, 0, s>>>(a);
+  if (cache->capacity <= SELECT_FEW * KEYS_FEW) {
+    evict_select_kernel<SELECT_FEW, KEYS_FEW><<<heads, SELECT_FEW, 0, s>>>(a);
+  } else if (cache->capacity <= SELECT_MANY * KEYS_FEW) {
+    evict_select_kernel<SELECT_MANY, KEYS_FEW><<<heads, SELECT_MANY, 0, s>>>(a);
+  } else if (cache->capacity <= SELECT_MANY * KEYS_MANY) {
+    evict_select_kernel<SELECT_MANY, KEYS_MANY><<<heads, SELECT_MANY, 0, s>>>(a);
   } else {
     const dim3 chunks((cache->capacity + CHUNK - 1) / CHUNK, cache->kv_heads, cache->batch);
     evict_clear_kernel<<<cache->batch * cache->kv_heads, 256, 0, s>>>(a);

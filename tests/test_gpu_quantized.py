@@ -386,11 +386,12 @@ def test_evict_orders_special_weights(device):
 
 @pytest.mark.parametrize("keep,num_sink,recent", [(5000, 10, 64), (1, 0, 0), (4096, 0, 4096), (12_287, 3, 5),
                                                   (8193, 100, 0)])
-def test_evict_several_workgroups(device, keep, num_sink, recent):
-    """Sequences long enough for several workgroups: special weights, many ties, lengths at and around the chunks."""
+@pytest.mark.parametrize("capacity", [12_288, 20_480])  # one workgroup, several
+def test_evict_long_with_ties(device, keep, num_sink, recent, capacity):
+    """Long sequences: special weights, many ties, lengths at and around the chunks."""
     gen = torch.Generator().manual_seed(keep)
     lengths = [12_288, 4096, 9001, 4097]
-    cache = _fill(device, gen, batch=4, heads=2, capacity=12_288, block=64, lengths=lengths)
+    cache = _fill(device, gen, batch=4, heads=2, capacity=capacity, block=64, lengths=lengths)
     special = torch.tensor([0.0, -0.0, 1.0, 1.0, float("inf"), -float("inf"), float("nan"), -3.0, 1e-45, 7.25])
     pick = torch.randint(0, 10, cache.weights.shape, generator=gen)
     cache.weights.copy_(torch.where(torch.rand(cache.weights.shape, generator=gen) < 0.7, special[pick],
@@ -399,6 +400,24 @@ def test_evict_several_workgroups(device, keep, num_sink, recent):
     evict(cache, keep=keep, num_sink=num_sink, recent=recent)
     torch.cuda.synchronize()
     oracle.evict(keep=keep, num_sink=num_sink, recent=recent)
+    _same(cache, oracle)
+
+
+@pytest.mark.parametrize("capacity,block", [(2048, 32), (2064, 16), (8192, 64), (8208, 16), (16_384, 128), (16_400, 16),
+                                            (20_480, 64)])
+@pytest.mark.parametrize("share", [0.0, 0.5, 1.0])
+def test_evict_at_each_capacity(device, capacity, block, share):
+    """Both sides of every capacity where the selection's form changes, full and nearly full sequences."""
+    print(f"evict capacity={capacity} block={block} share={share}", flush=True)
+    gen = torch.Generator().manual_seed(capacity)
+    keep = max(1, min(capacity - 1, int(capacity * share)))
+    cache = _fill(device, gen, batch=3, heads=1, capacity=capacity, block=block, lengths=[capacity, capacity - 1, 1500])
+    weights = torch.rand(cache.weights.shape, generator=gen)
+    cache.weights.copy_(torch.where(weights < 0.4, 0.25, weights))
+    oracle = oq.Cache.of(cache)
+    evict(cache, keep=keep, num_sink=min(2, keep // 2), recent=min(9, keep // 2))
+    torch.cuda.synchronize()
+    oracle.evict(keep=keep, num_sink=min(2, keep // 2), recent=min(9, keep // 2))
     _same(cache, oracle)
 
 
