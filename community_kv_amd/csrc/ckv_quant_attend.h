@@ -150,6 +150,17 @@ __device__ inline void query_range(const QuantAttendArgs& a, int row, int count,
   *lo = a.window > 0 && at >= a.window ? at - a.window + 1 : 0;  // no position is negative
 }
 
+// Positions that any of the query rows [first, first + rows) sees: [lo, hi].
+__device__ inline void rows_range(const QuantAttendArgs& a, int first, int rows, int count, int seen, int* lo, int* hi) {
+  const int t0 = token_of(a, first), t1 = min(token_of(a, min(first + rows, a.rows) - 1), count - 1);
+  *lo = 0;
+  *hi = -1;
+  if (t0 > t1) return;
+  int unused;
+  query_range(a, t0 * a.group, count, seen, lo, &unused);
+  query_range(a, t1 * a.group, count, seen, &unused, hi);
+}
+
 // Where query row `row` of KV head h goes: index of its first output element
 // and of its lse.
 __device__ inline void output_index(const QuantAttendArgs& a, int b, int h, int row, int64_t* out, int64_t* lse) {

@@ -246,6 +246,54 @@ __device__ inline void add_step(const float* sc, float vs, const uint4* vop, boo
   }
 }
 
+// Goes over this wave's steps of a part.  Without a window: the part's rows, STEP
+// of every WAVES * STEP.  With one most rows are out of every query's sight, and
+// those in it mostly stand together: a part is then every count-th unit of
+// WAVES * STEP rows, so that all parts have some of them, and a wave looks at the
+// positions of its STEP rows of eight units at once (four a lane) and passes over
+// steps that nobody sees.  Eight sequences of 16k-131k rows in order, window 4,096:
+// 35 us, where reading every row takes 304; of rows in any order, 251.
+struct StepWalk {
+  int t0, end;       // first row of the step; rows end before `end`
+  int unit, stride;  // with a window
+  int lo, hi;        // positions that the workgroup's queries see
+  uint64_t bits;     // steps to come of the eight units from `unit` on, eight bits each
+  __device__ StepWalk(const QuantAttendArgs& a, const Part& part, int n, int wave, int row0, int count, int seen)
+      : end(n), lo(0), hi(0), bits(0) {
+    if (a.window == 0) {
+      end = (int)min((int64_t)part.index * part.rows + part.rows, (int64_t)n);
+      t0 = part.index * part.rows + (wave - WAVES) * STEP;
+    } else {
+      rows_range(a, row0, 16, count, seen, &lo, &hi);
+      stride = part.count;
+      unit = part.index - 8 * stride;
+    }
+  }
+  __device__ bool next(const QuantAttendArgs& a, const QuantHead& q, int wave) {
+    if (a.window == 0) {
+      t0 += WAVES * STEP;
+      return t0 < end;
+    }
+    const int lane = threadIdx.x & 63;
+    while (bits == 0) {
+      unit += 8 * stride;  // at most 2^23 + 2^12 units
+      if (unit * (WAVES * STEP) >= end) return false;
+      const int row = (unit + (lane >> 3) * stride) * (WAVES * STEP) + wave * STEP + 4 * (lane & 7);
+      bool need = false;
+      if (row < end) {
+        const int4 p = __builtin_bit_cast(int4, gload16(q.positions + row));
+        need = (p.x >= lo && p.x <= hi) || (row + 1 < end && p.y >= lo && p.y <= hi) ||
+               (row + 2 < end && p.z >= lo && p.z <= hi) || (row + 3 < end && p.w >= lo && p.w <= hi);
+      }
+      bits = __ballot(need);
+    }
+    const int k = (__ffsll((unsigned long long)bits) - 1) >> 3;
+    bits &= ~(0xffull << (8 * k));
+    t0 = (unit + k * stride) * (WAVES * STEP) + wave * STEP;
+    return true;
+  }
+};
+
 // One workgroup of four waves takes a part of the cache rows of a (sequence,
 // head) for 16 query rows; its waves take steps in turn and join in LDS.
 // Bound by memory: eight sequences of 16k-131k rows (32/8 heads, one query,
@@ -260,12 +308,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_split_kernel(const Quant
   __shared__ float o_s[WAVES][16 * D];
   const ckv_quant_cache& c = a.cache;
   const int h = blockIdx.x % c.kv_heads, number = blockIdx.x / c.kv_heads, row0 = 16 * blockIdx.y;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, L = lane >> 4, col = lane & 15;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, L = lane >> 4, col = lane & 15;
   const Part part = find_part(c, a.parts, number, -1);
   const int b = part.sequence;
   if (b < 0) return;  // the join knows how many parts there are
   const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
-  const int lo_row = part.index * part.rows, hi_row = (int)min((int64_t)lo_row + part.rows, (int64_t)n);
   const QuantHead q = quant_head(c, b, h);
   const int block_log2 = 31 - __clz(c.block);
   QueryTile<DT> query;
@@ -280,7 +328,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_split_kernel(const Quant
   // with one new token and no window every row in use is at or before it
   const bool by_position = a.window > 0 || a.tokens > 1 || count < a.tokens;
   StepCodes cur;
-  for (int t0 = lo_row + wave * STEP; t0 < hi_row; t0 += WAVES * STEP) {
+  StepWalk walk(a, part, n, wave, row0, count, seen);
+  while (walk.next(a, q, wave)) {
+    const int t0 = walk.t0;
     load_step(q, t0, n - 1, block_log2, by_position, cur);
     const bool tail = t0 + STEP > n;
     bool fix_nan = false;
@@ -342,7 +392,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_split_kernel(const Quant
         acc += o_s[w][x] * f;
       }
       const int64_t bh = (int64_t)b * c.kv_heads + h;
-      if (a.parts == c.batch) {
+      if (part.count == 1) {
         int64_t at_out, at_lse;
         output_index(a, b, h, row, &at_out, &at_lse);
         store_out<DT>(a.out, at_out + d, sum == 0.0f ? 0.0f : acc / sum);
@@ -373,6 +423,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(const QuantAt
   const ckv_quant_cache& c = a.cache;
   const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const Part part = find_part(c, a.parts, 0, b);
+  if (part.count == 1) return;  // written already
   const float* pm = a.part_max + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
   const float* pl = a.part_sum + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
   float m = NEG_INF;
@@ -419,6 +470,50 @@ __global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(const QuantAt
   }
 }
 
+// The same for many query rows, of few parts mostly: a wave a row, two dims a lane
+// (702 queries in 3 parts, 28 heads: 14 us, a workgroup a row 38).
+template <int DT>
+__global__ __launch_bounds__(256) void attend_join_rows_kernel(const QuantAttendArgs a) {
+  const ckv_quant_cache& c = a.cache;
+  const int row = 4 * blockIdx.x + (threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
+  if (row >= a.rows) return;
+  const Part part = find_part(c, a.parts, 0, b);
+  if (part.count == 1) return;
+  const int64_t first = ((int64_t)h * a.row_pad + row) * a.parts + part.first;
+  float m = NEG_INF;
+  for (int s = lane; s < part.count; s += 64) m = fmaxf(m, a.part_max[first + s]);
+  m = wave_max(m);
+  const float at = m == NEG_INF ? 0.0f : m;
+  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.first) * a.row_pad + row) * D + 2 * lane;
+  float sum = 0.0f;
+  float2 acc{0.0f, 0.0f};
+  for (int s0 = 0; s0 < part.count; s0 += 64) {
+    const int left = min(part.count - s0, 64);
+    float f = 0.0f, share = 0.0f;
+    if (lane < left) {
+      f = __builtin_amdgcn_exp2f(a.part_max[first + s0 + lane] - at);
+      share = a.part_sum[first + s0 + lane] * f;
+    }
+    sum += wave_sum_tree(share);
+#pragma unroll 4
+    for (int s = 0; s < left; ++s) {
+      const float2 x = *reinterpret_cast<const float2*>(pa + (int64_t)(s0 + s) * a.row_pad * D);
+      const float of = ckv_u2f((uint32_t)__builtin_amdgcn_readlane((int)ckv_f2u(f), s));
+      acc.x += x.x * of;
+      acc.y += x.y * of;
+    }
+  }
+  int64_t at_out, at_lse;
+  output_index(a, b, h, row, &at_out, &at_lse);
+  store_out<DT>(a.out, at_out + 2 * lane, sum == 0.0f ? 0.0f : acc.x / sum);
+  store_out<DT>(a.out, at_out + 2 * lane + 1, sum == 0.0f ? 0.0f : acc.y / sum);
+  if (lane == 0) {
+    a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + __log2f(sum)) * LN2;
+    if (a.stats)
+      a.stats[((int64_t)b * c.kv_heads + h) * a.row_pad + row] = float2{at, sum == 0.0f ? 0.0f : 1.0f / sum};
+  }
+}
+
 // Received weight from the scores that the split kernel left (at most 16 query
 // rows a head): a thread adds up four cache rows over the query rows.  Writing
 // and reading 4 bytes a row and query costs less than the keys again.  A whole
@@ -434,6 +529,15 @@ __global__ __launch_bounds__(SUM_THREADS) void weights_of_scores_kernel(const Qu
   const int64_t r = 4 * ((int64_t)blockIdx.x * SUM_THREADS + threadIdx.x);
   if (r >= n) return;
   const int64_t bh = (int64_t)b * c.kv_heads + h;
+  const QuantHead q = quant_head(c, b, h);
+  if (a.window > 0) {  // scores were written only of steps with a row in sight
+    int lo, hi;
+    rows_range(a, 0, a.rows, new_count(a, b), c.cursors[c.batch + b], &lo, &hi);
+    const int4 p = __builtin_bit_cast(int4, gload16(q.positions + r));
+    const bool need = (p.x >= lo && p.x <= hi) || (r + 1 < n && p.y >= lo && p.y <= hi) ||
+                      (r + 2 < n && p.z >= lo && p.z <= hi) || (r + 3 < n && p.w >= lo && p.w <= hi);
+    if (!need) return;
+  }
   const float* from = a.scores + bh * a.rows * c.capacity + r;
   const float2* stats = a.stats + bh * a.row_pad;
   float got[4] = {};
@@ -445,7 +549,7 @@ __global__ __launch_bounds__(SUM_THREADS) void weights_of_scores_kernel(const Qu
 #pragma unroll
     for (int i = 0; i < 4; ++i) got[i] += v[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(v[i] - st.x) * st.y;
   }
-  float* to = quant_head(c, b, h).weights + r;
+  float* to = q.weights + r;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (r + i < n) to[i] += got[i];
@@ -464,6 +568,12 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendAr
   if (first >= n) return;
   const int t0 = (int)first;
   const QuantHead q = quant_head(c, b, h);
+  if (a.window > 0) {
+    int low, high;
+    rows_range(a, 0, a.rows, count, seen, &low, &high);
+    const int p = q.positions[min(t0 + (lane & 31), n - 1)];
+    if (__ballot(p >= low && p <= high) == 0) return;
+  }
   const bool by_position = a.window > 0 || a.tokens > 1 || count < a.tokens;
   StepCodes s;
   load_step<false>(q, t0, n - 1, 31 - __clz(c.block), by_position, s);
@@ -502,10 +612,13 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendAr
 // 10.4; replayed, 8 heads over 2).
 constexpr int ONE_PART_UNITS = 8;
 
-int parts_for(const ckv_quant_cache* c, int64_t row_blocks, int64_t workgroups, int64_t alone) {
+int parts_for(const ckv_quant_cache* c, int64_t row_blocks, bool many) {
+  const int64_t workgroups = many ? 256 : FEW_WORKGROUPS;
   const int64_t units = ((int64_t)c->capacity + PART_UNIT - 1) / PART_UNIT;
   const int64_t want = workgroups / ((int64_t)c->kv_heads * row_blocks);
-  if (want <= c->batch || units <= alone) return c->batch;
+  // many rows in fewer than two parts a sequence cost more in joins than they even out
+  // (8 prompts of 234 tokens, 28 heads over 4: whole 25 us, in 9 parts 120)
+  if (want < (many ? 2 * c->batch : c->batch + 1) || units <= (many ? 1 : ONE_PART_UNITS)) return c->batch;
   return (int)(want < c->batch * units ? want : c->batch * units);
 }
 
@@ -519,7 +632,7 @@ struct AttendLayout {
     row_pad = (rows + 15) / 16 * 16;
     many = rows > FEW_ROWS;
     const int64_t block = many ? many_row_block(dtype) : 16;
-    parts = parts_for(c, (rows + block - 1) / block, many ? 256 : FEW_WORKGROUPS, many ? 1 : ONE_PART_UNITS);
+    parts = parts_for(c, (rows + block - 1) / block, many);
     keep_scores = accumulate && rows <= 16;
     const size_t heads = (size_t)c->batch * c->kv_heads;
     size_t at = 0;
@@ -552,7 +665,8 @@ int launch_attend(const QuantAttendArgs& a, bool many, bool accumulate, hipStrea
     rc = launched("ckv_quant_attention");
   }
   if (!rc && a.parts > a.cache.batch) {
-    attend_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
+    if (many) attend_join_rows_kernel<DT><<<dim3((a.rows + 3) / 4, a.cache.kv_heads, a.cache.batch), 256, 0, s>>>(a);
+    else attend_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
     rc = launched("ckv_quant_attention");
   }
   if (!rc && accumulate) {

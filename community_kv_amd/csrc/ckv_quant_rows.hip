@@ -452,7 +452,7 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   if (row >= a.rows) return;
   const float sum = hi < 0 ? 0.0f : add_xor32(l);
   const float top = m == NEG_INF ? 0.0f : m * sl2;
-  if (a.parts > c.batch) {
+  if (part.count > 1) {
     float* acc = a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + row) * D;
 #pragma unroll
     for (int db = 0; db < 4; ++db) {

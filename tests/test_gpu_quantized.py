@@ -211,6 +211,32 @@ def test_attend_several_tokens(device, tokens, group, dtype, window):
                  counts=[tokens, 0, (tokens + 1) // 2])
 
 
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("tokens,dtype", [(1, torch.bfloat16), (4, torch.float16), (6, torch.float32), (30, torch.bfloat16)])
+def test_attend_window_over_long_caches(device, mixed, tokens, dtype):
+    """Most steps hold no row in sight and are passed over, in parts of one or several units; also where the window
+    begins or ends inside a step, with sequences that are shorter than it, empty or without a query."""
+    print(f"attend window mixed={mixed} tokens={tokens} dtype={dtype}", flush=True)
+    gen = torch.Generator().manual_seed(tokens + 100)
+    lengths = [4000, 2913, 35, 0, 1025]
+    cache = _fill(device, gen, batch=5, heads=1, capacity=4000, block=16, lengths=lengths, mixed=mixed)
+    counts = [tokens, 0, (tokens + 1) // 2, 0, tokens]
+    for window in (1, 33, 96, 1000):
+        _attend_case(device, gen, cache, group=4, tokens=tokens, dtype=dtype, window=window, accumulate=True,
+                     counts=counts, what=f"window {window}")
+    one = _fill(device, gen, batch=1, heads=8, capacity=9008, block=16, lengths=[9001], mixed=mixed)
+    _attend_case(device, gen, one, group=2, tokens=tokens, dtype=dtype, window=700, accumulate=True, what="one")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attend_parts_of_many_rows(device, dtype):
+    """Prompt rows in several parts, of sequences some of which are one part."""
+    gen = torch.Generator().manual_seed(31)
+    cache = _fill(device, gen, batch=3, heads=1, capacity=3200, block=64, lengths=[3200, 300, 90])
+    for counts in ([80, 80, 80], [80, 33, 0]):
+        _attend_case(device, gen, cache, group=1, tokens=80, dtype=dtype, accumulate=True, counts=counts)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attend_long_prompt_rows(device, dtype):
     """A whole prompt's queries at once (many row blocks, the causal diagonal)."""
