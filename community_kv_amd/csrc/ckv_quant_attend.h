@@ -86,11 +86,12 @@ __device__ inline int new_count(const QuantAttendArgs& a, int b) {
 }
 
 // The cache rows of all sequences in `parts` parts of nearly equal size, so that
-// every workgroup of a ragged batch has the same work: part size = the rows of
-// the batch over parts - batch (whole units), a sequence of n rows has
-// max(1, ceil(n / size)) parts, which together are at most `parts`.  With as
-// many parts as sequences each sequence is one part.  Every wave works this out
-// for itself, 64 sequences at a time.
+// every workgroup of a ragged batch has the same work: the least part size, in
+// whole units, with which the sequences' parts, max(1, ceil(n / size)) each, are
+// at most `parts` together.  The rows of the batch over parts is below it and
+// those over parts - batch above, between which it is searched for (up to 64
+// sequences; with more the upper one is taken).  With as many parts as sequences
+// each sequence is one part.  Every wave works this out for itself.
 struct Part {
   int sequence;    // -1: none
   int index;       // within the sequence
@@ -99,16 +100,36 @@ struct Part {
   int rows;        // rows of a part
 };
 
+__device__ inline int wave_sum_i32(int v) {
+  v += (int)xor_u32<1>((uint32_t)v);
+  v += (int)xor_u32<2>((uint32_t)v);
+  v += (int)xor_u32<4>((uint32_t)v);
+  v += (int)xor_u32<8>((uint32_t)v);
+  v += (int)xor_u32<16>((uint32_t)v);
+  return __builtin_amdgcn_readfirstlane(v + (int)xor_u32<32>((uint32_t)v));
+}
+
+// (No overflow: 2^31 units of codes would be 2^46 bytes.)
 __device__ inline int part_size(const ckv_quant_cache& c, int parts) {
   if (parts <= c.batch) return 0x7fffff80;
   const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int b0 = 0; b0 < c.batch; b0 += 64) total += b0 + lane < c.batch ? quant_length(c, b0 + lane) : 0;
-  for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
-  const int64_t spare = parts - c.batch;
-  const int64_t units = ((total + spare - 1) / spare + PART_UNIT - 1) / PART_UNIT;
-  // the same on every lane, and said so: what follows from it stays on the scalar unit
-  return __builtin_amdgcn_readfirstlane((int)min(max(units, (int64_t)1) * PART_UNIT, (int64_t)0x7fffff80));
+  int mine = 0, units = 0;
+  for (int b0 = 0; b0 < c.batch; b0 += 64) {
+    mine = b0 + lane < c.batch ? (quant_length(c, b0 + lane) + PART_UNIT - 1) / PART_UNIT : 0;
+    units += mine;
+  }
+  units = max(wave_sum_i32(units), 1);
+  uint32_t least = ((uint32_t)units + parts - 1) / (uint32_t)parts;
+  if (c.batch > 1) {
+    uint32_t most = ((uint32_t)units + parts - c.batch - 1) / (uint32_t)(parts - c.batch);
+    while (c.batch <= 64 && least < most) {
+      const uint32_t half = (least + most) / 2;
+      if (wave_sum_i32(lane < c.batch ? max((int)(((uint32_t)mine + half - 1) / half), 1) : 0) <= parts) most = half;
+      else least = half + 1;
+    }
+    least = most;
+  }
+  return (int)least * PART_UNIT;
 }
 
 __device__ inline int parts_of_sequence(int n, int size) { return n > size ? (n - 1) / size + 1 : 1; }

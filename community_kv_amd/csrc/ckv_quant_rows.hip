@@ -164,12 +164,16 @@ __device__ inline bool drop_nan_codes(uint32_t& w) {
   return is != 0;
 }
 
+constexpr int O_STRIDE = 64 + 4;     // floats of a row of 64 output dims: b128 writes of 16 rows hit distinct banks
+
 struct RowsLds {
   alignas(16) uint16_t k[2][K_TILE];
   alignas(16) uint16_t v[2][V_TILE];
   alignas(16) int32_t pos[2][KEYS];
   int nan[2];  // the tile, where its values held a NaN code that was staged as zero
 };
+
+static_assert(8 * 32 * O_STRIDE * sizeof(float) <= sizeof(RowsLds), "eight waves' output fits");
 
 template <int DT, int W>
 __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendArgs a) {
@@ -449,52 +453,69 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
     if (TURNS && !second && left == 0) __syncthreads();  // the second group's last slot
   }
 
-  if (row >= a.rows) return;
+  // The wave's rows go out through LDS (free by now), 64 dims at a time, so that
+  // whole lines are written: from the accumulators a store would touch 32 lines.
   const float sum = hi < 0 ? 0.0f : add_xor32(l);
   const float top = m == NEG_INF ? 0.0f : m * sl2;
-  if (part.count > 1) {
-    float* acc = a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + row) * D;
+  const bool joined = part.count > 1, none = joined ? hi < 0 : sum == 0.0f;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, factor = joined ? 1.0f : inv;
+  float* out_s = reinterpret_cast<float*>(lds_raw) + wave * 32 * O_STRIDE;
+  const int wave0 = block0 + 32 * wave;
 #pragma unroll
-    for (int db = 0; db < 4; ++db) {
+  for (int dims = 0; dims < 2; ++dims) {
+    asm volatile("" ::: "memory");
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<float4*>(acc + 32 * db + 8 * g + 4 * half) =
-            hi < 0 ? float4{0.0f, 0.0f, 0.0f, 0.0f}
-                   : float4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+    for (int i = 0; i < 8; ++i) {
+      const f32x16_t& x = o[2 * dims + (i >> 2)];
+      const int g = i & 3;
+      *reinterpret_cast<float4*>(&out_s[(lane & 31) * O_STRIDE + 32 * (i >> 2) + 8 * g + 4 * half]) =
+          none ? float4{0.0f, 0.0f, 0.0f, 0.0f}
+               : float4{x[4 * g] * factor, x[4 * g + 1] * factor, x[4 * g + 2] * factor, x[4 * g + 3] * factor};
     }
-    if (half == 0) {
-      a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m == NEG_INF || hi < 0 ? NEG_INF : top;
-      a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
+    asm volatile("" ::: "memory");  // a wave's own LDS operations stay in order
+    if (joined || DT == CKV_F32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int local = 4 * j + (lane >> 4), r = wave0 + local, dim = 64 * dims + 4 * (lane & 15);
+        const float4 x = *reinterpret_cast<const float4*>(&out_s[local * O_STRIDE + 4 * (lane & 15)]);
+        if (r >= a.rows) continue;
+        if (joined) {
+          *reinterpret_cast<float4*>(a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + r) * D + dim) = x;
+        } else {
+          int64_t at_out, at_lse;
+          output_index(a, b, h, r, &at_out, &at_lse);
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at_out + dim) = x;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int local = 8 * j + (lane >> 3), r = wave0 + local, dim = 64 * dims + 8 * (lane & 7);
+        const float* from = &out_s[local * O_STRIDE + 8 * (lane & 7)];
+        const float4 x = *reinterpret_cast<const float4*>(from), y = *reinterpret_cast<const float4*>(from + 4);
+        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = DT == CKV_BF16 ? pack_bf16x2_hw(v[2 * e], v[2 * e + 1])
+                                : (uint32_t)f16_bits_hw(v[2 * e]) | ((uint32_t)f16_bits_hw(v[2 * e + 1]) << 16);
+        if (r >= a.rows) continue;
+        int64_t at_out, at_lse;
+        output_index(a, b, h, r, &at_out, &at_lse);
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at_out + dim) = uint4{w[0], w[1], w[2], w[3]};
+      }
     }
+  }
+  if (half != 0 || row >= a.rows) return;
+  if (joined) {
+    a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m == NEG_INF || hi < 0 ? NEG_INF : top;
+    a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
     return;
   }
   int64_t at_out, at_lse;
   output_index(a, b, h, row, &at_out, &at_lse);
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-  for (int db = 0; db < 4; ++db) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int64_t at = at_out + 32 * db + 8 * g + 4 * half;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = sum == 0.0f ? 0.0f : o[db][4 * g + e] * inv;
-      if constexpr (DT == CKV_F32) {
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at) = float4{v[0], v[1], v[2], v[3]};
-      } else {
-        uint32_t w[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          w[e] = DT == CKV_BF16 ? pack_bf16x2_hw(v[2 * e], v[2 * e + 1])
-                                : (uint32_t)f16_bits_hw(v[2 * e]) | ((uint32_t)f16_bits_hw(v[2 * e + 1]) << 16);
-        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at) = uint2{w[0], w[1]};
-      }
-    }
-  }
-  if (half == 0) {
-    a.lse[at_lse] = sum == 0.0f ? NEG_INF : (top + __log2f(sum)) * LN2;
-    if (a.stats) a.stats[(int64_t)bh * a.row_pad + row] = float2{top, inv};
-  }
+  a.lse[at_lse] = sum == 0.0f ? NEG_INF : (top + __log2f(sum)) * LN2;
+  if (a.stats) a.stats[(int64_t)bh * a.row_pad + row] = float2{top, inv};
 }
 
 template <int DT>
