@@ -152,6 +152,8 @@ class QuantizedKVCache:
         """Takes back the newest ``counts`` tokens of every sequence (rejected
         draft tokens): at most those appended since the last eviction.  Block
         scales stay as they have grown."""
+        if isinstance(counts, int) and counts < 0:
+            raise ValueError("counts must be non-negative")
         self.cursors[:2].sub_(counts)
 
     def dequantize(self) -> tuple[torch.Tensor, torch.Tensor]:

@@ -21,6 +21,7 @@ attention function of this kind); ragged batches call ``quantized_append`` and
 
 from __future__ import annotations
 
+import weakref
 from typing import Any
 
 import torch
@@ -50,6 +51,7 @@ class QuantizedCacheLayer(CacheLayerMixin):
         self.store: QuantizedKVCache | None = None
         self.rows = 0  # in the cache
         self.seen = 0  # ever written: the next token's position
+        self._latest: Any = None  # the keys written last, to tell a call with another cache's keys
 
     # -- Hugging Face cache-layer protocol ----------------------------------
 
@@ -73,6 +75,7 @@ class QuantizedCacheLayer(CacheLayerMixin):
         quantized_append(self.store, key_states, value_states)
         self.rows += tokens
         self.seen += tokens
+        self._latest = weakref.ref(key_states)
         return key_states, value_states
 
     def get_mask_sizes(self, query_length: int, *args: object, **kwargs: object) -> tuple[int, int]:
@@ -88,6 +91,7 @@ class QuantizedCacheLayer(CacheLayerMixin):
         if self.store is not None:
             self.store.reset()
         self.rows = self.seen = 0
+        self._latest = None
 
     def crop(self, max_length: int) -> None:
         """Takes back the newest tokens, down to ``max_length`` (or by ``-max_length``)."""
@@ -110,11 +114,13 @@ class QuantizedCacheLayer(CacheLayerMixin):
 
     # -- attention -----------------------------------------------------------
 
-    def attend(self, query: torch.Tensor, scaling: float, window: int = 0) -> torch.Tensor:
-        """Attention of the queries of the tokens written last, then the
-        eviction where the layer holds more than its budget and slack."""
-        if self.store is None or query.shape[2] > self.rows:
-            raise RuntimeError("attention needs its tokens in the cache first")
+    def attend(self, query: torch.Tensor, key: torch.Tensor, scaling: float, window: int = 0) -> torch.Tensor:
+        """Attention of the queries of the tokens written last, whose keys are
+        ``key`` as ``update`` returned them, then the eviction where the layer
+        holds more than its budget and slack."""
+        if self.store is None or self._latest is None or self._latest() is not key or query.shape[2] != key.shape[2]:
+            raise RuntimeError("the tokens of this call were not written into this cache: pass the cache that the "
+                               "attention function was registered with as past_key_values")
         out, _ = quantized_attention(query, self.store, softmax_scale=scaling, window=window,
                                      accumulate=self.budget > 0)
         if self.budget and self.rows > self.budget + self.slack:
@@ -139,7 +145,9 @@ class QuantizedCache(Cache):
 
 
 class QuantizedCacheAttention:
-    """The attention function of a model whose cache is ``cache``."""
+    """The attention function of a model whose cache is ``cache``.  One
+    function is registered at a time; a model that runs with another cache than
+    the one registered last is told so (``RuntimeError``)."""
 
     IMPL_NAME = QUANTIZED_ATTENTION_IMPLEMENTATION
 
@@ -165,7 +173,7 @@ class QuantizedCacheAttention:
             if kwargs.get(name) is not None:
                 raise ValueError(f"attention over the 8-bit cache does not support {name}")
         layer = self.cache.layer(int(module.layer_idx))
-        return layer.attend(query, float(scaling), int(kwargs.get("sliding_window") or 0)), None
+        return layer.attend(query, key, float(scaling), int(kwargs.get("sliding_window") or 0)), None
 
 
 __all__ = ["QUANTIZED_ATTENTION_IMPLEMENTATION", "QuantizedCache", "QuantizedCacheAttention", "QuantizedCacheLayer"]

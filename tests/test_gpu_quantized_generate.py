@@ -95,3 +95,18 @@ def test_prompt_in_pieces_and_crop(device):
     for other in logits[1:]:
         # a query's output does not depend on the others of its call but for the order of 32-bit sums
         assert (other - logits[0]).abs().max() <= 1e-3 * logits[0].abs().max()
+
+
+def test_another_cache_is_refused(device):
+    """Two caches, one registered function: a model run with the other cache, or with none, raises."""
+    model = _model(device)
+    prompt = torch.randint(0, 512, (1, 20), generator=torch.Generator().manual_seed(3)).to(device)
+    caches = [QuantizedCache(num_hidden_layers=LAYERS, max_cache_len=64) for _ in range(2)]
+    for cache in caches:
+        model.set_attn_implementation(QuantizedCacheAttention(cache).register())
+    with torch.no_grad():
+        model(prompt, past_key_values=caches[1], use_cache=True)
+        with pytest.raises(RuntimeError, match="not written into this cache"):
+            model(prompt, past_key_values=caches[0], use_cache=True)
+        with pytest.raises(RuntimeError, match="not written into this cache"):
+            model(prompt, use_cache=False)

@@ -41,6 +41,8 @@ def test_reset_rewind_overflow_flag():
     cache.cursors.copy_(torch.tensor([[7, 5], [9, 5], [0, 0]], dtype=torch.int32))
     cache.rewind(torch.tensor([2, 0], dtype=torch.int32))
     cache.rewind(1)
+    with pytest.raises(ValueError):
+        cache.rewind(-1)
     assert cache.cursors.tolist() == [[4, 4], [6, 4], [0, 0]]
     cache.assert_no_overflow()
     cache.cursors[2, 1] = 1
@@ -242,8 +244,8 @@ def test_cache_layer_protocol():
     with pytest.raises(RuntimeError, match="GPU only"):
         cache.update(x[:, :, :3], x[:, :, :3], 1)
     assert layer.seen == 0 and layer.rows == 0
-    with pytest.raises(RuntimeError, match="in the cache first"):
-        layer.attend(x[:, :, :1], 1.0)
+    with pytest.raises(RuntimeError, match="not written into this cache"):
+        layer.attend(x[:, :, :1], x[:, :, :1], 1.0)
     with pytest.raises(NotImplementedError):
         layer.reorder_cache(torch.zeros(1, dtype=torch.long))
     with pytest.raises(NotImplementedError):
