@@ -260,9 +260,9 @@ __device__ inline uint32_t evict_key(float w, bool is_protected) {
 // One workgroup a (sequence, head) selects where its threads hold all keys, and
 // several where they do not.  A whole eviction of 8 heads, half the rows kept, in a
 // graph: capacity 1,000 13.6 us with 256 threads of 8 keys, 14.4 with 1,024 (their
-// barriers), 28.5 with several workgroups (the launches); 8,000 17.3 with 1,024
-// threads of 8 keys, 32.6; 12,000 24.0 with 1,024 of 16, 35.7; 16,300 27.9, 38.3;
-// 32 keys a thread, 32,000 48.9, 43.4.
+// barriers), 25.2 with several workgroups (the launches); 8,000 17.2 with 1,024
+// threads of 8 keys, 28.8; 12,000 23.9 with 1,024 of 16, 32.3; 16,300 27.8, 34.8;
+// 32,000 48.9 with 32 keys a thread, 40.2.
 constexpr int SELECT_FEW = 256, SELECT_MANY = 1024;
 constexpr int KEYS_FEW = 8, KEYS_MANY = 16;
 
