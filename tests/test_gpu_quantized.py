@@ -634,3 +634,49 @@ def test_same_call_twice_is_bit_equal(device):
     torch.cuda.synchronize()
     for a, b in zip(*seen):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("tokens,window,capacity,dtype", [(1, 200, 4096, torch.bfloat16), (9, 0, 20_480, torch.float16),
+                                                          (40, 300, 12_288, torch.float32),
+                                                          (130, 0, 2048, torch.bfloat16)])
+def test_replays_equal_eager_calls(device, tokens, window, capacity, dtype):
+    """Every form of the kernels captured: an append, attention with received weights and an eviction, replayed with
+    eager work of other caches between, against the same calls made eagerly; two graphs of one cache in turn."""
+    print(f"replay tokens={tokens} window={window} capacity={capacity}", flush=True)
+    gen = torch.Generator().manual_seed(capacity)
+    full = capacity - tokens - 3
+    caches = [_fill(device, torch.Generator().manual_seed(capacity), batch=2, heads=2, capacity=capacity, block=64,
+                    lengths=[full, full - 500]) for _ in range(2)]
+    key, value, query = (_rows(gen, 2, heads, tokens, dtype=dtype).to(device) for heads in (2, 2, 8))
+    other = _fill(device, gen, batch=1, heads=2, capacity=320, block=32, lengths=[300])
+
+    def step(cache):
+        quantized_append(cache, key, value)
+        out, lse = quantized_attention(query, cache, softmax_scale=SCALE, window=window, accumulate=True)
+        evict(cache, keep=full - 700, num_sink=2, recent=tokens + 5)
+        return out, lse
+
+    def drawn():
+        for x in (key, value, query):
+            x.copy_(_rows(gen, *x.shape[:3], dtype=dtype))
+
+    warm = torch.cuda.Stream(device)
+    warm.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(warm):
+        step(caches[0])
+    torch.cuda.current_stream(device).wait_stream(warm)
+    step(caches[1])
+    graphs, results = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            results.append(step(caches[0]))
+    for i in range(6):
+        drawn()
+        graphs[i % 2].replay()
+        quantized_attention(query[:1, :, :1], other, softmax_scale=SCALE, accumulate=True)
+        want = step(caches[1])
+        torch.cuda.synchronize()
+        for got, eager in zip(results[i % 2], want):
+            assert torch.equal(got, eager), i
+        _same(caches[0], oq.Cache.of(caches[1]), f"replay {i}")
