@@ -195,13 +195,24 @@ __device__ inline void output_index(const QuantAttendArgs& a, int b, int h, int 
   *lse = ((int64_t)b * heads + hq) * a.tokens + t;
 }
 
-// More query rows than this a head go to the many-row kernels (64 or 128 of them a
-// workgroup, where the few-row kernel takes 16 and reads the cache for each 16).
-// 32 heads over 8, in a graph, over 2,000 and 16,000 rows: 64 query rows 17.7 and
-// 41.2 us with few, 22.9 and 37.3 with many (bf16), 19.6 and 44.6, 27.1 and 48.0
-// (f32); 96 query rows 18.7 and 56, 24.5 and 39.3 (bf16), 20.5 and 61, 29.2 and
-// 49.4 (f32).
-constexpr int FEW_ROWS = 64;
+// Which query rows of a head go to the many-row kernels (128 or 256 of them a
+// workgroup): the few-row kernel takes 16 a workgroup and reads the cache for each
+// 16, but starts sooner.  It has all calls of up to 32 rows (bf16; 64 with two or
+// three pieces, whose many-row kernel is slower), and those whose cache rows, over
+// all heads and blocks of 16 query rows, are at most FEW_WORK; with received
+// weights only up to 128 query rows, beyond which their own kernels decide.
+// 32/8 heads, in a graph, few and many, us: 1 sequence of 1,000 rows, bf16, 128
+// query rows 19.9 and 22.0, 512 rows 20.4 and 29.5; 4,000 rows: 22.4 and 35.3, 52.1
+// and 41.1; 16,000 rows, 64 query rows 31.1 and 40.1, 128 rows 49.3 and 42.2; 8
+// sequences of 16,000 rows: 32 query rows 92 and 135, 64 rows 167 and 141 (f32: 192
+// and 259).  With weights, 1,000 rows: 128 query rows 34.6 and 32.4, 512 rows 61 and
+// 41.
+constexpr int64_t FEW_WORK = 720000;
+inline bool many_rows(const ckv_quant_cache* c, int rows, int dtype, bool accumulate) {
+  if (rows <= (dtype == CKV_BF16 ? 32 : 64)) return false;
+  if (accumulate && rows > 128) return true;
+  return (int64_t)c->batch * c->kv_heads * ((rows + 15) / 16) * c->capacity > FEW_WORK;
+}
 
 // Host-side launchers of the many-row kernels (ckv_quant_rows.hip).
 int launch_many_rows(const QuantAttendArgs& a, int dtype, hipStream_t stream);

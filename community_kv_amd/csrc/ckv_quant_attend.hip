@@ -606,11 +606,12 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendAr
 
 // Parts that the cache rows of the batch are split into: enough workgroups to
 // fill the chip (`workgroups`), no more than there are units.  A few units are
-// left in one part, which needs no join: with one query a sequence and up to
-// eight units (1,024 rows) one part takes 5.5, 6.8 and 9.6 us at 256, 512 and
-// 1,024 rows where parts and their join take 10.2 to 10.4 (2,048 rows: 15.1 and
-// 10.4; replayed, 8 heads over 2).
-constexpr int ONE_PART_UNITS = 8;
+// left in one part, which needs no join.  2 sequences, 32/8 heads, bf16, in a graph,
+// one part and several, us: up to 400 rows in 4 units 8.3 and 10.4 with 4 query
+// rows, 12.5 and 12.2 with 16, 12.7 and 16.9 with 128; 640 rows in 7 units 8.6 and
+// 10.0, 14.7 and 12.3, 15.1 and 18.2; 1,000 rows in 8 units 11.6 and 10.7, 19.7 and
+// 12.3, 20.2 and 19.2.
+constexpr int ONE_PART_UNITS = 6;
 
 int parts_for(const ckv_quant_cache* c, int64_t row_blocks, bool many) {
   const int64_t workgroups = many ? 256 : FEW_WORKGROUPS;
@@ -630,7 +631,7 @@ struct AttendLayout {
   size_t stats, ranges, scores, sums, max, sum, acc, bytes;
   AttendLayout(const ckv_quant_cache* c, int rows, int dtype, bool accumulate) {
     row_pad = (rows + 15) / 16 * 16;
-    many = rows > FEW_ROWS;
+    many = many_rows(c, rows, dtype, accumulate);
     const int64_t block = many ? many_row_block(dtype) : 16;
     parts = parts_for(c, (rows + block - 1) / block, many);
     keep_scores = accumulate && rows <= 16;
