@@ -211,6 +211,35 @@ def test_attend_several_tokens(device, tokens, group, dtype, window):
                  counts=[tokens, 0, (tokens + 1) // 2])
 
 
+@pytest.mark.parametrize("tokens,group,dtype", [(33, 2, torch.float16), (40, 5, torch.bfloat16), (80, 1, torch.bfloat16),
+                                                (30, 7, torch.float32)])
+@pytest.mark.parametrize("window", [0, 1, 37, 2**31 - 1])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_attend_many_rows_of_a_large_cache(device, tokens, group, dtype, window, accumulate):
+    """Short sequences in a large cache, whose capacity alone sends the calls to the many-row kernels."""
+    gen = torch.Generator().manual_seed(tokens + 7)
+    print(f"attend many rows tokens={tokens} group={group} dtype={dtype} window={window}", flush=True)
+    cache = _fill(device, gen, batch=3, heads=2, capacity=24_064, block=32, lengths=[tokens, 100 + tokens, 290])
+    for counts in (None, [tokens, 0, (tokens + 1) // 2]):
+        _attend_case(device, gen, cache, group=group, tokens=tokens, dtype=dtype, window=window, accumulate=accumulate,
+                     counts=counts)
+
+
+def test_attend_same_rows_in_a_small_and_a_large_cache(device):
+    """The kernels that a call goes to depend on the capacity: their results agree within the roundings of both."""
+    gen = torch.Generator().manual_seed(40)
+    key, value, query = (_rows(gen, 1, heads, 260) for heads in (2, 2, 8))
+    seen = []
+    for capacity in (320, 65_536):
+        cache = QuantizedKVCache.allocate(kv_heads=2, capacity=capacity, block=32, device=device)
+        quantized_append(cache, key.to(device), value.to(device))
+        seen.append(quantized_attention(query.to(device), cache, softmax_scale=SCALE))
+    torch.cuda.synchronize()
+    # both are within the oracle's bound (test_attend_several_tokens), here 2^-16 of values up to 5 at the least
+    assert (seen[0][0] - seen[1][0]).abs().max() <= 2 * 5 * 2.0 ** -16
+    assert (seen[0][1] - seen[1][1]).abs().max() <= 2 * 10 * 2.0 ** -16
+
+
 @pytest.mark.parametrize("mixed", [False, True])
 @pytest.mark.parametrize("tokens,dtype", [(1, torch.bfloat16), (4, torch.float16), (6, torch.float32), (30, torch.bfloat16)])
 def test_attend_window_over_long_caches(device, mixed, tokens, dtype):
@@ -259,10 +288,11 @@ def test_attend_many_sequences(device):
 
 @pytest.mark.parametrize("group,tokens,dtype", [(2, 3, torch.bfloat16), (4, 12, torch.bfloat16), (5, 40, torch.bfloat16),
                                                 (4, 20, torch.float32)])
-def test_attend_padded_queries_hold_anything(device, group, tokens, dtype):
+@pytest.mark.parametrize("capacity", [320, 65_536])  # few-row kernels, many-row ones
+def test_attend_padded_queries_hold_anything(device, group, tokens, dtype, capacity):
     """Queries past a sequence's count, NaN here, touch neither the others' outputs nor the received weights."""
     gen = torch.Generator().manual_seed(16)
-    cache = _fill(device, gen, batch=2, heads=2, capacity=320, block=64, lengths=[300, 129])
+    cache = _fill(device, gen, batch=2, heads=2, capacity=capacity, block=64, lengths=[300, 129])
     query = _rows(gen, 2, 2 * group, tokens, dtype=dtype)
     counts = [tokens - 1, tokens // 2]
     weights = cache.weights.clone()
@@ -288,11 +318,12 @@ def test_attend_window_leaves_rows_empty(device):
 
 @pytest.mark.parametrize("group,tokens,dtype", [(2, 4, torch.bfloat16), (16, 20, torch.bfloat16),
                                                 (5, 30, torch.float32)])
-def test_attend_ignores_nan_in_masked_rows(device, group, tokens, dtype):
+@pytest.mark.parametrize("capacity", [192, 131_072])
+def test_attend_ignores_nan_in_masked_rows(device, group, tokens, dtype, capacity):
     """NaN keys and values at masked positions and past the length change nothing; a NaN value that a query does
     see makes that query's dim NaN, and a NaN key the whole query.  Few query rows, and many."""
     gen = torch.Generator().manual_seed(10)
-    cache = _fill(device, gen, batch=1, heads=1, capacity=192, block=32, lengths=[100], mixed=False)
+    cache = _fill(device, gen, batch=1, heads=1, capacity=capacity, block=32, lengths=[100], mixed=False)
     query = _rows(gen, 1, group, tokens, dtype=dtype)
     last = tokens - 2  # queries from here on see position 98
     clean, clean_lse = quantized_attention(query.to(device), cache, softmax_scale=SCALE)
@@ -302,7 +333,7 @@ def test_attend_ignores_nan_in_masked_rows(device, group, tokens, dtype):
     torch.cuda.synchronize()
     assert torch.equal(got[:, :last], clean[:, :last]) and torch.equal(got_lse[..., :last], clean_lse[..., :last])
     assert bool(got[:, last:].isnan().all()) and bool(got_lse[..., last:].isnan().all())
-    cache = _fill(device, gen, batch=1, heads=1, capacity=192, block=32, lengths=[100], mixed=False)
+    cache = _fill(device, gen, batch=1, heads=1, capacity=capacity, block=32, lengths=[100], mixed=False)
     clean, _ = quantized_attention(query.to(device), cache, softmax_scale=SCALE)
     cache.value_codes.view(torch.uint8)[0, 0, 98, 5] = 0xFF
     cache.value_codes.view(torch.uint8)[0, 0, 7, 77] = 0x7F
