@@ -246,6 +246,44 @@ __device__ inline void add_step(const float* sc, float vs, const uint4* vop, boo
   }
 }
 
+// Received weight from the scores that the split kernel left (at most 16 query
+// rows a head): a thread adds up the four cache rows from r on over the query rows.
+// Writing and reading 4 bytes a row and query costs less than the keys again.  A
+// whole call, 2 sequences of 16,000 rows, 32 heads over 8: 4 query rows a head 27.4
+// us from kept scores and 36.4 with them computed again (weights_kernel), 16 rows
+// 35.9 and 44.0; 2,000 rows: 16.3 and 18.1, 21.2 and 21.2.  With more query rows
+// the kept scores would outgrow the cache itself (64 rows: 256 bytes a cache row).
+__device__ inline void add_scores(const QuantAttendArgs& a, int b, int h, int64_t r) {
+  const ckv_quant_cache& c = a.cache;
+  const int n = quant_length(c, b);
+  if (r >= n) return;
+  const int64_t bh = (int64_t)b * c.kv_heads + h;
+  const QuantHead q = quant_head(c, b, h);
+  if (a.window > 0) {  // scores were written only of steps with a row in sight
+    int lo, hi;
+    rows_range(a, 0, a.rows, new_count(a, b), c.cursors[c.batch + b], &lo, &hi);
+    const int4 p = __builtin_bit_cast(int4, gload16(q.positions + r));
+    const bool need = (p.x >= lo && p.x <= hi) || (r + 1 < n && p.y >= lo && p.y <= hi) ||
+                      (r + 2 < n && p.z >= lo && p.z <= hi) || (r + 3 < n && p.w >= lo && p.w <= hi);
+    if (!need) return;
+  }
+  const float* from = a.scores + bh * a.rows * c.capacity + r;
+  const float2* stats = a.stats + bh * a.row_pad;
+  float got[4] = {};
+#pragma unroll 4
+  for (int row = 0; row < a.rows; ++row) {
+    const float4 s = *reinterpret_cast<const float4*>(from + (int64_t)row * c.capacity);
+    const float2 st = stats[row];
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) got[i] += v[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(v[i] - st.x) * st.y;
+  }
+  float* to = q.weights + r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (r + i < n) to[i] += got[i];
+}
+
 // Goes over this wave's steps of a part.  Without a window: the part's rows, STEP
 // of every WAVES * STEP.  With one most rows are out of every query's sight, and
 // those in it mostly stand together: a part is then every count-th unit of
@@ -301,7 +339,10 @@ struct StepWalk {
 // waves a SIMD: 1,024 and 2,048 workgroups take 3 and 8 % longer there and 9 and
 // 20 % at one sequence of 131k; three waves a SIMD (168 registers) the same or
 // longer, reading a step ahead into a second set of registers the same.
-template <int DT>
+// SUMS: every sequence is one part and the scores are kept, so that the workgroup
+// adds up the received weights itself and no launch has to (8 sequences of 300 rows
+// 11.6 us, with a launch 12.5; 64 of 600 21.9 and 23.8).
+template <int DT, bool SUMS>
 __global__ __launch_bounds__(64 * WAVES, 2) void attend_split_kernel(const QuantAttendArgs a) {
   __shared__ float m_s[WAVES][16];
   __shared__ float l_s[WAVES][16];
@@ -409,6 +450,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_split_kernel(const Quant
       }
     }
   }
+  if constexpr (SUMS) {
+    __syncthreads();  // the scores and statistics are written
+    for (int64_t r = 4 * tid; r < n; r += 4 * 64 * WAVES) add_scores(a, b, h, r);
+  }
 }
 
 // Joins the parts of one query row: a workgroup of 256 threads, a part each for
@@ -514,45 +559,9 @@ __global__ __launch_bounds__(256) void attend_join_rows_kernel(const QuantAttend
   }
 }
 
-// Received weight from the scores that the split kernel left (at most 16 query
-// rows a head): a thread adds up four cache rows over the query rows.  Writing
-// and reading 4 bytes a row and query costs less than the keys again.  A whole
-// call, 2 sequences of 16,000 rows, 32 heads over 8: 4 query rows a head 27.4 us
-// from kept scores and 36.4 with them computed again (weights_kernel), 16 rows
-// 35.9 and 44.0; 2,000 rows: 16.3 and 18.1, 21.2 and 21.2.  With more query rows
-// the kept scores would outgrow the cache itself (64 rows: 256 bytes a cache row).
 constexpr int SUM_THREADS = 64;
 __global__ __launch_bounds__(SUM_THREADS) void weights_of_scores_kernel(const QuantAttendArgs a) {
-  const ckv_quant_cache& c = a.cache;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int n = quant_length(c, b);
-  const int64_t r = 4 * ((int64_t)blockIdx.x * SUM_THREADS + threadIdx.x);
-  if (r >= n) return;
-  const int64_t bh = (int64_t)b * c.kv_heads + h;
-  const QuantHead q = quant_head(c, b, h);
-  if (a.window > 0) {  // scores were written only of steps with a row in sight
-    int lo, hi;
-    rows_range(a, 0, a.rows, new_count(a, b), c.cursors[c.batch + b], &lo, &hi);
-    const int4 p = __builtin_bit_cast(int4, gload16(q.positions + r));
-    const bool need = (p.x >= lo && p.x <= hi) || (r + 1 < n && p.y >= lo && p.y <= hi) ||
-                      (r + 2 < n && p.z >= lo && p.z <= hi) || (r + 3 < n && p.w >= lo && p.w <= hi);
-    if (!need) return;
-  }
-  const float* from = a.scores + bh * a.rows * c.capacity + r;
-  const float2* stats = a.stats + bh * a.row_pad;
-  float got[4] = {};
-#pragma unroll 4
-  for (int row = 0; row < a.rows; ++row) {
-    const float4 s = *reinterpret_cast<const float4*>(from + (int64_t)row * c.capacity);
-    const float2 st = stats[row];
-    const float v[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) got[i] += v[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(v[i] - st.x) * st.y;
-  }
-  float* to = q.weights + r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (r + i < n) to[i] += got[i];
+  add_scores(a, blockIdx.z, blockIdx.y, 4 * ((int64_t)blockIdx.x * SUM_THREADS + threadIdx.x));
 }
 
 // Received weight: a wave owns 32 cache rows of a (sequence, head), goes over
@@ -662,7 +671,8 @@ int launch_attend(const QuantAttendArgs& a, bool many, bool accumulate, hipStrea
     rc = launch_many_rows(a, DT, s);
   } else {
     const dim3 grid(a.parts * a.cache.kv_heads, (a.rows + 15) / 16);
-    attend_split_kernel<DT><<<grid, 64 * WAVES, 0, s>>>(a);
+    if (a.scores && a.parts == a.cache.batch) attend_split_kernel<DT, true><<<grid, 64 * WAVES, 0, s>>>(a);
+    else attend_split_kernel<DT, false><<<grid, 64 * WAVES, 0, s>>>(a);
     rc = launched("ckv_quant_attention");
   }
   if (!rc && a.parts > a.cache.batch) {
@@ -673,6 +683,7 @@ int launch_attend(const QuantAttendArgs& a, bool many, bool accumulate, hipStrea
   if (!rc && accumulate) {
     if (many) return launch_many_rows_weights(a, DT, s);
     if (a.scores) {
+      if (a.parts == a.cache.batch) return rc;  // added by the attention itself
       const dim3 grid((a.cache.capacity + 4 * SUM_THREADS - 1) / (4 * SUM_THREADS), a.cache.kv_heads, a.cache.batch);
       weights_of_scores_kernel<<<grid, SUM_THREADS, 0, s>>>(a);
       return launched("ckv_quant_attention");
