@@ -94,8 +94,9 @@ class QuantizedCacheLayer(CacheLayerMixin):
         self._latest = None
 
     def crop(self, max_length: int) -> None:
-        """Takes back the newest tokens, down to ``max_length`` (or by ``-max_length``)."""
-        drop = self.seen - max_length if max_length >= 0 else -max_length
+        """Takes back the newest tokens, down to a positive ``max_length``, else ``-max_length`` of them (0: none,
+        what assisted generation asks for where every candidate was right)."""
+        drop = self.seen - max_length if max_length > 0 else -max_length
         if drop <= 0:
             return
         if drop > self.rows or (self.budget and self.seen != self.rows):

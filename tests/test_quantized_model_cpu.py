@@ -1,0 +1,111 @@
+"""A transformers model on the 8-bit cache without a GPU: the oracle stands in for the operators, so that what is
+tested is how the cache and the attention function meet the library's generation, masks and cache protocol."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from community_kv_amd import QuantizedCache, QuantizedCacheAttention
+from community_kv_amd.attention import quantized_cache
+from oracle import quantized as oq
+
+LAYERS = 2
+
+
+def _store(oracle, cache):
+    for i, (codes, scales) in enumerate(((cache.key_codes, cache.key_scales), (cache.value_codes, cache.value_scales))):
+        codes.view(torch.uint8).copy_(torch.from_numpy(oracle.codes[i]))
+        scales.copy_(torch.from_numpy(oracle.scales[i]))
+    cache.positions.copy_(torch.from_numpy(oracle.positions))
+    cache.cursors.copy_(torch.from_numpy(oracle.cursors))
+    if cache.weights is not None:
+        cache.weights.copy_(torch.from_numpy(oracle.weights))
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """The operators that the cache calls, as the oracle computes them."""
+
+    def append(cache, key, value):
+        oracle = oq.Cache.of(cache)
+        oracle.append(key.double().numpy(), value.double().numpy())
+        _store(oracle, cache)
+
+    def attention(query, cache, *, softmax_scale, window=0, accumulate=False):
+        (out, lse, got), _ = oq.Cache.of(cache).attend(query.double().numpy(), scale=softmax_scale, window=window)
+        if accumulate:
+            cache.weights.add_(torch.from_numpy(got.astype(np.float32)))
+        return torch.from_numpy(out).to(query.dtype), torch.from_numpy(lse).float()
+
+    def evict(cache, **kwargs):
+        oracle = oq.Cache.of(cache)
+        oracle.evict(**kwargs)
+        _store(oracle, cache)
+
+    monkeypatch.setattr(quantized_cache, "quantized_append", append)
+    monkeypatch.setattr(quantized_cache, "quantized_attention", attention)
+    monkeypatch.setattr(quantized_cache, "evict", evict)
+
+
+def _model(**change):
+    from transformers import Qwen3Config, Qwen3ForCausalLM
+
+    cfg = Qwen3Config(**(dict(vocab_size=64, hidden_size=128, intermediate_size=128, num_hidden_layers=LAYERS,
+                              num_attention_heads=2, num_key_value_heads=1, head_dim=128, max_position_embeddings=512,
+                              tie_word_embeddings=False) | change))
+    torch.manual_seed(0)
+    return Qwen3ForCausalLM(cfg).eval()
+
+
+def _on_cache(model, **kwargs):
+    cache = QuantizedCache(**(dict(num_hidden_layers=LAYERS, max_cache_len=96, block=16) | kwargs))
+    model.set_attn_implementation(QuantizedCacheAttention(cache).register())
+    return cache
+
+
+def _prompt(n, seed=1):
+    return torch.randint(0, 64, (1, n), generator=torch.Generator().manual_seed(seed))
+
+
+# ------------------------------------------------------------------------------------------ tokens taken back
+
+def test_crop_by_nothing_keeps_all(on_cpu):
+    """crop(0) takes nothing back, as the library's own cache, and crop(-n) the newest n."""
+    from transformers import DynamicCache
+
+    cache, dynamic = _on_cache(_model()), DynamicCache()
+    x = torch.randn(1, 1, 20, 128)
+    for layer in range(LAYERS):
+        cache.update(x, x, layer)
+        dynamic.update(x, x, layer)
+    for n, left in ((0, 20), (-4, 16), (0, 16)):
+        cache.crop(n)
+        dynamic.crop(n)
+        assert cache.get_seq_length() == dynamic.get_seq_length() == left
+        for layer in range(LAYERS):
+            assert cache.layer(layer).store.cursors.tolist() == [[left], [left], [0]]
+
+
+def test_assisted_generation(on_cpu):
+    """Prompt-lookup generation takes rejected candidates back after every verification, none where all were right,
+    and gives the tokens of plain greedy generation."""
+    model = _model()
+    prompt = torch.cat([_prompt(6), _prompt(6), _prompt(4)], 1)
+    taken = []
+
+    def generate(**kwargs):
+        cache = _on_cache(model)
+        crop = cache.crop
+        cache.crop = lambda n: (taken.append(n), crop(n))
+        out = model.generate(prompt, past_key_values=cache, max_new_tokens=24, do_sample=False, **kwargs)
+        for layer in range(LAYERS):
+            assert cache.layer(layer).rows == cache.layer(layer).seen == out.shape[1] - 1
+            assert cache.layer(layer).store.lengths.tolist() == [out.shape[1] - 1]
+        return out
+
+    plain = generate()
+    assert not taken
+    assert torch.equal(generate(prompt_lookup_num_tokens=3), plain)
+    assert 0 in taken and min(taken) < 0
