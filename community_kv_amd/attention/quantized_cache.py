@@ -95,8 +95,9 @@ class QuantizedCacheLayer(CacheLayerMixin):
 
     def crop(self, max_length: int) -> None:
         """Takes back the newest tokens, down to a positive ``max_length``, else ``-max_length`` of them (0: none,
-        what assisted generation asks for where every candidate was right)."""
-        drop = self.seen - max_length if max_length > 0 else -max_length
+        what assisted generation asks for where every candidate was right; the library passes 0-dim tensors too)."""
+        max_length = int(max_length)
+        drop = min(self.seen - max_length if max_length > 0 else -max_length, self.seen)
         if drop <= 0:
             return
         if drop > self.rows or (self.budget and self.seen != self.rows):

@@ -109,3 +109,25 @@ def test_assisted_generation(on_cpu):
     assert not taken
     assert torch.equal(generate(prompt_lookup_num_tokens=3), plain)
     assert 0 in taken and min(taken) < 0
+
+
+def test_crop_counts(on_cpu):
+    """Counts come as 0-dim tensors from the library; the host's own counts stay integers, which nothing waits for.
+    More than there are empties the cache, as the library's own does, also before anything was written."""
+    from transformers import DynamicCache
+
+    cache, dynamic = _on_cache(_model()), DynamicCache()
+    cache.crop(-3)
+    x = torch.randn(1, 1, 20, 128)
+    for layer in range(LAYERS):
+        cache.update(x, x, layer)
+        dynamic.update(x, x, layer)
+    for n in (torch.tensor(-3), torch.tensor(0), np.int64(-1), -100):
+        cache.crop(n)
+        dynamic.crop(n)
+        assert cache.get_seq_length() == dynamic.get_seq_length()
+        for layer in range(LAYERS):
+            held = cache.layer(layer)
+            assert type(held.rows) is int and type(held.seen) is int and held.rows == held.seen
+            assert held.store.cursors.tolist() == [[held.rows], [held.rows], [0]]
+    assert held.rows == 0
