@@ -14,8 +14,8 @@ call is cut to its ``budget`` most attended rows (the first ``num_sink``
 positions and the newest ``recent`` ones among them), so a request of any
 length runs in ``max(prompt, budget + slack + 1)`` rows.
 
-One sequence at a time, as the CommunityKV runtime (padding is not seen by an
-attention function of this kind); ragged batches call ``quantized_append`` and
+One sequence at a time, as the CommunityKV runtime, and without padding (a
+padding mask raises); ragged batches call ``quantized_append`` and
 ``quantized_attention`` with ``counts``.
 """
 
@@ -157,10 +157,24 @@ class QuantizedCacheAttention:
         self.cache = cache
 
     def register(self) -> str:
+        from transformers import AttentionMaskInterface
         from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
         ALL_ATTENTION_FUNCTIONS[self.IMPL_NAME] = self.forward
+        AttentionMaskInterface.register(self.IMPL_NAME, self.mask)
         return self.IMPL_NAME
+
+    @staticmethod
+    def mask(*args: Any, attention_mask: torch.Tensor | None = None, **kwargs: Any) -> None:
+        """The model's mask: none, as ``forward`` masks by position.  The library asks for it once a forward call,
+        with the padding mask [1, rows] (without a function of this name it drops that mask unseen).  Reading it
+        waits for the device; a caller who captures passes no mask."""
+        if attention_mask is None:
+            return
+        if attention_mask.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise ValueError("a captured call takes no attention_mask: it cannot be looked at for padding")
+        if not bool(attention_mask.all()):
+            raise ValueError("attention over the 8-bit cache takes no padding: pass the sequence without it")
 
     def forward(self, module: torch.nn.Module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                 attention_mask: torch.Tensor | None, scaling: float, dropout: float = 0.0,

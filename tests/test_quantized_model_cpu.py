@@ -26,7 +26,7 @@ def _store(oracle, cache):
 
 @pytest.fixture
 def on_cpu(monkeypatch):
-    """The operators that the cache calls, as the oracle computes them."""
+    """The operators that the cache calls, as the oracle computes them, without gradients."""
 
     def append(cache, key, value):
         oracle = oq.Cache.of(cache)
@@ -47,6 +47,8 @@ def on_cpu(monkeypatch):
     monkeypatch.setattr(quantized_cache, "quantized_append", append)
     monkeypatch.setattr(quantized_cache, "quantized_attention", attention)
     monkeypatch.setattr(quantized_cache, "evict", evict)
+    with torch.no_grad():
+        yield
 
 
 def _model(**change):
@@ -131,3 +133,48 @@ def test_crop_counts(on_cpu):
             assert type(held.rows) is int and type(held.seen) is int and held.rows == held.seen
             assert held.store.cursors.tolist() == [[held.rows], [held.rows], [0]]
     assert held.rows == 0
+
+
+# ------------------------------------------------------------------------------------------ masks
+
+def test_a_mask_of_ones_is_no_padding(on_cpu):
+    model = _model()
+    prompt, mask = _prompt(12), torch.ones(1, 12, dtype=torch.long)
+    want = model(prompt, past_key_values=_on_cache(model)).logits
+    assert torch.equal(model(prompt, attention_mask=mask, past_key_values=_on_cache(model)).logits, want)
+    model.generate(prompt, attention_mask=mask, past_key_values=_on_cache(model), max_new_tokens=2, do_sample=False)
+
+
+@pytest.mark.parametrize("padded", [slice(0, 1), slice(0, 5), slice(11, 12), slice(4, 6)])
+def test_padding_is_refused(on_cpu, padded):
+    """A padded sequence raises from the model's own call, left, right and within, before anything is written."""
+    model = _model()
+    prompt, mask = _prompt(12), torch.ones(1, 12, dtype=torch.long)
+    mask[:, padded] = 0
+    for call in (model, lambda *args, **kwargs: model.generate(*args, max_new_tokens=2, do_sample=False, **kwargs)):
+        cache = _on_cache(model)
+        with pytest.raises(ValueError, match="padding"):
+            call(prompt, attention_mask=mask, past_key_values=cache)
+        assert cache.get_seq_length() == 0
+
+
+def test_padding_is_refused_behind_a_prompt(on_cpu):
+    model = _model()
+    cache = _on_cache(model)
+    model(_prompt(12), past_key_values=cache)
+    mask = torch.ones(1, 13, dtype=torch.long)
+    mask[0, 3] = 0
+    with pytest.raises(ValueError, match="padding"):
+        model(_prompt(1), attention_mask=mask, past_key_values=cache)
+    assert cache.get_seq_length() == 12
+
+
+def test_a_mask_in_a_captured_call_is_refused(monkeypatch):
+    """Whether it masks anything cannot be read while a stream is captured."""
+    class Mask:
+        is_cuda = True
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    assert QuantizedCacheAttention.mask(attention_mask=None) is None
+    with pytest.raises(ValueError, match="captured"):
+        QuantizedCacheAttention.mask(attention_mask=Mask())
