@@ -169,6 +169,13 @@ class QuantizedCacheAttention:
         """The model's mask: none, as ``forward`` masks by position.  The library asks for it once a forward call,
         with the padding mask [1, rows] (without a function of this name it drops that mask unseen).  Reading it
         waits for the device; a caller who captures passes no mask."""
+        config, local = kwargs.get("config"), kwargs.get("local_size")
+        # the library may not skip a causal mask that a model adds to, or of packed sequences; chunks come as a local
+        # size, as a sliding window does
+        if (not kwargs.get("allow_is_causal_skip", True) or local not in (None, getattr(config, "sliding_window", None)) or
+                "chunked_attention" in (getattr(config, "layer_types", None) or ())):
+            raise ValueError("attention over the 8-bit cache is causal, with or without a sliding window, and takes no "
+                             "other mask")
         if attention_mask is None:
             return
         if attention_mask.is_cuda and torch.cuda.is_current_stream_capturing():

@@ -178,3 +178,27 @@ def test_a_mask_in_a_captured_call_is_refused(monkeypatch):
     assert QuantizedCacheAttention.mask(attention_mask=None) is None
     with pytest.raises(ValueError, match="captured"):
         QuantizedCacheAttention.mask(attention_mask=Mask())
+
+
+def test_other_patterns_than_causal_and_sliding_are_refused(on_cpu):
+    """Chunks of attention, packed sequences and a model's own additions to the causal mask: the operator has no such
+    mask, and would attend past it."""
+    from transformers import masking_utils
+
+    model = _model(sliding_window=8, use_sliding_window=True, max_window_layers=1)
+    cache = _on_cache(model)
+    call = dict(config=model.config, inputs_embeds=torch.zeros(1, 5, 128), attention_mask=None, past_key_values=cache)
+    model.config.attention_chunk_size = 4
+    assert masking_utils.create_causal_mask(**call) is None
+    assert masking_utils.create_sliding_window_causal_mask(**call) is None
+    for make, extra in ((masking_utils.create_chunked_causal_mask, {}),
+                        (masking_utils.create_causal_mask, dict(or_mask_function=lambda b, h, q, k: k < 3)),
+                        (masking_utils.create_sliding_window_causal_mask, dict(and_mask_function=lambda b, h, q, k: k < 3)),
+                        (masking_utils.create_causal_mask, dict(past_key_values=None,
+                                                                position_ids=torch.tensor([[0, 1, 2, 0, 1]])))):
+        with pytest.raises(ValueError, match="causal"):
+            make(**(call | extra))
+    model.config.attention_chunk_size = model.config.sliding_window
+    model.config.layer_types = ["full_attention", "chunked_attention"]
+    with pytest.raises(ValueError, match="causal"):
+        masking_utils.create_chunked_causal_mask(**call)
