@@ -691,7 +691,7 @@ __global__ __launch_bounds__(64 * WT_WAVES, DT == CKV_F32 ? 2 : 4) void rows_wei
           acc = mfma32(kop[s], *reinterpret_cast<const uint4*>(&lds.q[stage][p][qrow * K_STRIDE + 16 * s + 8 * half]),
                        acc);
       }
-      const float2 st = lds.stats[stage][qrow];
+      float2 st = lds.stats[stage][qrow];
       // the 32 query rows together first, on the scalar unit: all there and all seeing all of the wave's rows
       const int row = step * WT_ROWS + 32 * x, last = row + 31;
       bool clear = full && last < a.rows;
@@ -717,6 +717,16 @@ __global__ __launch_bounds__(64 * WT_WAVES, DT == CKV_F32 ? 2 : 4) void rows_wei
             see.mask(y, at[e]);
             acc[4 * g + e] = y;
           }
+        }
+        if (st.y != st.y) {
+          // The query is NaN (by its own values, a key's or an infinite score), and so is what the rows that it sees
+          // get; below, a masked row's zero times NaN would be NaN too.
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int p = lds.pos[32 * wave + 8 * (v >> 2) + 4 * half + (v & 3)];
+            if ((uint32_t)(p - see.lo) <= see.span) got[v] = st.y;
+          }
+          st = float2{0.0f, 0.0f};
         }
       }
 #pragma unroll

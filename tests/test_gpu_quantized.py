@@ -711,3 +711,50 @@ def test_replays_equal_eager_calls(device, tokens, window, capacity, dtype):
         for got, eager in zip(results[i % 2], want):
             assert torch.equal(got, eager), i
         _same(caches[0], oq.Cache.of(caches[1]), f"replay {i}")
+
+
+@pytest.mark.parametrize("group,tokens,dtype", [(4, 40, torch.bfloat16), (2, 50, torch.float16), (4, 30, torch.float32),
+                                                (2, 3, torch.bfloat16), (8, 15, torch.bfloat16)])
+@pytest.mark.parametrize("window", [0, 17])
+@pytest.mark.parametrize("capacity", [320, 65_536])  # few-row kernels, many-row ones
+@pytest.mark.parametrize("mixed", [False, True])
+def test_nan_reaches_the_weights_of_the_rows_seen_alone(device, group, tokens, dtype, window, capacity, mixed):
+    """A NaN query, or a NaN key among the rows that a query sees, makes the received weights of the rows which that
+    query sees NaN, and no others: those are as they are without it, to the bit."""
+    print(f"nan weights group={group} tokens={tokens} dtype={dtype} window={window} capacity={capacity}", flush=True)
+    gen = torch.Generator().manual_seed(51)
+    n = 300
+    cache = _fill(device, gen, batch=1, heads=2, capacity=capacity, block=32, lengths=[n], mixed=mixed)
+    query = _rows(gen, 1, 2 * group, tokens, dtype=dtype)
+    weights, at = cache.weights.clone(), torch.arange(n - tokens, n, device=device)
+    position = cache.positions[0, :, :n]
+
+    def received(q):
+        cache.weights.copy_(weights)
+        quantized_attention(q.to(device), cache, softmax_scale=SCALE, window=window, accumulate=True)
+        torch.cuda.synchronize()
+        return cache.weights[0, :, :n].clone()
+
+    def seen_by(t):  # rows that query t sees, by head
+        return (position <= at[t]) & ((position > at[t] - window) if window else True)
+
+    clean = received(query)
+    assert not clean.isnan().any()
+    bad = tokens // 2
+    for value in (float("nan"), float("inf")):
+        broken = query.clone()
+        broken[0, group - 1, bad] = value  # a query head of KV head 0
+        got = received(broken)
+        want = seen_by(bad)
+        want[1] = False
+        assert torch.equal(got.isnan(), want) and torch.equal(got[~want], clean[~want]), value
+    # a NaN key: every query that sees it gives NaN to all that it sees
+    row = int((position[1] == n - tokens // 2 - 1).nonzero()[0])
+    cache.key_codes.view(torch.uint8)[0, 1, row, 3] = 0x7F
+    got = received(query)
+    want = torch.zeros_like(position, dtype=torch.bool)
+    for t in range(tokens):
+        if bool(seen_by(t)[1, row]):
+            want[1] |= seen_by(t)[1]
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[1].isnan(), want[1])
+    assert torch.equal(got[1][~want[1]], clean[1][~want[1]])
