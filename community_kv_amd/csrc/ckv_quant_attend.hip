@@ -270,13 +270,28 @@ __device__ inline void add_scores(const QuantAttendArgs& a, int b, int h, int64_
   const float* from = a.scores + bh * a.rows * c.capacity + r;
   const float2* stats = a.stats + bh * a.row_pad;
   float got[4] = {};
+  bool nan = false;
 #pragma unroll 4
   for (int row = 0; row < a.rows; ++row) {
     const float4 s = *reinterpret_cast<const float4*>(from + (int64_t)row * c.capacity);
     const float2 st = stats[row];
     const float v[4] = {s.x, s.y, s.z, s.w};
+    nan |= st.y != st.y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) got[i] += v[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(v[i] - st.x) * st.y;
+  }
+  if (nan) {  // a NaN query makes what it sees NaN, scores of minus infinity too, which masked rows have as well
+    const int4 p = __builtin_bit_cast(int4, gload16(q.positions + r));
+    const int at[4] = {p.x, p.y, p.z, p.w};
+    const int count = new_count(a, b), seen = c.cursors[c.batch + b];
+    for (int row = 0; row < a.rows; ++row) {
+      const float share = stats[row].y;
+      if (share == share) continue;
+      int lo, hi;
+      query_range(a, row, count, seen, &lo, &hi);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) got[i] = at[i] >= lo && at[i] <= hi ? share : got[i];
+    }
   }
   float* to = q.weights + r;
 #pragma unroll
@@ -597,6 +612,13 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendAr
     float sc[8];
     step_scores<DT>(s, query, a.scale_log2, sc);
     mask_step(s, by_position, t0, n, lo, hi, sc);
+    if (st.y != st.y) {  // as in add_scores
+      float seen_rows[8] = {};
+      mask_step(s, by_position, t0, n, lo, hi, seen_rows);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) got[i] = seen_rows[i] == NEG_INF ? got[i] : st.y;
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       got[i] += sc[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(sc[i] - st.x) * st.y;

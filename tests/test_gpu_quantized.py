@@ -758,3 +758,31 @@ def test_nan_reaches_the_weights_of_the_rows_seen_alone(device, group, tokens, d
             want[1] |= seen_by(t)[1]
     assert torch.equal(got[0], clean[0]) and torch.equal(got[1].isnan(), want[1])
     assert torch.equal(got[1][~want[1]], clean[1][~want[1]])
+
+
+@pytest.mark.parametrize("group,tokens", [(4, 1), (2, 3), (8, 15), (4, 40)])
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("capacity", [320, 65_536])
+@pytest.mark.parametrize("lengths", [[300], [300, 300]])
+def test_an_infinite_query_makes_all_that_it_sees_nan(device, group, tokens, window, capacity, lengths):
+    """One infinite element: scores are infinities of both signs, the softmax is NaN, and every row that the query sees
+    gets NaN, those of minus infinity too."""
+    print(f"infinite query group={group} tokens={tokens} window={window} capacity={capacity}", flush=True)
+    gen = torch.Generator().manual_seed(52)
+    n, batch = 300, len(lengths)
+    cache = _fill(device, gen, batch=batch, heads=1, capacity=capacity, block=32, lengths=lengths)
+    query = _rows(gen, batch, group, tokens, dtype=torch.bfloat16)
+    weights, at = cache.weights.clone(), n - tokens + tokens // 2
+    quantized_attention(query.to(device), cache, softmax_scale=SCALE, window=window, accumulate=True)
+    clean = cache.weights.clone()
+    cache.weights.copy_(weights)
+    query[0, group - 1, tokens // 2, 7] = -float("inf")
+    out, lse = quantized_attention(query.to(device), cache, softmax_scale=SCALE, window=window, accumulate=True)
+    torch.cuda.synchronize()
+    position = cache.positions[0, 0, :n]
+    want = torch.zeros_like(cache.weights, dtype=torch.bool)
+    want[0, 0, :n] = (position <= at) & ((position > at - window) if window else True)
+    assert torch.equal(cache.weights.isnan(), want) and torch.equal(cache.weights[~want], clean[~want])
+    nan = torch.zeros_like(lse, dtype=torch.bool)
+    nan[0, group - 1, tokens // 2] = True
+    assert torch.equal(lse.isnan(), nan) and torch.equal(out.isnan(), nan.transpose(1, 2)[..., None].expand(out.shape))
