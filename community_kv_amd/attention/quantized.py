@@ -313,8 +313,9 @@ def evict(cache: QuantizedKVCache, *, keep: int, num_sink: int = 0, recent: int 
         if into.capacity < min(keep, cache.capacity):
             raise ValueError(f"into holds {into.capacity} rows, keep needs {min(keep, cache.capacity)}")
     device = nat.require_device(cache.key_codes, *(() if into is None else (into.key_codes,)))
-    keep = min(keep, cache.capacity)
-    num_sink, recent = min(num_sink, keep), min(recent, keep)
+    keep = min(keep, cache.capacity)  # a lower one holds the protected rows; at the capacity no row is chosen
+    num_sink = min(num_sink, keep)
+    recent = min(recent, keep - num_sink)
     lib = nat.lib()
     size = lib.ckv_quant_evict_workspace_bytes(cache._ref, keep)
     workspace = torch.empty(size, dtype=torch.uint8, device=device)

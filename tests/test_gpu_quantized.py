@@ -786,3 +786,19 @@ def test_an_infinite_query_makes_all_that_it_sees_nan(device, group, tokens, win
     nan = torch.zeros_like(lse, dtype=torch.bool)
     nan[0, group - 1, tokens // 2] = True
     assert torch.equal(lse.isnan(), nan) and torch.equal(out.isnan(), nan.transpose(1, 2)[..., None].expand(out.shape))
+
+
+@pytest.mark.parametrize("keep,num_sink,recent", [(1000, 10, 500), (200, 4, 126), (2**40, 2**39, 2**39)])
+@pytest.mark.parametrize("into", [False, True])
+def test_evict_to_more_rows_than_there_are(device, keep, num_sink, recent, into):
+    """In place nothing happens; another cache gets a copy."""
+    gen = torch.Generator().manual_seed(53)
+    cache = _fill(device, gen, batch=2, heads=2, capacity=128, block=32, lengths=[128, 70])
+    target = _fill(device, gen, batch=2, heads=2, capacity=160, block=32, lengths=[3, 0]) if into else None
+    oracle, to = oq.Cache.of(cache), oq.Cache.of(target) if into else None
+    evict(cache, keep=keep, num_sink=num_sink, recent=recent, into=target)
+    torch.cuda.synchronize()
+    _same(cache, oracle, "cache")
+    if into:
+        oracle.evict(keep=keep, into=to)
+        _same(target, to, "into")

@@ -274,3 +274,24 @@ def test_attention_function_refuses_what_it_does_not_do():
                   dict(attention_mask=torch.zeros(1, 1, 1, 1))):
         with pytest.raises(ValueError):
             attention.forward(module, x, x, x, **(dict(attention_mask=None, scaling=1.0) | extra))
+
+
+@pytest.mark.parametrize("keep,num_sink,recent", [(1000, 10, 500), (200, 4, 126), (129, 64, 65), (2**40, 2**39, 2**39),
+                                                  (128, 128, 0), (100, 0, 100)])
+@pytest.mark.parametrize("into", [False, True])
+def test_evict_to_more_rows_than_there_are(lib, monkeypatch, keep, num_sink, recent, into):
+    """`keep` may exceed the capacity, and the protected rows with it: the C entry gets numbers that it takes."""
+    from community_kv_amd.attention import quantized
+
+    cache, target = _cache(), _cache() if into else None  # 128 rows
+    calls = []
+    monkeypatch.setattr(nat, "require_device", lambda *tensors: torch.device("cpu"))
+    monkeypatch.setattr(quantized, "_call", lambda device, function, *args: calls.append(args))
+    evict(cache, keep=keep, num_sink=num_sink, recent=recent, into=target)
+    (_, _, c_keep, c_sink, c_recent, _), = calls
+    assert 0 < c_keep <= 128 and 0 <= c_sink and 0 <= c_recent and c_sink + c_recent <= c_keep
+    if keep <= 128:
+        assert (c_keep, c_sink, c_recent) == (keep, num_sink, recent)
+    if not into and c_keep == 128:
+        # no sequence can hold more, so nothing is launched and the entry itself may be called
+        assert lib.ckv_quant_evict(cache._ref, None, c_keep, c_sink, c_recent, 0x1000, None) == 0
