@@ -299,8 +299,9 @@ def evict(cache: QuantizedKVCache, *, keep: int, num_sink: int = 0, recent: int 
     unless its value is an E4M3 subnormal of the new block.  In place by
     default (the addresses stay, so a step may be captured around it);
     ``into``: the rows and cursors go to another cache of the same batch, heads
-    and block, and ``cache`` stays as it is.  Evict between steps: after a
-    call's attention, before the next append."""
+    and block that shares no memory with this one, which stays as it is; the
+    weights go along if the other cache tracks them.  Evict between steps: after
+    a call's attention, before the next append."""
     if cache.weights is None:
         raise ValueError("evict needs a cache that tracks weights")
     if keep <= 0 or num_sink < 0 or recent < 0 or num_sink + recent > keep:

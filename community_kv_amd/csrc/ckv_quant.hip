@@ -735,6 +735,25 @@ __global__ __launch_bounds__(THREADS) void evict_move_kernel(const EvictArgs a, 
   if (tid == 0 && (!in_place || scale != old)) dst.scales(tensor)[blk] = scale;
 }
 
+// Whether two caches share any of the memory that an eviction reads or writes.
+bool overlap(const ckv_quant_cache& x, const ckv_quant_cache& y) {
+  struct Spans {
+    uintptr_t at[7], end[7];
+    explicit Spans(const ckv_quant_cache& c) {
+      const uintptr_t rows = (uintptr_t)c.batch * c.kv_heads * c.capacity, scales = rows / c.block * sizeof(float);
+      const void* first[7] = {c.key_codes, c.value_codes, c.key_scales, c.value_scales, c.positions, c.weights, c.cursors};
+      const uintptr_t bytes[7] = {rows * D, rows * D, scales, scales, rows * 4, c.weights ? rows * 4 : 0,
+                                  (uintptr_t)c.batch * 12};
+      for (int i = 0; i < 7; ++i) end[i] = (at[i] = (uintptr_t)first[i]) + bytes[i];
+    }
+  };
+  const Spans a(x), b(y);
+  for (int i = 0; i < 7; ++i)
+    for (int j = 0; j < 7; ++j)
+      if (a.at[i] < b.end[j] && b.at[j] < a.end[i]) return true;
+  return false;
+}
+
 int check_rows(const ckv_quant_rows* r, int dtype, const char* what) {
   static thread_local char message[160];
   const int unit = dtype == CKV_F32 ? 4 : 8;
@@ -788,9 +807,7 @@ extern "C" int ckv_quant_evict(const ckv_quant_cache* cache, const ckv_quant_cac
     if (into->batch != cache->batch || into->kv_heads != cache->kv_heads || into->block != cache->block)
       return fail(CKV_E_INVALID, "ckv_quant_evict: into must have the cache's batch, heads and block");
     if (into->capacity < most) return fail(CKV_E_INVALID, "ckv_quant_evict: into holds fewer rows than keep");
-    if (into->key_codes == cache->key_codes || into->value_codes == cache->value_codes ||
-        into->cursors == cache->cursors)
-      return fail(CKV_E_INVALID, "ckv_quant_evict: into must be another cache");
+    if (overlap(*cache, *into)) return fail(CKV_E_INVALID, "ckv_quant_evict: into must be another cache, with no memory of this one");
   } else if (keep >= cache->capacity) {
     return CKV_OK;  // no sequence can hold more
   }

@@ -637,7 +637,8 @@ int ckv_quant_attention(const ckv_quant_cache* cache, const ckv_quant_rows* quer
  * their rows, lengths become min(length, keep), rows at and past the new
  * length are left as they are.  into (null: in place): the rows go to another
  * cache of the same batch, heads and block and at least min(keep, capacity)
- * rows, whose cursors are set, and `cache` stays as it is.  workspace:
+ * rows, whose cursors are set, and `cache`, which shares no memory with it,
+ * stays as it is; weights are written where `into` has them.  workspace:
  * ckv_quant_evict_workspace_bytes() bytes, this call's alone. */
 size_t ckv_quant_evict_workspace_bytes(const ckv_quant_cache* cache, int32_t keep);
 int ckv_quant_evict(const ckv_quant_cache* cache, const ckv_quant_cache* into, int32_t keep, int32_t num_sink,

@@ -802,3 +802,26 @@ def test_evict_to_more_rows_than_there_are(device, keep, num_sink, recent, into)
     if into:
         oracle.evict(keep=keep, into=to)
         _same(target, to, "into")
+
+
+@pytest.mark.parametrize("tracked", [False, True])
+def test_evict_into_the_other_half_of_one_storage(device, tracked):
+    """Two caches that lie behind one another in the same tensors share no memory; a target that keeps no weights gets
+    none."""
+    gen = torch.Generator().manual_seed(54)
+    both = _fill(device, gen, batch=2, heads=2, capacity=128, block=32, lengths=[128, 128])
+    cursors = [_i32([[n], [n], [0]], device) for n in (128, 0)]
+    halves = [QuantizedKVCache.from_tensors(
+        key_codes=both.key_codes[b:b + 1], value_codes=both.value_codes[b:b + 1], key_scales=both.key_scales[b:b + 1],
+        value_scales=both.value_scales[b:b + 1], positions=both.positions[b:b + 1], cursors=cursors[b], block=32,
+        weights=both.weights[b:b + 1] if b == 0 or tracked else None) for b in range(2)]
+    left = both.weights[1].clone()
+    oracle, to = oq.Cache.of(halves[0]), oq.Cache.of(halves[1])
+    evict(halves[0], keep=50, num_sink=2, recent=9, into=halves[1])
+    torch.cuda.synchronize()
+    oracle.evict(keep=50, num_sink=2, recent=9, into=to)
+    if not tracked:
+        to.weights[:] = 0
+        assert torch.equal(both.weights[1], left)
+    _same(halves[0], oracle, "cache")
+    _same(halves[1], to, "into")

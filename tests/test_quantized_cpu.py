@@ -295,3 +295,27 @@ def test_evict_to_more_rows_than_there_are(lib, monkeypatch, keep, num_sink, rec
     if not into and c_keep == 128:
         # no sequence can hold more, so nothing is launched and the entry itself may be called
         assert lib.ckv_quant_evict(cache._ref, None, c_keep, c_sink, c_recent, 0x1000, None) == 0
+
+
+@pytest.mark.parametrize("shared", ["key_codes", "value_codes", "key_scales", "value_scales", "positions", "weights",
+                                    "cursors"])
+@pytest.mark.parametrize("whole", [False, True])
+def test_evict_refuses_a_target_that_shares_memory(lib, shared, whole):
+    """Any tensor of the source's among the target's, or one that begins within it."""
+    cache, tensors = _cache(), _tensors(_cache())
+    if whole:
+        tensors[shared] = getattr(cache, shared)
+    else:
+        good = tensors[shared]
+        bytes_ = torch.zeros(2 * good.nbytes, dtype=torch.uint8)
+
+        def part(first):
+            return bytes_[first:first + good.nbytes].view(good.dtype).view(good.shape)
+
+        step = max(16, good.nbytes // 32 * 16)
+        cache = QuantizedKVCache.from_tensors(**(_tensors(cache) | {shared: part(0)}))
+        tensors[shared] = part(min(step, good.nbytes - 8))
+    into = QuantizedKVCache.from_tensors(**tensors)
+    for a, b in ((cache, into), (into, cache)):
+        assert lib.ckv_quant_evict(a._ref, b._ref, 16, 0, 0, 0x1000, None) == 1
+        assert b"another cache" in lib.ckv_last_error()
