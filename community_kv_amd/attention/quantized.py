@@ -77,6 +77,9 @@ class QuantizedKVCache:
                 raise ValueError("all tensors of a cache must share one device")
         if any(t.data_ptr() % 16 for t in (codes, self.value_codes, self.positions, self.weights) if t is not None):
             raise ValueError("codes, positions and weights must be 16-byte aligned")
+        spans = sorted((tensor.data_ptr(), tensor.data_ptr() + tensor.nbytes) for _, tensor, _, _ in expected)
+        if any(start < end for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise ValueError("the tensors of a cache must not share memory")
         counters = torch.zeros(batch * nat.QUANT_COUNTERS, dtype=torch.int32, device=codes.device)
         struct = nat.QuantCache(
             codes.data_ptr(), self.value_codes.data_ptr(), self.key_scales.data_ptr(), self.value_scales.data_ptr(),

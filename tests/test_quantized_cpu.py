@@ -319,3 +319,22 @@ def test_evict_refuses_a_target_that_shares_memory(lib, shared, whole):
     for a, b in ((cache, into), (into, cache)):
         assert lib.ckv_quant_evict(a._ref, b._ref, 16, 0, 0, 0x1000, None) == 1
         assert b"another cache" in lib.ckv_last_error()
+
+
+@pytest.mark.parametrize("one,other", [("key_codes", "value_codes"), ("key_scales", "value_scales"),
+                                       ("positions", "weights")])
+def test_a_cache_over_one_tensor_twice_is_refused(one, other):
+    tensors = _tensors(_cache())
+    tensors[other] = tensors[one].view(tensors[other].dtype)
+    with pytest.raises(ValueError, match="share"):
+        QuantizedKVCache.from_tensors(**tensors)
+    buffer = torch.zeros(tensors[one].nbytes * 2, dtype=torch.uint8)
+    for gap in (0, tensors[one].nbytes // 32 * 16):
+        first, second = buffer[:tensors[one].nbytes], buffer[tensors[one].nbytes - gap:2 * tensors[one].nbytes - gap]
+        for name, part in ((one, first), (other, second)):
+            tensors[name] = part.view(tensors[name].dtype).view(tensors[name].shape)
+        if gap:
+            with pytest.raises(ValueError, match="share"):
+                QuantizedKVCache.from_tensors(**tensors)
+        else:
+            QuantizedKVCache.from_tensors(**tensors)
