@@ -110,3 +110,80 @@ def test_another_cache_is_refused(device):
             model(prompt, past_key_values=caches[0], use_cache=True)
         with pytest.raises(RuntimeError, match="not written into this cache"):
             model(prompt, use_cache=False)
+
+
+def _windowed_model(device):
+    """As _model, in f32, with a sliding layer behind the full one."""
+    from transformers import Qwen3ForCausalLM
+
+    cfg = _model("cpu").config
+    cfg.use_sliding_window, cfg.sliding_window = True, 33
+    cfg.layer_types = ["full_attention", "sliding_attention"]
+    torch.manual_seed(0)
+    with torch.device(device):
+        model = Qwen3ForCausalLM(cfg)
+    return model.float().eval()
+
+
+@pytest.mark.parametrize("sizes", [[90, 61, 1, 1, 5, 1], [200], [1, 1, 1, 140, 1]])
+def test_unbounded_run_is_the_dense_model(device, sizes):
+    """Prompt pieces, drafts and single tokens of a model with a full and a sliding layer, f32, against the same model
+    with the library's masks and attention in 64 bits over the numbers that the codes stand for.
+
+    Queries and keys have norm sqrt(128) (RMS norm, weights of one), so sum|q k| / sqrt(128) <= 11.4, and the oracle's
+    bound puts a score within d = 772 * 2^-24 * 11.4 = 5.3e-4, a probability within e^(2 d) - 1 = 1.1e-3 < 2^-9, an
+    output within 2^-9 of the largest value.  What so much does to the logits, through codes that flip too, is measured
+    on the dense model."""
+    from tests import _dense_codes as dense_codes
+
+    model = _windowed_model(device)
+    assert [layer.self_attn.sliding_window for layer in model.model.layers] == [None, 33]
+    prompt = torch.randint(0, 512, (1, sum(sizes)), generator=torch.Generator().manual_seed(4)).to(device)
+    pieces = prompt.split(sizes, 1)
+    cache = QuantizedCache(num_hidden_layers=LAYERS, max_cache_len=256, block=32)
+    model.set_attn_implementation(QuantizedCacheAttention(cache).register())
+    got = dense_codes.logits(model, cache, pieces)
+
+    def dense(noise):
+        model.set_attn_implementation(dense_codes.register(noise))
+        return dense_codes.logits(model, dense_codes.dense_cache(quantized_append, layers=LAYERS, rows=256, block=32), pieces)
+
+    want, moved = dense(0.0), dense(2.0 ** -9)
+    off, tol = (max(float((a - b).abs().max()) for a, b in zip(want, other)) for other in (got, moved))
+    assert off <= 2 * tol < 0.2 * max(float(a.abs().max()) for a in want), (off, tol)
+
+
+def test_assisted_generation_gives_the_greedy_tokens(device):
+    """Prompt lookup: rejected candidates are taken back after every verification, none where all were right."""
+    model = _model(device, torch.float32)
+    some = torch.randint(0, 512, (1, 40), generator=torch.Generator().manual_seed(5))
+    prompt = torch.cat([some, some, some[:, :20]], 1).to(device)
+    taken, tokens = [], []
+    for kwargs in ({}, dict(prompt_lookup_num_tokens=3)):
+        cache = QuantizedCache(num_hidden_layers=LAYERS, max_cache_len=256, block=32)
+        crop = cache.crop
+        cache.crop = lambda n, crop=crop: (taken.append(int(n)), crop(n))
+        model.set_attn_implementation(QuantizedCacheAttention(cache).register())
+        with torch.no_grad():
+            tokens.append(model.generate(prompt, past_key_values=cache, max_new_tokens=60, do_sample=False, **kwargs))
+        for layer in range(LAYERS):
+            held = cache.layer(layer)
+            assert held.rows == held.seen == tokens[-1].shape[1] - 1 and held.store.lengths.tolist() == [held.rows]
+    assert torch.equal(tokens[0], tokens[1]) and 0 in taken and min(taken) < 0
+
+
+def test_padding_is_refused(device):
+    model = _model(device)
+    prompt = torch.randint(0, 512, (1, 20), generator=torch.Generator().manual_seed(6)).to(device)
+    mask = torch.ones_like(prompt)
+    for padded in (None, 0, 19):
+        cache = QuantizedCache(num_hidden_layers=LAYERS, max_cache_len=64)
+        model.set_attn_implementation(QuantizedCacheAttention(cache).register())
+        if padded is None:
+            model.generate(prompt, attention_mask=mask, past_key_values=cache, max_new_tokens=2, do_sample=False)
+            continue
+        mask[0, padded] = 0
+        with pytest.raises(ValueError, match="padding"):
+            model.generate(prompt, attention_mask=mask, past_key_values=cache, max_new_tokens=2, do_sample=False)
+        assert cache.get_seq_length() == 0
+        mask[0, padded] = 1

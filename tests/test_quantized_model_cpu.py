@@ -10,6 +10,7 @@ import torch
 from community_kv_amd import QuantizedCache, QuantizedCacheAttention
 from community_kv_amd.attention import quantized_cache
 from oracle import quantized as oq
+from tests import _dense_codes as dense_codes
 
 LAYERS = 2
 
@@ -202,3 +203,26 @@ def test_other_patterns_than_causal_and_sliding_are_refused(on_cpu):
     model.config.layer_types = ["full_attention", "chunked_attention"]
     with pytest.raises(ValueError, match="causal"):
         masking_utils.create_chunked_causal_mask(**call)
+
+
+# ------------------------------------------------------------------------------------------ the dense model
+
+def test_a_model_on_the_cache_is_the_dense_model(on_cpu):
+    """Prompt pieces and single tokens of a model with a full and a sliding layer, against dense attention over what the
+    codes stand for.  Both attentions are in 64 bits here and rounded to 32, so an output is off by far less than 2^-16 of
+    the largest value; how far so much moves the logits, through codes that flip too, is measured on the dense model.
+    The sliding mask lost moves them much further."""
+    model = _model(sliding_window=9, use_sliding_window=True, max_window_layers=1)
+    assert model.config.layer_types == ["full_attention", "sliding_attention"]
+    prompt = _prompt(36)
+    pieces = [prompt[:, :17], prompt[:, 17:30]] + [prompt[:, i:i + 1] for i in range(30, 36)]
+    got = dense_codes.logits(model, _on_cache(model), pieces)
+
+    def dense(**kwargs):
+        model.set_attn_implementation(dense_codes.register(**kwargs))
+        cache = dense_codes.dense_cache(quantized_cache.quantized_append, layers=LAYERS, rows=96, block=16)
+        return dense_codes.logits(model, cache, pieces)
+
+    want, moved, wrong = dense(), dense(noise=2.0 ** -16), dense(window=False)
+    off, tol, far = (max(float((a - b).abs().max()) for a, b in zip(want, other)) for other in (got, moved, wrong))
+    assert off <= 2 * tol and far > 100 * tol, (off, tol, far)
