@@ -154,7 +154,9 @@ class QuantizedKVCache:
     def rewind(self, counts: int | torch.Tensor) -> None:
         """Takes back the newest ``counts`` tokens of every sequence (rejected
         draft tokens): at most those appended since the last eviction.  Block
-        scales stay as they have grown."""
+        scales stay as they have grown, and other rows keep the weight that the
+        tokens' queries gave them (attend to drafts without ``accumulate`` where
+        it must not count)."""
         if isinstance(counts, int) and counts < 0:
             raise ValueError("counts must be non-negative")
         self.cursors[:2].sub_(counts)
@@ -254,7 +256,8 @@ def quantized_attention(query: torch.Tensor, cache: QuantizedKVCache, *, softmax
     at positions up to its own and, with ``window`` > 0, of the last
     ``window`` positions (its own among them).  ``accumulate`` adds the
     probability that each row received, summed over the queries and the heads
-    of its group, to ``cache.weights``.
+    of its group, to ``cache.weights``; a query whose softmax is NaN gives NaN
+    to the rows that it attends.
 
     Returns (output [batch, tokens, query heads, 128] in the queries' dtype,
     lse [batch, query heads, tokens] float32, natural log); a query that

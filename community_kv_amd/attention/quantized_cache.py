@@ -95,7 +95,8 @@ class QuantizedCacheLayer(CacheLayerMixin):
 
     def crop(self, max_length: int) -> None:
         """Takes back the newest tokens, down to a positive ``max_length``, else ``-max_length`` of them (0: none,
-        what assisted generation asks for where every candidate was right; the library passes 0-dim tensors too)."""
+        what assisted generation asks for where every candidate was right; the library passes 0-dim tensors too).
+        With a budget the weight that their queries gave to older rows stays, and counts in later evictions."""
         max_length = int(max_length)
         drop = min(self.seen - max_length if max_length > 0 else -max_length, self.seen)
         if drop <= 0:

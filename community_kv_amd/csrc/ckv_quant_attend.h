@@ -90,10 +90,11 @@ __device__ inline int new_count(const QuantAttendArgs& a, int b) {
 // whole units, with which the sequences' parts, max(1, ceil(n / size)) each, are
 // at most `parts` together.  The rows of the batch over parts is below it and
 // those over parts - batch above, between which it is searched for where they
-// are more than 15 % apart (8 sequences of 2,048 rows, 32/8 heads: 13.3 us, with
-// the upper one 14.5; 24 f32 query rows over 5 sequences of 10k to 20k rows: 136
-// and 144; 8 sequences of 8k to 16k rows, 14 % apart: 69.7 and 68.1) and there are
-// up to 64 sequences.  With as many parts as sequences each sequence is one part.
+// are more than 15 % apart (8 sequences of 2,048 rows, 32/8 heads, in a graph: 13.6
+// us, with the upper one 14.5; 24 f32 query rows over 5 sequences of 10k to 20k
+// rows: 137 and 144; 8 sequences of 8k to 16k rows, 14 % apart: 54.1 either way) and
+// there are up to 64 sequences.  With as many parts as sequences each sequence is
+// one part.
 // Every wave works this out for itself.
 struct Part {
   int sequence;    // -1: none
@@ -201,12 +202,13 @@ __device__ inline void output_index(const QuantAttendArgs& a, int b, int h, int 
 // three pieces, whose many-row kernel is slower), and those whose cache rows, over
 // all heads and blocks of 16 query rows, are at most FEW_WORK; with received
 // weights only up to 128 query rows, beyond which their own kernels decide.
-// 32/8 heads, in a graph, few and many, us: 1 sequence of 1,000 rows, bf16, 128
-// query rows 19.9 and 22.0, 512 rows 20.4 and 29.5; 4,000 rows: 22.4 and 35.3, 52.1
-// and 41.1; 16,000 rows, 64 query rows 31.1 and 40.1, 128 rows 49.3 and 42.2; 8
-// sequences of 16,000 rows: 32 query rows 92 and 135, 64 rows 167 and 141 (f32: 192
-// and 259).  With weights, 1,000 rows: 128 query rows 34.6 and 32.4, 512 rows 61 and
-// 41.
+// 32/8 heads, in a graph, full caches, few and many, us: 1 sequence of 1,000 rows,
+// bf16, 128 query rows 15.1 and 22.0, 512 rows 27.3 and 30.2; 4,000 rows: 22.4 and
+// 36.4, 53.2 and 42.0; 16,000 rows, 64 query rows 31.1 and 40.6, 128 rows 49.1 and
+// 42.3; 8 sequences of 16,000 rows: 32 query rows 93 and 143, 64 rows 165 and 147
+// (f32: 192 and 261).  With weights, 1,000 rows: 128 query rows 29.4 and 32.6, 512
+// rows 66 and 42.  The host knows the capacity alone: 36 query rows over 1,000 rows
+// take 12.0 us in a cache of up to 16,384 rows, 19.6 in one of 40,960.
 constexpr int64_t FEW_WORK = 720000;
 inline bool many_rows(const ckv_quant_cache* c, int rows, int dtype, bool accumulate) {
   if (rows <= (dtype == CKV_BF16 ? 32 : 64)) return false;

@@ -7,7 +7,11 @@
 // scales multiply the scores and the probabilities, in 32 bits.  Queries and
 // scaled probabilities are split into as many bf16 pieces as their type has
 // significant bits (bf16 queries 1, fp16 2, f32 3), each piece a product of its
-// own into the same 32-bit accumulator.
+// own into the same 32-bit accumulator.  The one piece of bf16 rounds a probability
+// by up to 2^-8 of it, where the sums and received weights keep 32 bits: against 64
+// bits, relative to the outputs' norm, 1.7e-3 for single queries and 1.9e-3 for
+// 2,048 over 32k rows, where rounding the exact output alone gives 1.6e-3; a second
+// piece would be another product.
 //
 // A head's query rows are packed as token * group + query head, so that one
 // read of a key or value serves the whole group.
@@ -304,8 +308,8 @@ __device__ inline void add_scores(const QuantAttendArgs& a, int b, int h, int64_
 // those in it mostly stand together: a part is then every count-th unit of
 // WAVES * STEP rows, so that all parts have some of them, and a wave looks at the
 // positions of its STEP rows of eight units at once (four a lane) and passes over
-// steps that nobody sees.  Eight sequences of 16k-131k rows in order, window 4,096:
-// 35 us, where reading every row takes 304; of rows in any order, 251.
+// steps that nobody sees.  Eight sequences of 16k-131k rows in order, window 4,096,
+// in a graph: 34 us, where reading every row takes 312; of rows in any order, 256.
 struct StepWalk {
   int t0, end;       // first row of the step; rows end before `end`
   int unit, stride;  // with a window
@@ -531,7 +535,8 @@ __global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(const QuantAt
 }
 
 // The same for many query rows, of few parts mostly: a wave a row, two dims a lane
-// (702 queries in 3 parts, 28 heads: 14 us, a workgroup a row 38).
+// (702 queries over 4,201 rows, 28 heads, in 3 parts: the whole call 75 us, with a
+// workgroup a row 94).
 template <int DT>
 __global__ __launch_bounds__(256) void attend_join_rows_kernel(const QuantAttendArgs a) {
   const ckv_quant_cache& c = a.cache;
@@ -641,7 +646,11 @@ __global__ __launch_bounds__(64 * WAVES) void weights_kernel(const QuantAttendAr
 // one part and several, us: up to 400 rows in 4 units 8.3 and 10.4 with 4 query
 // rows, 12.5 and 12.2 with 16, 12.7 and 16.9 with 128; 640 rows in 7 units 8.6 and
 // 10.0, 14.7 and 12.3, 15.1 and 18.2; 1,000 rows in 8 units 11.6 and 10.7, 19.7 and
-// 12.3, 20.2 and 19.2.
+// 12.3, 20.2 and 19.2.  (Units of the capacity: a larger cache has parts, one sequence of
+// 1,000 rows 10.2 in any.)  With about as many (sequence, head, 16 query rows) as
+// workgroups every sequence is one part.  Even batches lose nothing by that, but one long
+// sequence among short ones then runs on one workgroup a head: 64 sequences of 8 heads,
+// one of 131,072 rows and the rest of 1,000, take 1,060 us, 32 sequences 60.
 constexpr int ONE_PART_UNITS = 6;
 
 int parts_for(const ckv_quant_cache* c, int64_t row_blocks, bool many) {
@@ -649,7 +658,7 @@ int parts_for(const ckv_quant_cache* c, int64_t row_blocks, bool many) {
   const int64_t units = ((int64_t)c->capacity + PART_UNIT - 1) / PART_UNIT;
   const int64_t want = workgroups / ((int64_t)c->kv_heads * row_blocks);
   // many rows in fewer than two parts a sequence cost more in joins than they even out
-  // (8 prompts of 234 tokens, 28 heads over 4: whole 25 us, in 9 parts 120)
+  // (8 prompts of 234 tokens, 28 heads over 4: whole 23 us, in 9 parts 44)
   if (want < (many ? 2 * c->batch : c->batch + 1) || units <= (many ? 1 : ONE_PART_UNITS)) return c->batch;
   return (int)(want < c->batch * units ? want : c->batch * units);
 }

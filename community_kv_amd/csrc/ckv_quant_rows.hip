@@ -9,7 +9,8 @@
 // next tile.  Each wave computes S^T = K Q^T with v_mfma_f32_32x32x16_bf16, which
 // leaves one query row in a lane (lane % 32) and 16 of 32 cache rows in each half of
 // the wave, so the softmax is per-lane work; O^T = V^T P^T takes the same layout,
-// with V^T by transposing LDS reads.
+// with V^T by transposing LDS reads.  (P in one bf16 piece for bf16 queries, two for
+// fp16, three for f32, as in the few-row kernel; its row sums before that rounding.)
 //
 // Tiles that no query of the workgroup sees are skipped by their least and
 // largest position, which range_kernel writes beforehand; rows may stand in

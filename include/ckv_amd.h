@@ -620,7 +620,8 @@ int ckv_quant_append(const ckv_quant_cache* cache, const ckv_quant_rows* key, co
  * [batch][query_heads][tokens] (natural log); a query that attends no row, or
  * with t >= counts[b], gives zeros and -inf.  accumulate adds to
  * weights[b][h][row] the probabilities that the head's queries gave the row
- * (fixed summation order).  workspace:
+ * (fixed summation order; NaN from a query whose softmax is NaN, to the rows that
+ * it attends alone).  workspace:
  * ckv_quant_attention_workspace_bytes() bytes, this call's alone. */
 size_t ckv_quant_attention_workspace_bytes(const ckv_quant_cache* cache, int32_t query_heads, int32_t tokens,
                                            int32_t dtype, int32_t accumulate);
