@@ -14,7 +14,15 @@ from community_kv_amd.config import CommunityKVConfig, GraphAggregation, Partiti
 from community_kv_amd.graph.partition import leiden_max_iterations, partition_graphs, partition_query_groups
 from community_kv_amd.runtime import CommunityKVRuntime
 
-# the 8-bit cache has no counterpart in the reference, whose __all__ this keeps
+# the 8-bit and the paged cache have no counterpart in the reference, whose __all__ this keeps
+from community_kv_amd.attention.paged import (  # noqa: F401
+    DraftTree,
+    PagedKVCache,
+    RotaryTable,
+    paged_append,
+    paged_attention,
+    paged_commit,
+)
 from community_kv_amd.attention.quantized import (  # noqa: F401
     QuantizedKVCache,
     evict,

@@ -20,7 +20,8 @@ LIB_PATH = os.path.join(PACKAGE_DIR, "libckv_amd.so")
 SOURCES = [os.path.join(PACKAGE_DIR, "csrc", name)
            for name in ("ckv_decode.hip", "ckv_select.hip", "ckv_attend.hip", "ckv_prefill.hip", "ckv_diag.hip",
                                 "ckv_state.hip", "ckv_adjacency.hip", "ckv_leiden.hip", "ckv_noalloc.hip",
-                                "ckv_select_large.hip", "ckv_quant.hip", "ckv_quant_attend.hip", "ckv_quant_rows.hip")]
+                                "ckv_select_large.hip", "ckv_quant.hip", "ckv_quant_attend.hip", "ckv_quant_rows.hip",
+                                "ckv_paged.hip", "ckv_paged_attend.hip", "ckv_paged_rows.hip")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HIP_FLAGS = [
     "--offload-arch=gfx950",
@@ -54,6 +55,7 @@ MAX_DESCRIPTORS = 4096
 MAX_SINKS = 256
 MAX_WINDOW = 1024
 QUANT_COUNTERS = 32
+MAX_DRAFT = 512
 
 EXPORTED_SYMBOLS = (
     "ckv_score_select",
@@ -101,6 +103,11 @@ EXPORTED_SYMBOLS = (
     "ckv_quant_attention",
     "ckv_quant_evict_workspace_bytes",
     "ckv_quant_evict",
+    "ckv_draft_tree_plan",
+    "ckv_paged_append",
+    "ckv_paged_attention_workspace_bytes",
+    "ckv_paged_attention",
+    "ckv_paged_commit",
     "ckv_host_numerics",
     "ckv_device_numerics",
     "ckv_latency_probe",
@@ -194,6 +201,21 @@ class QuantCache(ctypes.Structure):
 
 class QuantRows(ctypes.Structure):
     _fields_ = [("data", _p), ("batch_stride", _i64), ("head_stride", _i64), ("token_stride", _i64)]
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [("key_pages", _p), ("value_pages", _p), ("page_table", _p), ("lengths", _p), ("overflow", _p),
+                ("layers", _i32), ("pages", _i32), ("kv_heads", _i32), ("page_size", _i32), ("table_pages", _i32),
+                ("batch", _i32), ("dtype", _i32), ("reserved", _i32)]
+
+
+class TreeMasks(ctypes.Structure):
+    _fields_ = [("depths", _p), ("masks", _p)]
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [("cosines", _p), ("sines", _p), ("positions", _i32), ("dim", _i32), ("interleaved", _i32),
+                ("reserved", _i32)]
 
 
 def build(verbose: bool = False) -> str:
@@ -332,6 +354,19 @@ def lib() -> ctypes.CDLL:
     handle.ckv_quant_evict_workspace_bytes.restype = ctypes.c_size_t
     handle.ckv_quant_evict.argtypes = [quant, quant, _i32, _i32, _i32, _p, _p]
     handle.ckv_quant_evict.restype = ctypes.c_int
+    paged = ctypes.POINTER(PagedCache)
+    handle.ckv_draft_tree_plan.argtypes = [_p, _p, _i32, _i32, _p, _p, _p]
+    handle.ckv_draft_tree_plan.restype = ctypes.c_int
+    handle.ckv_paged_append.argtypes = [paged, _i32, rows, rows, rows, _i32, _i32, _p, _p, ctypes.POINTER(Rotary), _i32,
+                                        _p, _p]
+    handle.ckv_paged_append.restype = ctypes.c_int
+    handle.ckv_paged_attention_workspace_bytes.argtypes = [paged, _i32, _i32, _i32]
+    handle.ckv_paged_attention_workspace_bytes.restype = ctypes.c_size_t
+    handle.ckv_paged_attention.argtypes = [paged, _i32, rows, _i32, _i32, _p, ctypes.POINTER(TreeMasks), _f32, _i32, _p, _p,
+                                           _p, _p]
+    handle.ckv_paged_attention.restype = ctypes.c_int
+    handle.ckv_paged_commit.argtypes = [paged, _i32, _p, _p, _i32, _p]
+    handle.ckv_paged_commit.restype = ctypes.c_int
     handle.ckv_host_numerics.argtypes = [ctypes.c_int, _p, _p, _i64]
     handle.ckv_host_numerics.restype = ctypes.c_int
     handle.ckv_device_numerics.argtypes = [ctypes.c_int, _p, _p, _i64, _p]

@@ -1,0 +1,511 @@
+// Attention of a step's tokens over the paged KV cache (gfx950).
+//
+//   s_r = softmax_scale * (q . k_r),  out = sum_r e^{s_r - lse} v_r,
+//
+// r over the committed rows and the step's tokens that the query sees.  The
+// products run on the matrix cores in the cache's own type with 32-bit sums.
+// Maxima, sums and outputs are kept in 32 bits; a probability enters the value
+// product rounded to the cache's type (by up to 2^-8 or 2^-11 of it, where the
+// sums keep it whole), the same rounding that the result itself gets at the end.
+//
+// A head's query rows are packed as token * group + query head, so that one
+// read of a key or value serves the whole group and all tokens of a tree.
+#include <hip/hip_runtime.h>
+
+#include "ckv_paged_attend.h"
+#include "ckv_tile.h"
+
+namespace {
+using namespace ckv;
+
+constexpr int STEP = 32;  // cache rows a wave takes at a time
+constexpr int WAVES = 4;
+static_assert(PART_UNIT == WAVES * STEP, "parts are whole rounds of the waves");
+
+template <int DT>
+__device__ inline f32x4_t mfma16(uint4 a, uint4 b, f32x4_t c) {
+  if constexpr (DT == CKV_BF16) {
+    return mfma_bf16(a, b, c);
+  } else {
+    typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  }
+}
+
+// One step's rows of a head, straight from memory into operands: keys as A
+// operands (row m of MFMA block j is cache row 8 (m / 4) + 4 j + m % 4 of the
+// step, so that an accumulator lane holds the eight rows 8 L .. 8 L + 7, just
+// what the P operand of the value product takes), values 8 dims a lane of the
+// rows 8 L + u.  Eight rows that stand together share a page.
+struct StepRows {
+  uint4 k[2][4];
+  uint4 v[8];
+};
+
+struct StepPages {
+  int k, v;  // of this lane's rows
+};
+
+__device__ inline StepPages step_pages(const PagedHead& q, int t0, int last) {
+  const int lane = threadIdx.x & 63;
+  return StepPages{q.page(min(t0 + 8 * ((lane & 15) >> 2), last)), q.page(min(t0 + 8 * (lane >> 4), last))};
+}
+
+// Rows past the last one are read as they are in its page, and masked.
+__device__ inline void load_step(const PagedHead& q, int t0, const StepPages& pages, StepRows& s) {
+  const int lane = threadIdx.x & 63, L = lane >> 4, c = lane & 15;
+  const uint16_t* k = q.keys + q.at(pages.k, t0 + 8 * (c >> 2) + (c & 3)) + 8 * L;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) s.k[j][x] = gload16(k + 4 * j * D + 32 * x);
+  }
+  const uint16_t* v = q.values + q.at(pages.v, t0 + 8 * L) + 8 * c;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) s.v[u] = gload16(v + u * D);
+}
+
+__device__ inline uint32_t word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+
+// B operands of the value product: for dims 8 c + d, the rows 8 L + u (an 8 x 8
+// transposition within the lane).
+__device__ inline void value_operands(const uint4* v, uint4* op) {
+#pragma unroll
+  for (int pair = 0; pair < 4; ++pair) {
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t a = word_of(v[2 * u], pair), b = word_of(v[2 * u + 1], pair);
+      lo[u] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+      hi[u] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    }
+    op[2 * pair] = uint4{lo[0], lo[1], lo[2], lo[3]};
+    op[2 * pair + 1] = uint4{hi[0], hi[1], hi[2], hi[3]};
+  }
+}
+
+// The running softmax of 16 query rows over the steps of one wave.  m: log2
+// maximum of query row c, the same on the four lane groups; l: sum over this
+// lane's rows alone; o: accumulators, element i of block nb is query row
+// 4 L + i, dim 8 c + nb.
+struct Running {
+  float m, l;
+  f32x4_t o[8];
+};
+
+template <int DT>
+__device__ inline void add_step(const float* sc, const uint4* vop, Running& r) {
+  float top = sc[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[i]);
+  if (__ballot(top > r.m + PAGED_RESCALE) != 0) {
+    float t = fmaxf(top, xor_f32<16>(top));
+    t = fmaxf(t, xor_f32<32>(t));
+    t = t > r.m + PAGED_RESCALE ? t : r.m;  // a query's own scores alone decide
+    const float corr = r.m == t ? 1.0f : __builtin_amdgcn_exp2f(r.m - t);
+    const int L = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = __shfl(corr, 4 * L + i, 64);
+#pragma unroll
+      for (int nb = 0; nb < 8; ++nb) r.o[nb][i] *= f;
+    }
+    r.l *= corr;
+    r.m = t;
+  }
+  const float m = (r.m == NEG_INF ? 0.0f : r.m) - prob_bias<DT>();
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(sc[i] - m);
+    r.l += p[i];
+  }
+  const uint4 aop = {pack_store<DT>(p[0], p[1]), pack_store<DT>(p[2], p[3]), pack_store<DT>(p[4], p[5]),
+                     pack_store<DT>(p[6], p[7])};
+#pragma unroll
+  for (int nb = 0; nb < 8; ++nb) r.o[nb] = mfma16<DT>(aop, vop[nb], r.o[nb]);
+}
+
+// One workgroup of four waves takes a part of the cache rows of a (sequence,
+// head) for 16 RT query rows; its waves take steps in turn and join in LDS.
+// Bound by memory.
+template <int DT, int RT>
+__global__ __launch_bounds__(64 * WAVES, RT <= 2 ? 2 : 1) void paged_split_kernel(const PagedAttendArgs a) {
+  __shared__ float m_s[WAVES][16];
+  __shared__ float l_s[WAVES][16];
+  __shared__ float o_s[WAVES][16 * D];
+  const ckv_paged_cache& c = a.cache;
+  const int h = blockIdx.x % c.kv_heads, number = blockIdx.x / c.kv_heads, row0 = 16 * RT * blockIdx.y;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, L = lane >> 4, col = lane & 15;
+  const Part part = find_part(PagedRows{a}, a.parts, number, -1);
+  const int b = part.sequence;
+  if (b < 0) return;  // the join knows how many parts there are
+  const PagedStep step(a, b);
+  const PagedHead q(a, b, h);
+  // tokens of this workgroup's rows, and the rows that all and that any of them see
+  const int first_token = paged_token(a, row0);
+  const int last_token = min(paged_token(a, min(row0 + 16 * RT, a.rows) - 1), step.count - 1);
+  int begin = step.first(a) + part.index * part.rows;
+  int end = (int)min((int64_t)begin + part.rows, (int64_t)step.total);
+  int clear_hi = step.start - 1, clear_lo = 0;
+  if (!a.masks) {
+    clear_hi = step.start + first_token;
+    end = min(end, step.start + last_token + 1);
+    if (a.window > 0) begin = max(begin, max(step.start + first_token - a.window + 1, 0) & -PART_UNIT);
+  }
+  if (a.window > 0) clear_lo = step.start + (a.masks ? step.count - 1 : last_token) - a.window + 1;
+  if (first_token >= step.count) end = begin;
+  clear_hi = min(clear_hi, step.total - 1);
+
+  uint4 query[RT][4];
+  Running run[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int64_t from = paged_query_index(a, b, h, min(row0 + 16 * r + col, a.rows - 1));
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      query[r][x] = gload16(reinterpret_cast<const uint16_t*>(a.query.data) + from + 32 * x + 8 * L);
+    run[r].m = NEG_INF;
+    run[r].l = 0.0f;
+#pragma unroll
+    for (int nb = 0; nb < 8; ++nb) run[r].o[nb] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  int t0 = begin + wave * STEP;
+  const int last = step.total - 1;
+  StepPages pages{0, 0};
+  if (t0 < end) pages = step_pages(q, t0, last);
+  for (; t0 < end; t0 += WAVES * STEP) {
+    StepRows rows;
+    load_step(q, t0, pages, rows);
+    const bool bad = __ballot(!q.good(pages.k) || !q.good(pages.v)) != 0;
+    const bool good_rows = q.good(pages.v);
+    if (t0 + WAVES * STEP < end) pages = step_pages(q, t0 + WAVES * STEP, last);
+    const bool masked = bad || t0 < clear_lo || t0 + STEP - 1 > clear_hi;
+    bool special = false;
+    if (masked) {  // a masked row's zero probability times infinity or NaN would spread it
+      bool found = false;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) found |= has_special<DT>(word_of(rows.v[u], i));
+      }
+      special = __ballot(found) != 0;
+      if (special) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          rows.v[u] = uint4{without_special<DT>(rows.v[u].x), without_special<DT>(rows.v[u].y),
+                            without_special<DT>(rows.v[u].z), without_special<DT>(rows.v[u].w)};
+      }
+    }
+    uint4 vop[8];
+    value_operands(rows.v, vop);
+    uint32_t seen[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float sc[8];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc = mfma16<DT>(rows.k[j][x], query[r][x], acc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[4 * j + i] = acc[i] * a.scale_log2;
+      }
+      if (masked) {
+        const Sight sight(a, step, b, row0 + 16 * r + col);
+        seen[r] = good_rows ? (uint32_t)sight.rows(a, step, b, t0 + 8 * L) & 0xffu : 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sc[i] = (seen[r] >> i) & 1 ? sc[i] : NEG_INF;
+      }
+      add_step<DT>(sc, vop, run[r]);
+    }
+    if (special) {
+      // values that were taken as zeros above, added for the queries that see their row
+#pragma nounroll
+      for (int g = 0; g < 4; ++g) {
+        const int page = q.page(min(t0 + 8 * g, last));
+        const uint16_t* from = q.values + q.at(page, t0 + 8 * g) + 8 * col;
+#pragma nounroll
+        for (int u = 0; u < 8; ++u) {
+          const uint4 w = gload16(from + u * D);
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[2 * i] = special_value<DT>(word_of(w, i) & 0xffffu);
+            x[2 * i + 1] = special_value<DT>(word_of(w, i) >> 16);
+          }
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t sees = (uint32_t)__shfl((int)seen[r], 16 * g + 4 * L + i, 64) >> u & 1u;
+#pragma unroll
+              for (int nb = 0; nb < 8; ++nb) run[r].o[nb][i] += sees ? x[nb] : 0.0f;
+            }
+          }
+        }
+      }
+    }
+  }
+  // join the waves, 16 query rows at a time
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int at0 = row0 + 16 * r;
+    float l = add_xor16(run[r].l);
+    l = add_xor32(l);
+    __syncthreads();
+    if (L == 0) {
+      m_s[wave][col] = run[r].m;
+      l_s[wave][col] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float4* p = reinterpret_cast<float4*>(&o_s[wave][(4 * L + i) * D + 8 * col]);
+      p[0] = float4{run[r].o[0][i], run[r].o[1][i], run[r].o[2][i], run[r].o[3][i]};
+      p[1] = float4{run[r].o[4][i], run[r].o[5][i], run[r].o[6][i], run[r].o[7][i]};
+    }
+    __syncthreads();
+    for (int x = tid; x < 16 * D; x += 64 * WAVES) {
+      const int i = x >> 7, d = x & (D - 1), row = at0 + i;
+      if (row >= a.rows) continue;
+      const bool live = paged_token(a, row) < step.count;
+      float m = m_s[0][i];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) m = fmaxf(m, m_s[w][i]);
+      const float at = m == NEG_INF ? 0.0f : m;
+      float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        // a wave without a row has zeros and a maximum of -inf
+        const float f = __builtin_amdgcn_exp2f(m_s[w][i] - at);
+        sum += l_s[w][i] * f;
+        acc += o_s[w][x] * f;
+      }
+      if (!live) {
+        m = NEG_INF;
+        sum = acc = 0.0f;
+      }
+      if (part.count == 1) {
+        int64_t at_out, at_lse;
+        paged_output_index(a, b, h, row, &at_out, &at_lse);
+        store_value<DT>(a.out, at_out + d, sum == 0.0f ? 0.0f : acc / sum);
+        if (d == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+      } else {
+        a.part_acc[(((int64_t)h * a.parts + number) * a.row_pad + row) * D + d] = acc;
+        if (d == 0) {
+          a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m;
+          a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
+        }
+      }
+    }
+  }
+}
+
+// Joins the parts of one query row: a workgroup of 256 threads, four dims and
+// every eighth part each.
+constexpr int JOIN_THREADS = 256;
+constexpr int MAX_PARTS = 512;  // of one sequence
+
+template <int DT>
+__global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAttendArgs a) {
+  __shared__ float factor[MAX_PARTS];
+  __shared__ float scratch[4];
+  __shared__ float4 acc_s[JOIN_THREADS];
+  const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const Part part = find_part(PagedRows{a}, a.parts, 0, b);
+  if (part.count == 1) return;  // written already
+  const float* pm = a.part_max + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
+  const float* pl = a.part_sum + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
+  float m = NEG_INF;
+  for (int s = tid & 63; s < part.count; s += 64) m = fmaxf(m, pm[s]);
+  m = wave_max(m);  // every wave for itself
+  const float at = m == NEG_INF ? 0.0f : m;
+  float sum = 0.0f;
+  for (int s = tid; s < part.count; s += JOIN_THREADS) {
+    const float f = __builtin_amdgcn_exp2f(pm[s] - at);
+    factor[s] = f;
+    sum += pl[s] * f;
+  }
+  sum = wave_sum_tree(sum);
+  if ((tid & 63) == 0) scratch[tid >> 6] = sum;
+  __syncthreads();
+  sum = (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
+  const int dim = 4 * (tid & 31);
+  float4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.first) * a.row_pad + row) * D + dim;
+#pragma unroll 4
+  for (int s = tid >> 5; s < part.count; s += JOIN_THREADS / 32) {
+    const float4 x = *reinterpret_cast<const float4*>(pa + (int64_t)s * a.row_pad * D);
+    const float f = factor[s];
+    acc.x += x.x * f;
+    acc.y += x.y * f;
+    acc.z += x.z * f;
+    acc.w += x.w * f;
+  }
+  acc_s[tid] = acc;
+  __syncthreads();
+  int64_t at_out, at_lse;
+  paged_output_index(a, b, h, row, &at_out, &at_lse);
+  if (tid < D) {
+    float x = 0.0f;
+#pragma unroll
+    for (int g = 0; g < JOIN_THREADS / 32; ++g) x += reinterpret_cast<const float*>(acc_s)[g * D + tid];
+    store_value<DT>(a.out, at_out + tid, sum == 0.0f ? 0.0f : x / sum);
+  }
+  if (tid == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+}
+
+// The same for many query rows, of few parts mostly: a wave a row, two dims a lane.
+template <int DT>
+__global__ __launch_bounds__(256) void paged_join_rows_kernel(const PagedAttendArgs a) {
+  const int row = 4 * blockIdx.x + (threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
+  if (row >= a.rows) return;
+  const Part part = find_part(PagedRows{a}, a.parts, 0, b);
+  if (part.count == 1) return;
+  const int64_t first = ((int64_t)h * a.row_pad + row) * a.parts + part.first;
+  float m = NEG_INF;
+  for (int s = lane; s < part.count; s += 64) m = fmaxf(m, a.part_max[first + s]);
+  m = wave_max(m);
+  const float at = m == NEG_INF ? 0.0f : m;
+  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.first) * a.row_pad + row) * D + 2 * lane;
+  float sum = 0.0f;
+  float2 acc{0.0f, 0.0f};
+  for (int s0 = 0; s0 < part.count; s0 += 64) {
+    const int left = min(part.count - s0, 64);
+    float f = 0.0f, share = 0.0f;
+    if (lane < left) {
+      f = __builtin_amdgcn_exp2f(a.part_max[first + s0 + lane] - at);
+      share = a.part_sum[first + s0 + lane] * f;
+    }
+    sum += wave_sum_tree(share);
+#pragma unroll 4
+    for (int s = 0; s < left; ++s) {
+      const float2 x = *reinterpret_cast<const float2*>(pa + (int64_t)(s0 + s) * a.row_pad * D);
+      const float of = ckv_u2f((uint32_t)__builtin_amdgcn_readlane((int)ckv_f2u(f), s));
+      acc.x += x.x * of;
+      acc.y += x.y * of;
+    }
+  }
+  int64_t at_out, at_lse;
+  paged_output_index(a, b, h, row, &at_out, &at_lse);
+  const float x = sum == 0.0f ? 0.0f : acc.x / sum, y = sum == 0.0f ? 0.0f : acc.y / sum;
+  *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + at_out + 2 * lane) = pack_store<DT>(x, y);
+  if (lane == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+}
+
+constexpr int64_t MAX_ROWS = 1 << 21;  // query rows of a head: the grids' second dimension holds their blocks
+
+// How a call is laid out: which kernel, how many parts, and the workspace.
+struct PagedLayout {
+  int parts, row_pad, tiles;  // tiles of 16 query rows a workgroup of the few-row kernel, 0: the many-row kernel
+  size_t max, sum, acc, bytes;
+  PagedLayout(const ckv_paged_cache* c, int tokens, int group, int window) {
+    const int rows = tokens * group;
+    row_pad = (rows + 15) / 16 * 16;
+    tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 0;
+    const int64_t block = tiles ? 16 * tiles : paged_row_block(rows);
+    const int64_t blocks = (rows + block - 1) / block;
+    int64_t most = (int64_t)c->table_pages * c->page_size;  // rows that a sequence's tokens may see
+    if (window > 0 && (int64_t)window + tokens + 2 * PART_UNIT < most) most = (int64_t)window + tokens + 2 * PART_UNIT;
+    const int64_t units = (most + PART_UNIT - 1) / PART_UNIT;
+    const int64_t workgroups = tiles == 1 || tiles == 2 ? 512 : 256;
+    const int64_t want = workgroups / (c->kv_heads * blocks);
+    if (want < (tiles ? c->batch + 1 : 2 * c->batch) || units <= (tiles ? 6 : 1)) parts = c->batch;
+    else parts = (int)(want < c->batch * units ? want : c->batch * units);
+    size_t at = 0;
+    auto take = [&](size_t size) {
+      const size_t here = at;
+      at += (size + 15) & ~(size_t)15;
+      return here;
+    };
+    const size_t each = parts > c->batch ? (size_t)c->kv_heads * row_pad * parts * sizeof(float) : 0;
+    max = take(each);
+    sum = take(each);
+    acc = take(each * D);
+    bytes = at;
+  }
+};
+
+template <int DT>
+int launch_few(const PagedAttendArgs& a, int tiles, hipStream_t s) {
+  const dim3 grid(a.parts * a.cache.kv_heads, (a.rows + 16 * tiles - 1) / (16 * tiles));
+  if (tiles == 1) paged_split_kernel<DT, 1><<<grid, 64 * WAVES, 0, s>>>(a);
+  else if (tiles == 2) paged_split_kernel<DT, 2><<<grid, 64 * WAVES, 0, s>>>(a);
+  else paged_split_kernel<DT, 4><<<grid, 64 * WAVES, 0, s>>>(a);
+  return paged_launched("ckv_paged_attention");
+}
+
+template <int DT>
+int launch_attend(const PagedAttendArgs& a, int tiles, hipStream_t s) {
+  const int rc = tiles ? launch_few<DT>(a, tiles, s) : launch_paged_rows(a, s);
+  if (rc || a.parts == a.cache.batch) return rc;
+  if (tiles) paged_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
+  else paged_join_rows_kernel<DT><<<dim3((a.rows + 3) / 4, a.cache.kv_heads, a.cache.batch), 256, 0, s>>>(a);
+  return paged_launched("ckv_paged_attention");
+}
+
+}  // namespace
+
+extern "C" size_t ckv_paged_attention_workspace_bytes(const ckv_paged_cache* cache, int32_t query_heads, int32_t tokens,
+                                                      int32_t window) {
+  if (validate_paged_cache(cache, "ckv_paged_attention") || tokens <= 0 || query_heads <= 0 ||
+      query_heads % cache->kv_heads || window < 0)
+    return 0;
+  const int64_t group = query_heads / cache->kv_heads;
+  if (tokens * group > MAX_ROWS) return 0;
+  return PagedLayout(cache, tokens, (int)group, window).bytes;
+}
+
+extern "C" int ckv_paged_attention(const ckv_paged_cache* cache, int32_t layer, const ckv_quant_rows* query,
+                                   int32_t query_heads, int32_t tokens, const int32_t* counts,
+                                   const ckv_draft_tree* tree, float softmax_scale, int32_t window, void* out, float* lse,
+                                   void* workspace, void* stream) {
+  const char* what = "ckv_paged_attention";
+  int rc = validate_paged_cache(cache, what);
+  if (rc) return rc;
+  if (layer < 0 || layer >= cache->layers) return paged_error(CKV_E_INVALID, what, "no such layer");
+  if (!out || !lse) return paged_error(CKV_E_INVALID, what, "null argument");
+  rc = check_paged_rows(query, cache->dtype, what);
+  if (rc) return rc;
+  if (query_heads <= 0 || query_heads % cache->kv_heads)
+    return paged_error(CKV_E_INVALID, what, "query heads must be a multiple of the cache's heads");
+  const int group = query_heads / cache->kv_heads;
+  if (group > CKV_MAX_GROUP) return paged_error(CKV_E_LIMIT, what, "group size exceeds 16");
+  if (tokens <= 0 || window < 0) return paged_error(CKV_E_INVALID, what, "tokens must be positive, window not negative");
+  if ((int64_t)tokens * group > MAX_ROWS) return paged_error(CKV_E_LIMIT, what, "more than 2^21 query rows a head");
+  if (tree && (!tree->depths || !tree->masks)) return paged_error(CKV_E_INVALID, what, "null argument");
+  if (tree && tokens > CKV_MAX_DRAFT) return paged_error(CKV_E_LIMIT, what, "a tree of more than 512 tokens");
+  if (!(softmax_scale > 0.0f) || softmax_scale > 1e30f)
+    return paged_error(CKV_E_INVALID, what, "softmax_scale must be positive");
+  const PagedLayout lay(cache, tokens, group, window);
+  if (lay.bytes && (!workspace || ((uintptr_t)workspace & 15))) return paged_error(CKV_E_INVALID, what, "workspace");
+  char* ws = reinterpret_cast<char*>(workspace);
+  PagedAttendArgs a{};
+  a.cache = *cache;
+  const size_t layer_bytes = (size_t)cache->pages * cache->kv_heads * cache->page_size * D * 2;
+  a.cache.key_pages = reinterpret_cast<char*>(cache->key_pages) + layer * layer_bytes;
+  a.cache.value_pages = reinterpret_cast<char*>(cache->value_pages) + layer * layer_bytes;
+  a.query = *query;
+  a.counts = counts;
+  a.depths = tree ? tree->depths : nullptr;
+  a.masks = tree ? tree->masks : nullptr;
+  a.out = out;
+  a.lse = lse;
+  a.part_max = reinterpret_cast<float*>(ws + lay.max);
+  a.part_sum = reinterpret_cast<float*>(ws + lay.sum);
+  a.part_acc = reinterpret_cast<float*>(ws + lay.acc);
+  a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
+  a.tokens = tokens;
+  a.group = group;
+  a.group_magic = group > 1 ? (uint32_t)(((1ull << 32) + group - 1) / group) : 0u;
+  a.rows = tokens * group;
+  a.row_pad = lay.row_pad;
+  a.window = window;
+  a.parts = lay.parts;
+  a.words = (tokens + 63) / 64;
+  a.page_log2 = 31 - __builtin_clz((unsigned)cache->page_size);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (cache->dtype == CKV_BF16) return launch_attend<CKV_BF16>(a, lay.tiles, s);
+  return launch_attend<CKV_F16>(a, lay.tiles, s);
+}

@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_split_kernel(const Quant
   const int h = blockIdx.x % c.kv_heads, number = blockIdx.x / c.kv_heads, row0 = 16 * blockIdx.y;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, L = lane >> 4, col = lane & 15;
-  const Part part = find_part(c, a.parts, number, -1);
+  const Part part = find_part(QuantLengths{c}, a.parts, number, -1);
   const int b = part.sequence;
   if (b < 0) return;  // the join knows how many parts there are
   const int n = quant_length(c, b), seen = c.cursors[c.batch + b], count = new_count(a, b);
@@ -486,7 +486,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void attend_join_kernel(const QuantAt
   __shared__ float4 acc_s[JOIN_THREADS];
   const ckv_quant_cache& c = a.cache;
   const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-  const Part part = find_part(c, a.parts, 0, b);
+  const Part part = find_part(QuantLengths{c}, a.parts, 0, b);
   if (part.count == 1) return;  // written already
   const float* pm = a.part_max + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
   const float* pl = a.part_sum + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
@@ -542,7 +542,7 @@ __global__ __launch_bounds__(256) void attend_join_rows_kernel(const QuantAttend
   const ckv_quant_cache& c = a.cache;
   const int row = 4 * blockIdx.x + (threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
   if (row >= a.rows) return;
-  const Part part = find_part(c, a.parts, 0, b);
+  const Part part = find_part(QuantLengths{c}, a.parts, 0, b);
   if (part.count == 1) return;
   const int64_t first = ((int64_t)h * a.row_pad + row) * a.parts + part.first;
   float m = NEG_INF;

@@ -187,7 +187,7 @@ __global__ __launch_bounds__(64 * W) void attend_rows_kernel(const QuantAttendAr
   // the blocks of the newest rows see the most: they go first
   const int block0 = (int)(gridDim.y - 1 - blockIdx.y) * 32 * W;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
-  const Part part = find_part(c, a.parts, number, -1);
+  const Part part = find_part(QuantLengths{c}, a.parts, number, -1);
   const int b = part.sequence;
   if (b < 0) return;
   const int64_t bh = (int64_t)b * c.kv_heads + h;

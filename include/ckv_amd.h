@@ -645,6 +645,93 @@ size_t ckv_quant_evict_workspace_bytes(const ckv_quant_cache* cache, int32_t kee
 int ckv_quant_evict(const ckv_quant_cache* cache, const ckv_quant_cache* into, int32_t keep, int32_t num_sink,
                     int32_t recent, void* workspace, void* stream);
 
+/* Paged KV cache of a batch (no reference counterpart; the reference's cache is
+ * one sequence's).  Row r of sequence b lies in page page_table[b][r / page_size]
+ * at r % page_size, of every layer alike.  Rows below lengths[b] are committed;
+ * the tokens of a step stand behind them, token t in row lengths[b] + t, until
+ * ckv_paged_commit takes them over or the next step overwrites them.  A page
+ * number outside [0, pages) is no page: its rows are not written and not
+ * attended.  Sequences may share pages that are only read. */
+typedef struct ckv_paged_cache {
+  void* key_pages;             /* [layers][pages][kv_heads][page_size][128] bf16 or fp16, 16-byte aligned */
+  void* value_pages;           /* same */
+  const int32_t* page_table;   /* [batch][table_pages] */
+  int32_t* lengths;            /* [batch] committed rows, taken as clamped to [0, table_pages * page_size] */
+  int32_t* overflow;           /* [batch] 1: tokens found no row */
+  int32_t layers;
+  int32_t pages;
+  int32_t kv_heads;
+  int32_t page_size;           /* 16, 32, 64, 128 or 256 */
+  int32_t table_pages;         /* at most 2^30 rows a sequence */
+  int32_t batch;
+  int32_t dtype;               /* CKV_BF16 or CKV_F16 */
+  int32_t reserved;
+} ckv_paged_cache;
+
+/* A step's drafted tokens as trees over the committed rows: token t's position
+ * is lengths[b] + depths[b][t], and it attends the drafted tokens whose bit is
+ * set in its mask (bit j % 64 of word j / 64; ceil(tokens / 64) words). */
+typedef struct ckv_draft_tree {
+  const int32_t* depths;       /* [batch][tokens] */
+  const uint64_t* masks;       /* [batch][tokens][ceil(tokens / 64)] */
+} ckv_draft_tree;
+
+/* Position rotation: cosines and sines of position p's dim / 2 angles.  Pairs
+ * (i, i + dim / 2), or (2 i, 2 i + 1) where interleaved, of the first dim
+ * dimensions turn by angle i; the others stay. */
+typedef struct ckv_rotary {
+  const float* cosines;        /* [positions][dim / 2], 16-byte aligned */
+  const float* sines;          /* same */
+  int32_t positions;           /* at least the cache's rows a sequence */
+  int32_t dim;                 /* a multiple of 16, 16 to 128 */
+  int32_t interleaved;
+  int32_t reserved;
+} ckv_rotary;
+
+#define CKV_MAX_DRAFT 512      /* tokens of a tree, entries of a path */
+
+/* Depths and ancestor masks of drafted tokens from their parents: token t < counts[b]
+ * (null: tokens) is a child of token parents[b][t] where that is in [0, t), else of
+ * the last committed token.  Mask t holds t and its ancestors, depth t their number;
+ * both are 0 for tokens past the count.  tokens <= CKV_MAX_DRAFT. */
+int ckv_draft_tree_plan(const int32_t* parents, const int32_t* counts, int32_t batch, int32_t tokens,
+                        int32_t* depths, uint64_t* masks, void* stream);
+
+/* Writes a step's keys and values into layer `layer`: token t < counts[b] (null:
+ * tokens) into row lengths[b] + t, its key turned by the angles of position
+ * lengths[b] + t (tree: + depths[b][t]) where rotary is given, each value rounded
+ * once.  query (with rotary alone, may be null) [batch][query_heads][tokens][128]
+ * strided goes to query_out [batch][tokens][query_heads][128] in the cache's dtype,
+ * turned likewise; zeros past the count.  A token whose row is past the table or
+ * whose page is none is dropped and sets overflow[b].  dtype: the inputs',
+ * CKV_BF16, CKV_F16 or CKV_F32.  lengths stay as they are. */
+int ckv_paged_append(const ckv_paged_cache* cache, int32_t layer, const ckv_quant_rows* key,
+                     const ckv_quant_rows* value, const ckv_quant_rows* query, int32_t query_heads, int32_t tokens,
+                     const int32_t* counts, const int32_t* depths, const ckv_rotary* rotary, int32_t dtype,
+                     void* query_out, void* stream);
+
+/* Attention of a step's tokens, already written, over layer `layer`: token
+ * t < counts[b] (null: tokens) attends the committed rows and the step's tokens
+ * up to itself, or with a tree those of its mask; with window > 0 only rows whose
+ * position is above its own minus window.  query strided as above in the cache's
+ * dtype, out [batch][tokens][query_heads][128], lse [batch][query_heads][tokens]
+ * (natural log); a query that attends no row, or with t >= counts[b], gives zeros
+ * and -inf.  workspace: ckv_paged_attention_workspace_bytes() bytes, this call's alone. */
+size_t ckv_paged_attention_workspace_bytes(const ckv_paged_cache* cache, int32_t query_heads, int32_t tokens,
+                                           int32_t window);
+int ckv_paged_attention(const ckv_paged_cache* cache, int32_t layer, const ckv_quant_rows* query, int32_t query_heads,
+                        int32_t tokens, const int32_t* counts, const ckv_draft_tree* tree, float softmax_scale,
+                        int32_t window, void* out, float* lse, void* workspace, void* stream);
+
+/* Commits a step's tokens in all layers.  Without a path the first counts[b] (null:
+ * tokens) are taken: lengths[b] += count, up to the table's rows.  path
+ * [batch][path_tokens] (path_tokens <= CKV_MAX_DRAFT) names the tokens to keep in
+ * ascending order: row lengths[b] + j takes row lengths[b] + path[b][j] for
+ * j < counts[b], and lengths[b] grows by their number.  The path ends at the first
+ * entry that does not ascend or lies past the table's rows. */
+int ckv_paged_commit(const ckv_paged_cache* cache, int32_t tokens, const int32_t* counts, const int32_t* path,
+                     int32_t path_tokens, void* stream);
+
 /* Diagnostic, no counterpart in the reference: latency probes behind the
  * decode step's measured cost model (bench.py --workload floor).  kind 0: one
  * empty kernel of blocks x threads with lds_bytes of dynamic LDS (the host
