@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 import subprocess
 
 import torch
@@ -205,7 +206,7 @@ class QuantRows(ctypes.Structure):
 
 class PagedCache(ctypes.Structure):
     _fields_ = [("key_pages", _p), ("value_pages", _p), ("page_table", _p), ("lengths", _p), ("overflow", _p),
-                ("layers", _i32), ("pages", _i32), ("kv_heads", _i32), ("page_size", _i32), ("table_pages", _i32),
+                ("counters", _p), ("layers", _i32), ("pages", _i32), ("kv_heads", _i32), ("page_size", _i32), ("table_pages", _i32),
                 ("batch", _i32), ("dtype", _i32), ("reserved", _i32)]
 
 
@@ -216,6 +217,12 @@ class TreeMasks(ctypes.Structure):
 class Rotary(ctypes.Structure):
     _fields_ = [("cosines", _p), ("sines", _p), ("positions", _i32), ("dim", _i32), ("interleaved", _i32),
                 ("reserved", _i32)]
+
+
+# ckv_paged_append_args and ckv_paged_attention_args: packed in one call, where a
+# ctypes structure costs a call's worth of microseconds
+PAGED_APPEND_ARGS = struct.Struct("@PqqqPqqqPqqqPPPPiiii")
+PAGED_ATTENTION_ARGS = struct.Struct("@PqqqPPPPPiiiifi")
 
 
 def build(verbose: bool = False) -> str:
@@ -357,13 +364,11 @@ def lib() -> ctypes.CDLL:
     paged = ctypes.POINTER(PagedCache)
     handle.ckv_draft_tree_plan.argtypes = [_p, _p, _i32, _i32, _p, _p, _p]
     handle.ckv_draft_tree_plan.restype = ctypes.c_int
-    handle.ckv_paged_append.argtypes = [paged, _i32, rows, rows, rows, _i32, _i32, _p, _p, ctypes.POINTER(Rotary), _i32,
-                                        _p, _p]
+    handle.ckv_paged_append.argtypes = [paged, ctypes.c_char_p, _p]
     handle.ckv_paged_append.restype = ctypes.c_int
     handle.ckv_paged_attention_workspace_bytes.argtypes = [paged, _i32, _i32, _i32]
     handle.ckv_paged_attention_workspace_bytes.restype = ctypes.c_size_t
-    handle.ckv_paged_attention.argtypes = [paged, _i32, rows, _i32, _i32, _p, ctypes.POINTER(TreeMasks), _f32, _i32, _p, _p,
-                                           _p, _p]
+    handle.ckv_paged_attention.argtypes = [paged, ctypes.c_char_p, _p]
     handle.ckv_paged_attention.restype = ctypes.c_int
     handle.ckv_paged_commit.argtypes = [paged, _i32, _p, _p, _i32, _p]
     handle.ckv_paged_commit.restype = ctypes.c_int

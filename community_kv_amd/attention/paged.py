@@ -31,7 +31,7 @@ from dataclasses import dataclass, field
 import torch
 
 from community_kv_amd import _native as nat
-from community_kv_amd.attention.quantized import _call, _rows
+from community_kv_amd.attention.quantized import _rows
 
 HEAD_DIM = nat.HEAD_DIM
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -66,8 +66,11 @@ class PagedKVCache:
     page_table: torch.Tensor   # [batch, pages a sequence] int32
     lengths: torch.Tensor      # [batch] int32: committed rows
     overflow: torch.Tensor = field(init=False)  # [batch] int32: 1 where tokens found no row
+    _counters: torch.Tensor = field(init=False, repr=False)
+    # made once: a call costs microseconds
     _struct: nat.PagedCache = field(init=False, repr=False)
-    _ref: object = field(init=False, repr=False)  # the struct by reference, made once: a call costs microseconds
+    _ref: object = field(init=False, repr=False)  # the struct by reference
+    _facts: tuple = field(init=False, repr=False)  # layers, batch, kv_heads, capacity, device number
     _sizes: dict = field(init=False, repr=False)  # workspace bytes by call shape
 
     def __post_init__(self) -> None:
@@ -96,11 +99,14 @@ class PagedKVCache:
         spans = sorted((tensor.data_ptr(), tensor.data_ptr() + tensor.nbytes) for _, tensor, _, _ in expected)
         if any(start < end for (_, end), (start, _) in zip(spans, spans[1:])):
             raise ValueError("the tensors of a cache must not share memory")
-        overflow = torch.zeros(batch, dtype=torch.int32, device=pages.device)
+        overflow, counters = (torch.zeros(batch * each, dtype=torch.int32, device=pages.device)
+                              for each in (1, nat.QUANT_COUNTERS))
         struct = nat.PagedCache(pages.data_ptr(), self.value_pages.data_ptr(), self.page_table.data_ptr(),
-                                self.lengths.data_ptr(), overflow.data_ptr(), layers, count, heads, size, table_pages, batch,
-                                _STORES[pages.dtype], 0)
-        for name, value in (("overflow", overflow), ("_struct", struct), ("_ref", ctypes.byref(struct)), ("_sizes", {})):
+                                self.lengths.data_ptr(), overflow.data_ptr(), counters.data_ptr(), layers, count, heads, size,
+                                table_pages, batch, _STORES[pages.dtype], 0)
+        facts = (layers, batch, heads, table_pages * size, pages.get_device())
+        for name, value in (("overflow", overflow), ("_counters", counters), ("_struct", struct), ("_ref", ctypes.byref(struct)), ("_facts", facts),
+                            ("_sizes", {})):
             object.__setattr__(self, name, value)
 
     @classmethod
@@ -171,7 +177,8 @@ class RotaryTable:
     cosines: torch.Tensor
     sines: torch.Tensor
     interleaved: bool = False
-    _ref: object = field(init=False, repr=False)
+    _struct: nat.Rotary = field(init=False, repr=False)
+    _facts: tuple = field(init=False, repr=False)  # the struct's address, positions, device number
 
     def __post_init__(self) -> None:
         if self.cosines.ndim != 2 or self.cosines.shape[0] == 0:
@@ -186,7 +193,8 @@ class RotaryTable:
             if tensor.data_ptr() % 16:
                 raise ValueError(f"{name} must be 16-byte aligned")
         struct = nat.Rotary(self.cosines.data_ptr(), self.sines.data_ptr(), positions, 2 * half, int(self.interleaved), 0)
-        object.__setattr__(self, "_ref", ctypes.byref(struct))
+        object.__setattr__(self, "_struct", struct)
+        object.__setattr__(self, "_facts", (ctypes.addressof(struct), positions, self.cosines.get_device()))
 
     @classmethod
     def from_frequencies(cls, frequencies: torch.Tensor, positions: int, *, interleaved: bool = False,
@@ -205,30 +213,35 @@ class RotaryTable:
         return self.cosines.shape[0]
 
 
-@dataclass(frozen=True, eq=False)
 class DraftTree:
     """The drafted tokens of a step, made once and used by every layer.  Token
     ``t`` stands ``depths[b, t]`` positions behind the first drafted ones, and
     bit ``j % 64`` of ``masks[b, t, j // 64]`` is set where ``j`` is ``t`` or one
-    of its ancestors."""
+    of its ancestors.
 
-    depths: torch.Tensor              # [batch, tokens] int32
-    masks: torch.Tensor               # [batch, tokens, ceil(tokens / 64)] int64
-    counts: torch.Tensor | None = None  # [batch] int32: tokens of each sequence
-    _ref: object = field(init=False, repr=False)
+    ``depths`` [batch, tokens] int32, ``masks`` [batch, tokens, ceil(tokens / 64)]
+    int64, ``counts`` [batch] int32 (tokens of each sequence) or None."""
 
-    def __post_init__(self) -> None:
-        if self.depths.ndim != 2 or 0 in self.depths.shape:
+    __slots__ = ("depths", "masks", "counts", "_struct", "_facts")
+
+    def __init__(self, depths: torch.Tensor, masks: torch.Tensor, counts: torch.Tensor | None = None) -> None:
+        if depths.ndim != 2 or 0 in depths.shape:
             raise ValueError("depths must be a non-empty [batch, tokens] tensor")
-        batch, tokens = self.depths.shape
+        batch, tokens = depths.shape
         if tokens > MAX_DRAFT:
             raise ValueError(f"a tree may have at most {MAX_DRAFT} tokens, not {tokens}")
-        _expect("depths", self.depths, torch.int32, (batch, tokens), self.depths.device)
-        _expect("masks", self.masks, torch.int64, (batch, tokens, -(-tokens // 64)), self.depths.device)
-        if self.counts is not None:
-            _expect("counts", self.counts, torch.int32, (batch,), self.depths.device)
-        struct = nat.TreeMasks(self.depths.data_ptr(), self.masks.data_ptr())
-        object.__setattr__(self, "_ref", ctypes.byref(struct))
+        _expect("depths", depths, torch.int32, (batch, tokens), depths.device)
+        _expect("masks", masks, torch.int64, (batch, tokens, -(-tokens // 64)), depths.device)
+        if counts is not None:
+            _expect("counts", counts, torch.int32, (batch,), depths.device)
+        self._hold(depths, masks, counts, batch, tokens, depths.get_device())
+
+    def _hold(self, depths, masks, counts, batch, tokens, device) -> None:
+        self.depths, self.masks, self.counts = depths, masks, counts
+        at = depths.data_ptr()
+        self._struct = nat.TreeMasks(at, masks.data_ptr())
+        # batch, tokens, device number, addresses of the struct, the depths and the counts
+        self._facts = (batch, tokens, device, ctypes.addressof(self._struct), at, 0 if counts is None else counts.data_ptr())
 
     @classmethod
     def from_parents(cls, parents: torch.Tensor, *, counts: torch.Tensor | None = None) -> "DraftTree":
@@ -238,22 +251,27 @@ class DraftTree:
         tokens of each sequence that are there."""
         if parents.dtype != torch.int32:
             raise TypeError(f"parents must use int32, not {parents.dtype}")
-        if parents.ndim != 2 or 0 in parents.shape:
+        shape = parents.shape
+        if len(shape) != 2 or 0 in shape:
             raise ValueError("parents must be a non-empty [batch, tokens] tensor")
-        batch, tokens = parents.shape
+        batch, tokens = shape
         if tokens > MAX_DRAFT:
             raise ValueError(f"a tree may have at most {MAX_DRAFT} tokens, not {tokens}")
+        device = parents.get_device()
+        counts_at = 0
         if counts is not None:
-            if counts.dtype != torch.int32 or counts.shape != (batch,):
-                raise TypeError(f"counts must be an int32 vector of one entry a sequence ({batch})")
-            counts = counts.contiguous()
-        device = nat.require_device(parents, *(() if counts is None else (counts,)))
+            counts = _counts_vector(counts, batch, device)
+            counts_at = counts.data_ptr()
+        if device < 0:
+            raise RuntimeError(_NEED_GPU)
         parents = parents.contiguous()
-        depths = torch.empty((batch, tokens), dtype=torch.int32, device=device)
-        masks = torch.empty((batch, tokens, -(-tokens // 64)), dtype=torch.int64, device=device)
-        _call(device, nat.lib().ckv_draft_tree_plan, parents.data_ptr(), nat.ptr(counts), batch, tokens, depths.data_ptr(),
-              masks.data_ptr())
-        return cls(depths, masks, counts)
+        depths = parents.new_empty((batch, tokens))
+        masks = parents.new_empty((batch, tokens, (tokens + 63) // 64), dtype=torch.int64)
+        tree = cls.__new__(cls)
+        tree._hold(depths, masks, counts, batch, tokens, device)
+        _launch(device, nat.lib().ckv_draft_tree_plan, parents.data_ptr(), counts_at, batch, tokens, depths.data_ptr(),
+                masks.data_ptr())
+        return tree
 
     @property
     def batch(self) -> int:
@@ -264,33 +282,73 @@ class DraftTree:
         return self.depths.shape[1]
 
 
-def _check_step(cache: PagedKVCache, layer: int, name: str, tensor: torch.Tensor) -> None:
-    shape = tensor.shape
-    if len(shape) != 4 or shape[0] != cache._struct.batch or shape[3] != HEAD_DIM:
-        raise ValueError(f"{name} must have shape [{cache.batch}, heads, tokens, {HEAD_DIM}], not {tuple(shape)}")
-    if not 0 <= layer < cache._struct.layers:
-        raise ValueError(f"layer {layer} of a cache of {cache.layers}")
-    if tensor.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} requires a gradient; the paged cache has no backward pass (use torch.no_grad())")
+_NEED_GPU = "the paged cache runs on the GPU only (got a CPU tensor)"
 
 
-def _step_counts(cache: PagedKVCache, tokens: int, tree: DraftTree | None,
-                 counts: torch.Tensor | None) -> torch.Tensor | None:
-    if tree is not None:
-        if counts is not None:
-            raise ValueError("a tree has its own counts")
-        if tree.depths.shape != (cache._struct.batch, tokens):
-            raise ValueError(f"the tree holds {tuple(tree.depths.shape)} tokens, the call [{cache.batch}, {tokens}]")
-        return tree.counts
-    if counts is None:
-        return None
-    if counts.dtype != torch.int32 or counts.shape != (cache._struct.batch,):
-        raise TypeError(f"counts must be an int32 vector of one entry a sequence ({cache.batch})")
+def _launch(device: int, function, *args) -> None:
+    """Calls a C entry on the current stream of device number ``device``."""
+    if device == torch._C._cuda_getDevice():
+        rc = function(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        nat.check(rc)
+
+
+def _counts_vector(counts: torch.Tensor, batch: int, device: int) -> torch.Tensor:
+    if counts.dtype != torch.int32 or counts.shape != (batch,):
+        raise TypeError(f"counts must be an int32 vector of one entry a sequence ({batch})")
+    if counts.get_device() != device:
+        raise ValueError("all tensors must share one device")
     return counts.contiguous()
 
 
-def _devices(cache: PagedKVCache, *tensors: torch.Tensor | None) -> torch.device:
-    return nat.require_device(cache.key_pages, *(t for t in tensors if t is not None))
+def _check_step(cache: PagedKVCache, layer: int, name: str, tensor: torch.Tensor) -> torch.Size:
+    shape = tensor.shape
+    layers, batch, _, _, device = cache._facts
+    if len(shape) != 4 or shape[0] != batch or shape[3] != HEAD_DIM:
+        raise ValueError(f"{name} must have shape [{batch}, heads, tokens, {HEAD_DIM}], not {tuple(shape)}")
+    if not 0 <= layer < layers:
+        raise ValueError(f"layer {layer} of a cache of {layers}")
+    if tensor.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient; the paged cache has no backward pass (use torch.no_grad())")
+    if tensor.get_device() != device:
+        raise ValueError("all tensors must share one device")
+    return shape
+
+
+def _step_counts(cache: PagedKVCache, tokens: int, tree: DraftTree | None,
+                 counts: torch.Tensor | None) -> tuple[int, torch.Tensor | None]:
+    """Address of a step's counts (0: all tokens), and the tensor that holds them."""
+    _, batch, _, _, device = cache._facts
+    if tree is not None:
+        if counts is not None:
+            raise ValueError("a tree has its own counts")
+        facts = tree._facts
+        if facts[0] != batch or facts[1] != tokens:
+            raise ValueError(f"the tree holds {facts[:2]} tokens, the call {(batch, tokens)}")
+        if facts[2] != device:
+            raise ValueError("all tensors must share one device")
+        return facts[5], tree.counts
+    if counts is None:
+        return 0, None
+    counts = _counts_vector(counts, batch, device)
+    return counts.data_ptr(), counts
+
+
+def _view(tensor: torch.Tensor) -> tuple[tuple[int, int, int, int], torch.Tensor]:
+    """Address and strides of [batch, heads, tokens, 128], and the tensor that they are of (a copy where they do not
+    suit 16-byte loads)."""
+    b, h, t, d = tensor.stride()
+    at = tensor.data_ptr()
+    if d == 1 and not ((b | h | t) * tensor.element_size() | at) & 15:
+        return (at, b, h, t), tensor
+    rows, tensor = _rows(tensor)
+    return (rows.data, rows.batch_stride, rows.head_stride, rows.token_stride), tensor
+
+
+_NO_ROWS = (0, 0, 0, 0)
 
 
 def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, *, layer: int = 0,
@@ -308,43 +366,52 @@ def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, *,
 
     Tokens whose row is past the capacity or has no page are dropped and raise the
     overflow flag (``assert_no_overflow``)."""
+    layers, batch, heads, capacity, device = cache._facts
+    shape, kind = key.shape, key.dtype
+    dtype = _DTYPES.get(kind)
+    if (dtype is None or value.dtype != kind or value.shape != shape or len(shape) != 4 or shape[1] != heads or
+            value.requires_grad or value.get_device() != device):
+        _check_step(cache, layer, "value", value)
+        if dtype is None:
+            raise TypeError(f"key must use bfloat16, float16 or float32, not {key.dtype}")
+        if len(shape) != 4 or shape[1] != heads or value.shape != shape:
+            raise ValueError(f"key and value must both have {heads} heads and the same tokens")
+        if value.dtype != kind:
+            raise TypeError("key and value must share a dtype")
     _check_step(cache, layer, "key", key)
-    _check_step(cache, layer, "value", value)
-    if key.dtype not in _DTYPES:
-        raise TypeError(f"key must use bfloat16, float16 or float32, not {key.dtype}")
-    if key.shape[1] != cache._struct.kv_heads or value.shape != key.shape:
-        raise ValueError(f"key and value must both have {cache.kv_heads} heads and the same tokens")
-    if value.dtype != key.dtype:
-        raise TypeError("key and value must share a dtype")
-    batch, _, tokens, _ = key.shape
+    tokens = shape[2]
+    rotary_at = query_heads = turned_at = 0
+    query_view = _NO_ROWS
+    if rotary is not None:
+        rotary_at, positions, table_device = rotary._facts
+        if positions < capacity:
+            raise ValueError(f"the rotation table holds {positions} positions, the cache {capacity} rows")
+        if table_device != device:
+            raise ValueError("all tensors must share one device")
     if query is not None:
-        _check_step(cache, layer, "query", query)
         if rotary is None:
             raise ValueError("queries are only turned: query needs rotary")
+        _, query_heads, query_tokens, _ = _check_step(cache, layer, "query", query)
         if query.dtype != key.dtype:
             raise TypeError("query and key must share a dtype")
-        if query.shape[1] == 0 or query.shape[2] != tokens:
+        if query_heads == 0 or query_tokens != tokens:
             raise ValueError(f"query must have heads and the keys' {tokens} tokens")
-    if rotary is not None and rotary.cosines.shape[0] < cache.capacity:
-        raise ValueError(f"the rotation table holds {rotary.positions} positions, the cache {cache.capacity} rows")
-    counts = _step_counts(cache, tokens, tree, counts)
-    device = _devices(cache, key, value, query, counts, None if rotary is None else rotary.cosines,
-                      None if tree is None else tree.depths)
+    counts_at, counts = _step_counts(cache, tokens, tree, counts)
+    if device < 0:
+        raise RuntimeError(_NEED_GPU)
     turned = None
     if query is not None:
-        turned = torch.empty((batch, tokens, query.shape[1], HEAD_DIM), dtype=cache.key_pages.dtype, device=device)
+        row = query_heads * HEAD_DIM
+        turned = cache.key_pages.new_empty_strided((batch, query_heads, tokens, HEAD_DIM), (tokens * row, HEAD_DIM, row, 1))
+        turned_at = turned.data_ptr()
+        query_view, query = _view(query)
     if tokens:
-        key_rows, key = _rows(key)
-        value_rows, value = _rows(value)
-        query_ref = None
-        if query is not None:
-            query_rows, query = _rows(query)
-            query_ref = ctypes.byref(query_rows)
-        _call(device, nat.lib().ckv_paged_append, cache._ref, layer, ctypes.byref(key_rows), ctypes.byref(value_rows),
-              query_ref, 0 if query is None else query.shape[1], tokens, nat.ptr(counts),
-              None if tree is None else tree.depths.data_ptr(), None if rotary is None else rotary._ref, _DTYPES[key.dtype],
-              nat.ptr(turned))
-    return None if turned is None else turned.transpose(1, 2)
+        key_view, key = _view(key)
+        value_view, value = _view(value)
+        args = nat.PAGED_APPEND_ARGS.pack(*key_view, *value_view, *query_view, counts_at, 0 if tree is None else tree._facts[4],
+                                          rotary_at, turned_at, layer, tokens, query_heads, dtype)
+        _launch(device, nat.lib().ckv_paged_append, cache._ref, args)
+    return turned
 
 
 def paged_attention(query: torch.Tensor, cache: PagedKVCache, *, softmax_scale: float, layer: int = 0,
@@ -362,21 +429,21 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, *, softmax_scale: 
     [batch, query heads, tokens] float32, natural log); a query past the counts gives
     zeros and -inf.  What a query does not see does not reach it, infinities and NaN
     included; an infinite value that it sees makes its output infinite or NaN."""
-    _check_step(cache, layer, "query", query)
+    _, batch, kv_heads, _, device = cache._facts
+    _, heads, tokens, _ = _check_step(cache, layer, "query", query)
     if query.dtype != cache.key_pages.dtype:
         raise TypeError(f"query must use the cache's {cache.dtype}, not {query.dtype}")
-    heads = query.shape[1]
-    if heads % cache._struct.kv_heads or not 1 <= heads // cache._struct.kv_heads <= nat.MAX_GROUP:
-        raise ValueError(f"query heads must be 1 to {nat.MAX_GROUP} times the {cache.kv_heads} KV heads, not {heads}")
+    if heads % kv_heads or not 1 <= heads // kv_heads <= nat.MAX_GROUP:
+        raise ValueError(f"query heads must be 1 to {nat.MAX_GROUP} times the {kv_heads} KV heads, not {heads}")
     if not 0.0 < softmax_scale <= 1e30:
         raise ValueError("softmax_scale must be positive and finite")
     if window < 0:
         raise ValueError("window must be non-negative")
-    batch, _, tokens, _ = query.shape
-    counts = _step_counts(cache, tokens, tree, counts)
-    device = _devices(cache, query, counts, None if tree is None else tree.depths)
-    out = torch.empty((batch, tokens, heads, HEAD_DIM), dtype=query.dtype, device=device)
-    lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=device)
+    counts_at, counts = _step_counts(cache, tokens, tree, counts)
+    if device < 0:
+        raise RuntimeError(_NEED_GPU)
+    out = query.new_empty((batch, tokens, heads, HEAD_DIM))
+    lse = query.new_empty((batch, heads, tokens), dtype=torch.float32)
     if tokens == 0:
         return out, lse
     lib = nat.lib()
@@ -385,10 +452,12 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, *, softmax_scale: 
     size = cache._sizes.get(call)
     if size is None:
         size = cache._sizes[call] = lib.ckv_paged_attention_workspace_bytes(cache._ref, heads, tokens, window)
-    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    rows, query = _rows(query)
-    _call(device, lib.ckv_paged_attention, cache._ref, layer, ctypes.byref(rows), heads, tokens, nat.ptr(counts),
-          None if tree is None else tree._ref, softmax_scale, window, out.data_ptr(), lse.data_ptr(), nat.ptr(workspace))
+    workspace = query.new_empty(size, dtype=torch.uint8) if size else None
+    view, query = _view(query)
+    args = nat.PAGED_ATTENTION_ARGS.pack(*view, counts_at, 0 if tree is None else tree._facts[3], out.data_ptr(),
+                                         lse.data_ptr(), workspace.data_ptr() if size else 0, layer, heads, tokens, window,
+                                         softmax_scale, 0)
+    _launch(device, lib.ckv_paged_attention, cache._ref, args)
     return out, lse
 
 
@@ -399,31 +468,33 @@ def paged_commit(cache: PagedKVCache, counts: int | torch.Tensor, *, path: torch
     n <= 512) the tokens ``path[b, :counts[b]]``, in ascending order, as a branch of a
     tree has them: their rows move together behind the committed ones.  A path ends
     at the first entry that does not ascend or lies past the capacity."""
-    amount = 0
+    _, batch, _, _, device = cache._facts
+    amount = counts_at = path_at = entries = 0
     if isinstance(counts, torch.Tensor):
-        if counts.dtype != torch.int32 or counts.shape != (cache.batch,):
-            raise TypeError(f"counts must be an int32 vector of one entry a sequence ({cache.batch})")
-        counts = counts.contiguous()
+        counts = _counts_vector(counts, batch, device)
+        counts_at = counts.data_ptr()
         amount = 2**31 - 1
     else:
         if counts < 0:
             raise ValueError("counts must be non-negative")
         amount, counts = min(counts, 2**31 - 1), None
-    entries = 0
     if path is not None:
-        if path.dtype != torch.int32 or path.ndim != 2 or path.shape[0] != cache.batch:
-            raise TypeError(f"path must be an int32 tensor [{cache.batch}, entries]")
-        if not 1 <= path.shape[1] <= MAX_DRAFT:
-            raise ValueError(f"a path may have 1 to {MAX_DRAFT} entries, not {path.shape[1]}")
-        path = path.contiguous()
-        entries = path.shape[1]
+        shape = path.shape
+        if path.dtype != torch.int32 or len(shape) != 2 or shape[0] != batch:
+            raise TypeError(f"path must be an int32 tensor [{batch}, entries]")
+        if not 1 <= shape[1] <= MAX_DRAFT:
+            raise ValueError(f"a path may have 1 to {MAX_DRAFT} entries, not {shape[1]}")
+        if path.get_device() != device:
+            raise ValueError("all tensors must share one device")
         if counts is None:
-            path = path[:, :amount].contiguous()
-            entries = path.shape[1]
-            if entries == 0:
-                return
-    device = _devices(cache, counts, path)
-    _call(device, nat.lib().ckv_paged_commit, cache._ref, amount, nat.ptr(counts), nat.ptr(path), entries)
+            path = path[:, :amount]
+        path = path.contiguous()
+        path_at, entries = path.data_ptr(), path.shape[1]
+        if entries == 0:
+            return
+    if device < 0:
+        raise RuntimeError(_NEED_GPU)
+    _launch(device, nat.lib().ckv_paged_commit, cache._ref, amount, counts_at, path_at, entries)
 
 
 __all__ = ["DraftTree", "PagedKVCache", "RotaryTable", "paged_append", "paged_attention", "paged_commit"]

@@ -18,7 +18,7 @@ int paged_launched(const char* what) {
 }
 
 int validate_paged_cache(const ckv_paged_cache* c, const char* what) {
-  if (!c || !c->key_pages || !c->value_pages || !c->page_table || !c->lengths || !c->overflow)
+  if (!c || !c->key_pages || !c->value_pages || !c->page_table || !c->lengths || !c->overflow || !c->counters)
     return paged_error(CKV_E_INVALID, what, "null argument");
   if (c->layers <= 0 || c->pages <= 0 || c->kv_heads <= 0 || c->table_pages <= 0 || c->batch <= 0)
     return paged_error(CKV_E_INVALID, what, "layers, pages, kv_heads, table_pages and batch must be positive");
@@ -74,16 +74,20 @@ __global__ __launch_bounds__(CKV_MAX_DRAFT) void tree_plan_kernel(const int32_t*
   uint64_t mine[MAX_WORDS];
 #pragma unroll
   for (int w = 0; w < MAX_WORDS; ++w) mine[w] = t < count && w == t >> 6 ? 1ull << (t & 63) : 0ull;
+  bool changed = true;
   while (__syncthreads_or(jump >= 0)) {
-    jump_s[t] = jump;
-#pragma unroll
-    for (int w = 0; w < MAX_WORDS; ++w)
-      if (w < words) mask_s[w][t] = mine[w];
-    __syncthreads();
-    if (jump >= 0) {
+    if (changed) {
+      jump_s[t] = jump;
 #pragma unroll
       for (int w = 0; w < MAX_WORDS; ++w)
-        if (w < words) mine[w] |= mask_s[w][jump];
+        if (w <= t >> 6) mask_s[w][t] = mine[w];
+    }
+    __syncthreads();
+    changed = jump >= 0;
+    if (changed) {
+#pragma unroll
+      for (int w = 0; w < MAX_WORDS; ++w)
+        if (w <= jump >> 6) mine[w] |= mask_s[w][jump];  // ancestors are earlier tokens
       jump = jump_s[jump];
     }
   }
@@ -279,50 +283,59 @@ __device__ inline int path_length(const CommitArgs& a, int b, int room) {
   return count;
 }
 
+constexpr int COUNTER_STRIDE = CKV_QUANT_COUNTERS;  // words between two sequences' counters: a cache line each
 constexpr int MOVE_LOADS = 4;  // of four rows each
+constexpr int MOVE_WORKGROUPS = 64;  // of a sequence: each takes a ticket of its counter
 
-// A wave a (sequence, layer, head, keys or values): 16 lanes a row, 16 rows at a time.  The entries ascend, so
+// A wave takes (layer, head, keys or values) of a sequence in turn: 16 lanes a row, 16 rows at a time.  The entries ascend, so
 // entry j's source is row j or a later one and no later entry reads what an earlier one wrote; within a batch every
 // load is issued before the first store.  Rows whose page is none stay where they are.  Bound by latency: a chain of
 // cursor, path, pages, rows.
 __global__ __launch_bounds__(THREADS) void move_kernel(const CommitArgs a) {
   const ckv_paged_cache& c = a.cache;
   const int b = blockIdx.y, lane = threadIdx.x & 63;
-  const int number = __builtin_amdgcn_readfirstlane(blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6));
-  const int head = number % c.kv_heads, plane = number / c.kv_heads, layer = plane >> 1;
-  if (layer >= c.layers) return;
   const int start = paged_length(c, b), size = path_length(a, b, paged_capacity(c) - start);
+  // every wave has read the length: the last workgroup to come here writes the new one
+  __syncthreads();
+  if (threadIdx.x == 0 && atomicAdd(c.counters + b * COUNTER_STRIDE, 1u) == gridDim.x - 1) {
+    c.counters[b * COUNTER_STRIDE] = 0;
+    c.lengths[b] = start + size;
+  }
   const int64_t head_rows = (int64_t)c.kv_heads * c.page_size;
-  uint16_t* pages = reinterpret_cast<uint16_t*>(plane & 1 ? c.value_pages : c.key_pages) +
-                    ((int64_t)layer * c.pages * head_rows + (int64_t)head * c.page_size) * D + 8 * (lane & 15);
   const int32_t* table = c.page_table + (int64_t)b * c.table_pages;
   const int32_t* path = a.path + (int64_t)b * a.path_tokens;
-  for (int j0 = 0; j0 < size; j0 += 4 * MOVE_LOADS) {
-    uint4 w[MOVE_LOADS];
-    int64_t to[MOVE_LOADS];
+  const int planes = 2 * c.layers * c.kv_heads;
+  for (int number = blockIdx.x * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); number < planes;
+       number += gridDim.x * (THREADS / 64)) {
+    const int head = number % c.kv_heads, plane = number / c.kv_heads, layer = plane >> 1;
+    uint16_t* pages = reinterpret_cast<uint16_t*>(plane & 1 ? c.value_pages : c.key_pages) +
+                      ((int64_t)layer * c.pages * head_rows + (int64_t)head * c.page_size) * D + 8 * (lane & 15);
+    for (int j0 = 0; j0 < size; j0 += 4 * MOVE_LOADS) {
+      uint4 w[MOVE_LOADS];
+      int64_t to[MOVE_LOADS];
 #pragma unroll
-    for (int i = 0; i < MOVE_LOADS; ++i) {
-      const int j = j0 + 4 * i + (lane >> 4);
-      to[i] = -1;
-      if (j >= size || path[j] == j) continue;
-      const int source = start + path[j], row = start + j;
-      const int from_page = gload_i32(table + source / c.page_size), page = gload_i32(table + row / c.page_size);
-      if ((uint32_t)from_page >= (uint32_t)c.pages || (uint32_t)page >= (uint32_t)c.pages) continue;
-      w[i] = gload16(pages + (from_page * head_rows + (source & (c.page_size - 1))) * D);
-      to[i] = (page * head_rows + (row & (c.page_size - 1))) * D;
+      for (int i = 0; i < MOVE_LOADS; ++i) {
+        const int j = j0 + 4 * i + (lane >> 4);
+        to[i] = -1;
+        if (j >= size || path[j] == j) continue;
+        const int source = start + path[j], row = start + j;
+        const int from_page = gload_i32(table + source / c.page_size), page = gload_i32(table + row / c.page_size);
+        if ((uint32_t)from_page >= (uint32_t)c.pages || (uint32_t)page >= (uint32_t)c.pages) continue;
+        w[i] = gload16(pages + (from_page * head_rows + (source & (c.page_size - 1))) * D);
+        to[i] = (page * head_rows + (row & (c.page_size - 1))) * D;
+      }
+#pragma unroll
+      for (int i = 0; i < MOVE_LOADS; ++i)
+        if (to[i] >= 0) *reinterpret_cast<uint4*>(pages + to[i]) = w[i];
     }
-#pragma unroll
-    for (int i = 0; i < MOVE_LOADS; ++i)
-      if (to[i] >= 0) *reinterpret_cast<uint4*>(pages + to[i]) = w[i];
   }
 }
 
-// A wave a sequence, behind the moves, which read the lengths.
+// Without a path: a wave a sequence.
 __global__ __launch_bounds__(64) void advance_kernel(const CommitArgs a) {
   const ckv_paged_cache& c = a.cache;
-  const int b = blockIdx.x, start = paged_length(c, b), room = paged_capacity(c) - start;
-  const int size = a.path ? path_length(a, b, room) : min(step_count(a.counts, a.tokens, b), room);
-  if (threadIdx.x == 0) c.lengths[b] = start + size;
+  const int b = blockIdx.x, start = paged_length(c, b);
+  if (threadIdx.x == 0) c.lengths[b] = start + min(step_count(a.counts, a.tokens, b), paged_capacity(c) - start);
 }
 
 }  // namespace
@@ -338,22 +351,23 @@ extern "C" int ckv_draft_tree_plan(const int32_t* parents, const int32_t* counts
   return paged_launched(what);
 }
 
-extern "C" int ckv_paged_append(const ckv_paged_cache* cache, int32_t layer, const ckv_quant_rows* key,
-                                const ckv_quant_rows* value, const ckv_quant_rows* query, int32_t query_heads,
-                                int32_t tokens, const int32_t* counts, const int32_t* depths, const ckv_rotary* rotary,
-                                int32_t dtype, void* query_out, void* stream) {
+extern "C" int ckv_paged_append(const ckv_paged_cache* cache, const ckv_paged_append_args* args, void* stream) {
   const char* what = "ckv_paged_append";
   int rc = validate_paged_cache(cache, what);
   if (rc) return rc;
-  if (layer < 0 || layer >= cache->layers) return paged_error(CKV_E_INVALID, what, "no such layer");
-  if (dtype != CKV_BF16 && dtype != CKV_F16 && dtype != CKV_F32)
+  if (!args) return paged_error(CKV_E_INVALID, what, "null argument");
+  const ckv_rotary* rotary = args->rotary;
+  const bool query = args->query.data != nullptr;
+  if (args->layer < 0 || args->layer >= cache->layers) return paged_error(CKV_E_INVALID, what, "no such layer");
+  if (args->dtype != CKV_BF16 && args->dtype != CKV_F16 && args->dtype != CKV_F32)
     return paged_error(CKV_E_INVALID, what, "dtype must be bf16, fp16 or f32");
-  if (tokens <= 0) return paged_error(CKV_E_INVALID, what, "tokens must be positive");
-  rc = check_paged_rows(key, dtype, what);
-  if (!rc) rc = check_paged_rows(value, dtype, what);
-  if (!rc && query) rc = check_paged_rows(query, dtype, what);
+  if (args->tokens <= 0) return paged_error(CKV_E_INVALID, what, "tokens must be positive");
+  rc = check_paged_rows(&args->key, args->dtype, what);
+  if (!rc) rc = check_paged_rows(&args->value, args->dtype, what);
+  if (!rc && query) rc = check_paged_rows(&args->query, args->dtype, what);
   if (rc) return rc;
-  if (query && (!query_out || !rotary || query_heads <= 0 || query_heads > (1 << 20)))
+  if (query && (!args->query_out || ((uintptr_t)args->query_out & 15) || !rotary || args->query_heads <= 0 ||
+                args->query_heads > (1 << 20)))
     return paged_error(CKV_E_INVALID, what, "a query needs its output, its heads and the rotation");
   if (rotary) {
     if (!rotary->cosines || !rotary->sines || (((uintptr_t)rotary->cosines | (uintptr_t)rotary->sines) & 15))
@@ -365,19 +379,19 @@ extern "C" int ckv_paged_append(const ckv_paged_cache* cache, int32_t layer, con
   }
   AppendArgs a{};
   a.cache = *cache;
-  a.key = *key;
-  a.value = *value;
-  if (query) a.query = *query;
+  a.key = args->key;
+  a.value = args->value;
+  a.query = args->query;
   if (rotary) a.rotary = *rotary;
-  a.counts = counts;
-  a.depths = depths;
-  a.query_out = query_out;
-  a.layer_offset = (int64_t)layer * cache->pages * cache->kv_heads * cache->page_size * D;
-  a.tokens = tokens;
-  a.query_heads = query ? query_heads : 0;
+  a.counts = args->counts;
+  a.depths = args->depths;
+  a.query_out = args->query_out;
+  a.layer_offset = (int64_t)args->layer * cache->pages * cache->kv_heads * cache->page_size * D;
+  a.tokens = args->tokens;
+  a.query_heads = query ? args->query_heads : 0;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == CKV_BF16) return launch_append<CKV_BF16>(a, s);
-  if (dtype == CKV_F16) return launch_append<CKV_F16>(a, s);
+  if (args->dtype == CKV_BF16) return launch_append<CKV_BF16>(a, s);
+  if (args->dtype == CKV_F16) return launch_append<CKV_F16>(a, s);
   return launch_append<CKV_F32>(a, s);
 }
 
@@ -392,11 +406,10 @@ extern "C" int ckv_paged_commit(const ckv_paged_cache* cache, int32_t tokens, co
   const CommitArgs a{*cache, counts, path, tokens, path_tokens};
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (path) {
-    const int64_t waves = 2 * (int64_t)cache->layers * cache->kv_heads;
-    if (waves > 0x7fffffff) return paged_error(CKV_E_LIMIT, what, "too many layers");
-    move_kernel<<<dim3((uint32_t)((waves + THREADS / 64 - 1) / (THREADS / 64)), cache->batch), THREADS, 0, s>>>(a);
-    const int moved = paged_launched(what);
-    if (moved) return moved;
+    const int64_t waves = 2 * (int64_t)cache->layers * cache->kv_heads, blocks = (waves + THREADS / 64 - 1) / (THREADS / 64);
+    if (waves > 0x3fffffff) return paged_error(CKV_E_LIMIT, what, "too many layers");
+    move_kernel<<<dim3((uint32_t)(blocks < MOVE_WORKGROUPS ? blocks : MOVE_WORKGROUPS), cache->batch), THREADS, 0, s>>>(a);
+    return paged_launched(what);
   }
   advance_kernel<<<cache->batch, 64, 0, s>>>(a);
   return paged_launched(what);

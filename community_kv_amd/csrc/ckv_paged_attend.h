@@ -27,6 +27,7 @@ struct PagedAttendArgs {
   float* part_max;         // [kv_heads][row_pad][parts], log2
   float* part_sum;
   float* part_acc;         // [kv_heads][parts][row_pad][128]
+  int2* part_of;           // [batch]: a sequence's first part and their number
   float scale_log2;        // softmax_scale * log2 e
   int32_t tokens, group, rows, row_pad, window, parts, words, page_log2;
   uint32_t group_magic;    // ceil(2^32 / group), 0 for a group of one
@@ -54,6 +55,12 @@ struct PagedRows {
     return max(s.total - s.first(a), 0);
   }
 };
+
+// The parts of a sequence, told to the join by its first one.
+__device__ inline void tell_parts(const PagedAttendArgs& a, const Part& part) {
+  if (a.parts > a.cache.batch && part.index == 0 && blockIdx.x % a.cache.kv_heads == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+    a.part_of[part.sequence] = int2{part.first, part.count};
+}
 
 // row / group without a division: exact while row * group < 2^32 (rows are below 2^22, groups at most 16).
 __device__ inline int paged_token(const PagedAttendArgs& a, int row) {
@@ -93,14 +100,23 @@ struct PagedHead {
   }
 };
 
-// What one query row sees: rows lo .. hi, and of a tree's rows (start and on) those of its mask.
+// What one query row sees: rows lo .. hi, and of a tree's rows (start and on) those of its mask, whose first word is
+// kept (trees of up to 64 tokens have no other).
 struct Sight {
   int lo, hi, token;
   bool live;
+  uint64_t kin0;
+  Sight() = default;
   __device__ Sight(const PagedAttendArgs& a, const PagedStep& s, int b, int row) {
     token = min(paged_token(a, row), a.tokens - 1);
     live = row < a.rows && token < s.count;
-    const int position = s.start + (a.masks ? gload_i32(a.depths + (int64_t)b * a.tokens + token) : token);
+    int position = s.start + token;
+    kin0 = 0;
+    if (a.masks) {
+      const int64_t at = (int64_t)b * a.tokens + token;
+      kin0 = a.masks[at * a.words];
+      position = s.start + gload_i32(a.depths + at);
+    }
     lo = a.window > 0 ? max(position - a.window + 1, 0) : 0;
     hi = min(a.masks ? s.total : s.start + token + 1, s.total) - 1;
     if (!live) hi = -1;
@@ -112,17 +128,20 @@ struct Sight {
     uint64_t seen = (~0ull >> (63 - high)) & (~0ull << low);
     if (a.masks && first + 63 >= s.start) {
       const int j = first - s.start;  // the draft's token in the first row
-      const uint64_t* mask = a.masks + ((int64_t)b * a.tokens + token) * a.words;
       uint64_t kin;
       if (j < 0) {
-        kin = (mask[0] << -j) | (~0ull >> (64 + j));  // -64 < j: rows before the draft are all there
+        kin = (kin0 << -j) | (~0ull >> (64 + j));  // -64 < j: rows before the draft are all there
       } else {
         const int w = j >> 6, shift = j & 63;
-        kin = w < a.words ? mask[w] >> shift : 0;
-        if (shift && w + 1 < a.words) kin |= mask[w + 1] << (64 - shift);
+        kin = w == 0 ? kin0 >> shift : 0;
+        if (a.words > 1) {
+          const uint64_t* mask = a.masks + ((int64_t)b * a.tokens + token) * a.words;
+          if (w && w < a.words) kin = mask[w] >> shift;
+          if (shift && w + 1 < a.words) kin |= mask[w + 1] << (64 - shift);
+        }
       }
       seen &= kin;
-      if (a.window > 0) {  // ancestors out of the window: a draft row's position goes by its depth
+      if (lo > s.start) {  // ancestors out of the window: a draft row's position goes by its depth
         uint64_t drafted = seen & (j < 0 ? ~0ull << -j : ~0ull);
         while (drafted) {
           const int i = __ffsll((unsigned long long)drafted) - 1;

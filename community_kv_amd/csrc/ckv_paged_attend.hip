@@ -130,7 +130,7 @@ __device__ inline void add_step(const float* sc, const uint4* vop, Running& r) {
 // head) for 16 RT query rows; its waves take steps in turn and join in LDS.
 // Bound by memory.
 template <int DT, int RT>
-__global__ __launch_bounds__(64 * WAVES, RT <= 2 ? 2 : 1) void paged_split_kernel(const PagedAttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedAttendArgs a) {
   __shared__ float m_s[WAVES][16];
   __shared__ float l_s[WAVES][16];
   __shared__ float o_s[WAVES][16 * D];
@@ -141,6 +141,7 @@ __global__ __launch_bounds__(64 * WAVES, RT <= 2 ? 2 : 1) void paged_split_kerne
   const Part part = find_part(PagedRows{a}, a.parts, number, -1);
   const int b = part.sequence;
   if (b < 0) return;  // the join knows how many parts there are
+  tell_parts(a, part);
   const PagedStep step(a, b);
   const PagedHead q(a, b, h);
   // tokens of this workgroup's rows, and the rows that all and that any of them see
@@ -171,16 +172,13 @@ __global__ __launch_bounds__(64 * WAVES, RT <= 2 ? 2 : 1) void paged_split_kerne
 #pragma unroll
     for (int nb = 0; nb < 8; ++nb) run[r].o[nb] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  int t0 = begin + wave * STEP;
+  Sight sight[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) sight[r] = Sight(a, step, b, row0 + 16 * r + col);
   const int last = step.total - 1;
-  StepPages pages{0, 0};
-  if (t0 < end) pages = step_pages(q, t0, last);
-  for (; t0 < end; t0 += WAVES * STEP) {
-    StepRows rows;
-    load_step(q, t0, pages, rows);
+  auto add = [&](StepRows& rows, const StepPages& pages, int t0) __attribute__((always_inline)) {
     const bool bad = __ballot(!q.good(pages.k) || !q.good(pages.v)) != 0;
     const bool good_rows = q.good(pages.v);
-    if (t0 + WAVES * STEP < end) pages = step_pages(q, t0 + WAVES * STEP, last);
     const bool masked = bad || t0 < clear_lo || t0 + STEP - 1 > clear_hi;
     bool special = false;
     if (masked) {  // a masked row's zero probability times infinity or NaN would spread it
@@ -213,8 +211,7 @@ __global__ __launch_bounds__(64 * WAVES, RT <= 2 ? 2 : 1) void paged_split_kerne
         for (int i = 0; i < 4; ++i) sc[4 * j + i] = acc[i] * a.scale_log2;
       }
       if (masked) {
-        const Sight sight(a, step, b, row0 + 16 * r + col);
-        seen[r] = good_rows ? (uint32_t)sight.rows(a, step, b, t0 + 8 * L) & 0xffu : 0u;
+        seen[r] = good_rows ? (uint32_t)sight[r].rows(a, step, b, t0 + 8 * L) & 0xffu : 0u;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sc[i] = (seen[r] >> i) & 1 ? sc[i] : NEG_INF;
       }
@@ -247,6 +244,19 @@ __global__ __launch_bounds__(64 * WAVES, RT <= 2 ? 2 : 1) void paged_split_kerne
         }
       }
     }
+  };
+  // A step's pages are read a step ahead.  (Reading its rows ahead too, into a second set of registers, changes nothing:
+  // two waves a SIMD have enough in flight.)
+  constexpr int STRIDE = WAVES * STEP;
+  int t0 = begin + wave * STEP;
+  StepPages pages{0, 0};
+  if (t0 < end) pages = step_pages(q, t0, last);
+  for (; t0 < end; t0 += STRIDE) {
+    StepRows rows;
+    load_step(q, t0, pages, rows);
+    const StepPages of = pages;
+    if (t0 + STRIDE < end) pages = step_pages(q, t0 + STRIDE, last);
+    add(rows, of, t0);
   }
   // join the waves, 16 query rows at a time
 #pragma unroll
@@ -266,37 +276,47 @@ __global__ __launch_bounds__(64 * WAVES, RT <= 2 ? 2 : 1) void paged_split_kerne
       p[1] = float4{run[r].o[4][i], run[r].o[5][i], run[r].o[6][i], run[r].o[7][i]};
     }
     __syncthreads();
-    for (int x = tid; x < 16 * D; x += 64 * WAVES) {
-      const int i = x >> 7, d = x & (D - 1), row = at0 + i;
-      if (row >= a.rows) continue;
-      const bool live = paged_token(a, row) < step.count;
-      float m = m_s[0][i];
+    // 16 threads a query row, eight dims each
+    const int i = tid >> 4, d = 8 * (tid & 15), row = at0 + i;
+    if (row >= a.rows) continue;
+    float m = m_s[0][i];
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) m = fmaxf(m, m_s[w][i]);
-      const float at = m == NEG_INF ? 0.0f : m;
-      float sum = 0.0f, acc = 0.0f;
+    for (int w = 1; w < WAVES; ++w) m = fmaxf(m, m_s[w][i]);
+    const float at = m == NEG_INF ? 0.0f : m;
+    float sum = 0.0f, acc[8] = {};
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        // a wave without a row has zeros and a maximum of -inf
-        const float f = __builtin_amdgcn_exp2f(m_s[w][i] - at);
-        sum += l_s[w][i] * f;
-        acc += o_s[w][x] * f;
-      }
-      if (!live) {
-        m = NEG_INF;
-        sum = acc = 0.0f;
-      }
-      if (part.count == 1) {
-        int64_t at_out, at_lse;
-        paged_output_index(a, b, h, row, &at_out, &at_lse);
-        store_value<DT>(a.out, at_out + d, sum == 0.0f ? 0.0f : acc / sum);
-        if (d == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
-      } else {
-        a.part_acc[(((int64_t)h * a.parts + number) * a.row_pad + row) * D + d] = acc;
-        if (d == 0) {
-          a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m;
-          a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
-        }
+    for (int w = 0; w < WAVES; ++w) {
+      // a wave without a row has zeros and a maximum of -inf
+      const float f = __builtin_amdgcn_exp2f(m_s[w][i] - at);
+      const float4 x = *reinterpret_cast<const float4*>(&o_s[w][i * D + d]), y = *reinterpret_cast<const float4*>(&o_s[w][i * D + d + 4]);
+      sum += l_s[w][i] * f;
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += v[e] * f;
+    }
+    if (paged_token(a, row) >= step.count) {  // no token
+      m = NEG_INF;
+      sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+    }
+    if (part.count == 1) {
+      int64_t at_out, at_lse;
+      paged_output_index(a, b, h, row, &at_out, &at_lse);
+      const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = sum == 0.0f ? 0.0f : acc[e] * scale;
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at_out + d) =
+          uint4{pack_store<DT>(acc[0], acc[1]), pack_store<DT>(acc[2], acc[3]), pack_store<DT>(acc[4], acc[5]),
+                pack_store<DT>(acc[6], acc[7])};
+      if (d == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+    } else {
+      float4* to = reinterpret_cast<float4*>(a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + row) * D + d);
+      to[0] = float4{acc[0], acc[1], acc[2], acc[3]};
+      to[1] = float4{acc[4], acc[5], acc[6], acc[7]};
+      if (d == 0) {
+        a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m;
+        a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
       }
     }
   }
@@ -313,16 +333,16 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAtt
   __shared__ float scratch[4];
   __shared__ float4 acc_s[JOIN_THREADS];
   const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-  const Part part = find_part(PagedRows{a}, a.parts, 0, b);
-  if (part.count == 1) return;  // written already
-  const float* pm = a.part_max + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
-  const float* pl = a.part_sum + ((int64_t)h * a.row_pad + row) * a.parts + part.first;
+  const int2 part = a.part_of[b];  // the first and their number
+  if (part.y == 1) return;  // written already
+  const int64_t first = ((int64_t)h * a.row_pad + row) * a.parts + part.x;
+  const float *pm = a.part_max + first, *pl = a.part_sum + first;
   float m = NEG_INF;
-  for (int s = tid & 63; s < part.count; s += 64) m = fmaxf(m, pm[s]);
+  for (int s = tid & 63; s < part.y; s += 64) m = fmaxf(m, pm[s]);
   m = wave_max(m);  // every wave for itself
   const float at = m == NEG_INF ? 0.0f : m;
   float sum = 0.0f;
-  for (int s = tid; s < part.count; s += JOIN_THREADS) {
+  for (int s = tid; s < part.y; s += JOIN_THREADS) {
     const float f = __builtin_amdgcn_exp2f(pm[s] - at);
     factor[s] = f;
     sum += pl[s] * f;
@@ -333,9 +353,9 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAtt
   sum = (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
   const int dim = 4 * (tid & 31);
   float4 acc{0.0f, 0.0f, 0.0f, 0.0f};
-  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.first) * a.row_pad + row) * D + dim;
+  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.x) * a.row_pad + row) * D + dim;
 #pragma unroll 4
-  for (int s = tid >> 5; s < part.count; s += JOIN_THREADS / 32) {
+  for (int s = tid >> 5; s < part.y; s += JOIN_THREADS / 32) {
     const float4 x = *reinterpret_cast<const float4*>(pa + (int64_t)s * a.row_pad * D);
     const float f = factor[s];
     acc.x += x.x * f;
@@ -356,63 +376,85 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAtt
   if (tid == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
 }
 
-// The same for many query rows, of few parts mostly: a wave a row, two dims a lane.
+// The same for many query rows, of few parts mostly: half a wave a row, four dims a lane; the first parts' outputs are
+// read along with their maxima.
 template <int DT>
-__global__ __launch_bounds__(256) void paged_join_rows_kernel(const PagedAttendArgs a) {
-  const int row = 4 * blockIdx.x + (threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63;
+__global__ __launch_bounds__(JOIN_THREADS) void paged_join_rows_kernel(const PagedAttendArgs a) {
+  constexpr int TOGETHER = 4;  // parts in flight
+  const int row = (JOIN_THREADS / 32) * blockIdx.x + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
   if (row >= a.rows) return;
-  const Part part = find_part(PagedRows{a}, a.parts, 0, b);
-  if (part.count == 1) return;
-  const int64_t first = ((int64_t)h * a.row_pad + row) * a.parts + part.first;
-  float m = NEG_INF;
-  for (int s = lane; s < part.count; s += 64) m = fmaxf(m, a.part_max[first + s]);
-  m = wave_max(m);
-  const float at = m == NEG_INF ? 0.0f : m;
-  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.first) * a.row_pad + row) * D + 2 * lane;
-  float sum = 0.0f;
-  float2 acc{0.0f, 0.0f};
-  for (int s0 = 0; s0 < part.count; s0 += 64) {
-    const int left = min(part.count - s0, 64);
-    float f = 0.0f, share = 0.0f;
-    if (lane < left) {
-      f = __builtin_amdgcn_exp2f(a.part_max[first + s0 + lane] - at);
-      share = a.part_sum[first + s0 + lane] * f;
+  const int2 part = a.part_of[b];
+  if (part.y == 1) return;
+  const int64_t first = ((int64_t)h * a.row_pad + row) * a.parts + part.x;
+  const float *pm = a.part_max + first, *pl = a.part_sum + first;
+  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.x) * a.row_pad + row) * D + 4 * lane;
+  const int64_t stride = (int64_t)a.row_pad * D;
+  float m = NEG_INF, sum = 0.0f;
+  float4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = 0; s0 < part.y; s0 += TOGETHER) {
+    float ms[TOGETHER], ls[TOGETHER];
+    float4 xs[TOGETHER];
+    const int left = part.y - s0;
+#pragma unroll
+    for (int i = 0; i < TOGETHER; ++i) {
+      const int s = s0 + min(i, left - 1);
+      xs[i] = *reinterpret_cast<const float4*>(pa + s * stride);
+      ms[i] = pm[s];
+      ls[i] = pl[s];
     }
-    sum += wave_sum_tree(share);
-#pragma unroll 4
-    for (int s = 0; s < left; ++s) {
-      const float2 x = *reinterpret_cast<const float2*>(pa + (int64_t)(s0 + s) * a.row_pad * D);
-      const float of = ckv_u2f((uint32_t)__builtin_amdgcn_readlane((int)ckv_f2u(f), s));
-      acc.x += x.x * of;
-      acc.y += x.y * of;
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < TOGETHER; ++i) top = fmaxf(top, ms[i]);
+    const float at = top == NEG_INF ? 0.0f : top, before = __builtin_amdgcn_exp2f(m - at);
+    m = top;
+    sum *= before;
+    acc = float4{acc.x * before, acc.y * before, acc.z * before, acc.w * before};
+#pragma unroll
+    for (int i = 0; i < TOGETHER; ++i) {
+      if (i >= left) break;
+      const float f = __builtin_amdgcn_exp2f(ms[i] - at);
+      sum += ls[i] * f;
+      acc.x += xs[i].x * f;
+      acc.y += xs[i].y * f;
+      acc.z += xs[i].z * f;
+      acc.w += xs[i].w * f;
     }
   }
   int64_t at_out, at_lse;
   paged_output_index(a, b, h, row, &at_out, &at_lse);
-  const float x = sum == 0.0f ? 0.0f : acc.x / sum, y = sum == 0.0f ? 0.0f : acc.y / sum;
-  *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + at_out + 2 * lane) = pack_store<DT>(x, y);
+  const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float4 x = sum == 0.0f ? float4{0.0f, 0.0f, 0.0f, 0.0f} : float4{acc.x * scale, acc.y * scale, acc.z * scale, acc.w * scale};
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at_out + 4 * lane) =
+      uint2{pack_store<DT>(x.x, x.y), pack_store<DT>(x.z, x.w)};
   if (lane == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
 }
 
 constexpr int64_t MAX_ROWS = 1 << 21;  // query rows of a head: the grids' second dimension holds their blocks
 
+// Cache rows times blocks of 16 query rows, over all heads, up to which the few-row kernel takes a call, and up to which
+// it does so with one tile of query rows a workgroup instead of two.
+constexpr int64_t FEW_WORK = 400000, ONE_TILE_WORK = 128000;
+
 // How a call is laid out: which kernel, how many parts, and the workspace.
 struct PagedLayout {
   int parts, row_pad, tiles;  // tiles of 16 query rows a workgroup of the few-row kernel, 0: the many-row kernel
-  size_t max, sum, acc, bytes;
+  bool wide_join;
+  size_t max, sum, acc, of, bytes;
   PagedLayout(const ckv_paged_cache* c, int tokens, int group, int window) {
     const int rows = tokens * group;
     row_pad = (rows + 15) / 16 * 16;
-    tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 0;
-    const int64_t block = tiles ? 16 * tiles : paged_row_block(rows);
-    const int64_t blocks = (rows + block - 1) / block;
     int64_t most = (int64_t)c->table_pages * c->page_size;  // rows that a sequence's tokens may see
     if (window > 0 && (int64_t)window + tokens + 2 * PART_UNIT < most) most = (int64_t)window + tokens + 2 * PART_UNIT;
+    const int64_t work = (int64_t)c->batch * c->kv_heads * (row_pad / 16) * most;
+    tiles = rows <= 16 || work <= ONE_TILE_WORK ? 1 : rows <= 32 || work <= FEW_WORK ? 2 : 0;
+    const int64_t block = tiles ? 16 * tiles : paged_row_block(rows);
+    const int64_t blocks = (rows + block - 1) / block;
     const int64_t units = (most + PART_UNIT - 1) / PART_UNIT;
-    const int64_t workgroups = tiles == 1 || tiles == 2 ? 512 : 256;
+    const int64_t workgroups = tiles || paged_row_block(rows) == 128 ? 512 : 256;
     const int64_t want = workgroups / (c->kv_heads * blocks);
     if (want < (tiles ? c->batch + 1 : 2 * c->batch) || units <= (tiles ? 6 : 1)) parts = c->batch;
     else parts = (int)(want < c->batch * units ? want : c->batch * units);
+    wide_join = parts > 8 * c->batch;  // parts of a sequence, on average
     size_t at = 0;
     auto take = [&](size_t size) {
       const size_t here = at;
@@ -423,6 +465,7 @@ struct PagedLayout {
     max = take(each);
     sum = take(each);
     acc = take(each * D);
+    of = take(each ? c->batch * sizeof(int2) : 0);
     bytes = at;
   }
 };
@@ -431,17 +474,16 @@ template <int DT>
 int launch_few(const PagedAttendArgs& a, int tiles, hipStream_t s) {
   const dim3 grid(a.parts * a.cache.kv_heads, (a.rows + 16 * tiles - 1) / (16 * tiles));
   if (tiles == 1) paged_split_kernel<DT, 1><<<grid, 64 * WAVES, 0, s>>>(a);
-  else if (tiles == 2) paged_split_kernel<DT, 2><<<grid, 64 * WAVES, 0, s>>>(a);
-  else paged_split_kernel<DT, 4><<<grid, 64 * WAVES, 0, s>>>(a);
+  else paged_split_kernel<DT, 2><<<grid, 64 * WAVES, 0, s>>>(a);
   return paged_launched("ckv_paged_attention");
 }
 
 template <int DT>
-int launch_attend(const PagedAttendArgs& a, int tiles, hipStream_t s) {
-  const int rc = tiles ? launch_few<DT>(a, tiles, s) : launch_paged_rows(a, s);
+int launch_attend(const PagedAttendArgs& a, const PagedLayout& lay, hipStream_t s) {
+  const int rc = lay.tiles ? launch_few<DT>(a, lay.tiles, s) : launch_paged_rows(a, s);
   if (rc || a.parts == a.cache.batch) return rc;
-  if (tiles) paged_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
-  else paged_join_rows_kernel<DT><<<dim3((a.rows + 3) / 4, a.cache.kv_heads, a.cache.batch), 256, 0, s>>>(a);
+  if (lay.wide_join) paged_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
+  else paged_join_rows_kernel<DT><<<dim3((a.rows + 7) / 8, a.cache.kv_heads, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
   return paged_launched("ckv_paged_attention");
 }
 
@@ -457,16 +499,16 @@ extern "C" size_t ckv_paged_attention_workspace_bytes(const ckv_paged_cache* cac
   return PagedLayout(cache, tokens, (int)group, window).bytes;
 }
 
-extern "C" int ckv_paged_attention(const ckv_paged_cache* cache, int32_t layer, const ckv_quant_rows* query,
-                                   int32_t query_heads, int32_t tokens, const int32_t* counts,
-                                   const ckv_draft_tree* tree, float softmax_scale, int32_t window, void* out, float* lse,
-                                   void* workspace, void* stream) {
+extern "C" int ckv_paged_attention(const ckv_paged_cache* cache, const ckv_paged_attention_args* args, void* stream) {
   const char* what = "ckv_paged_attention";
   int rc = validate_paged_cache(cache, what);
   if (rc) return rc;
+  if (!args) return paged_error(CKV_E_INVALID, what, "null argument");
+  const int layer = args->layer, query_heads = args->query_heads, tokens = args->tokens, window = args->window;
+  const ckv_draft_tree* tree = args->tree;
   if (layer < 0 || layer >= cache->layers) return paged_error(CKV_E_INVALID, what, "no such layer");
-  if (!out || !lse) return paged_error(CKV_E_INVALID, what, "null argument");
-  rc = check_paged_rows(query, cache->dtype, what);
+  if (!args->out || ((uintptr_t)args->out & 15) || !args->lse) return paged_error(CKV_E_INVALID, what, "null argument");
+  rc = check_paged_rows(&args->query, cache->dtype, what);
   if (rc) return rc;
   if (query_heads <= 0 || query_heads % cache->kv_heads)
     return paged_error(CKV_E_INVALID, what, "query heads must be a multiple of the cache's heads");
@@ -476,26 +518,27 @@ extern "C" int ckv_paged_attention(const ckv_paged_cache* cache, int32_t layer, 
   if ((int64_t)tokens * group > MAX_ROWS) return paged_error(CKV_E_LIMIT, what, "more than 2^21 query rows a head");
   if (tree && (!tree->depths || !tree->masks)) return paged_error(CKV_E_INVALID, what, "null argument");
   if (tree && tokens > CKV_MAX_DRAFT) return paged_error(CKV_E_LIMIT, what, "a tree of more than 512 tokens");
-  if (!(softmax_scale > 0.0f) || softmax_scale > 1e30f)
+  if (!(args->softmax_scale > 0.0f) || args->softmax_scale > 1e30f)
     return paged_error(CKV_E_INVALID, what, "softmax_scale must be positive");
   const PagedLayout lay(cache, tokens, group, window);
-  if (lay.bytes && (!workspace || ((uintptr_t)workspace & 15))) return paged_error(CKV_E_INVALID, what, "workspace");
-  char* ws = reinterpret_cast<char*>(workspace);
+  if (lay.bytes && (!args->workspace || ((uintptr_t)args->workspace & 15))) return paged_error(CKV_E_INVALID, what, "workspace");
+  char* ws = reinterpret_cast<char*>(args->workspace);
   PagedAttendArgs a{};
   a.cache = *cache;
   const size_t layer_bytes = (size_t)cache->pages * cache->kv_heads * cache->page_size * D * 2;
   a.cache.key_pages = reinterpret_cast<char*>(cache->key_pages) + layer * layer_bytes;
   a.cache.value_pages = reinterpret_cast<char*>(cache->value_pages) + layer * layer_bytes;
-  a.query = *query;
-  a.counts = counts;
+  a.query = args->query;
+  a.counts = args->counts;
   a.depths = tree ? tree->depths : nullptr;
   a.masks = tree ? tree->masks : nullptr;
-  a.out = out;
-  a.lse = lse;
+  a.out = args->out;
+  a.lse = args->lse;
   a.part_max = reinterpret_cast<float*>(ws + lay.max);
   a.part_sum = reinterpret_cast<float*>(ws + lay.sum);
   a.part_acc = reinterpret_cast<float*>(ws + lay.acc);
-  a.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
+  a.part_of = reinterpret_cast<int2*>(ws + lay.of);
+  a.scale_log2 = (float)((double)args->softmax_scale * 1.4426950408889634);
   a.tokens = tokens;
   a.group = group;
   a.group_magic = group > 1 ? (uint32_t)(((1ull << 32) + group - 1) / group) : 0u;
@@ -506,6 +549,6 @@ extern "C" int ckv_paged_attention(const ckv_paged_cache* cache, int32_t layer, 
   a.words = (tokens + 63) / 64;
   a.page_log2 = 31 - __builtin_clz((unsigned)cache->page_size);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (cache->dtype == CKV_BF16) return launch_attend<CKV_BF16>(a, lay.tiles, s);
-  return launch_attend<CKV_F16>(a, lay.tiles, s);
+  if (cache->dtype == CKV_BF16) return launch_attend<CKV_BF16>(a, lay, s);
+  return launch_attend<CKV_F16>(a, lay, s);
 }

@@ -2,13 +2,13 @@
 // the paged KV cache (gfx950).
 //
 // A workgroup of W waves takes 32 W packed query rows of a KV head (row = token *
-// group + query head).  Tiles of 64 cache rows come from memory into registers two
+// group + query head).  Tiles of 64 (or 32) cache rows come from memory into registers two
 // tiles ahead, page by page, and are stored to LDS for the next tile.  Each wave
 // computes S^T = K Q^T with the 32 x 32 x 16 matrix instructions, which leaves one
 // query row in a lane (lane % 32) and 16 of 32 cache rows in each half of the wave,
 // so the softmax is per-lane work; O^T = V^T P^T takes the same layout, with V^T by
 // transposing LDS reads.  A tile that not every query of a wave sees whole is masked
-// by 64 bits a lane.
+// by a bit a row and lane.
 #include <hip/hip_runtime.h>
 
 #include "ckv_paged_attend.h"
@@ -19,11 +19,8 @@ using namespace ckv;
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
-constexpr int KEYS = 64;             // cache rows of an LDS tile
 constexpr int K_STRIDE = D + 8;      // 17 chunks of 16 bytes: b128 reads of 16 lanes hit distinct banks
 constexpr int V_STRIDE = D + 32;     // 20 chunks: transposed b64 reads hit distinct banks
-constexpr int K_TILE = KEYS * K_STRIDE;
-constexpr int V_TILE = KEYS * V_STRIDE;
 constexpr int O_STRIDE = 64 + 4;     // floats of a row of 64 output dims: b128 writes of 16 rows hit distinct banks
 
 template <int DT>
@@ -43,52 +40,60 @@ __device__ inline float max3(float x, float y, float z) {
   return r;
 }
 
-// A thread's share of a tile: piece i is 8 dims from 8 (tid % 16) on of local row tid / 16 + 4 W i.  A wave's four rows of
-// a piece share a page.
-template <int W>
+// A thread's share of a tile of KEYS cache rows: piece i is 8 dims from 8 (tid % 16) on of local row
+// tid / 16 + 4 W i.  A wave's four rows of a piece share a page.
+template <int W, int KEYS>
 struct TilePieces {
-  static constexpr int C = 16 / W;
+  static constexpr int C = KEYS / (4 * W);
   uint4 w[C];
 };
-template <int W>
+template <int W, int KEYS>
 struct TilePages {
-  int32_t page[TilePieces<W>::C];
+  int32_t page[TilePieces<W, KEYS>::C];
 };
 
-template <int W>
-__device__ inline void load_pages(const PagedHead& q, int tile, int last, TilePages<W>& p) {
+template <int W, int KEYS>
+__device__ inline void load_pages(const PagedHead& q, int tile, int last, TilePages<W, KEYS>& p) {
 #pragma unroll
-  for (int i = 0; i < TilePieces<W>::C; ++i)
+  for (int i = 0; i < TilePieces<W, KEYS>::C; ++i)
     p.page[i] = q.page(min(tile * KEYS + (int)(threadIdx.x >> 4) + i * 4 * W, last));
 }
 
 // Rows past the last one are read as they are in its page, and masked.
-template <int W>
-__device__ inline void load_tile(const PagedHead& q, const uint16_t* base, int tile, const TilePages<W>& p, TilePieces<W>& t) {
+template <int W, int KEYS>
+__device__ inline void load_tile(const PagedHead& q, const uint16_t* base, int tile, const TilePages<W, KEYS>& p,
+                                 TilePieces<W, KEYS>& t) {
 #pragma unroll
-  for (int i = 0; i < TilePieces<W>::C; ++i)
+  for (int i = 0; i < TilePieces<W, KEYS>::C; ++i)
     t.w[i] = gload16(base + q.at(p.page[i], tile * KEYS + (threadIdx.x >> 4) + i * 4 * W) + 8 * (threadIdx.x & 15));
 }
 
-template <int W>
-__device__ inline void store_tile(const TilePieces<W>& t, uint16_t* tile, int stride) {
+template <int W, int KEYS>
+__device__ inline void store_tile(const TilePieces<W, KEYS>& t, uint16_t* tile, int stride) {
 #pragma unroll
-  for (int i = 0; i < TilePieces<W>::C; ++i)
+  for (int i = 0; i < TilePieces<W, KEYS>::C; ++i)
     *reinterpret_cast<uint4*>(tile + ((threadIdx.x >> 4) + i * 4 * W) * stride + 8 * (threadIdx.x & 15)) = t.w[i];
 }
 
-struct RowsLds {
-  alignas(16) uint16_t k[2][K_TILE];
-  alignas(16) uint16_t v[2][V_TILE];
+template <int KEYS>
+struct TilesLds {
+  alignas(16) uint16_t k[2][KEYS * K_STRIDE];
+  alignas(16) uint16_t v[2][KEYS * V_STRIDE];
   int special[2];  // the tile, where its values held infinity or NaN that was staged as zero
 };
 
-static_assert(8 * 32 * O_STRIDE * sizeof(float) <= sizeof(RowsLds), "eight waves' output fits");
+// LDS of a workgroup: the tiles, or the output rows on their way out.
+template <int W, int KEYS>
+constexpr size_t rows_lds_bytes() {
+  const size_t out = W * 32 * O_STRIDE * sizeof(float);
+  return out > sizeof(TilesLds<KEYS>) ? out : sizeof(TilesLds<KEYS>);
+}
 
-template <int DT, int W>
-__global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAttendArgs a) {
+template <int DT, int W, int KEYS>
+__global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttendArgs a) {
   extern __shared__ __align__(16) unsigned char lds_raw[];
-  RowsLds& lds = *reinterpret_cast<RowsLds*>(lds_raw);
+  constexpr int NI = KEYS / 32;  // blocks of 32 cache rows a tile
+  TilesLds<KEYS>& lds = *reinterpret_cast<TilesLds<KEYS>*>(lds_raw);
   const ckv_paged_cache& c = a.cache;
   // workgroups that follow one another go to different XCDs: one head's to one, where they share its L2
   const int h = blockIdx.x, number = blockIdx.z;
@@ -98,6 +103,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
   const Part part = find_part(PagedRows{a}, a.parts, number, -1);
   const int b = part.sequence;
   if (b < 0) return;
+  tell_parts(a, part);
   const PagedStep step(a, b);
   const PagedHead q(a, b, h);
   const int row = block0 + 32 * wave + (lane & 31);
@@ -134,7 +140,6 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
     const int low = first_tile * KEYS >> a.page_log2, high = min(end_tile * KEYS - 1, last) >> a.page_log2;
     for (int p = low + tid; p <= high; p += 64 * W) bad |= !q.good(gload_i32(q.table + p));
   }
-  bad = __syncthreads_or(bad);
 
   uint4 qreg[8];
   {
@@ -156,17 +161,17 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
   auto is_masked = [&](int tile, int all_lo, int all_hi) __attribute__((always_inline)) {
     return bad || tile * KEYS < all_lo || tile * KEYS + KEYS - 1 > all_hi;
   };
-  // 64 bits: which rows of a tile this lane's query sees
+  // Which rows of a tile this lane's query sees, a bit each
   auto seen_rows = [&](int tile) {
     uint64_t seen = see.rows(a, step, b, tile * KEYS);
     if (bad) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < KEYS / 16; ++g)
         if (!q.good(q.page(min(tile * KEYS + 16 * g, last)))) seen &= ~(0xffffull << (16 * g));
     }
     return seen;
   };
-  TilePieces<W> kc, vc;
+  TilePieces<W, KEYS> kc, vc;
   // Before a tile's values go to LDS: where some query does not see some row, values that are not finite become zeros
   // (a masked row's zero probability times infinity or NaN would spread it) and are added afterwards.
   auto prepare_values = [&](int tile, int stage) __attribute__((always_inline)) {
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
     asm volatile("");
     bool found = false;
 #pragma unroll
-    for (int i = 0; i < TilePieces<W>::C; ++i) {
+    for (int i = 0; i < TilePieces<W, KEYS>::C; ++i) {
       uint4& w = vc.w[i];
       found |= has_special<DT>(w.x) || has_special<DT>(w.y) || has_special<DT>(w.z) || has_special<DT>(w.w);
       w = uint4{without_special<DT>(w.x), without_special<DT>(w.y), without_special<DT>(w.z), without_special<DT>(w.w)};
@@ -195,33 +200,35 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
   const bool second = TURNS && wave >= 4;
   const int last_tile = end_tile - 1;
   int t0 = first_tile;
-  TilePages<W> ahead;  // of the tile whose keys are loaded next
+  TilePages<W, KEYS> ahead;  // of the tile whose keys are loaded next
   int stage = 0;  // X_i has its values in v[i & 1], its keys in k[(i + 1) & 1]
-  f32x16_t sc[2];
+  f32x16_t sc[NI];
   if (tid < 2) lds.special[tid] = -1;
-  __syncthreads();
-  TilePages<W> vpages;  // of the tile whose values are loaded next
+  TilePages<W, KEYS> vpages;  // of the tile whose values are loaded next
+  const int t1 = min(t0 + 1, last_tile), t2 = min(t0 + 2, last_tile), t3 = min(t0 + 3, last_tile);
   if (left > 0) {
-    TilePages<W> p0;
-    const int t1 = min(t0 + 1, last_tile), t2 = min(t0 + 2, last_tile), t3 = min(t0 + 3, last_tile);
-    load_pages<W>(q, t0, last, p0);
-    load_pages<W>(q, t1, last, vpages);
-    load_pages<W>(q, t2, last, ahead);
-    load_tile<W>(q, q.keys, t0, p0, kc);
-    load_tile<W>(q, q.values, t0, p0, vc);
-    store_tile<W>(kc, lds.k[0], K_STRIDE);
-    load_tile<W>(q, q.keys, t1, vpages, kc);
+    TilePages<W, KEYS> p0;
+    load_pages<W, KEYS>(q, t0, last, p0);
+    load_pages<W, KEYS>(q, t1, last, vpages);
+    load_pages<W, KEYS>(q, t2, last, ahead);
+    load_tile<W, KEYS>(q, q.keys, t0, p0, kc);
+    load_tile<W, KEYS>(q, q.values, t0, p0, vc);
+  }
+  bad = __syncthreads_or(bad);  // with the first rows on their way
+  if (left > 0) {
+    store_tile<W, KEYS>(kc, lds.k[0], K_STRIDE);
+    load_tile<W, KEYS>(q, q.keys, t1, vpages, kc);
     prepare_values(t0, 0);
-    store_tile<W>(vc, lds.v[0], V_STRIDE);
-    store_tile<W>(kc, lds.k[1], K_STRIDE);
-    load_tile<W>(q, q.values, t1, vpages, vc);
-    load_tile<W>(q, q.keys, t2, ahead, kc);
+    store_tile<W, KEYS>(vc, lds.v[0], V_STRIDE);
+    store_tile<W, KEYS>(kc, lds.k[1], K_STRIDE);
+    load_tile<W, KEYS>(q, q.values, t1, vpages, vc);
+    load_tile<W, KEYS>(q, q.keys, t2, ahead, kc);
     vpages = ahead;
-    load_pages<W>(q, t3, last, ahead);
+    load_pages<W, KEYS>(q, t3, last, ahead);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int i = k & 1, x = k >> 1;
+    for (int k = 0; k < 8 * NI; ++k) {
+      const int i = k % NI, x = k / NI;
       const uint4 kf = *reinterpret_cast<const uint4*>(&lds.k[0][(32 * i + (lane & 31)) * K_STRIDE + 16 * x + 8 * half]);
       sc[i] = mfma32<DT>(kf, qreg[x], x == 0 ? f32x16_t{} : sc[i]);
     }
@@ -229,27 +236,30 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
     if (second) __syncthreads();
   }
 
-  uint32_t pb[2][8];
+  uint32_t pb[NI][8];
   while (left > 0) {
     // ---- V_i: the vector ALUs ----
     if (is_masked(t0, wave_lo, wave_hi)) {
       asm volatile("");  // a branch, not selects on every tile
       const uint64_t seen = seen_rows(t0) >> (4 * half);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < NI; ++i) {
         const uint32_t bits = (uint32_t)(seen >> (32 * i));
 #pragma unroll
         for (int v = 0; v < 16; ++v) sc[i][v] = bits >> (8 * (v >> 2) + (v & 3)) & 1u ? sc[i][v] : NEG_INF;
       }
     }
-    float tops[4];
+    float tops[2 * NI];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    for (int x = 0; x < 2 * NI; ++x) {
       const f32x16_t& v = sc[x >> 1];
       const int e = 8 * (x & 1);
       tops[x] = max3(max3(v[e], v[e + 1], v[e + 2]), max3(v[e + 3], v[e + 4], v[e + 5]), max3(v[e + 6], v[e + 7], v[e + 7]));
     }
-    const float top = max_xor32(max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]));
+    float all = tops[0];
+#pragma unroll
+    for (int x = 1; x < 2 * NI; ++x) all = max3(all, tops[x], tops[x]);
+    const float top = max_xor32(all);
     if (__ballot(top > m + grow_by) != 0) {
       const float t = top > m + grow_by ? top : m;  // a query's own scores alone decide
       const float f = m == t ? 1.0f : __builtin_amdgcn_exp2f((m - t) * sl2);
@@ -261,7 +271,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
     const float mc = (m == NEG_INF ? 0.0f : m * sl2) - prob_bias<DT>();
     float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NI; ++i) {
 #pragma unroll
       for (int v = 0; v < 16; v += 2) {
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i][v], sl2, -mc));
@@ -278,18 +288,19 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
     // ---- M_i: the matrix cores, and the staging of X_(i + 1) between the products ----
     if (TURNS) __builtin_amdgcn_s_setprio(1);
     const int t1 = min(t0 + 1, last_tile), t2 = min(t0 + 2, last_tile), t3 = min(t0 + 3, last_tile), t4 = min(t0 + 4, last_tile);
-    // Operands from LDS are read AHEAD products before they are used: 16 of
-    // values (rows 16 (k / 4) of the tile, dims 32 (k % 4)), then 16 of keys.
+    // Operands from LDS are read AHEAD products before they are used: first those of
+    // values (rows 16 (k / 4) of the tile, dims 32 (k % 4)), then as many of keys.
+    constexpr int HALF = 8 * NI;
     const uint16_t* v_at = lds.v[stage] + (4 * half + ((lane & 15) >> 2)) * V_STRIDE + 16 * ((lane >> 4) & 1) +
                            4 * (lane & 3);
     const uint16_t* k_at = lds.k[stage ^ 1] + (lane & 31) * K_STRIDE + 8 * half;
     auto operand = [&](int k) __attribute__((always_inline)) {
-      if (k < 16) {
+      if (k < HALF) {
         const uint16_t* p = v_at + 16 * (k >> 2) * V_STRIDE + 32 * (k & 3);
         const uint2 x = lds_read_tr16(p), y = lds_read_tr16(p + 8 * V_STRIDE);
         return uint4{x.x, x.y, y.x, y.y};
       }
-      return *reinterpret_cast<const uint4*>(k_at + 32 * (k & 1) * K_STRIDE + 16 * ((k - 16) >> 1));
+      return *reinterpret_cast<const uint4*>(k_at + 32 * ((k - HALF) % NI) * K_STRIDE + 16 * ((k - HALF) / NI));
     };
     constexpr int AHEAD = 6;
     uint4 op[AHEAD];
@@ -298,23 +309,23 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
     prepare_values(t1, stage ^ 1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
+    for (int k = 0; k < 2 * HALF; ++k) {
       const uint4 now = op[k % AHEAD];
-      if (k < 16) {
+      if (k < HALF) {
         const int i = k >> 3, vb = 4 * ((k >> 2) & 1), db = k & 3;
         o[db] = mfma32<DT>(now, uint4{pb[i][vb], pb[i][vb + 1], pb[i][vb + 2], pb[i][vb + 3]}, o[db]);
       } else {
-        const int i = k & 1, x = (k - 16) >> 1;
-        sc[i] = mfma32<DT>(now, qreg[x], k < 18 ? f32x16_t{} : sc[i]);
+        const int i = (k - HALF) % NI, x = (k - HALF) / NI;
+        sc[i] = mfma32<DT>(now, qreg[x], x == 0 ? f32x16_t{} : sc[i]);
       }
-      if (k + AHEAD < 32) op[k % AHEAD] = operand(k + AHEAD);
-      if (k == 4) store_tile<W>(vc, lds.v[stage ^ 1], V_STRIDE);
-      if (k == 10) store_tile<W>(kc, lds.k[stage], K_STRIDE);
-      if (k == 14) load_tile<W>(q, q.values, t2, vpages, vc);
-      if (k == 18) load_tile<W>(q, q.keys, t3, ahead, kc);
-      if (k == 22) {
+      if (k + AHEAD < 2 * HALF) op[k % AHEAD] = operand(k + AHEAD);
+      if (k == 2 * NI) store_tile<W, KEYS>(vc, lds.v[stage ^ 1], V_STRIDE);
+      if (k == 5 * NI) store_tile<W, KEYS>(kc, lds.k[stage], K_STRIDE);
+      if (k == 7 * NI) load_tile<W, KEYS>(q, q.values, t2, vpages, vc);
+      if (k == 9 * NI) load_tile<W, KEYS>(q, q.keys, t3, ahead, kc);
+      if (k == 11 * NI) {
         vpages = ahead;
-        load_pages<W>(q, t4, last, ahead);
+        load_pages<W, KEYS>(q, t4, last, ahead);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -403,15 +414,15 @@ __global__ __launch_bounds__(64 * W, W / 4) void paged_rows_kernel(const PagedAt
   a.lse[at_lse] = sum == 0.0f ? NEG_INF : (top + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
 }
 
-template <int DT, int W>
+template <int DT, int W, int KEYS>
 int launch_rows(const PagedAttendArgs& a, hipStream_t s) {
   const ckv_paged_cache& c = a.cache;
-  auto kernel = paged_rows_kernel<DT, W>;
+  auto kernel = paged_rows_kernel<DT, W, KEYS>;
   static bool ready[64] = {};  // one flag a device; setting it twice does no harm
   int device = 0;
   if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !ready[device]) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RowsLds));
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)rows_lds_bytes<W, KEYS>());
     if (e != hipSuccess) {
       (void)hipGetLastError();
       return paged_error(CKV_E_LAUNCH, "ckv_paged_attention", hipGetErrorString(e));
@@ -419,7 +430,7 @@ int launch_rows(const PagedAttendArgs& a, hipStream_t s) {
     if (device >= 0 && device < 64) ready[device] = true;
   }
   const dim3 grid(c.kv_heads, (a.rows + 32 * W - 1) / (32 * W), a.parts);
-  kernel<<<grid, 64 * W, sizeof(RowsLds), s>>>(a);
+  kernel<<<grid, 64 * W, rows_lds_bytes<W, KEYS>(), s>>>(a);
   return paged_launched("ckv_paged_attention");
 }
 
@@ -431,8 +442,8 @@ int paged_row_block(int rows) { return rows <= 128 ? 128 : 256; }
 
 int launch_paged_rows(const PagedAttendArgs& a, hipStream_t stream) {
   if (paged_row_block(a.rows) == 128)
-    return a.cache.dtype == CKV_BF16 ? launch_rows<CKV_BF16, 4>(a, stream) : launch_rows<CKV_F16, 4>(a, stream);
-  return a.cache.dtype == CKV_BF16 ? launch_rows<CKV_BF16, 8>(a, stream) : launch_rows<CKV_F16, 8>(a, stream);
+    return a.cache.dtype == CKV_BF16 ? launch_rows<CKV_BF16, 4, 32>(a, stream) : launch_rows<CKV_F16, 4, 32>(a, stream);
+  return a.cache.dtype == CKV_BF16 ? launch_rows<CKV_BF16, 8, 64>(a, stream) : launch_rows<CKV_F16, 8, 64>(a, stream);
 }
 
 }  // namespace ckv

@@ -658,6 +658,7 @@ typedef struct ckv_paged_cache {
   const int32_t* page_table;   /* [batch][table_pages] */
   int32_t* lengths;            /* [batch] committed rows, taken as clamped to [0, table_pages * page_size] */
   int32_t* overflow;           /* [batch] 1: tokens found no row */
+  uint32_t* counters;          /* [batch][CKV_QUANT_COUNTERS], zero before first use; the kernels leave it zero */
   int32_t layers;
   int32_t pages;
   int32_t kv_heads;
@@ -699,16 +700,21 @@ int ckv_draft_tree_plan(const int32_t* parents, const int32_t* counts, int32_t b
 
 /* Writes a step's keys and values into layer `layer`: token t < counts[b] (null:
  * tokens) into row lengths[b] + t, its key turned by the angles of position
- * lengths[b] + t (tree: + depths[b][t]) where rotary is given, each value rounded
- * once.  query (with rotary alone, may be null) [batch][query_heads][tokens][128]
- * strided goes to query_out [batch][tokens][query_heads][128] in the cache's dtype,
- * turned likewise; zeros past the count.  A token whose row is past the table or
- * whose page is none is dropped and sets overflow[b].  dtype: the inputs',
- * CKV_BF16, CKV_F16 or CKV_F32.  lengths stay as they are. */
-int ckv_paged_append(const ckv_paged_cache* cache, int32_t layer, const ckv_quant_rows* key,
-                     const ckv_quant_rows* value, const ckv_quant_rows* query, int32_t query_heads, int32_t tokens,
-                     const int32_t* counts, const int32_t* depths, const ckv_rotary* rotary, int32_t dtype,
-                     void* query_out, void* stream);
+ * lengths[b] + t (with depths: + depths[b][t]) where rotary is given, each value
+ * rounded once.  query (with rotary alone; data may be null) [batch][query_heads][tokens]
+ * [128] strided goes to query_out [batch][tokens][query_heads][128] in the cache's
+ * dtype, turned likewise; zeros past the count.  A token whose row is past the
+ * table or whose page is none is dropped and sets overflow[b].  lengths stay. */
+typedef struct ckv_paged_append_args {
+  ckv_quant_rows key, value, query;
+  const int32_t* counts;
+  const int32_t* depths;       /* [batch][tokens] */
+  const ckv_rotary* rotary;
+  void* query_out;
+  int32_t layer, tokens, query_heads;
+  int32_t dtype;               /* the inputs': CKV_BF16, CKV_F16 or CKV_F32 */
+} ckv_paged_append_args;
+int ckv_paged_append(const ckv_paged_cache* cache, const ckv_paged_append_args* args, void* stream);
 
 /* Attention of a step's tokens, already written, over layer `layer`: token
  * t < counts[b] (null: tokens) attends the committed rows and the step's tokens
@@ -717,11 +723,20 @@ int ckv_paged_append(const ckv_paged_cache* cache, int32_t layer, const ckv_quan
  * dtype, out [batch][tokens][query_heads][128], lse [batch][query_heads][tokens]
  * (natural log); a query that attends no row, or with t >= counts[b], gives zeros
  * and -inf.  workspace: ckv_paged_attention_workspace_bytes() bytes, this call's alone. */
+typedef struct ckv_paged_attention_args {
+  ckv_quant_rows query;
+  const int32_t* counts;
+  const ckv_draft_tree* tree;
+  void* out;
+  float* lse;
+  void* workspace;
+  int32_t layer, query_heads, tokens, window;
+  float softmax_scale;
+  int32_t reserved;
+} ckv_paged_attention_args;
 size_t ckv_paged_attention_workspace_bytes(const ckv_paged_cache* cache, int32_t query_heads, int32_t tokens,
                                            int32_t window);
-int ckv_paged_attention(const ckv_paged_cache* cache, int32_t layer, const ckv_quant_rows* query, int32_t query_heads,
-                        int32_t tokens, const int32_t* counts, const ckv_draft_tree* tree, float softmax_scale,
-                        int32_t window, void* out, float* lse, void* workspace, void* stream);
+int ckv_paged_attention(const ckv_paged_cache* cache, const ckv_paged_attention_args* args, void* stream);
 
 /* Commits a step's tokens in all layers.  Without a path the first counts[b] (null:
  * tokens) are taken: lengths[b] += count, up to the table's rows.  path

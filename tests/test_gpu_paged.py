@@ -31,12 +31,16 @@ def _host(t):
     return t.detach().cpu().double().numpy()
 
 
-def _cache(device, gen, *, lengths, heads=2, page=16, room=64, dtype=BF16, layers=1, spare=2):
-    """A cache with `lengths` committed rows in pages of any order, random rows everywhere, and `room` rows more."""
+LARGE = 262_144  # rows a sequence's table may name: which kernel takes a call goes by that, the host knows no lengths
+
+
+def _cache(device, gen, *, lengths, heads=2, page=16, room=64, dtype=BF16, layers=1, spare=2, capacity=0):
+    """A cache with `lengths` committed rows in pages of any order, random rows everywhere, and `room` rows more;
+    `capacity`: so many rows' entries in the page table, most of them without a page."""
     need = [-(-(n + room) // page) for n in lengths]
     pool = sum(need) + spare
     order = torch.randperm(pool, generator=gen).tolist()
-    table = torch.full((len(lengths), max(need)), -1, dtype=torch.int32)
+    table = torch.full((len(lengths), max(max(need), capacity // page)), -1, dtype=torch.int32)
     at = 0
     for b, pages in enumerate(need):
         table[b, :pages] = torch.tensor(order[at:at + pages], dtype=torch.int32)
@@ -239,19 +243,19 @@ def _attend_case(device, gen, cache, *, group, tokens, shape="chain", counts=Non
 
 FORMS = [  # heads, group, tokens: all forms of the kernels
     (2, 1, 1), (2, 4, 1), (1, 16, 1), (3, 7, 2), (2, 4, 8), (2, 2, 15), (1, 16, 3), (2, 7, 9), (1, 1, 100), (2, 4, 31),
-    (1, 16, 16), (2, 3, 50), (1, 8, 65)]
+    (1, 16, 16), (2, 3, 50), (1, 8, 65), (1, 4, 90)]
 
 
 @pytest.mark.parametrize("heads,group,tokens", FORMS)
-@pytest.mark.parametrize("dtype,page", [(BF16, 16), (F16, 64)])
-def test_attend_matches_oracle(device, heads, group, tokens, dtype, page):
+@pytest.mark.parametrize("dtype,page,capacity", [(BF16, 16, 0), (F16, 64, 0), (F16, 16, LARGE), (BF16, 128, LARGE)])
+def test_attend_matches_oracle(device, heads, group, tokens, dtype, page, capacity):
     """Ragged lengths (none, one row, page and tile ends), chains and trees, counts from none to all, windows."""
     gen = torch.Generator().manual_seed(heads * group + tokens)
-    cache = _cache(device, gen, lengths=[0, 1, 63, 64, 200, 391], heads=heads, page=page, room=tokens, dtype=dtype)
+    cache = _cache(device, gen, lengths=[0, 1, 63, 64, 200, 391], heads=heads, page=page, room=tokens, dtype=dtype, capacity=capacity)
     counts = [tokens, 0, max(tokens - 1, 0), tokens + 3, tokens // 2, -1]
     for shape, count, window in (("chain", None, 0), ("chain", counts, 0), ("chain", None, 1), ("chain", None, 70), ("wide", None, 0),
                                  ("deep", counts, 0), ("deep", None, 5), ("wide", counts, 129)):
-        print(f"attend {heads} x {group} x {tokens} {dtype} page={page} {shape} counts={count is not None} window={window}", flush=True)
+        print(f"attend {heads} x {group} x {tokens} {dtype} page={page} capacity={capacity} {shape} counts={count is not None} window={window}", flush=True)
         _attend_case(device, gen, cache, group=group, tokens=tokens, shape=shape, counts=count, window=window)
 
 
@@ -259,19 +263,21 @@ def test_attend_matches_oracle(device, heads, group, tokens, dtype, page):
     (2, 4, 1, [3000, 17, 2049], 128), (1, 2, 12, [2500], 256), (2, 4, 16, [1800, 900], 32), (1, 4, 30, [2600, 0], 64),
     (1, 4, 70, [2300, 640], 16)])
 @pytest.mark.parametrize("shape,window", [("chain", 0), ("deep", 0), ("chain", 700), ("wide", 300)])
-def test_attend_long_caches_in_parts(device, heads, group, tokens, lengths, page, shape, window):
+@pytest.mark.parametrize("capacity", [0, LARGE])
+def test_attend_long_caches_in_parts(device, heads, group, tokens, lengths, page, shape, window, capacity):
     print(f"attend parts {heads} x {group} x {tokens} over {lengths} page={page} {shape} window={window}", flush=True)
     gen = torch.Generator().manual_seed(sum(lengths))
-    cache = _cache(device, gen, lengths=lengths, heads=heads, page=page, room=tokens)
+    cache = _cache(device, gen, lengths=lengths, heads=heads, page=page, room=tokens, capacity=capacity)
     _attend_case(device, gen, cache, group=group, tokens=tokens, shape=shape, window=window)
 
 
 @pytest.mark.parametrize("group,tokens,shape", [(4, 300, "deep"), (1, 512, "wide"), (2, 512, "deep"), (3, 511, "chain")])
-def test_attend_large_trees(device, group, tokens, shape):
+@pytest.mark.parametrize("capacity", [0, LARGE])
+def test_attend_large_trees(device, group, tokens, shape, capacity):
     """Masks of many words whose draft starts inside a tile."""
     print(f"attend large {group} x {tokens} {shape}", flush=True)
     gen = torch.Generator().manual_seed(tokens + group)
-    cache = _cache(device, gen, lengths=[77, 128], heads=1, page=32, room=tokens, dtype=F16)
+    cache = _cache(device, gen, lengths=[77, 128], heads=1, page=32, room=tokens, dtype=F16, capacity=capacity)
     _attend_case(device, gen, cache, group=group, tokens=tokens, shape=shape, counts=[tokens, tokens - 70])
 
 
@@ -299,8 +305,8 @@ def test_attend_extreme_scores(device, dtype):
     """Scores of hundreds: one row takes all; a rising order moves the running maximum again and again."""
     gen = torch.Generator().manual_seed(9)
     for order in (1, -1):
-        for group, tokens in ((4, 1), (8, 40)):
-            cache = _cache(device, gen, lengths=[500], heads=1, room=tokens, dtype=dtype)
+        for group, tokens, capacity in ((4, 1, 0), (8, 40, 0), (8, 10, LARGE), (8, 40, LARGE)):
+            cache = _cache(device, gen, lengths=[500], heads=1, room=tokens, dtype=dtype, capacity=capacity)
             ramp = order * torch.linspace(-40, 40, 500 + tokens)
             for r in range(500 + tokens):
                 cache.key_pages[0, cache.page_table[0, r // 16], 0, r % 16] = ramp[r].to(device, dtype)
@@ -314,7 +320,7 @@ def test_attend_fp16_keeps_small_probabilities(device, group):
     n = 12_000
     gen = torch.Generator().manual_seed(10)
     for tokens in (1, 20):
-        cache = _cache(device, gen, lengths=[n], heads=1, page=256, room=tokens, dtype=F16)
+        cache = _cache(device, gen, lengths=[n], heads=1, page=256, room=tokens, dtype=F16, capacity=LARGE)
         cache.key_pages.zero_()
         cache.value_pages.fill_(1.0)
         query = torch.zeros(1, group, tokens, D, dtype=F16)
@@ -331,9 +337,10 @@ def test_attend_fp16_keeps_small_probabilities(device, group):
             assert abs(float(out[0, t, 0, 0]) * (weight + rest) / rest - 1) < 2 * 2.0 ** -11 + 2.0 ** -13 + 2.0 ** -24 * weight / rest * 4
 
 
-@pytest.mark.parametrize("group,tokens", [(2, 1), (2, 6), (4, 8), (4, 16), (4, 30), (8, 40)])
+@pytest.mark.parametrize("group,tokens,capacity", [(2, 1, 0), (2, 6, 0), (4, 8, 0), (4, 30, 0), (4, 16, LARGE), (4, 30, LARGE),
+                                                   (8, 40, LARGE)])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_attend_special_values_reach_only_who_sees_them(device, group, tokens, dtype):
+def test_attend_special_values_reach_only_who_sees_them(device, group, tokens, capacity, dtype):
     """Infinities and NaN in rows of other branches, before a window, past the length, in spare pages: no change; a
     value that is not finite and seen appears in its dim alone, a NaN key makes the query NaN."""
     print(f"special {group} x {tokens} {dtype}", flush=True)
@@ -348,7 +355,7 @@ def test_attend_special_values_reach_only_who_sees_them(device, group, tokens, d
         return put
 
     for shape, window in (("chain", 0), ("chain", 30), ("wide", 0), ("deep", 30)):
-        cache = _cache(device, gen, lengths=[100], heads=1, room=tokens, dtype=dtype)
+        cache = _cache(device, gen, lengths=[100], heads=1, room=tokens, dtype=dtype, capacity=capacity)
         parents = _parents(gen, 1, tokens, shape)
         tree = None if parents is None else DraftTree.from_parents(parents.to(device))
         query = _rand(gen, 1, group, tokens, dtype=dtype).to(device)
@@ -403,12 +410,12 @@ def test_attend_special_values_reach_only_who_sees_them(device, group, tokens, d
                 assert torch.equal(got_lse[:, t], clean_lse[:, t]) and not bool(got[t].isnan().any())
 
 
-@pytest.mark.parametrize("group,tokens", [(2, 1), (2, 12), (4, 16), (4, 32), (4, 70)])
-def test_attend_passes_over_missing_pages(device, group, tokens):
+@pytest.mark.parametrize("group,tokens,capacity", [(2, 1, 0), (2, 12, 0), (4, 16, 0), (4, 16, LARGE), (4, 32, LARGE), (4, 70, LARGE)])
+def test_attend_passes_over_missing_pages(device, group, tokens, capacity):
     """Rows whose page number is none are not attended, whatever the number is; a draft without pages sees the rest."""
     print(f"missing pages {group} x {tokens}", flush=True)
     gen = torch.Generator().manual_seed(group + tokens)
-    cache = _cache(device, gen, lengths=[150, 70, 40], heads=2, room=tokens)
+    cache = _cache(device, gen, lengths=[150, 70, 40], heads=2, room=tokens, capacity=capacity)
     cache.page_table[0, 3], cache.page_table[0, 7] = -1, cache.pages
     cache.page_table[1, 0], cache.page_table[1, 2] = -2**31, 2**31 - 1
     cache.page_table[2] = -1
@@ -432,16 +439,17 @@ def test_attend_past_the_capacity(device):
 def test_attend_shared_pages(device):
     """Two sequences over the pages of one prompt, with drafts of their own."""
     gen = torch.Generator().manual_seed(12)
-    cache = _cache(device, gen, lengths=[64, 64], room=20)
-    cache.page_table[1, :4] = cache.page_table[0, :4]
-    _attend_case(device, gen, cache, group=4, tokens=20, shape="wide")
-    _attend_case(device, gen, cache, group=4, tokens=1)
+    for capacity in (0, LARGE):
+        cache = _cache(device, gen, lengths=[64, 64], room=20, capacity=capacity)
+        cache.page_table[1, :4] = cache.page_table[0, :4]
+        _attend_case(device, gen, cache, group=4, tokens=20, shape="wide")
+        _attend_case(device, gen, cache, group=4, tokens=1)
 
 
 def test_attend_strides(device):
     gen = torch.Generator().manual_seed(13)
-    cache = _cache(device, gen, lengths=[100, 77])
-    for tokens in (3, 40):
+    for tokens, capacity in ((3, 0), (40, LARGE)):
+        cache = _cache(device, gen, lengths=[100, 77], capacity=capacity)
         fused = _rand(gen, 2, tokens, 12, dtype=BF16).to(device)
         view = fused[:, :, 2:10].transpose(1, 2)
         odd = torch.empty(view.numel() + 1, dtype=BF16, device=device)[1:].view(view.shape)
@@ -666,14 +674,15 @@ def test_speculative_run(device, dtype):
     assert torch.equal(a.key_pages, b.key_pages) and torch.equal(a.value_pages, b.value_pages) and torch.equal(a.lengths, b.lengths)
 
 
-@pytest.mark.parametrize("group,tokens,lengths,window", [(4, 1, [4000, 300], 0), (2, 16, [2000, 100], 0), (4, 16, [900, 3000], 100),
-                                                         (4, 32, [2500, 700], 0), (4, 64, [1500, 2100], 500), (4, 100, [90, 3000], 0)])
-def test_replays_equal_eager_calls(device, group, tokens, lengths, window):
+@pytest.mark.parametrize("group,tokens,lengths,window,capacity", [
+    (4, 1, [4000, 300], 0, 0), (2, 16, [2000, 100], 0, 0), (4, 16, [900, 3000], 100, 0), (4, 16, [900, 3000], 0, LARGE),
+    (4, 32, [2500, 700], 0, LARGE), (4, 64, [1500, 2100], 500, LARGE), (4, 100, [90, 3000], 0, LARGE)])
+def test_replays_equal_eager_calls(device, group, tokens, lengths, window, capacity):
     """Every form of the kernels captured, two graphs of one cache in turn with eager work between, lengths and tables that
     change between replays."""
     print(f"replay {group} x {tokens} over {lengths}", flush=True)
     gen = torch.Generator().manual_seed(tokens)
-    cache = _cache(device, gen, lengths=lengths, page=32, room=tokens + 8)
+    cache = _cache(device, gen, lengths=lengths, page=32, room=tokens + 8, capacity=capacity)
     query = _rand(gen, 2, 2 * group, tokens, dtype=BF16).to(device)
     parents = _parents(gen, 2, tokens, "wide").to(device)
 
@@ -725,8 +734,8 @@ def test_calls_on_a_side_stream(device):
 def test_same_call_twice_is_bit_equal(device):
     """No atomics on results: the same calls give equal bits."""
     gen = torch.Generator().manual_seed(22)
-    cache = _cache(device, gen, lengths=[3000, 40, 900], page=64, room=70)
-    for group, tokens in ((4, 1), (4, 8), (4, 16), (4, 32), (4, 70)):
+    for group, tokens, capacity in ((4, 1, 0), (4, 8, 0), (4, 16, 0), (4, 32, LARGE), (4, 70, LARGE)):
+        cache = _cache(device, gen, lengths=[3000, 40, 900], page=64, room=70, capacity=capacity)
         query = _rand(gen, 3, 2 * group, tokens, dtype=BF16).to(device)
         a, b = (paged_attention(query, cache, softmax_scale=SCALE) for _ in range(2))
         torch.cuda.synchronize()
@@ -736,8 +745,8 @@ def test_same_call_twice_is_bit_equal(device):
 def test_results_do_not_depend_on_the_batch(device):
     """Dead queries (counts) with NaN change nothing for the others."""
     gen = torch.Generator().manual_seed(23)
-    cache = _cache(device, gen, lengths=[300, 40], room=70)
-    for group, tokens in ((4, 3), (4, 8), (4, 16), (4, 64)):
+    for group, tokens, capacity in ((4, 3, 0), (4, 8, 0), (4, 16, LARGE), (4, 64, LARGE)):
+        cache = _cache(device, gen, lengths=[300, 40], room=70, capacity=capacity)
         counts = [tokens - 1, 1]
         query = _rand(gen, 2, 2 * group, tokens, dtype=BF16)
         clean = paged_attention(query.to(device), cache, softmax_scale=SCALE, counts=_i32(counts, device))

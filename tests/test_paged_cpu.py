@@ -217,26 +217,37 @@ def test_commit_refuses():
 
 
 def _c_cache(lib, **change):
-    c = nat.PagedCache(0x1000, 0x2000, 0x3000, 0x4000, 0x5000, 2, 8, 2, 32, 4, 2, nat.CKV_BF16, 0)
+    c = nat.PagedCache(0x1000, 0x2000, 0x3000, 0x4000, 0x5000, 0x6000, 2, 8, 2, 32, 4, 2, nat.CKV_BF16, 0)
     for name, value in change.items():
         setattr(c, name, value)
     return ctypes.byref(c)
 
 
 def _rows(address=0x1000, stride=128):
-    return ctypes.byref(nat.QuantRows(address, stride, stride, stride))
+    return (address, stride, stride, stride)
+
+
+def _append_args(**change):
+    args = dict(key=_rows(), value=_rows(), query=_rows(0), counts=0, depths=0, rotary=0, out=0, layer=0, tokens=1, heads=0,
+                dtype=nat.CKV_BF16) | change
+    return nat.PAGED_APPEND_ARGS.pack(*args.pop("key"), *args.pop("value"), *args.pop("query"), *args.values())
+
+
+def _attention_args(**change):
+    args = dict(query=_rows(), counts=0, tree=0, out=0x1000, lse=0x1000, workspace=0x1000, layer=0, heads=4, tokens=3, window=0,
+                scale=1.0, reserved=0) | change
+    return nat.PAGED_ATTENTION_ARGS.pack(*args.pop("query"), *args.values())
 
 
 @pytest.mark.parametrize("change,rc", [
     (dict(key_pages=None), 1), (dict(value_pages=0x2008), 1), (dict(page_table=None), 1), (dict(lengths=None), 1),
-    (dict(overflow=None), 1), (dict(layers=0), 1), (dict(pages=0), 1), (dict(kv_heads=-1), 1), (dict(page_size=24), 1),
+    (dict(overflow=None), 1), (dict(counters=None), 1), (dict(layers=0), 1), (dict(pages=0), 1), (dict(kv_heads=-1), 1), (dict(page_size=24), 1),
     (dict(page_size=8), 1), (dict(page_size=512), 1), (dict(table_pages=0), 1), (dict(batch=0), 1), (dict(dtype=nat.CKV_F32), 1),
     (dict(table_pages=(1 << 25) + 1), 2), (dict(batch=32768), 2), (dict(kv_heads=32768), 2),
     (dict(batch=300, kv_heads=300), 2), (dict(batch=16384, table_pages=1 << 25), 2)])
 def test_c_entries_refuse_bad_caches(lib, change, rc):
     c = _c_cache(lib, **change)
-    for got in (lib.ckv_paged_append(c, 0, _rows(), _rows(), None, 0, 1, None, None, None, nat.CKV_BF16, None, None),
-                lib.ckv_paged_attention(c, 0, _rows(), 2, 1, None, None, 1.0, 0, 0x1000, 0x1000, 0x1000, None),
+    for got in (lib.ckv_paged_append(c, _append_args(), None), lib.ckv_paged_attention(c, _attention_args(), None),
                 lib.ckv_paged_commit(c, 1, None, None, 0, None)):
         assert got == rc, lib.ckv_last_error()
     assert lib.ckv_paged_attention_workspace_bytes(c, 2, 1, 0) == 0
@@ -244,37 +255,36 @@ def test_c_entries_refuse_bad_caches(lib, change, rc):
 
 def test_c_entries_refuse_bad_arguments(lib):
     c = _c_cache(lib)
-    good = dict(layer=0, key=_rows(), value=_rows(), query=None, heads=0, tokens=1, counts=None, depths=None, rotary=None,
-                dtype=nat.CKV_BF16, out=None, stream=None)
-    table = nat.Rotary(0x1000, 0x1000, 128, 64, 0, 0)
+    tables = []
 
     def rotary(**change):
         t = nat.Rotary(0x1000, 0x1000, 128, 64, 0, 0)
         for name, value in change.items():
             setattr(t, name, value)
-        return ctypes.byref(t)
+        tables.append(t)
+        return ctypes.addressof(t)
 
-    for change in (dict(layer=2), dict(layer=-1), dict(key=None), dict(key=_rows(0)), dict(key=_rows(0x1008)),
+    for change in (dict(layer=2), dict(layer=-1), dict(key=_rows(0)), dict(key=_rows(0x1008)), dict(value=_rows(0)),
                    dict(value=_rows(0x1000, 4)), dict(dtype=2), dict(tokens=0), dict(query=_rows()),
-                   dict(query=_rows(), heads=4, out=0x1000), dict(query=_rows(), heads=4, rotary=ctypes.byref(table)),
-                   dict(query=_rows(), heads=0, rotary=ctypes.byref(table), out=0x1000),
-                   dict(query=_rows(0x1002), heads=4, rotary=ctypes.byref(table), out=0x1000),
+                   dict(query=_rows(), heads=4, out=0x1000), dict(query=_rows(), heads=4, rotary=rotary()),
+                   dict(query=_rows(), heads=4, rotary=rotary(), out=0x1008),
+                   dict(query=_rows(), heads=0, rotary=rotary(), out=0x1000),
+                   dict(query=_rows(0x1002), heads=4, rotary=rotary(), out=0x1000),
                    dict(rotary=rotary(cosines=None)), dict(rotary=rotary(sines=0x1004)), dict(rotary=rotary(dim=0)),
                    dict(rotary=rotary(dim=24)), dict(rotary=rotary(dim=144)), dict(rotary=rotary(positions=127))):
-        assert lib.ckv_paged_append(c, *(good | change).values()) == 1, change
-    good = dict(layer=0, query=_rows(), heads=4, tokens=3, counts=None, tree=None, scale=1.0, window=0, out=0x1000, lse=0x1000,
-                workspace=0x1000, stream=None)
-    half = nat.TreeMasks(0x1000, None)
-    for change, rc in ((dict(layer=2), 1), (dict(query=None), 1), (dict(query=_rows(0x1008)), 1), (dict(heads=3), 1),
+        assert lib.ckv_paged_append(c, _append_args(**change), None) == 1, change
+    assert lib.ckv_paged_append(c, None, None) == 1 and lib.ckv_paged_attention(c, None, None) == 1
+    half, whole = nat.TreeMasks(0x1000, None), nat.TreeMasks(0x1000, 0x1000)
+    for change, rc in ((dict(layer=2), 1), (dict(query=_rows(0)), 1), (dict(query=_rows(0x1008)), 1), (dict(heads=3), 1),
                        (dict(heads=0), 1), (dict(heads=34), 2), (dict(tokens=0), 1), (dict(window=-1), 1), (dict(scale=0.0), 1),
-                       (dict(scale=float("nan")), 1), (dict(scale=2e30), 1), (dict(out=None), 1), (dict(lse=None), 1),
-                       (dict(tree=ctypes.byref(half)), 1), (dict(tokens=(1 << 20) + 1), 2),
-                       (dict(tokens=513, tree=ctypes.byref(nat.TreeMasks(0x1000, 0x1000))), 2)):
-        assert lib.ckv_paged_attention(c, *(good | change).values()) == rc, change
+                       (dict(scale=float("nan")), 1), (dict(scale=2e30), 1), (dict(out=0), 1), (dict(out=0x1008), 1),
+                       (dict(lse=0), 1), (dict(tree=ctypes.addressof(half)), 1), (dict(tokens=(1 << 20) + 1), 2),
+                       (dict(tokens=513, tree=ctypes.addressof(whole)), 2)):
+        assert lib.ckv_paged_attention(c, _attention_args(**change), None) == rc, change
     large = _c_cache(lib, table_pages=1 << 16)
-    for workspace in (None, 0x1008):  # several parts a sequence
+    for workspace in (0, 0x1008):  # several parts a sequence
         assert lib.ckv_paged_attention_workspace_bytes(large, 4, 1, 0) > 0
-        assert lib.ckv_paged_attention(large, *(good | dict(tokens=1, workspace=workspace)).values()) == 1
+        assert lib.ckv_paged_attention(large, _attention_args(tokens=1, workspace=workspace), None) == 1
     for args in ((0, None, None, 1, 0x1000, 0x1000, None), (0x1000, None, 0, 1, 0x1000, 0x1000, None),
                  (0x1000, None, 1, 0, 0x1000, 0x1000, None), (0x1000, None, 1, 1, None, 0x1000, None),
                  (0x1000, None, 1, 1, 0x1000, None, None)):
