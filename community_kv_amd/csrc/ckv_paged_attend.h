@@ -85,18 +85,23 @@ __device__ inline int64_t paged_query_index(const PagedAttendArgs& a, int b, int
 struct PagedHead {
   const uint16_t *keys, *values;
   const int32_t* table;
-  int64_t page_elems;  // of all heads
+  uint32_t page_elems;  // of all heads: at most 2^30
   int pages, page_log2;
   __device__ PagedHead(const PagedAttendArgs& a, int b, int h)
       : keys(reinterpret_cast<const uint16_t*>(a.cache.key_pages) + ((int64_t)h << a.page_log2) * D),
         values(reinterpret_cast<const uint16_t*>(a.cache.value_pages) + ((int64_t)h << a.page_log2) * D),
         table(a.cache.page_table + (int64_t)b * a.cache.table_pages),
-        page_elems(((int64_t)a.cache.kv_heads << a.page_log2) * D), pages(a.cache.pages), page_log2(a.page_log2) {}
+        page_elems(((uint32_t)a.cache.kv_heads << a.page_log2) * D), pages(a.cache.pages), page_log2(a.page_log2) {}
   __device__ int page(int row) const { return gload_i32(table + (row >> page_log2)); }
+  // The same for a row that is the same in the whole wave: a scalar load (the table does not change during a call).
+  __device__ int uniform_page(int row) const {
+    typedef const __attribute__((address_space(4))) int32_t* constant_i32_ptr;
+    return *(constant_i32_ptr)(uintptr_t)(table + (row >> page_log2));
+  }
   __device__ bool good(int page) const { return (uint32_t)page < (uint32_t)pages; }
   // Element offset of a row; of some row where the page is none.
   __device__ int64_t at(int page, int row) const {
-    return (good(page) ? page : 0) * page_elems + (int64_t)(row & ((1 << page_log2) - 1)) * D;
+    return (int64_t)((uint64_t)(good(page) ? (uint32_t)page : 0u) * page_elems) + (row & ((1 << page_log2) - 1)) * D;
   }
 };
 

@@ -41,7 +41,8 @@ __device__ inline float max3(float x, float y, float z) {
 }
 
 // A thread's share of a tile of KEYS cache rows: piece i is 8 dims from 8 (tid % 16) on of local row
-// tid / 16 + 4 W i.  A wave's four rows of a piece share a page.
+// tid / 16 + 4 W i.  A wave's four rows of a piece share a page, so pages and the addresses of their rows are the
+// scalar unit's work: the vector ALUs have the softmax, and no time to spare.
 template <int W, int KEYS>
 struct TilePieces {
   static constexpr int C = KEYS / (4 * W);
@@ -53,19 +54,20 @@ struct TilePages {
 };
 
 template <int W, int KEYS>
-__device__ inline void load_pages(const PagedHead& q, int tile, int last, TilePages<W, KEYS>& p) {
+__device__ inline void load_pages(const PagedHead& q, int wave, int tile, int last, TilePages<W, KEYS>& p) {
 #pragma unroll
-  for (int i = 0; i < TilePieces<W, KEYS>::C; ++i)
-    p.page[i] = q.page(min(tile * KEYS + (int)(threadIdx.x >> 4) + i * 4 * W, last));
+  for (int i = 0; i < TilePieces<W, KEYS>::C; ++i) p.page[i] = q.uniform_page(min(tile * KEYS + 4 * wave + i * 4 * W, last));
 }
 
 // Rows past the last one are read as they are in its page, and masked.
 template <int W, int KEYS>
-__device__ inline void load_tile(const PagedHead& q, const uint16_t* base, int tile, const TilePages<W, KEYS>& p,
+__device__ inline void load_tile(const PagedHead& q, const uint16_t* base, int wave, int tile, const TilePages<W, KEYS>& p,
                                  TilePieces<W, KEYS>& t) {
 #pragma unroll
-  for (int i = 0; i < TilePieces<W, KEYS>::C; ++i)
-    t.w[i] = gload16(base + q.at(p.page[i], tile * KEYS + (threadIdx.x >> 4) + i * 4 * W) + 8 * (threadIdx.x & 15));
+  for (int i = 0; i < TilePieces<W, KEYS>::C; ++i) {
+    const uint16_t* row = base + q.at(p.page[i], tile * KEYS + 4 * wave + i * 4 * W);
+    t.w[i] = gload16(row + (uint32_t)(((threadIdx.x & 63) >> 4) * D + 8 * (threadIdx.x & 15)));
+  }
 }
 
 template <int W, int KEYS>
@@ -89,6 +91,93 @@ constexpr size_t rows_lds_bytes() {
   return out > sizeof(TilesLds<KEYS>) ? out : sizeof(TilesLds<KEYS>);
 }
 
+// Rows that some of the query rows `first` to `first + rows` see, and those that all of them see.
+__device__ inline void ranges_of(const PagedAttendArgs& a, const PagedStep& step, int first, int rows, int* some_lo,
+                                 int* some_hi, int* all_lo, int* all_hi) {
+  const int t0 = paged_token(a, first), t1 = min(paged_token(a, min(first + rows, a.rows) - 1), step.count - 1);
+  const int last = step.total - 1;
+  *some_lo = *all_lo = 0;
+  *some_hi = -1;
+  *all_hi = 0x7ffffffe;  // without a query nothing is masked: the rows are dropped at the end
+  if (first >= a.rows || t0 > t1) return;
+  const int newest = a.masks ? step.count - 1 : t1, oldest = a.masks ? 0 : t0;  // positions of the tokens, from start on
+  *some_hi = min(step.start + newest, last);
+  *all_hi = min(a.masks ? step.start - 1 : step.start + t0, last);
+  if (a.window > 0) {
+    *some_lo = max(step.start + oldest - a.window + 1, 0);
+    *all_lo = max(step.start + newest - a.window + 1, 0);
+  }
+}
+
+// Zeros in place of the values that are not finite; whether there were any.
+template <int DT, int W, int KEYS>
+__device__ inline bool drop_special(TilePieces<W, KEYS>& t) {
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < TilePieces<W, KEYS>::C; ++i) {
+    uint4& w = t.w[i];
+    found |= has_special<DT>(w.x) || has_special<DT>(w.y) || has_special<DT>(w.z) || has_special<DT>(w.w);
+    w = uint4{without_special<DT>(w.x), without_special<DT>(w.y), without_special<DT>(w.z), without_special<DT>(w.w)};
+  }
+  return found;
+}
+
+// Results of 32 query rows from `row0` on, one a lane of each half: m the maximum of its unscaled scores, l the lane's
+// share of the sum, o the outputs (o[i][v]: dim 32 i + 8 (v / 4) + 4 half + v % 4).  They go out through `out_s`, LDS of
+// the wave alone, 64 dims at a time, so that whole lines are written: from the accumulators a store would touch 32 lines.
+template <int DT>
+__device__ inline void write_rows(const PagedAttendArgs& a, int b, int h, int number, bool joined, int row0, bool live, float m,
+                                  float l, const f32x16_t* o, float* out_s) {
+  const int lane = threadIdx.x & 63, half = lane >> 5, row = row0 + (lane & 31);
+  const float sum = live ? add_xor32(l) : 0.0f;
+  const float top = m == NEG_INF ? 0.0f : m * a.scale_log2;
+  const bool none = joined ? !live : sum == 0.0f;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, factor = joined ? 1.0f : inv;
+#pragma unroll
+  for (int dims = 0; dims < 2; ++dims) {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const f32x16_t& x = o[2 * dims + (i >> 2)];
+      const int g = i & 3;
+      *reinterpret_cast<float4*>(&out_s[(lane & 31) * O_STRIDE + 32 * (i >> 2) + 8 * g + 4 * half]) =
+          none ? float4{0.0f, 0.0f, 0.0f, 0.0f}
+               : float4{x[4 * g] * factor, x[4 * g + 1] * factor, x[4 * g + 2] * factor, x[4 * g + 3] * factor};
+    }
+    asm volatile("" ::: "memory");  // a wave's own LDS operations stay in order
+    if (joined) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int local = 4 * j + (lane >> 4), r = row0 + local, dim = 64 * dims + 4 * (lane & 15);
+        const float4 x = *reinterpret_cast<const float4*>(&out_s[local * O_STRIDE + 4 * (lane & 15)]);
+        if (r < a.rows)
+          *reinterpret_cast<float4*>(a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + r) * D + dim) = x;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int local = 8 * j + (lane >> 3), r = row0 + local, dim = 64 * dims + 8 * (lane & 7);
+        const float* from = &out_s[local * O_STRIDE + 8 * (lane & 7)];
+        const float4 x = *reinterpret_cast<const float4*>(from), y = *reinterpret_cast<const float4*>(from + 4);
+        if (r >= a.rows) continue;
+        int64_t at_out, at_lse;
+        paged_output_index(a, b, h, r, &at_out, &at_lse);
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at_out + dim) =
+            uint4{pack_store<DT>(x.x, x.y), pack_store<DT>(x.z, x.w), pack_store<DT>(y.x, y.y), pack_store<DT>(y.z, y.w)};
+      }
+    }
+  }
+  if (half != 0 || row >= a.rows) return;
+  if (joined) {
+    a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m == NEG_INF || !live ? NEG_INF : top;
+    a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
+    return;
+  }
+  int64_t at_out, at_lse;
+  paged_output_index(a, b, h, row, &at_out, &at_lse);
+  a.lse[at_lse] = sum == 0.0f ? NEG_INF : (top + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+}
+
 template <int DT, int W, int KEYS>
 __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttendArgs a) {
   extern __shared__ __align__(16) unsigned char lds_raw[];
@@ -110,24 +199,9 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
   const Sight see(a, step, b, row);
   const int last = step.total - 1;
 
-  // Rows that some of `rows` query rows from `first` on see, and those that all of them see.
-  auto ranges_of = [&](int first, int rows, int* some_lo, int* some_hi, int* all_lo, int* all_hi) {
-    const int t0 = paged_token(a, first), t1 = min(paged_token(a, min(first + rows, a.rows) - 1), step.count - 1);
-    *some_lo = *all_lo = 0;
-    *some_hi = -1;
-    *all_hi = 0x7ffffffe;  // without a query nothing is masked: the rows are dropped at the end
-    if (first >= a.rows || t0 > t1) return;
-    const int newest = a.masks ? step.count - 1 : t1, oldest = a.masks ? 0 : t0;  // positions of the tokens, from start on
-    *some_hi = min(step.start + newest, last);
-    *all_hi = min(a.masks ? step.start - 1 : step.start + t0, last);
-    if (a.window > 0) {
-      *some_lo = max(step.start + oldest - a.window + 1, 0);
-      *all_lo = max(step.start + newest - a.window + 1, 0);
-    }
-  };
   int walk_lo, walk_hi, group_lo, group_hi, wave_lo, wave_hi, unused;
-  ranges_of(block0, 32 * W, &walk_lo, &walk_hi, &group_lo, &group_hi);
-  ranges_of(block0 + 32 * wave, 32, &unused, &unused, &wave_lo, &wave_hi);
+  ranges_of(a, step, block0, 32 * W, &walk_lo, &walk_hi, &group_lo, &group_hi);
+  ranges_of(a, step, block0 + 32 * wave, 32, &unused, &unused, &wave_lo, &wave_hi);
   // tiles of this part that are walked (its first row opens one)
   const int lo_row = step.first(a) + part.index * part.rows;
   const int hi_row = (int)min((int64_t)lo_row + part.rows, (int64_t)walk_hi + 1);
@@ -177,14 +251,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
   auto prepare_values = [&](int tile, int stage) __attribute__((always_inline)) {
     if (!is_masked(tile, group_lo, group_hi)) return;
     asm volatile("");
-    bool found = false;
-#pragma unroll
-    for (int i = 0; i < TilePieces<W, KEYS>::C; ++i) {
-      uint4& w = vc.w[i];
-      found |= has_special<DT>(w.x) || has_special<DT>(w.y) || has_special<DT>(w.z) || has_special<DT>(w.w);
-      w = uint4{without_special<DT>(w.x), without_special<DT>(w.y), without_special<DT>(w.z), without_special<DT>(w.w)};
-    }
-    if (found) lds.special[stage] = tile;
+    if (drop_special<DT>(vc)) lds.special[stage] = tile;
   };
 
   // Two groups of four waves, one of each on a SIMD, take turns: while one has
@@ -200,31 +267,28 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
   const bool second = TURNS && wave >= 4;
   const int last_tile = end_tile - 1;
   int t0 = first_tile;
-  TilePages<W, KEYS> ahead;  // of the tile whose keys are loaded next
+  TilePages<W, KEYS> ahead;  // of tile i + 2, from V_i on of tile i + 3, whose keys are loaded in M_i
   int stage = 0;  // X_i has its values in v[i & 1], its keys in k[(i + 1) & 1]
   f32x16_t sc[NI];
   if (tid < 2) lds.special[tid] = -1;
-  TilePages<W, KEYS> vpages;  // of the tile whose values are loaded next
-  const int t1 = min(t0 + 1, last_tile), t2 = min(t0 + 2, last_tile), t3 = min(t0 + 3, last_tile);
+  TilePages<W, KEYS> p0, p1;
+  const int t1 = min(t0 + 1, last_tile), t2 = min(t0 + 2, last_tile);
   if (left > 0) {
-    TilePages<W, KEYS> p0;
-    load_pages<W, KEYS>(q, t0, last, p0);
-    load_pages<W, KEYS>(q, t1, last, vpages);
-    load_pages<W, KEYS>(q, t2, last, ahead);
-    load_tile<W, KEYS>(q, q.keys, t0, p0, kc);
-    load_tile<W, KEYS>(q, q.values, t0, p0, vc);
+    load_pages<W, KEYS>(q, wave, t0, last, p0);
+    load_pages<W, KEYS>(q, wave, t1, last, p1);
+    load_pages<W, KEYS>(q, wave, t2, last, ahead);
+    load_tile<W, KEYS>(q, q.keys, wave, t0, p0, kc);
+    load_tile<W, KEYS>(q, q.values, wave, t0, p0, vc);
   }
   bad = __syncthreads_or(bad);  // with the first rows on their way
   if (left > 0) {
     store_tile<W, KEYS>(kc, lds.k[0], K_STRIDE);
-    load_tile<W, KEYS>(q, q.keys, t1, vpages, kc);
+    load_tile<W, KEYS>(q, q.keys, wave, t1, p1, kc);
     prepare_values(t0, 0);
     store_tile<W, KEYS>(vc, lds.v[0], V_STRIDE);
     store_tile<W, KEYS>(kc, lds.k[1], K_STRIDE);
-    load_tile<W, KEYS>(q, q.values, t1, vpages, vc);
-    load_tile<W, KEYS>(q, q.keys, t2, ahead, kc);
-    vpages = ahead;
-    load_pages<W, KEYS>(q, t3, last, ahead);
+    load_tile<W, KEYS>(q, q.values, wave, t1, p1, vc);
+    load_tile<W, KEYS>(q, q.keys, wave, t2, ahead, kc);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 8 * NI; ++k) {
@@ -239,6 +303,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
   uint32_t pb[NI][8];
   while (left > 0) {
     // ---- V_i: the vector ALUs ----
+    const TilePages<W, KEYS> vpages = ahead;  // of tile i + 2, whose values are loaded in M_i
+    load_pages<W, KEYS>(q, wave, min(t0 + 3, last_tile), last, ahead);  // by scalar loads: away from the LDS reads of M_i
     if (is_masked(t0, wave_lo, wave_hi)) {
       asm volatile("");  // a branch, not selects on every tile
       const uint64_t seen = seen_rows(t0) >> (4 * half);
@@ -284,10 +350,11 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
       }
     }
     l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    if (TURNS) asm volatile("" : "+v"(l));  // and the sums
     if (TURNS) __syncthreads();
     // ---- M_i: the matrix cores, and the staging of X_(i + 1) between the products ----
     if (TURNS) __builtin_amdgcn_s_setprio(1);
-    const int t1 = min(t0 + 1, last_tile), t2 = min(t0 + 2, last_tile), t3 = min(t0 + 3, last_tile), t4 = min(t0 + 4, last_tile);
+    const int t1 = min(t0 + 1, last_tile), t2 = min(t0 + 2, last_tile), t3 = min(t0 + 3, last_tile);
     // Operands from LDS are read AHEAD products before they are used: first those of
     // values (rows 16 (k / 4) of the tile, dims 32 (k % 4)), then as many of keys.
     constexpr int HALF = 8 * NI;
@@ -321,12 +388,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
       if (k + AHEAD < 2 * HALF) op[k % AHEAD] = operand(k + AHEAD);
       if (k == 2 * NI) store_tile<W, KEYS>(vc, lds.v[stage ^ 1], V_STRIDE);
       if (k == 5 * NI) store_tile<W, KEYS>(kc, lds.k[stage], K_STRIDE);
-      if (k == 7 * NI) load_tile<W, KEYS>(q, q.values, t2, vpages, vc);
-      if (k == 9 * NI) load_tile<W, KEYS>(q, q.keys, t3, ahead, kc);
-      if (k == 11 * NI) {
-        vpages = ahead;
-        load_pages<W, KEYS>(q, t4, last, ahead);
-      }
+      if (k == 7 * NI) load_tile<W, KEYS>(q, q.values, wave, t2, vpages, vc);
+      if (k == 9 * NI) load_tile<W, KEYS>(q, q.keys, wave, t3, ahead, kc);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (TURNS) __builtin_amdgcn_s_setprio(0);
@@ -361,77 +424,34 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
     if (TURNS && !second && left == 0) __syncthreads();  // the second group's last slot
   }
 
-  // The wave's rows go out through LDS (free by now), 64 dims at a time, so that
-  // whole lines are written: from the accumulators a store would touch 32 lines.
-  const float sum = see.live ? add_xor32(l) : 0.0f;
-  const float top = m == NEG_INF ? 0.0f : m * sl2;
-  const bool joined = part.count > 1, none = joined ? !see.live : sum == 0.0f;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, factor = joined ? 1.0f : inv;
-  float* out_s = reinterpret_cast<float*>(lds_raw) + wave * 32 * O_STRIDE;
-  const int wave0 = block0 + 32 * wave;
-#pragma unroll
-  for (int dims = 0; dims < 2; ++dims) {
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const f32x16_t& x = o[2 * dims + (i >> 2)];
-      const int g = i & 3;
-      *reinterpret_cast<float4*>(&out_s[(lane & 31) * O_STRIDE + 32 * (i >> 2) + 8 * g + 4 * half]) =
-          none ? float4{0.0f, 0.0f, 0.0f, 0.0f}
-               : float4{x[4 * g] * factor, x[4 * g + 1] * factor, x[4 * g + 2] * factor, x[4 * g + 3] * factor};
-    }
-    asm volatile("" ::: "memory");  // a wave's own LDS operations stay in order
-    if (joined) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int local = 4 * j + (lane >> 4), r = wave0 + local, dim = 64 * dims + 4 * (lane & 15);
-        const float4 x = *reinterpret_cast<const float4*>(&out_s[local * O_STRIDE + 4 * (lane & 15)]);
-        if (r < a.rows)
-          *reinterpret_cast<float4*>(a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + r) * D + dim) = x;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int local = 8 * j + (lane >> 3), r = wave0 + local, dim = 64 * dims + 8 * (lane & 7);
-        const float* from = &out_s[local * O_STRIDE + 8 * (lane & 7)];
-        const float4 x = *reinterpret_cast<const float4*>(from), y = *reinterpret_cast<const float4*>(from + 4);
-        if (r >= a.rows) continue;
-        int64_t at_out, at_lse;
-        paged_output_index(a, b, h, r, &at_out, &at_lse);
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at_out + dim) =
-            uint4{pack_store<DT>(x.x, x.y), pack_store<DT>(x.z, x.w), pack_store<DT>(y.x, y.y), pack_store<DT>(y.z, y.w)};
-      }
-    }
-  }
-  if (half != 0 || row >= a.rows) return;
-  if (joined) {
-    a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m == NEG_INF || !see.live ? NEG_INF : top;
-    a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
-    return;
-  }
-  int64_t at_out, at_lse;
-  paged_output_index(a, b, h, row, &at_out, &at_lse);
-  a.lse[at_lse] = sum == 0.0f ? NEG_INF : (top + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+  write_rows<DT>(a, b, h, number, part.count > 1, block0 + 32 * wave, see.live, m, l, o,
+                 reinterpret_cast<float*>(lds_raw) + wave * 32 * O_STRIDE);
 }
 
-template <int DT, int W, int KEYS>
-int launch_rows(const PagedAttendArgs& a, hipStream_t s) {
-  const ckv_paged_cache& c = a.cache;
-  auto kernel = paged_rows_kernel<DT, W, KEYS>;
-  static bool ready[64] = {};  // one flag a device; setting it twice does no harm
+// Dynamic LDS of a kernel, set once a device; setting it twice does no harm.
+template <class Kernel>
+int launch_tiles(Kernel kernel, bool* ready, int rows, int threads, size_t lds, const PagedAttendArgs& a, hipStream_t s) {
   int device = 0;
   if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64 || !ready[device]) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)rows_lds_bytes<W, KEYS>());
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)lds);
     if (e != hipSuccess) {
       (void)hipGetLastError();
       return paged_error(CKV_E_LAUNCH, "ckv_paged_attention", hipGetErrorString(e));
     }
     if (device >= 0 && device < 64) ready[device] = true;
   }
-  const dim3 grid(c.kv_heads, (a.rows + 32 * W - 1) / (32 * W), a.parts);
-  kernel<<<grid, 64 * W, rows_lds_bytes<W, KEYS>(), s>>>(a);
+  const dim3 grid(a.cache.kv_heads, (a.rows + rows - 1) / rows, a.parts);
+  kernel<<<grid, threads, lds, s>>>(a);
   return paged_launched("ckv_paged_attention");
+}
+
+template <int DT>
+int launch_rows(const PagedAttendArgs& a, hipStream_t s) {
+  static bool small[64] = {}, large[64] = {};
+  if (paged_row_block(a.rows) == 128)
+    return launch_tiles(paged_rows_kernel<DT, 4, 32>, small, 128, 256, rows_lds_bytes<4, 32>(), a, s);
+  return launch_tiles(paged_rows_kernel<DT, 8, 64>, large, 256, 512, rows_lds_bytes<8, 64>(), a, s);
 }
 
 }  // namespace
@@ -441,9 +461,7 @@ namespace ckv {
 int paged_row_block(int rows) { return rows <= 128 ? 128 : 256; }
 
 int launch_paged_rows(const PagedAttendArgs& a, hipStream_t stream) {
-  if (paged_row_block(a.rows) == 128)
-    return a.cache.dtype == CKV_BF16 ? launch_rows<CKV_BF16, 4, 32>(a, stream) : launch_rows<CKV_F16, 4, 32>(a, stream);
-  return a.cache.dtype == CKV_BF16 ? launch_rows<CKV_BF16, 8, 64>(a, stream) : launch_rows<CKV_F16, 8, 64>(a, stream);
+  return a.cache.dtype == CKV_BF16 ? launch_rows<CKV_BF16>(a, stream) : launch_rows<CKV_F16>(a, stream);
 }
 
 }  // namespace ckv
