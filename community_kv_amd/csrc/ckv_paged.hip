@@ -54,41 +54,43 @@ constexpr int MAX_WORDS = CKV_MAX_DRAFT / 64;
 // ---------------------------------------------------------------------------
 // Plan of drafted trees
 // ---------------------------------------------------------------------------
-// A workgroup a sequence, a thread a token.  Each token starts with its own bit and
-// jumps to its parent; a round adds the mask of the token jumped to and doubles the
-// jump, so ceil(log2(depth)) rounds reach every ancestor.  Bound by latency: a few
-// rounds of LDS reads between barriers.
+// A workgroup a sequence, a thread a token, a wave a word of the masks.  In its wave each token starts with its own bit
+// and jumps to its parent; a round adds the bits of the token jumped to and doubles the jump, so at most six rounds of
+// shuffles reach every ancestor of the wave, and the token before the wave's that the chain goes on to.  After one
+// barrier each token follows these to the earlier waves, a word a hop.  Bound by latency: 512 tokens in up to 7 hops.
 __global__ __launch_bounds__(CKV_MAX_DRAFT) void tree_plan_kernel(const int32_t* __restrict__ parents,
                                                                   const int32_t* __restrict__ counts, int tokens,
                                                                   int32_t* __restrict__ depths,
                                                                   uint64_t* __restrict__ masks) {
-  __shared__ uint64_t mask_s[MAX_WORDS][CKV_MAX_DRAFT];
-  __shared__ int jump_s[CKV_MAX_DRAFT];
-  const int b = blockIdx.x, t = threadIdx.x, words = (tokens + 63) >> 6;
+  __shared__ uint64_t own_s[CKV_MAX_DRAFT];  // a token's bits in its own word
+  __shared__ int before_s[CKV_MAX_DRAFT];    // its last ancestor before that word, or -1
+  const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, words = (tokens + 63) >> 6;
   const int count = step_count(counts, tokens, b);
-  int jump = -1;
+  int parent = -1;
   if (t < count) {
     const int p = parents[(int64_t)b * tokens + t];
-    jump = p >= 0 && p < t ? p : -1;
+    parent = p >= 0 && p < t ? p : -1;
   }
+  const bool inside = parent >= t - lane;  // in the same wave
+  int jump = inside ? parent & 63 : -1, before = inside ? -1 : parent;
+  uint64_t own = t < count ? 1ull << lane : 0ull;
+  while (__ballot(jump >= 0) != 0) {
+    const int from = jump >= 0 ? jump : lane;
+    own |= (uint64_t)__shfl((unsigned long long)own, from, 64);
+    before = __shfl(before, from, 64);
+    const int next = __shfl(jump, from, 64);
+    if (jump >= 0) jump = next;
+  }
+  own_s[t] = own;
+  before_s[t] = before;
+  __syncthreads();
   uint64_t mine[MAX_WORDS];
 #pragma unroll
-  for (int w = 0; w < MAX_WORDS; ++w) mine[w] = t < count && w == t >> 6 ? 1ull << (t & 63) : 0ull;
-  bool changed = true;
-  while (__syncthreads_or(jump >= 0)) {
-    if (changed) {
-      jump_s[t] = jump;
-#pragma unroll
-      for (int w = 0; w < MAX_WORDS; ++w)
-        if (w <= t >> 6) mask_s[w][t] = mine[w];
-    }
-    __syncthreads();
-    changed = jump >= 0;
-    if (changed) {
-#pragma unroll
-      for (int w = 0; w < MAX_WORDS; ++w)
-        if (w <= jump >> 6) mine[w] |= mask_s[w][jump];  // ancestors are earlier tokens
-      jump = jump_s[jump];
+  for (int w = MAX_WORDS - 1; w >= 0; --w) {
+    mine[w] = w == t >> 6 ? own : 0ull;
+    if (before >= 0 && before >> 6 == w) {
+      mine[w] = own_s[before];
+      before = before_s[before];
     }
   }
   if (t >= tokens) return;
