@@ -431,9 +431,22 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_rows_kernel(const Pag
 
 constexpr int64_t MAX_ROWS = 1 << 21;  // query rows of a head: the grids' second dimension holds their blocks
 
-// Cache rows times blocks of 16 query rows, over all heads, up to which the few-row kernel takes a call, and up to which
-// it does so with one tile of query rows a workgroup instead of two.
-constexpr int64_t FEW_WORK = 400000, ONE_TILE_WORK = 128000;
+// Which kernel, by the call's work: cache rows times blocks of 16 query rows, over all heads and sequences.  Times of the
+// attention alone, one tile | two tiles | many rows, on heads of 32/8 unless said:
+//   136k (8/8 heads, 128 tokens, 2k rows)              15.7 | 17.5 | 20.4 us
+//   256k (64 query rows, 8k cache rows)                20.4 | 18.5 | 22.0
+//   544k (512 query rows, 2k cache rows)               27.8 | 24.3 | 30.2
+//   848k (4 sequences, 512 query rows, 700 cache rows)  38.3 | 27.4 | 30.2
+//   1,032k (256 query rows, 8k cache rows)             50.0 | 36.0 | 29.3
+// Up to 16 query rows one tile holds all, and up to 32 two do: the many-row kernel's tile would be empty mostly (8
+// sequences, 32 query rows, 32k cache rows: 194 us against 214).
+constexpr int64_t FEW_WORK = 850000, ONE_TILE_WORK = 200000;
+
+// Workgroups that parts are cut for.  A workgroup a compute unit, for parts cost a join (two tiles, 32 query rows, one
+// sequence of 32k: 31.5 us against 33.2 with two, 39.9 with four); two where a wave hides another's waits: one tile over
+// long caches (8 sequences of 32k: 191 us against 200; of 8k, below the limit: 57 against 54) and the many-row kernel of
+// 128 rows, of which two fit a compute unit (72 us against 74; 256 rows: 105 against 93).
+constexpr int64_t LONG_WORK = 700000;
 
 // How a call is laid out: which kernel, how many parts, and the workspace.
 struct PagedLayout {
@@ -450,11 +463,18 @@ struct PagedLayout {
     const int64_t block = tiles ? 16 * tiles : paged_row_block(rows);
     const int64_t blocks = (rows + block - 1) / block;
     const int64_t units = (most + PART_UNIT - 1) / PART_UNIT;
-    const int64_t workgroups = tiles || paged_row_block(rows) == 128 ? 512 : 256;
+    const int64_t workgroups = (tiles == 1 && work > LONG_WORK) || (!tiles && block == 128) ? 512 : 256;
     const int64_t want = workgroups / (c->kv_heads * blocks);
-    if (want < (tiles ? c->batch + 1 : 2 * c->batch) || units <= (tiles ? 6 : 1)) parts = c->batch;
+    // A sequence stays whole where a join costs more than it saves: up to 512 rows for a token or two (380 rows: 8.3 us
+    // whole, 9.0 cut; 640: 9.9, 8.7), 768 for a small tree (640 rows: 13.5, 13.8; 890: 15.8, 12.8), 128 for many rows (250
+    // rows, 8 sequences: 16 us, 25; 380, one sequence: 16.6, 14.4).
+    if (want < (tiles ? c->batch + 1 : 2 * c->batch) || units <= (!tiles ? 1 : rows <= 16 ? 4 : 6)) parts = c->batch;
     else parts = (int)(want < c->batch * units ? want : c->batch * units);
-    wide_join = parts > 8 * c->batch;  // parts of a sequence, on average
+    // A workgroup a query row joins faster than half a wave a row that reads the parts in turn where the parts are many
+    // and the rows few.  Rows of all heads and sequences, parts of a sequence, half waves | workgroups, in us of the whole
+    // call: 384, 5: 77.1 | 76.4;  128, 32: 27 | 18;  2,048, 32: 39 | 30;  4,096, 16: 40.5 | 38.6;  5,120, 13: 42 | 43;
+    // 8,192, 8: 55 | 60.
+    wide_join = parts > 4 * c->batch && (int64_t)rows * c->kv_heads * c->batch <= 4096;
     size_t at = 0;
     auto take = [&](size_t size) {
       const size_t here = at;
