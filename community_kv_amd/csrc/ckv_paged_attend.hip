@@ -323,7 +323,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedA
 }
 
 // Joins the parts of one query row: a workgroup of 256 threads, four dims and
-// every eighth part each.
+// every eighth part each.  Heads run along the grid's first dimension as they do
+// in the kernels that wrote the parts, so where their number is a multiple of
+// eight an XCD reads what its own compute units wrote (one sequence, 512 queries
+// over 2k rows: 39.4 us against 42.0 for the call with rows first).
 constexpr int JOIN_THREADS = 256;
 constexpr int MAX_PARTS = 512;  // of one sequence
 
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAtt
   __shared__ float factor[MAX_PARTS];
   __shared__ float scratch[4];
   __shared__ float4 acc_s[JOIN_THREADS];
-  const int row = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int h = blockIdx.x, row = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int2 part = a.part_of[b];  // the first and their number
   if (part.y == 1) return;  // written already
   const int64_t first = ((int64_t)h * a.row_pad + row) * a.parts + part.x;
@@ -381,7 +384,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAtt
 template <int DT>
 __global__ __launch_bounds__(JOIN_THREADS) void paged_join_rows_kernel(const PagedAttendArgs a) {
   constexpr int TOGETHER = 4;  // parts in flight
-  const int row = (JOIN_THREADS / 32) * blockIdx.x + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
+  const int h = blockIdx.x, row = (JOIN_THREADS / 32) * blockIdx.y + (threadIdx.x >> 5), b = blockIdx.z, lane = threadIdx.x & 31;
   if (row >= a.rows) return;
   const int2 part = a.part_of[b];
   if (part.y == 1) return;
@@ -502,8 +505,8 @@ template <int DT>
 int launch_attend(const PagedAttendArgs& a, const PagedLayout& lay, hipStream_t s) {
   const int rc = lay.tiles ? launch_few<DT>(a, lay.tiles, s) : launch_paged_rows(a, s);
   if (rc || a.parts == a.cache.batch) return rc;
-  if (lay.wide_join) paged_join_kernel<DT><<<dim3(a.rows, a.cache.kv_heads, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
-  else paged_join_rows_kernel<DT><<<dim3((a.rows + 7) / 8, a.cache.kv_heads, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
+  if (lay.wide_join) paged_join_kernel<DT><<<dim3(a.cache.kv_heads, a.rows, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
+  else paged_join_rows_kernel<DT><<<dim3(a.cache.kv_heads, (a.rows + 7) / 8, a.cache.batch), JOIN_THREADS, 0, s>>>(a);
   return paged_launched("ckv_paged_attention");
 }
 
