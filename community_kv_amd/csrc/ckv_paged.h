@@ -12,6 +12,7 @@ namespace ckv {
 
 // Rows of sequence b that are committed; a cursor out of its range must not lead a kernel out of the table.
 __host__ __device__ inline int paged_capacity(const ckv_paged_cache& c) { return c.table_pages * c.page_size; }
+__device__ inline int paged_log2(const ckv_paged_cache& c) { return __builtin_ctz((unsigned)c.page_size); }
 __device__ inline int paged_length(const ckv_paged_cache& c, int b) {
   return min(max(gload_i32(c.lengths + b), 0), paged_capacity(c));
 }

@@ -116,7 +116,7 @@ struct AppendArgs {
   const int32_t* depths;
   void* query_out;
   int64_t layer_offset;  // elements before this layer's pages
-  int32_t tokens, query_heads, shares;
+  int32_t tokens, query_heads, shares;  // a token's rows are shared out, eight a wave
 };
 
 // Eight values as 32 bits (the loads alone; a later use waits for them).
@@ -153,9 +153,10 @@ __device__ inline uint4 pack8(const float* v) {
                pack_store<DT>(v[6], v[7])};
 }
 
-// A wave takes one of `shares` shares of a token's rows (keys, queries, values of all heads), eight rows at a
-// time: eight lanes a row, two pieces of eight dims a lane, which pair up under the rotation, so that a token's
-// angles are read once and stay in registers.  Bound by memory.
+// A wave takes eight of a token's rows (keys, queries, values of all heads): eight lanes a row, two pieces of eight dims
+// a lane, which pair up under the rotation.  Bound by memory: 32,768 tokens of 32/8 heads take 140 us, 5.8 TB/s (a large
+// copy reaches 4.8).  A wave that takes more rows of its token reads the angles once for them, but they come from cache
+// anyway and it has less in flight: 152 us against 145 with a quarter of the waves; 4,096 tokens 19.1 against 18.4.
 template <int IN, int STORE>
 __global__ __launch_bounds__(THREADS) void append_kernel(const AppendArgs a) {
   const ckv_paged_cache& c = a.cache;
@@ -170,17 +171,23 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendArgs a) {
   // this lane's two pieces of a row: partners under the rotation, or two of the dims that stay
   const int first = x < pairs ? (a.rotary.interleaved ? 2 * x : x) : 2 * x;
   const int second = x < pairs ? (a.rotary.interleaved ? 2 * x + 1 : x + pairs) : 2 * x + 1;
+  const int r = 8 * share + group;
+  const bool is_query = r >= heads && r < turned;
+  const int head = r < heads ? r : is_query ? r - heads : r - turned;
+  const ckv_quant_rows& from = r < heads ? a.key : is_query ? a.query : a.value;
+  Eight<IN> piece[2];
+  if (live && r < rows) {  // before the page is known: its latency and the angles' pass meanwhile
+    const int64_t base = (int64_t)b * from.batch_stride + (int64_t)head * from.head_stride + (int64_t)t * from.token_stride;
+    piece[0].load(from.data, base + 8 * first);
+    piece[1].load(from.data, base + 8 * second);
+  }
   float cosine[8], sine[8];
   int64_t to = -1;  // this token's row in head 0
   if (live) {
     const int row = start + t;
     int page = -1;
-    if (row < paged_capacity(c)) page = gload_i32(c.page_table + (int64_t)b * c.table_pages + row / c.page_size);
-    if ((uint32_t)page < (uint32_t)c.pages)
-      to = a.layer_offset + ((int64_t)page * heads * c.page_size + (row & (c.page_size - 1))) * D;
-    else if (share == 0 && lane == 0)
-      c.overflow[b] = 1;
-    if (x < pairs) {
+    if (row < paged_capacity(c)) page = gload_i32(c.page_table + (int64_t)b * c.table_pages + (row >> paged_log2(c)));
+    if (x < pairs && 8 * share < turned) {
       const int depth = a.depths ? gload_i32(a.depths + (int64_t)b * a.tokens + t) : t;
       const int64_t at = (int64_t)min(max(start + depth, 0), a.rotary.positions - 1) * half + 8 * x;
       Eight<CKV_F32> table[2];
@@ -189,69 +196,59 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendArgs a) {
       table[0].values(cosine);
       table[1].values(sine);
     }
+    if ((uint32_t)page < (uint32_t)c.pages)
+      to = a.layer_offset + ((int64_t)page * heads * c.page_size + (row & (c.page_size - 1))) * D;
+    else if (share == 0 && lane == 0)
+      c.overflow[b] = 1;
   }
-  for (int r = 8 * share + group; r < rows; r += 8 * a.shares) {
-    const bool is_query = r >= heads && r < turned;
-    if (is_query ? false : to < 0) continue;
-    const int head = r < heads ? r : is_query ? r - heads : r - turned;
-    const ckv_quant_rows& from = r < heads ? a.key : is_query ? a.query : a.value;
-    uint16_t* out;
-    if (is_query)
-      out = reinterpret_cast<uint16_t*>(a.query_out) + (((int64_t)b * a.tokens + t) * a.query_heads + head) * D;
-    else
-      out = reinterpret_cast<uint16_t*>(r < heads ? c.key_pages : c.value_pages) + to + (int64_t)head * c.page_size * D;
-    if (!live) {  // a query past the count
-      *reinterpret_cast<uint4*>(out + 8 * first) = uint4{0, 0, 0, 0};
-      *reinterpret_cast<uint4*>(out + 8 * second) = uint4{0, 0, 0, 0};
-      continue;
-    }
-    const int64_t base = (int64_t)b * from.batch_stride + (int64_t)head * from.head_stride + (int64_t)t * from.token_stride;
-    Eight<IN> piece[2];
-    piece[0].load(from.data, base + 8 * first);
-    piece[1].load(from.data, base + 8 * second);
-    if (IN == STORE && (r >= turned || x >= pairs)) {
-      *reinterpret_cast<uint4*>(out + 8 * first) = piece[0].raw[0];
-      *reinterpret_cast<uint4*>(out + 8 * second) = piece[1].raw[0];
-      continue;
-    }
-    float u[8], v[8];
-    piece[0].values(u);
-    piece[1].values(v);
-    if (r < turned && x < pairs) {
-      if (a.rotary.interleaved) {
-        // the two pieces hold the pairs 8 x .. 8 x + 7, four each
+  if (r >= rows || (!is_query && to < 0)) return;
+  uint16_t* out;
+  if (is_query)
+    out = reinterpret_cast<uint16_t*>(a.query_out) + (((int64_t)b * a.tokens + t) * a.query_heads + head) * D;
+  else
+    out = reinterpret_cast<uint16_t*>(r < heads ? c.key_pages : c.value_pages) + to + (int64_t)head * c.page_size * D;
+  if (!live) {  // a query past the count
+    *reinterpret_cast<uint4*>(out + 8 * first) = uint4{0, 0, 0, 0};
+    *reinterpret_cast<uint4*>(out + 8 * second) = uint4{0, 0, 0, 0};
+    return;
+  }
+  if (IN == STORE && (r >= turned || x >= pairs)) {
+    *reinterpret_cast<uint4*>(out + 8 * first) = piece[0].raw[0];
+    *reinterpret_cast<uint4*>(out + 8 * second) = piece[1].raw[0];
+    return;
+  }
+  float u[8], v[8];
+  piece[0].values(u);
+  piece[1].values(v);
+  if (r < turned && x < pairs) {
+    if (a.rotary.interleaved) {
+      // the two pieces hold the pairs 8 x .. 8 x + 7, four each
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = u[2 * i], q = u[2 * i + 1], s = v[2 * i], w = v[2 * i + 1];
-          u[2 * i] = __builtin_fmaf(p, cosine[i], -(q * sine[i]));
-          u[2 * i + 1] = __builtin_fmaf(q, cosine[i], p * sine[i]);
-          v[2 * i] = __builtin_fmaf(s, cosine[4 + i], -(w * sine[4 + i]));
-          v[2 * i + 1] = __builtin_fmaf(w, cosine[4 + i], s * sine[4 + i]);
-        }
-      } else {
+      for (int i = 0; i < 4; ++i) {
+        const float p = u[2 * i], q = u[2 * i + 1], s = v[2 * i], w = v[2 * i + 1];
+        u[2 * i] = __builtin_fmaf(p, cosine[i], -(q * sine[i]));
+        u[2 * i + 1] = __builtin_fmaf(q, cosine[i], p * sine[i]);
+        v[2 * i] = __builtin_fmaf(s, cosine[4 + i], -(w * sine[4 + i]));
+        v[2 * i + 1] = __builtin_fmaf(w, cosine[4 + i], s * sine[4 + i]);
+      }
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = u[i], q = v[i];
-          u[i] = __builtin_fmaf(p, cosine[i], -(q * sine[i]));
-          v[i] = __builtin_fmaf(q, cosine[i], p * sine[i]);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float p = u[i], q = v[i];
+        u[i] = __builtin_fmaf(p, cosine[i], -(q * sine[i]));
+        v[i] = __builtin_fmaf(q, cosine[i], p * sine[i]);
       }
     }
-    *reinterpret_cast<uint4*>(out + 8 * first) = pack8<STORE>(u);
-    *reinterpret_cast<uint4*>(out + 8 * second) = pack8<STORE>(v);
   }
+  *reinterpret_cast<uint4*>(out + 8 * first) = pack8<STORE>(u);
+  *reinterpret_cast<uint4*>(out + 8 * second) = pack8<STORE>(v);
 }
-
-constexpr int64_t FILL_WAVES = 8192;  // waves that fill the chip
 
 template <int IN>
 int launch_append(AppendArgs& a, hipStream_t s) {
-  const int64_t tokens = (int64_t)a.cache.batch * a.tokens, rows = 2 * (int64_t)a.cache.kv_heads + a.query_heads;
-  // a wave a token reads its angles once; few tokens are shared out, down to eight rows a wave
-  const int64_t most = (rows + 7) / 8, want = (FILL_WAVES + tokens - 1) / tokens;
-  a.shares = (int32_t)(want < most ? want : most);
+  a.shares = (2 * a.cache.kv_heads + a.query_heads + 7) / 8;
   const int64_t blocks = ((int64_t)a.tokens * a.shares + THREADS / 64 - 1) / (THREADS / 64);
-  if (blocks > 0x7fffffff) return paged_error(CKV_E_LIMIT, "ckv_paged_append", "too many tokens");
+  if (blocks * THREADS > 0xffffffffll) return paged_error(CKV_E_LIMIT, "ckv_paged_append", "too many tokens");
   const dim3 grid((uint32_t)blocks, a.cache.batch);
   if (a.cache.dtype == CKV_BF16) append_kernel<IN, CKV_BF16><<<grid, THREADS, 0, s>>>(a);
   else append_kernel<IN, CKV_F16><<<grid, THREADS, 0, s>>>(a);
@@ -321,7 +318,7 @@ __global__ __launch_bounds__(THREADS) void move_kernel(const CommitArgs a) {
         to[i] = -1;
         if (j >= size || path[j] == j) continue;
         const int source = start + path[j], row = start + j;
-        const int from_page = gload_i32(table + source / c.page_size), page = gload_i32(table + row / c.page_size);
+        const int from_page = gload_i32(table + (source >> paged_log2(c))), page = gload_i32(table + (row >> paged_log2(c)));
         if ((uint32_t)from_page >= (uint32_t)c.pages || (uint32_t)page >= (uint32_t)c.pages) continue;
         w[i] = gload16(pages + (from_page * head_rows + (source & (c.page_size - 1))) * D);
         to[i] = (page * head_rows + (row & (c.page_size - 1))) * D;
