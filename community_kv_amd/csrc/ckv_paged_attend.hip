@@ -128,7 +128,11 @@ __device__ inline void add_step(const float* sc, const uint4* vop, Running& r) {
 
 // One workgroup of four waves takes a part of the cache rows of a (sequence,
 // head) for 16 RT query rows; its waves take steps in turn and join in LDS.
-// Bound by memory.
+// Keys and values go from memory into operands without LDS: each is used by one
+// wave alone.  Bound by memory on long caches: a token over 8 sequences of up to
+// 131k rows, 32/8 heads, in 418 us, 5.8 TB/s, where reading alone reaches 6.1;
+// by latency on short ones (one sequence of 300 rows: 7.1 us).  Two tiles of
+// query rows share what is read; four spill.
 template <int DT, int RT>
 __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedAttendArgs a) {
   __shared__ float m_s[WAVES][16];
@@ -471,8 +475,13 @@ struct PagedLayout {
     // A sequence stays whole where a join costs more than it saves: up to 512 rows for a token or two (380 rows: 8.3 us
     // whole, 9.0 cut; 640: 9.9, 8.7), 768 for a small tree (640 rows: 13.5, 13.8; 890: 15.8, 12.8), 128 for many rows (250
     // rows, 8 sequences: 16 us, 25; 380, one sequence: 16.6, 14.4).
-    if (want < (tiles ? c->batch + 1 : 2 * c->batch) || units <= (!tiles ? 1 : rows <= 16 ? 4 : 6)) parts = c->batch;
-    else parts = (int)(want < c->batch * units ? want : c->batch * units);
+    if (units <= (!tiles ? 1 : rows <= 16 ? 4 : 6)) parts = c->batch;
+    else if (want >= (tiles ? c->batch + 1 : 2 * c->batch)) parts = (int)(want < c->batch * units ? want : c->batch * units);
+    // A batch that fills the chip with whole sequences gets half as many parts again, so that one long sequence among short
+    // ones is cut all the same (equal ones stay whole).  64 sequences, 32/8 heads, a token each: 1,396 us -> 164 with one of
+    // 131k rows among ones of 1,000, 512 -> 458 with 1k to 16k rows, for 181 -> 188 with 4,000 rows in each; 24 trees of 64
+    // tokens: 379 -> 310 with 1k to 16k rows, 257 either way with 8,000.
+    else parts = c->batch + (want >= 2 && units > 32 ? (int)(want < c->batch / 2 ? want : c->batch / 2) : 0);
     // A workgroup a query row joins faster than half a wave a row that reads the parts in turn where the parts are many
     // and the rows few.  Rows of all heads and sequences, parts of a sequence, half waves | workgroups, in us of the whole
     // call: 384, 5: 77.1 | 76.4;  128, 32: 27 | 18;  2,048, 32: 39 | 30;  4,096, 16: 40.5 | 38.6;  5,120, 13: 42 | 43;

@@ -2,13 +2,28 @@
 // the paged KV cache (gfx950).
 //
 // A workgroup of W waves takes 32 W packed query rows of a KV head (row = token *
-// group + query head).  Tiles of 64 (or 32) cache rows come from memory into registers two
-// tiles ahead, page by page, and are stored to LDS for the next tile.  Each wave
-// computes S^T = K Q^T with the 32 x 32 x 16 matrix instructions, which leaves one
-// query row in a lane (lane % 32) and 16 of 32 cache rows in each half of the wave,
-// so the softmax is per-lane work; O^T = V^T P^T takes the same layout, with V^T by
-// transposing LDS reads.  A tile that not every query of a wave sees whole is masked
-// by a bit a row and lane.
+// group + query head).  Tiles of 64 (or 32) cache rows come from memory into
+// registers two tiles ahead, page by page, and are stored to LDS for the next
+// tile.  Each wave computes S^T = K Q^T with the 32 x 32 x 16 matrix instructions,
+// which leaves one query row in a lane (lane % 32) and 16 of 32 cache rows in each
+// half of the wave, so the softmax is per-lane work; O^T = V^T P^T takes the same
+// layout, with V^T by transposing LDS reads.  A tile that not every query of a wave
+// sees whole is masked by a bit a row and lane.
+//
+// Bound by the matrix cores together with the softmax beside them: 2,048 queries
+// over 32k rows (32/8 heads, bf16) take 976 to 1,012 us from card to card, 1,050 to
+// 1,090 TFLOP/s; the products alone take 787 us, the softmax alone 615, and what the
+// one does not hide of the other is the rest.  The matrix cores are busy 58 % of the
+// cycles at the 1.85 GHz that the card keeps under this load (a library product of
+// 16,384^3: 1,385 TFLOP/s).  8 trees of 64 tokens over 4k to 16k rows each: 111 to
+// 124 us, 2.8 TB/s; there each workgroup walks some 38 tiles of its own, 2 us each,
+// and its first rows, its outputs and the join take a quarter of the time.
+//
+// Measured and not taken, for the 2,048 queries: matrix and vector work interleaved
+// in every wave in place of the groups' turns (1,147 us); copies from memory into LDS
+// past the registers, four stages deep (1,004 against 982; trees 130 against 121);
+// row addresses on the vector ALUs (1,005); 64 query rows a wave at one wave a SIMD
+// (spills).
 #include <hip/hip_runtime.h>
 
 #include "ckv_paged_attend.h"
@@ -458,6 +473,8 @@ int launch_rows(const PagedAttendArgs& a, hipStream_t s) {
 
 namespace ckv {
 
+// 256 rows share what is read, 128 leave fewer of a small call's rows empty: 128 query rows of 8 sequences over 8k rows
+// take 71 us with 128 and 81 with 256; 192 query rows of 4 sequences (16/2 heads) over 32k rows 63 and 53.
 int paged_row_block(int rows) { return rows <= 128 ? 128 : 256; }
 
 int launch_paged_rows(const PagedAttendArgs& a, hipStream_t stream) {

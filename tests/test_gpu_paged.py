@@ -300,6 +300,17 @@ def test_attend_many_sequences(device):
     _attend_case(device, gen, cache, group=1, tokens=1)
 
 
+@pytest.mark.parametrize("batch,group,tokens,shape,long", [(70, 1, 1, "chain", 5000), (40, 3, 9, "deep", 3000), (18, 2, 65, "wide", 2500)])
+def test_attend_one_long_sequence_among_many(device, batch, group, tokens, shape, long):
+    """Whole sequences fill the chip, and the long one is cut all the same: some parts are joined, some are not."""
+    print(f"attend one long of {batch} {group} x {tokens}", flush=True)
+    gen = torch.Generator().manual_seed(batch)
+    lengths = [int(x) for x in torch.randint(0, 60, (batch,), generator=gen)]
+    lengths[batch // 3] = long
+    cache = _cache(device, gen, lengths=lengths, heads=8, room=tokens, capacity=8192)
+    _attend_case(device, gen, cache, group=group, tokens=tokens, shape=shape)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_attend_extreme_scores(device, dtype):
     """Scores of hundreds: one row takes all; a rising order moves the running maximum again and again."""
