@@ -435,8 +435,8 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, *, softmax_scale: 
         raise TypeError(f"query must use the cache's {cache.dtype}, not {query.dtype}")
     if heads % kv_heads or not 1 <= heads // kv_heads <= nat.MAX_GROUP:
         raise ValueError(f"query heads must be 1 to {nat.MAX_GROUP} times the {kv_heads} KV heads, not {heads}")
-    if not 0.0 < softmax_scale <= 1e30:
-        raise ValueError("softmax_scale must be positive and finite")
+    if not 1e-30 <= softmax_scale <= 1e30:
+        raise ValueError("softmax_scale must be between 1e-30 and 1e30")
     if window < 0:
         raise ValueError("window must be non-negative")
     counts_at, counts = _step_counts(cache, tokens, tree, counts)
@@ -451,6 +451,8 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, *, softmax_scale: 
     call = (heads, tokens, window)
     size = cache._sizes.get(call)
     if size is None:
+        if len(cache._sizes) >= 1024:
+            cache._sizes.clear()
         size = cache._sizes[call] = lib.ckv_paged_attention_workspace_bytes(cache._ref, heads, tokens, window)
     workspace = query.new_empty(size, dtype=torch.uint8) if size else None
     view, query = _view(query)

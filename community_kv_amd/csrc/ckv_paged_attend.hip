@@ -550,8 +550,9 @@ extern "C" int ckv_paged_attention(const ckv_paged_cache* cache, const ckv_paged
   if ((int64_t)tokens * group > MAX_ROWS) return paged_error(CKV_E_LIMIT, what, "more than 2^21 query rows a head");
   if (tree && (!tree->depths || !tree->masks)) return paged_error(CKV_E_INVALID, what, "null argument");
   if (tree && tokens > CKV_MAX_DRAFT) return paged_error(CKV_E_LIMIT, what, "a tree of more than 512 tokens");
-  if (!(args->softmax_scale > 0.0f) || args->softmax_scale > 1e30f)
-    return paged_error(CKV_E_INVALID, what, "softmax_scale must be positive");
+  // below, the step that a running maximum makes would not be a number in 32 bits
+  if (!(args->softmax_scale >= 0.99e-30f) || args->softmax_scale > 1.01e30f)
+    return paged_error(CKV_E_INVALID, what, "softmax_scale must be between 1e-30 and 1e30");
   const PagedLayout lay(cache, tokens, group, window);
   if (lay.bytes && (!args->workspace || ((uintptr_t)args->workspace & 15))) return paged_error(CKV_E_INVALID, what, "workspace");
   char* ws = reinterpret_cast<char*>(args->workspace);

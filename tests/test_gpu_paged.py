@@ -311,6 +311,14 @@ def test_attend_one_long_sequence_among_many(device, batch, group, tokens, shape
     _attend_case(device, gen, cache, group=group, tokens=tokens, shape=shape)
 
 
+@pytest.mark.parametrize("group,tokens,capacity", [(2, 3, 0), (4, 16, LARGE), (4, 70, LARGE)])
+@pytest.mark.parametrize("scale", [1e-30, 1e-10])
+def test_attend_smallest_scales(device, group, tokens, capacity, scale):
+    gen = torch.Generator().manual_seed(tokens)
+    cache = _cache(device, gen, lengths=[700, 5, 1500], room=tokens, page=64, capacity=capacity)
+    _attend_case(device, gen, cache, group=group, tokens=tokens, scale=scale)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_attend_extreme_scores(device, dtype):
     """Scores of hundreds: one row takes all; a rising order moves the running maximum again and again."""

@@ -185,6 +185,7 @@ def test_attention_refuses():
             (ValueError, lambda: paged_attention(q[..., :64], cache, softmax_scale=1.0)),
             (ValueError, lambda: paged_attention(q, cache, softmax_scale=1.0, layer=2)),
             (ValueError, lambda: paged_attention(q, cache, softmax_scale=0.0)),
+            (ValueError, lambda: paged_attention(q, cache, softmax_scale=1e-38)),
             (ValueError, lambda: paged_attention(q, cache, softmax_scale=float("nan"))),
             (ValueError, lambda: paged_attention(q, cache, softmax_scale=float("inf"))),
             (ValueError, lambda: paged_attention(q, cache, softmax_scale=1.0, window=-1)),
