@@ -11,13 +11,14 @@
 // sees whole is masked by a bit a row and lane.
 //
 // Bound by the matrix cores together with the softmax beside them: 2,048 queries
-// over 32k rows (32/8 heads, bf16) take 976 to 1,012 us from card to card, 1,050 to
-// 1,090 TFLOP/s; the products alone take 787 us, the softmax alone 615, and what the
-// one does not hide of the other is the rest.  The matrix cores are busy 58 % of the
-// cycles at the 1.85 GHz that the card keeps under this load (a library product of
-// 16,384^3: 1,385 TFLOP/s).  8 trees of 64 tokens over 4k to 16k rows each: 111 to
-// 124 us, 2.8 TB/s; there each workgroup walks some 38 tiles of its own, 2 us each,
-// and its first rows, its outputs and the join take a quarter of the time.
+// over 32k rows (32/8 heads, bf16) take 967 to 1,003 us from card to card, 1,060 to
+// 1,100 TFLOP/s, where a library product of 16,384^3 reaches 1,373 on the faster card.
+// The products alone took 787 us and the softmax alone 615 before the last two steps;
+// what the one does not hide of the other is the rest.  The matrix cores are busy 58 %
+// of the cycles at the 1.85 GHz that the card keeps under this load.  8 trees of 64
+// tokens over 4k to 16k rows each: 108 to 121 us, 3.0 TB/s; there each workgroup
+// walks some 38 tiles of its own, 2 us each, and its first rows, its outputs and the
+// join take a quarter of the time.
 //
 // Measured and not taken, for the 2,048 queries: matrix and vector work interleaved
 // in every wave in place of the groups' turns (1,147 us); copies from memory into LDS
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
       }
       return *reinterpret_cast<const uint4*>(k_at + 32 * ((k - HALF) % NI) * K_STRIDE + 16 * ((k - HALF) / NI));
     };
-    constexpr int AHEAD = 6;
+    constexpr int AHEAD = 3;  // 2,048 queries over 32k rows, one card: 1,004 us with 2, 1,003 with 3, 1,006 with 4, 1,016 with 6
     uint4 op[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) op[k] = operand(k);
