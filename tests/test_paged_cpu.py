@@ -278,7 +278,7 @@ def test_c_entries_refuse_bad_arguments(lib):
     half, whole = nat.TreeMasks(0x1000, None), nat.TreeMasks(0x1000, 0x1000)
     for change, rc in ((dict(layer=2), 1), (dict(query=_rows(0)), 1), (dict(query=_rows(0x1008)), 1), (dict(heads=3), 1),
                        (dict(heads=0), 1), (dict(heads=34), 2), (dict(tokens=0), 1), (dict(window=-1), 1), (dict(scale=0.0), 1),
-                       (dict(scale=float("nan")), 1), (dict(scale=2e30), 1), (dict(out=0), 1), (dict(out=0x1008), 1),
+                       (dict(scale=float("nan")), 1), (dict(scale=2e30), 1), (dict(scale=1e-31), 1), (dict(out=0), 1), (dict(out=0x1008), 1),
                        (dict(lse=0), 1), (dict(tree=ctypes.addressof(half)), 1), (dict(tokens=(1 << 20) + 1), 2),
                        (dict(tokens=513, tree=ctypes.addressof(whole)), 2)):
         assert lib.ckv_paged_attention(c, _attention_args(**change), None) == rc, change
