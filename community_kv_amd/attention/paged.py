@@ -428,7 +428,9 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, *, softmax_scale: 
     Returns (output [batch, tokens, query heads, 128] in the queries' dtype, lse
     [batch, query heads, tokens] float32, natural log); a query past the counts gives
     zeros and -inf.  What a query does not see does not reach it, infinities and NaN
-    included; an infinite value that it sees makes its output infinite or NaN."""
+    included; an infinite value that it sees makes its output infinite or NaN.  Scores
+    may be as large as products of finite queries and keys in 32 bits are, times the
+    scale; an lse beyond 32 bits is infinite."""
     _, batch, kv_heads, _, device = cache._facts
     _, heads, tokens, _ = _check_step(cache, layer, "query", query)
     if query.dtype != cache.key_pages.dtype:

@@ -10,6 +10,10 @@ namespace ckv {
 constexpr float PAGED_LN2 = 0.6931471805599453f;
 constexpr float PAGED_RESCALE = 8.0f;  // log2: how far scores may exceed the running maximum before it moves
 
+// Running maxima are kept of the products q . k, without the scale, and an exponent is (q . k - maximum) times the
+// scale: the difference first, which is exact where it matters, so the largest score's exponent is the 0 that it is.
+// Scaled first, a product of M log2 units is off by 2^-24 M, and from 2^25 on probabilities leave the types' range.
+
 // Probabilities are kept 2^bias times as large: at most 2^(8 + 7) fits fp16, and
 // ones below 2^-14 of the maximum, of which a long context has many, keep their
 // bits down to 2^-21 (2^-31 in steps).  bf16 has the exponents without it.
@@ -24,11 +28,12 @@ struct PagedAttendArgs {
   const uint64_t* masks;
   void* out;
   float* lse;
-  float* part_max;         // [kv_heads][row_pad][parts], log2
+  float* part_max;         // [kv_heads][row_pad][parts], unscaled
   float* part_sum;
   float* part_acc;         // [kv_heads][parts][row_pad][128]
   int2* part_of;           // [batch]: a sequence's first part and their number
   float scale_log2;        // softmax_scale * log2 e
+  float grow_by;           // PAGED_RESCALE / scale_log2
   int32_t tokens, group, rows, row_pad, window, parts, words, page_log2;
   uint32_t group_magic;    // ceil(2^32 / group), 0 for a group of one
 };
@@ -158,6 +163,12 @@ struct Sight {
     return seen;
   }
 };
+
+// The natural log of a sum of probabilities 2^bias times as large, relative to the maximum m.
+template <int DT>
+__device__ inline float paged_lse(const PagedAttendArgs& a, float m, float sum) {
+  return sum == 0.0f ? NEG_INF : (m * a.scale_log2 + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+}
 
 // Does a word hold a value that is not finite?
 template <int DT>

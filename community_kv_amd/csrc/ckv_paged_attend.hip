@@ -84,7 +84,7 @@ __device__ inline void value_operands(const uint4* v, uint4* op) {
   }
 }
 
-// The running softmax of 16 query rows over the steps of one wave.  m: log2
+// The running softmax of 16 query rows over the steps of one wave.  m: unscaled
 // maximum of query row c, the same on the four lane groups; l: sum over this
 // lane's rows alone; o: accumulators, element i of block nb is query row
 // 4 L + i, dim 8 c + nb.
@@ -94,15 +94,15 @@ struct Running {
 };
 
 template <int DT>
-__device__ inline void add_step(const float* sc, const uint4* vop, Running& r) {
+__device__ inline void add_step(const PagedAttendArgs& a, const float* sc, const uint4* vop, Running& r) {
   float top = sc[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[i]);
-  if (__ballot(top > r.m + PAGED_RESCALE) != 0) {
+  if (__ballot(top - r.m > a.grow_by) != 0) {
     float t = fmaxf(top, xor_f32<16>(top));
     t = fmaxf(t, xor_f32<32>(t));
-    t = t > r.m + PAGED_RESCALE ? t : r.m;  // a query's own scores alone decide
-    const float corr = r.m == t ? 1.0f : __builtin_amdgcn_exp2f(r.m - t);
+    t = t - r.m > a.grow_by ? t : r.m;  // a query's own scores alone decide
+    const float corr = r.m == t ? 1.0f : __builtin_amdgcn_exp2f((r.m - t) * a.scale_log2);
     const int L = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -113,11 +113,11 @@ __device__ inline void add_step(const float* sc, const uint4* vop, Running& r) {
     r.l *= corr;
     r.m = t;
   }
-  const float m = (r.m == NEG_INF ? 0.0f : r.m) - prob_bias<DT>();
+  const float m = r.m == NEG_INF ? 0.0f : r.m;
   float p[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    p[i] = __builtin_amdgcn_exp2f(sc[i] - m);
+    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i] - m, a.scale_log2, prob_bias<DT>()));
     r.l += p[i];
   }
   const uint4 aop = {pack_store<DT>(p[0], p[1]), pack_store<DT>(p[2], p[3]), pack_store<DT>(p[4], p[5]),
@@ -212,14 +212,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedA
 #pragma unroll
         for (int x = 0; x < 4; ++x) acc = mfma16<DT>(rows.k[j][x], query[r][x], acc);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[4 * j + i] = acc[i] * a.scale_log2;
+        for (int i = 0; i < 4; ++i) sc[4 * j + i] = acc[i];
       }
       if (masked) {
         seen[r] = good_rows ? (uint32_t)sight[r].rows(a, step, b, t0 + 8 * L) & 0xffu : 0u;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sc[i] = (seen[r] >> i) & 1 ? sc[i] : NEG_INF;
       }
-      add_step<DT>(sc, vop, run[r]);
+      add_step<DT>(a, sc, vop, run[r]);
     }
     if (special) {
       // values that were taken as zeros above, added for the queries that see their row
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedA
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       // a wave without a row has zeros and a maximum of -inf
-      const float f = __builtin_amdgcn_exp2f(m_s[w][i] - at);
+      const float f = __builtin_amdgcn_exp2f((m_s[w][i] - at) * a.scale_log2);
       const float4 x = *reinterpret_cast<const float4*>(&o_s[w][i * D + d]), y = *reinterpret_cast<const float4*>(&o_s[w][i * D + d + 4]);
       sum += l_s[w][i] * f;
       const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedA
       *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at_out + d) =
           uint4{pack_store<DT>(acc[0], acc[1]), pack_store<DT>(acc[2], acc[3]), pack_store<DT>(acc[4], acc[5]),
                 pack_store<DT>(acc[6], acc[7])};
-      if (d == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+      if (d == 0) a.lse[at_lse] = paged_lse<DT>(a, m, sum);
     } else {
       float4* to = reinterpret_cast<float4*>(a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + row) * D + d);
       to[0] = float4{acc[0], acc[1], acc[2], acc[3]};
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAtt
   const float at = m == NEG_INF ? 0.0f : m;
   float sum = 0.0f;
   for (int s = tid; s < part.y; s += JOIN_THREADS) {
-    const float f = __builtin_amdgcn_exp2f(pm[s] - at);
+    const float f = __builtin_amdgcn_exp2f((pm[s] - at) * a.scale_log2);
     factor[s] = f;
     sum += pl[s] * f;
   }
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAtt
     for (int g = 0; g < JOIN_THREADS / 32; ++g) x += reinterpret_cast<const float*>(acc_s)[g * D + tid];
     store_value<DT>(a.out, at_out + tid, sum == 0.0f ? 0.0f : x / sum);
   }
-  if (tid == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+  if (tid == 0) a.lse[at_lse] = paged_lse<DT>(a, m, sum);
 }
 
 // The same for many query rows, of few parts mostly: half a wave a row, four dims a lane; the first parts' outputs are
@@ -412,14 +412,14 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_rows_kernel(const Pag
     float top = m;
 #pragma unroll
     for (int i = 0; i < TOGETHER; ++i) top = fmaxf(top, ms[i]);
-    const float at = top == NEG_INF ? 0.0f : top, before = __builtin_amdgcn_exp2f(m - at);
+    const float at = top == NEG_INF ? 0.0f : top, before = __builtin_amdgcn_exp2f((m - at) * a.scale_log2);
     m = top;
     sum *= before;
     acc = float4{acc.x * before, acc.y * before, acc.z * before, acc.w * before};
 #pragma unroll
     for (int i = 0; i < TOGETHER; ++i) {
       if (i >= left) break;
-      const float f = __builtin_amdgcn_exp2f(ms[i] - at);
+      const float f = __builtin_amdgcn_exp2f((ms[i] - at) * a.scale_log2);
       sum += ls[i] * f;
       acc.x += xs[i].x * f;
       acc.y += xs[i].y * f;
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_rows_kernel(const Pag
   const float4 x = sum == 0.0f ? float4{0.0f, 0.0f, 0.0f, 0.0f} : float4{acc.x * scale, acc.y * scale, acc.z * scale, acc.w * scale};
   *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at_out + 4 * lane) =
       uint2{pack_store<DT>(x.x, x.y), pack_store<DT>(x.z, x.w)};
-  if (lane == 0) a.lse[at_lse] = sum == 0.0f ? NEG_INF : (m + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+  if (lane == 0) a.lse[at_lse] = paged_lse<DT>(a, m, sum);
 }
 
 constexpr int64_t MAX_ROWS = 1 << 21;  // query rows of a head: the grids' second dimension holds their blocks
@@ -572,6 +572,7 @@ extern "C" int ckv_paged_attention(const ckv_paged_cache* cache, const ckv_paged
   a.part_acc = reinterpret_cast<float*>(ws + lay.acc);
   a.part_of = reinterpret_cast<int2*>(ws + lay.of);
   a.scale_log2 = (float)((double)args->softmax_scale * 1.4426950408889634);
+  a.grow_by = (float)((double)PAGED_RESCALE / (double)a.scale_log2);
   a.tokens = tokens;
   a.group = group;
   a.group_magic = group > 1 ? (uint32_t)(((1ull << 32) + group - 1) / group) : 0u;

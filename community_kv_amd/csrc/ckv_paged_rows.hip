@@ -146,7 +146,6 @@ __device__ inline void write_rows(const PagedAttendArgs& a, int b, int h, int nu
                                   float l, const f32x16_t* o, float* out_s) {
   const int lane = threadIdx.x & 63, half = lane >> 5, row = row0 + (lane & 31);
   const float sum = live ? add_xor32(l) : 0.0f;
-  const float top = m == NEG_INF ? 0.0f : m * a.scale_log2;
   const bool none = joined ? !live : sum == 0.0f;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, factor = joined ? 1.0f : inv;
 #pragma unroll
@@ -185,13 +184,13 @@ __device__ inline void write_rows(const PagedAttendArgs& a, int b, int h, int nu
   }
   if (half != 0 || row >= a.rows) return;
   if (joined) {
-    a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m == NEG_INF || !live ? NEG_INF : top;
+    a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = live ? m : NEG_INF;
     a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
     return;
   }
   int64_t at_out, at_lse;
   paged_output_index(a, b, h, row, &at_out, &at_lse);
-  a.lse[at_lse] = sum == 0.0f ? NEG_INF : (top + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+  a.lse[at_lse] = paged_lse<DT>(a, m, sum);
 }
 
 template <int DT, int W, int KEYS>
@@ -240,7 +239,6 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
   }
 
   const float sl2 = a.scale_log2;
-  const float grow_by = PAGED_RESCALE / sl2;
   float m = NEG_INF;  // running maximum of the unscaled scores, shared by a row's two lanes
   float l = 0.0f;     // this lane's share of the sum
   // S^T of a tile: accumulator i holds cache rows 32 i + 8 (v / 4) + 4 half + v % 4 of the lane's query
@@ -342,15 +340,31 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
 #pragma unroll
     for (int x = 1; x < 2 * NI; ++x) all = max3(all, tops[x], tops[x]);
     const float top = max_xor32(all);
-    if (__ballot(top > m + grow_by) != 0) {
-      const float t = top > m + grow_by ? top : m;  // a query's own scores alone decide
+    if (__ballot(top - m > a.grow_by) != 0) {
+      const float t = top - m > a.grow_by ? top : m;  // a query's own scores alone decide
       const float f = m == t ? 1.0f : __builtin_amdgcn_exp2f((m - t) * sl2);
       m = t;
       l *= f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] *= f;
     }
-    const float mc = (m == NEG_INF ? 0.0f : m * sl2) - prob_bias<DT>();
+    // The scaled maximum's rounding is a factor of all of a query's probabilities, 2^-14 away from one at most up to
+    // EXACT, and saves a subtraction a score.  Beyond, the differences are taken before they are scaled.
+    constexpr float EXACT = 1024.0f;
+    const float m0 = m == NEG_INF ? 0.0f : m;
+    float mc = m0 * sl2;
+    const bool far = !(fabsf(mc) <= EXACT);
+    if (__ballot(far) != 0) {
+      asm volatile("");
+      const float base = far ? m0 : 0.0f;  // the other queries' scores stay as they are
+      if (far) mc = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sc[i][v] -= base;
+      }
+    }
+    mc -= prob_bias<DT>();
     float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NI; ++i) {

@@ -722,7 +722,8 @@ int ckv_paged_append(const ckv_paged_cache* cache, const ckv_paged_append_args* 
  * position is above its own minus window.  query strided as above in the cache's
  * dtype, out [batch][tokens][query_heads][128], lse [batch][query_heads][tokens]
  * (natural log); a query that attends no row, or with t >= counts[b], gives zeros
- * and -inf.  softmax_scale: 1e-30 to 1e30.  workspace:
+ * and -inf.  softmax_scale: 1e-30 to 1e30; an lse beyond 32 bits is infinite, the
+ * output right all the same.  workspace:
  * ckv_paged_attention_workspace_bytes() bytes, this call's alone. */
 typedef struct ckv_paged_attention_args {
   ckv_quant_rows query;
