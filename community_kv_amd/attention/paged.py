@@ -217,7 +217,9 @@ class DraftTree:
     """The drafted tokens of a step, made once and used by every layer.  Token
     ``t`` stands ``depths[b, t]`` positions behind the first drafted ones, and
     bit ``j % 64`` of ``masks[b, t, j // 64]`` is set where ``j`` is ``t`` or one
-    of its ancestors.
+    of its ancestors.  A caller's own depths and masks may be any: tokens in any
+    order, depths from 0 on (negative ones count as 0, ones from 2**30 on as
+    2**30 - 1), any set of drafted tokens to attend.
 
     ``depths`` [batch, tokens] int32, ``masks`` [batch, tokens, ceil(tokens / 64)]
     int64, ``counts`` [batch] int32 (tokens of each sequence) or None."""

@@ -19,6 +19,8 @@ __device__ inline int paged_length(const ckv_paged_cache& c, int b) {
 __device__ inline int step_count(const int32_t* counts, int tokens, int b) {
   return counts ? min(max(gload_i32(counts + b), 0), tokens) : tokens;
 }
+// A drafted token's depth: any number from 0 on, in any order of the tokens; below 2^30, so positions stay in 31 bits.
+__device__ inline int draft_depth(const int32_t* depths, int64_t at) { return min(max(gload_i32(depths + at), 0), (1 << 30) - 1); }
 
 // Two values rounded to the cache's type (to nearest even).
 template <int DT>

@@ -190,8 +190,8 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const AppendArgs a) {
     int page = -1;
     if (row < paged_capacity(c)) page = gload_i32(c.page_table + (int64_t)b * c.table_pages + (row >> paged_log2(c)));
     if (x < pairs && 8 * share < turned) {
-      const int depth = a.depths ? gload_i32(a.depths + (int64_t)b * a.tokens + t) : t;
-      const int64_t at = (int64_t)min(max(start + depth, 0), a.rotary.positions - 1) * half + 8 * x;
+      const int depth = a.depths ? draft_depth(a.depths, (int64_t)b * a.tokens + t) : t;
+      const int64_t at = (int64_t)min(start + depth, a.rotary.positions - 1) * half + 8 * x;
       Eight<CKV_F32> table[2];
       table[0].load(a.rotary.cosines, at);
       table[1].load(a.rotary.sines, at);

@@ -110,8 +110,9 @@ struct PagedHead {
   }
 };
 
-// What one query row sees: rows lo .. hi, and of a tree's rows (start and on) those of its mask, whose first word is
-// kept (trees of up to 64 tokens have no other).
+// What one query row sees: positions from lo on in rows up to hi, and of a tree's rows (start and on) those of its mask,
+// whose first word is kept (trees of up to 64 tokens have no other).  A committed row's position is its number, a draft
+// row's goes by its depth alone, which may be less or more than its place in the draft.
 struct Sight {
   int lo, hi, token;
   bool live;
@@ -125,7 +126,7 @@ struct Sight {
     if (a.masks) {
       const int64_t at = (int64_t)b * a.tokens + token;
       kin0 = a.masks[at * a.words];
-      position = s.start + gload_i32(a.depths + at);
+      position = s.start + draft_depth(a.depths, at);
     }
     lo = a.window > 0 ? max(position - a.window + 1, 0) : 0;
     hi = min(a.masks ? s.total : s.start + token + 1, s.total) - 1;
@@ -133,7 +134,7 @@ struct Sight {
   }
   // Bit i: row `first` + i is seen, i below 64 (or as many as the caller reads).
   __device__ uint64_t rows(const PagedAttendArgs& a, const PagedStep& s, int b, int first) const {
-    const int low = max(lo - first, 0), high = min(hi - first, 63);
+    const int low = max((a.masks ? min(lo, s.start) : lo) - first, 0), high = min(hi - first, 63);
     if (high < low || low > 63) return 0;
     uint64_t seen = (~0ull >> (63 - high)) & (~0ull << low);
     if (a.masks && first + 63 >= s.start) {
@@ -151,12 +152,12 @@ struct Sight {
         }
       }
       seen &= kin;
-      if (lo > s.start) {  // ancestors out of the window: a draft row's position goes by its depth
+      if (lo > s.start) {  // draft rows out of the window
         uint64_t drafted = seen & (j < 0 ? ~0ull << -j : ~0ull);
         while (drafted) {
           const int i = __ffsll((unsigned long long)drafted) - 1;
           drafted &= drafted - 1;
-          if (s.start + gload_i32(a.depths + (int64_t)b * a.tokens + j + i) < lo) seen &= ~(1ull << i);
+          if (s.start + draft_depth(a.depths, (int64_t)b * a.tokens + j + i) < lo) seen &= ~(1ull << i);
         }
       }
     }
@@ -168,6 +169,20 @@ struct Sight {
 template <int DT>
 __device__ inline float paged_lse(const PagedAttendArgs& a, float m, float sum) {
   return sum == 0.0f ? NEG_INF : (m * a.scale_log2 + (__log2f(sum) - prob_bias<DT>())) * PAGED_LN2;
+}
+
+// The first position that all of a wave's queries see in a window over a tree.
+template <int N>
+__device__ inline int wave_newest_lo(const Sight (&sight)[N]) {
+  int most = 0;
+#pragma unroll
+  for (int r = 0; r < N; ++r) most = max(most, sight[r].live ? sight[r].lo : 0);
+  most = max(most, (int)xor_u32<1>((uint32_t)most));
+  most = max(most, (int)xor_u32<2>((uint32_t)most));
+  most = max(most, (int)xor_u32<4>((uint32_t)most));
+  most = max(most, (int)xor_u32<8>((uint32_t)most));
+  most = max(most, (int)xor_u32<16>((uint32_t)most));
+  return __builtin_amdgcn_readfirstlane(max(most, (int)xor_u32<32>((uint32_t)most)));
 }
 
 // Does a word hold a value that is not finite?

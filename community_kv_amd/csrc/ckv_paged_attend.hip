@@ -159,7 +159,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedA
     end = min(end, step.start + last_token + 1);
     if (a.window > 0) begin = max(begin, max(step.start + first_token - a.window + 1, 0) & -PART_UNIT);
   }
-  if (a.window > 0) clear_lo = step.start + (a.masks ? step.count - 1 : last_token) - a.window + 1;
+  if (a.window > 0 && !a.masks) clear_lo = step.start + last_token - a.window + 1;
   if (first_token >= step.count) end = begin;
   clear_hi = min(clear_hi, step.total - 1);
 
@@ -179,6 +179,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedA
   Sight sight[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) sight[r] = Sight(a, step, b, row0 + 16 * r + col);
+  if (a.window > 0 && a.masks) clear_lo = wave_newest_lo(sight);
   const int last = step.total - 1;
   auto add = [&](StepRows& rows, const StepPages& pages, int t0) __attribute__((always_inline)) {
     const bool bad = __ballot(!q.good(pages.k) || !q.good(pages.v)) != 0;

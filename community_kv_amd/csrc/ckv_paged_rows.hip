@@ -98,6 +98,7 @@ struct TilesLds {
   alignas(16) uint16_t k[2][KEYS * K_STRIDE];
   alignas(16) uint16_t v[2][KEYS * V_STRIDE];
   int special[2];  // the tile, where its values held infinity or NaN that was staged as zero
+  int newest_lo[8];  // of each wave's queries, with a window over a tree
 };
 
 // LDS of a workgroup: the tiles, or the output rows on their way out.
@@ -107,7 +108,8 @@ constexpr size_t rows_lds_bytes() {
   return out > sizeof(TilesLds<KEYS>) ? out : sizeof(TilesLds<KEYS>);
 }
 
-// Rows that some of the query rows `first` to `first + rows` see, and those that all of them see.
+// Rows that some of the query rows `first` to `first + rows` see, and those that all of them see (but for all_lo of a
+// tree, where it goes by the depths).
 __device__ inline void ranges_of(const PagedAttendArgs& a, const PagedStep& step, int first, int rows, int* some_lo,
                                  int* some_hi, int* all_lo, int* all_hi) {
   const int t0 = paged_token(a, first), t1 = min(paged_token(a, min(first + rows, a.rows) - 1), step.count - 1);
@@ -116,12 +118,11 @@ __device__ inline void ranges_of(const PagedAttendArgs& a, const PagedStep& step
   *some_hi = -1;
   *all_hi = 0x7ffffffe;  // without a query nothing is masked: the rows are dropped at the end
   if (first >= a.rows || t0 > t1) return;
-  const int newest = a.masks ? step.count - 1 : t1, oldest = a.masks ? 0 : t0;  // positions of the tokens, from start on
-  *some_hi = min(step.start + newest, last);
+  *some_hi = min(step.start + (a.masks ? step.count - 1 : t1), last);
   *all_hi = min(a.masks ? step.start - 1 : step.start + t0, last);
   if (a.window > 0) {
-    *some_lo = max(step.start + oldest - a.window + 1, 0);
-    *all_lo = max(step.start + newest - a.window + 1, 0);
+    *some_lo = max(step.start + (a.masks ? 0 : t0) - a.window + 1, 0);
+    if (!a.masks) *all_lo = max(step.start + t1 - a.window + 1, 0);
   }
 }
 
@@ -285,6 +286,12 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
   int stage = 0;  // X_i has its values in v[i & 1], its keys in k[(i + 1) & 1]
   f32x16_t sc[NI];
   if (tid < 2) lds.special[tid] = -1;
+  const bool tree_window = a.masks && a.window > 0;
+  if (tree_window) {
+    const Sight mine[1] = {see};
+    wave_lo = wave_newest_lo(mine);
+    if (lane == 0) lds.newest_lo[wave] = wave_lo;
+  }
   TilePages<W, KEYS> p0, p1;
   const int t1 = min(t0 + 1, last_tile), t2 = min(t0 + 2, last_tile);
   if (left > 0) {
@@ -295,6 +302,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
     load_tile<W, KEYS>(q, q.values, wave, t0, p0, vc);
   }
   bad = __syncthreads_or(bad);  // with the first rows on their way
+  if (tree_window) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) group_lo = max(group_lo, __builtin_amdgcn_readfirstlane(lds.newest_lo[w]));
+  }
   if (left > 0) {
     store_tile<W, KEYS>(kc, lds.k[0], K_STRIDE);
     load_tile<W, KEYS>(q, q.keys, wave, t1, p1, kc);

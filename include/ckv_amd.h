@@ -671,7 +671,9 @@ typedef struct ckv_paged_cache {
 
 /* A step's drafted tokens as trees over the committed rows: token t's position
  * is lengths[b] + depths[b][t], and it attends the drafted tokens whose bit is
- * set in its mask (bit j % 64 of word j / 64; ceil(tokens / 64) words). */
+ * set in its mask (bit j % 64 of word j / 64; ceil(tokens / 64) words).  Depths
+ * and masks may be any: parents behind their children, depths beyond the tokens'
+ * number; negative depths count as 0, ones from 2^30 on as 2^30 - 1. */
 typedef struct ckv_draft_tree {
   const int32_t* depths;       /* [batch][tokens] */
   const uint64_t* masks;       /* [batch][tokens][ceil(tokens / 64)] */

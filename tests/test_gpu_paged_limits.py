@@ -7,9 +7,9 @@ import numpy as np
 import pytest
 import torch
 
-from community_kv_amd import paged_attention
+from community_kv_amd import DraftTree, RotaryTable, paged_append, paged_attention
 from oracle import paged as op
-from tests.test_gpu_paged import BF16, D, F16, HALF_STEP, LARGE, SCALE, _cache, _host
+from tests.test_gpu_paged import BF16, D, F16, HALF_STEP, LARGE, SCALE, _cache, _host, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,102 @@ def test_attend_far_scores_beside_ordinary_ones(device, group, tokens, capacity,
     want, size, _ = _best_rows(cache, query, SCALE)
     off = np.abs(_host(b[0]) - want)[:, :, 1] - (HALF_STEP[dtype] * np.abs(want) + 2.0 ** -25 + 32 * op.U * size)[:, :, 1]
     assert (off <= 0).all()
+
+
+# ------------------------------------------------------------------------------------------ trees that the caller makes
+
+class _Given(op.Paged):
+    """The oracle over given (depths, kin) of every sequence in the place of parents."""
+
+    @staticmethod
+    def _steps(tokens, trees, counts, b):
+        count = tokens if counts is None else min(max(int(counts[b]), 0), tokens)
+        depths, kin = trees[b]
+        return [min(max(d, 0), 2 ** 30 - 1) for d in depths[:count]], [[j for j in k if j < count] for k in kin[:count]]
+
+
+def _given_tree(gen, device, batch, tokens, order, counts=None):
+    """Depths and masks in orders that no plan makes."""
+    trees = []
+    for _ in range(batch):
+        if order == "backwards":  # a chain whose last token comes first
+            depths = list(range(tokens - 1, -1, -1))
+            kin = [list(range(t, tokens)) for t in range(tokens)]
+        else:
+            most = {"near": 2, "far": 3 * tokens + 40, "limits": 1}[order]
+            depths = torch.randint(0, most, (tokens,), generator=gen).tolist()
+            if order == "limits":
+                depths = [(-5, 0, 2 ** 31 - 1, 2 ** 30 - 1, -2 ** 31)[t % 5] for t in range(tokens)]
+            kin = [sorted(torch.randperm(tokens, generator=gen)[:int(torch.randint(0, tokens + 1, (1,), generator=gen))].tolist())
+                   for _ in range(tokens)]
+            kin = [sorted(set(k) | {t}) if t % 3 else k for t, k in enumerate(kin)]  # some do not see themselves
+        trees.append((depths, kin))
+    masks = np.zeros((batch, tokens, -(-tokens // 64)), np.uint64)
+    for b, (_, kin) in enumerate(trees):
+        for t, k in enumerate(kin):
+            for j in k:
+                masks[b, t, j // 64] |= np.uint64(1) << np.uint64(j % 64)
+    tree = DraftTree(_i32([d for d, _ in trees], device), torch.from_numpy(masks.view(np.int64)).to(device),
+                     None if counts is None else _i32(counts, device))
+    return tree, trees
+
+
+@pytest.mark.parametrize("group,tokens,capacity", [(2, 2, 0), (1, 9, 0), (4, 7, 0), (4, 9, LARGE), (4, 40, LARGE), (2, 130, LARGE),
+                                                   (1, 200, 0)])
+@pytest.mark.parametrize("order", ["backwards", "near", "far", "limits"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attend_given_trees(device, group, tokens, capacity, order, dtype):
+    """A window goes by positions, a draft row's by its depth: trees listed from their ends, depths beyond the tokens'
+    number, equal ones, negative ones and ones near 2^31."""
+    gen = torch.Generator().manual_seed(tokens)
+    cache = _cache(device, gen, lengths=[300, 0, 65], room=tokens, page=32, dtype=dtype, capacity=capacity)
+    query = torch.randn(3, 2 * group, tokens, D, generator=gen).to(dtype)
+    for counts, window in ((None, 0), (None, 1), (None, 2), ([tokens, 2, tokens - 1], 6), (None, tokens + 20), (None, 3 * tokens + 90)):
+        print(f"given tree {order} {group} x {tokens} capacity={capacity} window={window} counts={counts}", flush=True)
+        tree, trees = _given_tree(gen, device, 3, tokens, order, counts)
+        out, lse = paged_attention(query.to(device), cache, softmax_scale=SCALE, tree=tree, window=window)
+        torch.cuda.synchronize()
+        want, tol = _Given.of(cache).attend(0, _host(query), scale=SCALE, parents=trees, counts=counts, window=window,
+                                            half_step=HALF_STEP[dtype])
+        live = ~np.isneginf(want[1])
+        assert np.array_equal(~np.isneginf(_host(lse)), live)
+        assert (np.abs(_host(lse)[live] - want[1][live]) <= tol[1][live]).all()
+        assert (np.abs(_host(out) - want[0]) <= tol[0]).all()
+
+
+@pytest.mark.parametrize("group,tokens,capacity", [(4, 7, 0), (4, 40, LARGE), (8, 40, LARGE)])
+def test_given_trees_keep_special_values_out(device, group, tokens, capacity):
+    """Values that are not finite in committed rows before every query's window, where depths are far beyond the tokens'
+    number: not seen, so no trace of them."""
+    gen = torch.Generator().manual_seed(31)
+    cache = _cache(device, gen, lengths=[300], heads=1, room=tokens, page=16, capacity=capacity)
+    query = torch.randn(1, group, tokens, D, generator=gen).to(device, BF16)
+    masks = torch.full((1, tokens, 1), (1 << tokens) - 1, dtype=torch.int64, device=device)
+    tree = DraftTree(torch.full((1, tokens), 250, dtype=torch.int32, device=device), masks)
+    window = 300  # positions 251 to 550: rows up to 250 are out of it
+    clean = paged_attention(query, cache, softmax_scale=SCALE, tree=tree, window=window)
+    for r in range(251):
+        cache.value_pages[0, cache.page_table[0, r // 16], 0, r % 16] = float("nan")
+        cache.key_pages[0, cache.page_table[0, r // 16], 0, r % 16] = float("inf")
+    got = paged_attention(query, cache, softmax_scale=SCALE, tree=tree, window=window)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[1], clean[1])
+
+
+@pytest.mark.parametrize("order", ["backwards", "near", "far", "limits"])
+def test_append_given_trees(device, order):
+    """Keys and queries turn by their depth, whatever it is; past the table's end by its last position."""
+    gen = torch.Generator().manual_seed(32)
+    batch, heads, tokens = 2, 2, 19
+    cache = _cache(device, gen, lengths=[60, 3], room=tokens + 120)
+    table = RotaryTable.from_frequencies((1e4 ** -(torch.arange(32) / 32)).double().to(device), cache.capacity)
+    key, value, query = (torch.randn(batch, n, tokens, D, generator=gen) for n in (heads, heads, 4))
+    tree, trees = _given_tree(gen, device, batch, tokens, order)
+    oracle = _Given.of(cache)
+    got = paged_append(cache, key.to(device), value.to(device), query=query.to(device), rotary=table, tree=tree)
+    torch.cuda.synchronize()
+    turned, written = oracle.append(0, _host(key), _host(value), _host(query), (_host(table.cosines), _host(table.sines)), False, trees)
+    size = 2.0 ** -8 * np.abs(turned) + 8 * op.U * float(query.abs().max()) + 2.0 ** -25
+    assert (np.abs(_host(got) - turned) <= size).all()
+    off = np.abs(_host(cache.key_pages) - oracle.keys)[0]
+    assert (off <= 2.0 ** -8 * np.abs(oracle.keys[0]) + 8 * op.U * float(key.abs().max()) + 2.0 ** -25)[written].all()
