@@ -242,6 +242,13 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
   const float sl2 = a.scale_log2;
   float m = NEG_INF;  // running maximum of the unscaled scores, shared by a row's two lanes
   float l = 0.0f;     // this lane's share of the sum
+  // Of the maximum, as it last moved: the score that moves it, and the exponents, (score - base) * sl2 - mc.  The rounding
+  // of the scaled maximum mc is a factor of all of a query's probabilities, 2^-14 away from one at most up to EXACT log2
+  // units, and it saves a subtraction a score (base is 0).  Beyond, mc is 0, and differences are taken before they are
+  // scaled.
+  constexpr float EXACT = 1024.0f;
+  float limit = NEG_INF, base = 0.0f, mc = -prob_bias<DT>();
+  bool any_far = false;  // in the wave
   // S^T of a tile: accumulator i holds cache rows 32 i + 8 (v / 4) + 4 half + v % 4 of the lane's query
   f32x16_t o[4];
 #pragma unroll
@@ -351,31 +358,28 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
 #pragma unroll
     for (int x = 1; x < 2 * NI; ++x) all = max3(all, tops[x], tops[x]);
     const float top = max_xor32(all);
-    if (__ballot(top - m > a.grow_by) != 0) {
-      const float t = top - m > a.grow_by ? top : m;  // a query's own scores alone decide
+    if (__ballot(top > limit) != 0) {
+      const float t = top > limit ? top : m;  // a query's own scores alone decide
       const float f = m == t ? 1.0f : __builtin_amdgcn_exp2f((m - t) * sl2);
       m = t;
       l *= f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] *= f;
+      mc = m == NEG_INF ? 0.0f : m * sl2;
+      const bool far = !(fabsf(mc) <= EXACT);
+      base = far ? m : 0.0f;  // the scores of the wave's other queries stay as they are
+      mc = (far ? 0.0f : mc) - prob_bias<DT>();
+      limit = far ? m : m + a.grow_by;  // far from 0 the sum is rounded by more than a probability may exceed its type
+      any_far = __ballot(far) != 0;
     }
-    // The scaled maximum's rounding is a factor of all of a query's probabilities, 2^-14 away from one at most up to
-    // EXACT, and saves a subtraction a score.  Beyond, the differences are taken before they are scaled.
-    constexpr float EXACT = 1024.0f;
-    const float m0 = m == NEG_INF ? 0.0f : m;
-    float mc = m0 * sl2;
-    const bool far = !(fabsf(mc) <= EXACT);
-    if (__ballot(far) != 0) {
+    if (any_far) {
       asm volatile("");
-      const float base = far ? m0 : 0.0f;  // the other queries' scores stay as they are
-      if (far) mc = 0.0f;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) sc[i][v] -= base;
       }
     }
-    mc -= prob_bias<DT>();
     float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
