@@ -105,6 +105,7 @@ EXPORTED_SYMBOLS = (
     "ckv_quant_evict_workspace_bytes",
     "ckv_quant_evict",
     "ckv_draft_tree_plan",
+    "ckv_draft_tree_plan_counts",
     "ckv_paged_append",
     "ckv_paged_attention_workspace_bytes",
     "ckv_paged_attention",
@@ -364,6 +365,8 @@ def lib() -> ctypes.CDLL:
     paged = ctypes.POINTER(PagedCache)
     handle.ckv_draft_tree_plan.argtypes = [_p, _p, _i32, _i32, _p, _p, _p]
     handle.ckv_draft_tree_plan.restype = ctypes.c_int
+    handle.ckv_draft_tree_plan_counts.argtypes = [_p, _p, _i32, _i32, _p, _p, _p, _p]
+    handle.ckv_draft_tree_plan_counts.restype = ctypes.c_int
     handle.ckv_paged_append.argtypes = [paged, ctypes.c_char_p, _p]
     handle.ckv_paged_append.restype = ctypes.c_int
     handle.ckv_paged_attention_workspace_bytes.argtypes = [paged, _i32, _i32, _i32]

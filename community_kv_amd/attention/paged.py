@@ -3,7 +3,7 @@
 No reference counterpart (its cache holds one sequence at fixed addresses): this
 is the cache of a server whose requests come and go, and of speculative
 decoding, where a step's tokens are a tree of drafts of which one path is kept.
-The kernels are ``ckv_draft_tree_plan``, ``ckv_paged_append``,
+The kernels are ``ckv_draft_tree_plan_counts``, ``ckv_paged_append``,
 ``ckv_paged_attention`` and ``ckv_paged_commit``.
 
 A step writes its tokens behind every sequence's committed rows and attends to
@@ -222,7 +222,9 @@ class DraftTree:
     2**30 - 1), any set of drafted tokens to attend.
 
     ``depths`` [batch, tokens] int32, ``masks`` [batch, tokens, ceil(tokens / 64)]
-    int64, ``counts`` [batch] int32 (tokens of each sequence) or None."""
+    int64, ``counts`` [batch] int32 (tokens of each sequence) or None: a caller's
+    own are kept by reference and stay as they are until the last layer's call;
+    those of ``from_parents`` are the tree's."""
 
     __slots__ = ("depths", "masks", "counts", "_struct", "_facts")
 
@@ -250,7 +252,7 @@ class DraftTree:
         """``parents`` [batch, tokens] int32 names each token's parent, an earlier
         token of the draft; any other value (-1) makes it a child of the last
         committed token.  ``counts`` (int32, clamped to [0, tokens]): the first
-        tokens of each sequence that are there."""
+        tokens of each sequence that are there.  Neither is needed afterwards."""
         if parents.dtype != torch.int32:
             raise TypeError(f"parents must use int32, not {parents.dtype}")
         shape = parents.shape
@@ -260,19 +262,23 @@ class DraftTree:
         if tokens > MAX_DRAFT:
             raise ValueError(f"a tree may have at most {MAX_DRAFT} tokens, not {tokens}")
         device = parents.get_device()
-        counts_at = 0
+        counts_at = kept_at = 0
+        kept = None
         if counts is not None:
             counts = _counts_vector(counts, batch, device)
             counts_at = counts.data_ptr()
         if device < 0:
             raise RuntimeError(_NEED_GPU)
+        if counts is not None:
+            kept = counts.new_empty(batch)
+            kept_at = kept.data_ptr()
         parents = parents.contiguous()
         depths = parents.new_empty((batch, tokens))
         masks = parents.new_empty((batch, tokens, (tokens + 63) // 64), dtype=torch.int64)
         tree = cls.__new__(cls)
-        tree._hold(depths, masks, counts, batch, tokens, device)
-        _launch(device, nat.lib().ckv_draft_tree_plan, parents.data_ptr(), counts_at, batch, tokens, depths.data_ptr(),
-                masks.data_ptr())
+        tree._hold(depths, masks, kept, batch, tokens, device)
+        _launch(device, nat.lib().ckv_draft_tree_plan_counts, parents.data_ptr(), counts_at, batch, tokens, depths.data_ptr(),
+                masks.data_ptr(), kept_at)
         return tree
 
     @property

@@ -63,11 +63,12 @@ constexpr int MAX_WORDS = CKV_MAX_DRAFT / 64;
 __global__ __launch_bounds__(CKV_MAX_DRAFT) void tree_plan_kernel(const int32_t* __restrict__ parents,
                                                                   const int32_t* __restrict__ counts, int tokens,
                                                                   int32_t* __restrict__ depths,
-                                                                  uint64_t* __restrict__ masks) {
+                                                                  uint64_t* __restrict__ masks, int32_t* kept) {
   __shared__ uint64_t own_s[CKV_MAX_DRAFT];  // a token's bits in its own word
   __shared__ int before_s[CKV_MAX_DRAFT];    // its last ancestor before that word, or -1
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, words = (tokens + 63) >> 6;
   const int count = step_count(counts, tokens, b);
+  if (kept && t == 0) kept[b] = count;
   int parent = -1;
   if (t < count) {
     const int p = parents[(int64_t)b * tokens + t];
@@ -344,15 +345,20 @@ __global__ __launch_bounds__(64) void advance_kernel(const CommitArgs a) {
 
 }  // namespace
 
-extern "C" int ckv_draft_tree_plan(const int32_t* parents, const int32_t* counts, int32_t batch, int32_t tokens,
-                                   int32_t* depths, uint64_t* masks, void* stream) {
+extern "C" int ckv_draft_tree_plan_counts(const int32_t* parents, const int32_t* counts, int32_t batch, int32_t tokens,
+                                          int32_t* depths, uint64_t* masks, int32_t* counts_out, void* stream) {
   const char* what = "ckv_draft_tree_plan";
   if (!parents || !depths || !masks) return paged_error(CKV_E_INVALID, what, "null argument");
   if (batch <= 0 || tokens <= 0) return paged_error(CKV_E_INVALID, what, "batch and tokens must be positive");
   if (tokens > CKV_MAX_DRAFT) return paged_error(CKV_E_LIMIT, what, "more than 512 tokens");
   tree_plan_kernel<<<batch, (tokens + 63) / 64 * 64, 0, reinterpret_cast<hipStream_t>(stream)>>>(parents, counts, tokens,
-                                                                                                 depths, masks);
+                                                                                                 depths, masks, counts_out);
   return paged_launched(what);
+}
+
+extern "C" int ckv_draft_tree_plan(const int32_t* parents, const int32_t* counts, int32_t batch, int32_t tokens,
+                                   int32_t* depths, uint64_t* masks, void* stream) {
+  return ckv_draft_tree_plan_counts(parents, counts, batch, tokens, depths, masks, nullptr, stream);
 }
 
 extern "C" int ckv_paged_append(const ckv_paged_cache* cache, const ckv_paged_append_args* args, void* stream) {

@@ -700,6 +700,12 @@ typedef struct ckv_rotary {
 int ckv_draft_tree_plan(const int32_t* parents, const int32_t* counts, int32_t batch, int32_t tokens,
                         int32_t* depths, uint64_t* masks, void* stream);
 
+/* The same, with the clamped counts that the masks were made for written to
+ * counts_out [batch] (may be null): the layers' calls take those, whatever becomes
+ * of counts. */
+int ckv_draft_tree_plan_counts(const int32_t* parents, const int32_t* counts, int32_t batch, int32_t tokens,
+                               int32_t* depths, uint64_t* masks, int32_t* counts_out, void* stream);
+
 /* Writes a step's keys and values into layer `layer`: token t < counts[b] (null:
  * tokens) into row lengths[b] + t, its key turned by the angles of position
  * lengths[b] + t (with depths: + depths[b][t]) where rotary is given, each value

@@ -9,7 +9,7 @@ import torch
 
 from community_kv_amd import DraftTree, RotaryTable, paged_append, paged_attention
 from oracle import paged as op
-from tests.test_gpu_paged import BF16, D, F16, HALF_STEP, LARGE, SCALE, _cache, _host, _i32
+from tests.test_gpu_paged import BF16, D, F16, HALF_STEP, LARGE, SCALE, _cache, _host, _i32, _parents
 
 pytestmark = pytest.mark.gpu
 
@@ -196,3 +196,29 @@ def test_append_given_trees(device, order):
     assert (np.abs(_host(got) - turned) <= size).all()
     off = np.abs(_host(cache.key_pages) - oracle.keys)[0]
     assert (off <= 2.0 ** -8 * np.abs(oracle.keys[0]) + 8 * op.U * float(key.abs().max()) + 2.0 ** -25)[written].all()
+
+
+def test_a_tree_keeps_its_counts(device):
+    """Parents and counts that are used again before the last layer leave the tree as it was planned."""
+    gen = torch.Generator().manual_seed(33)
+    tokens, given = 9, [9, 0, 4, 30, -2]
+    cache = _cache(device, gen, lengths=[40, 7, 90, 20, 3], room=tokens)
+    parents = _parents(gen, 5, tokens, "wide").to(device)
+    query = torch.randn(5, 4, tokens, D, generator=gen).to(device, BF16)
+    for counts in (_i32(given, device), _i32([x for x in given for _ in range(2)], device)[::2]):
+        tree = DraftTree.from_parents(parents, counts=counts)
+        before = paged_attention(query, cache, softmax_scale=SCALE, tree=tree)
+        counts.fill_(2)
+        parents_before = parents.clone()
+        parents.zero_()
+        after = paged_attention(query, cache, softmax_scale=SCALE, tree=tree)
+        pages = cache.key_pages.clone()
+        paged_append(cache, query[:, :2], query[:, 2:], tree=tree)
+        torch.cuda.synchronize()
+        assert tree.counts.tolist() == [9, 0, 4, 9, 0]
+        assert torch.equal(before[0], after[0]) and torch.equal(before[1], after[1])
+        changed = (cache.key_pages != pages).any(-1).sum().item()
+        assert changed == 2 * sum(tree.counts.tolist())  # rows of both heads
+        parents.copy_(parents_before)
+        cache.key_pages.copy_(pages)
+    assert DraftTree.from_parents(parents).counts is None
