@@ -268,9 +268,12 @@ struct CommitArgs {
   int32_t tokens, path_tokens;
 };
 
+// Tokens of sequence b to commit, as far as there are so many.
+__device__ inline int commit_count(const CommitArgs& a, int b) { return a.counts ? max(gload_i32(a.counts + b), 0) : a.tokens; }
+
 // Entries of sequence b's path that count: up to the first that does not ascend or lies past the table's rows (`room`).
 __device__ inline int path_length(const CommitArgs& a, int b, int room) {
-  const int lane = threadIdx.x & 63, count = step_count(a.counts, a.path_tokens, b);
+  const int lane = threadIdx.x & 63, count = min(commit_count(a, b), a.path_tokens);
   const int32_t* path = a.path + (int64_t)b * a.path_tokens;
   for (int j0 = 0; j0 < count; j0 += 64) {
     const int j = j0 + lane;
@@ -340,7 +343,7 @@ __global__ __launch_bounds__(THREADS) void move_kernel(const CommitArgs a) {
 __global__ __launch_bounds__(64) void advance_kernel(const CommitArgs a) {
   const ckv_paged_cache& c = a.cache;
   const int b = blockIdx.x, start = paged_length(c, b);
-  if (threadIdx.x == 0) c.lengths[b] = start + min(step_count(a.counts, a.tokens, b), paged_capacity(c) - start);
+  if (threadIdx.x == 0) c.lengths[b] = start + min(commit_count(a, b), paged_capacity(c) - start);
 }
 
 }  // namespace

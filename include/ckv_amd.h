@@ -748,12 +748,13 @@ size_t ckv_paged_attention_workspace_bytes(const ckv_paged_cache* cache, int32_t
                                            int32_t window);
 int ckv_paged_attention(const ckv_paged_cache* cache, const ckv_paged_attention_args* args, void* stream);
 
-/* Commits a step's tokens in all layers.  Without a path the first counts[b] (null:
- * tokens) are taken: lengths[b] += count, up to the table's rows.  path
+/* Commits a step's tokens in all layers: counts[b] of them, or where counts is null
+ * `tokens` of every sequence (with counts it is not read).  Without a path the first
+ * ones are taken: lengths[b] += count, up to the table's rows.  path
  * [batch][path_tokens] (path_tokens <= CKV_MAX_DRAFT) names the tokens to keep in
  * ascending order: row lengths[b] + j takes row lengths[b] + path[b][j] for
- * j < counts[b], and lengths[b] grows by their number.  The path ends at the first
- * entry that does not ascend or lies past the table's rows. */
+ * j < min(count, path_tokens), and lengths[b] grows by their number.  The path ends
+ * at the first entry that does not ascend or lies past the table's rows. */
 int ckv_paged_commit(const ckv_paged_cache* cache, int32_t tokens, const int32_t* counts, const int32_t* path,
                      int32_t path_tokens, void* stream);
 

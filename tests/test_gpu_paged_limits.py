@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from community_kv_amd import DraftTree, RotaryTable, paged_append, paged_attention
+from community_kv_amd import _native as nat
 from oracle import paged as op
 from tests.test_gpu_paged import BF16, D, F16, HALF_STEP, LARGE, SCALE, _cache, _host, _i32, _parents
 
@@ -222,3 +223,25 @@ def test_a_tree_keeps_its_counts(device):
         parents.copy_(parents_before)
         cache.key_pages.copy_(pages)
     assert DraftTree.from_parents(parents).counts is None
+
+
+# ------------------------------------------------------------------------------------------ commits through the C entry
+
+@pytest.mark.parametrize("counts", [None, [1, 3, 0], [9, -1, 4]])
+@pytest.mark.parametrize("tokens", [0, 2, 4, 2 ** 31 - 1])
+@pytest.mark.parametrize("with_path", [False, True])
+def test_commit_c_entry_counts(device, counts, tokens, with_path):
+    """`tokens` of every sequence where counts is null, with a path too (whose padding ascends); counts alone otherwise."""
+    gen = torch.Generator().manual_seed(34)
+    cache = _cache(device, gen, lengths=[10, 0, 33], room=20, layers=2)
+    path = [[0, 2, 5, 7], [1, 2, 3, 9], [3, 4, 5, 6]] if with_path else None
+    oracle = op.Paged.of(cache)
+    path_t, counts_t = (None if x is None else _i32(x, device) for x in (path, counts))
+    rc = nat.lib().ckv_paged_commit(cache._ref, tokens, None if counts is None else counts_t.data_ptr(),
+                                    path_t.data_ptr() if with_path else None, 4 if with_path else 0,
+                                    torch.cuda.current_stream(device).cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0
+    oracle.commit([tokens] * 3 if counts is None else counts, path)
+    assert np.array_equal(cache.lengths.cpu().numpy(), oracle.lengths)
+    assert np.array_equal(_host(cache.key_pages), oracle.keys) and np.array_equal(_host(cache.value_pages), oracle.values)
