@@ -28,13 +28,13 @@ struct PagedAttendArgs {
   const uint64_t* masks;
   void* out;
   float* lse;
-  float* part_max;         // [kv_heads][row_pad][parts], unscaled
+  float* part_max;         // [kv_heads][row_pad][slots], unscaled
   float* part_sum;
-  float* part_acc;         // [kv_heads][parts][row_pad][128]
-  int2* part_of;           // [batch]: a sequence's first part and their number
+  float* part_acc;         // [kv_heads][slots][row_pad][128]
+  int2* part_of;           // [batch]: the slot of a sequence's first part, and the number of parts
   float scale_log2;        // softmax_scale * log2 e
   float grow_by;           // PAGED_RESCALE / scale_log2
-  int32_t tokens, group, rows, row_pad, window, parts, words, page_log2;
+  int32_t tokens, group, rows, row_pad, window, parts, slots, words, page_log2;
   uint32_t group_magic;    // ceil(2^32 / group), 0 for a group of one
 };
 
@@ -61,10 +61,15 @@ struct PagedRows {
   }
 };
 
+// Where a part leaves its results for the join: -1, nowhere, where the sequence has no other.  With `extra` parts more than
+// sequences at most `extra` are cut, into 2 `extra` parts together.
+__device__ inline int part_slot(const Part& part) { return part.count > 1 ? part.first - part.whole + part.index : -1; }
+inline int part_slots(int parts, int batch) { return min(parts, 2 * (parts - batch)); }
+
 // The parts of a sequence, told to the join by its first one.
 __device__ inline void tell_parts(const PagedAttendArgs& a, const Part& part) {
   if (a.parts > a.cache.batch && part.index == 0 && blockIdx.x % a.cache.kv_heads == 0 && blockIdx.y == 0 && threadIdx.x == 0)
-    a.part_of[part.sequence] = int2{part.first, part.count};
+    a.part_of[part.sequence] = int2{part_slot(part), part.count};
 }
 
 // row / group without a division: exact while row * group < 2^32 (rows are below 2^22, groups at most 16).

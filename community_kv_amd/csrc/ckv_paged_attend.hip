@@ -146,6 +146,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedA
   const int b = part.sequence;
   if (b < 0) return;  // the join knows how many parts there are
   tell_parts(a, part);
+  const int slot = part_slot(part);
   const PagedStep step(a, b);
   const PagedHead q(a, b, h);
   // tokens of this workgroup's rows, and the rows that all and that any of them see
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedA
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
     }
-    if (part.count == 1) {
+    if (slot < 0) {
       int64_t at_out, at_lse;
       paged_output_index(a, b, h, row, &at_out, &at_lse);
       const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -316,12 +317,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedA
                 pack_store<DT>(acc[6], acc[7])};
       if (d == 0) a.lse[at_lse] = paged_lse<DT>(a, m, sum);
     } else {
-      float4* to = reinterpret_cast<float4*>(a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + row) * D + d);
+      float4* to = reinterpret_cast<float4*>(a.part_acc + (((int64_t)h * a.slots + slot) * a.row_pad + row) * D + d);
       to[0] = float4{acc[0], acc[1], acc[2], acc[3]};
       to[1] = float4{acc[4], acc[5], acc[6], acc[7]};
       if (d == 0) {
-        a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = m;
-        a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
+        a.part_max[((int64_t)h * a.row_pad + row) * a.slots + slot] = m;
+        a.part_sum[((int64_t)h * a.row_pad + row) * a.slots + slot] = sum;
       }
     }
   }
@@ -341,9 +342,9 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAtt
   __shared__ float scratch[4];
   __shared__ float4 acc_s[JOIN_THREADS];
   const int h = blockIdx.x, row = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-  const int2 part = a.part_of[b];  // the first and their number
+  const int2 part = a.part_of[b];  // the first one's slot and their number
   if (part.y == 1) return;  // written already
-  const int64_t first = ((int64_t)h * a.row_pad + row) * a.parts + part.x;
+  const int64_t first = ((int64_t)h * a.row_pad + row) * a.slots + part.x;
   const float *pm = a.part_max + first, *pl = a.part_sum + first;
   float m = NEG_INF;
   for (int s = tid & 63; s < part.y; s += 64) m = fmaxf(m, pm[s]);
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_kernel(const PagedAtt
   sum = (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
   const int dim = 4 * (tid & 31);
   float4 acc{0.0f, 0.0f, 0.0f, 0.0f};
-  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.x) * a.row_pad + row) * D + dim;
+  const float* pa = a.part_acc + (((int64_t)h * a.slots + part.x) * a.row_pad + row) * D + dim;
 #pragma unroll 4
   for (int s = tid >> 5; s < part.y; s += JOIN_THREADS / 32) {
     const float4 x = *reinterpret_cast<const float4*>(pa + (int64_t)s * a.row_pad * D);
@@ -393,9 +394,9 @@ __global__ __launch_bounds__(JOIN_THREADS) void paged_join_rows_kernel(const Pag
   if (row >= a.rows) return;
   const int2 part = a.part_of[b];
   if (part.y == 1) return;
-  const int64_t first = ((int64_t)h * a.row_pad + row) * a.parts + part.x;
+  const int64_t first = ((int64_t)h * a.row_pad + row) * a.slots + part.x;
   const float *pm = a.part_max + first, *pl = a.part_sum + first;
-  const float* pa = a.part_acc + (((int64_t)h * a.parts + part.x) * a.row_pad + row) * D + 4 * lane;
+  const float* pa = a.part_acc + (((int64_t)h * a.slots + part.x) * a.row_pad + row) * D + 4 * lane;
   const int64_t stride = (int64_t)a.row_pad * D;
   float m = NEG_INF, sum = 0.0f;
   float4 acc{0.0f, 0.0f, 0.0f, 0.0f};
@@ -458,7 +459,7 @@ constexpr int64_t LONG_WORK = 700000;
 
 // How a call is laid out: which kernel, how many parts, and the workspace.
 struct PagedLayout {
-  int parts, row_pad, tiles;  // tiles of 16 query rows a workgroup of the few-row kernel, 0: the many-row kernel
+  int parts, slots, row_pad, tiles;  // tiles of 16 query rows a workgroup of the few-row kernel, 0: the many-row kernel
   bool wide_join;
   size_t max, sum, acc, of, bytes;
   PagedLayout(const ckv_paged_cache* c, int tokens, int group, int window) {
@@ -494,7 +495,8 @@ struct PagedLayout {
       at += (size + 15) & ~(size_t)15;
       return here;
     };
-    const size_t each = parts > c->batch ? (size_t)c->kv_heads * row_pad * parts * sizeof(float) : 0;
+    slots = part_slots(parts, c->batch);
+    const size_t each = (size_t)c->kv_heads * row_pad * slots * sizeof(float);
     max = take(each);
     sum = take(each);
     acc = take(each * D);
@@ -581,6 +583,7 @@ extern "C" int ckv_paged_attention(const ckv_paged_cache* cache, const ckv_paged
   a.row_pad = lay.row_pad;
   a.window = window;
   a.parts = lay.parts;
+  a.slots = lay.slots;
   a.words = (tokens + 63) / 64;
   a.page_log2 = 31 - __builtin_clz((unsigned)cache->page_size);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -143,9 +143,10 @@ __device__ inline bool drop_special(TilePieces<W, KEYS>& t) {
 // share of the sum, o the outputs (o[i][v]: dim 32 i + 8 (v / 4) + 4 half + v % 4).  They go out through `out_s`, LDS of
 // the wave alone, 64 dims at a time, so that whole lines are written: from the accumulators a store would touch 32 lines.
 template <int DT>
-__device__ inline void write_rows(const PagedAttendArgs& a, int b, int h, int number, bool joined, int row0, bool live, float m,
+__device__ inline void write_rows(const PagedAttendArgs& a, int b, int h, int slot, int row0, bool live, float m,
                                   float l, const f32x16_t* o, float* out_s) {
   const int lane = threadIdx.x & 63, half = lane >> 5, row = row0 + (lane & 31);
+  const bool joined = slot >= 0;
   const float sum = live ? add_xor32(l) : 0.0f;
   const bool none = joined ? !live : sum == 0.0f;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, factor = joined ? 1.0f : inv;
@@ -167,7 +168,7 @@ __device__ inline void write_rows(const PagedAttendArgs& a, int b, int h, int nu
         const int local = 4 * j + (lane >> 4), r = row0 + local, dim = 64 * dims + 4 * (lane & 15);
         const float4 x = *reinterpret_cast<const float4*>(&out_s[local * O_STRIDE + 4 * (lane & 15)]);
         if (r < a.rows)
-          *reinterpret_cast<float4*>(a.part_acc + (((int64_t)h * a.parts + number) * a.row_pad + r) * D + dim) = x;
+          *reinterpret_cast<float4*>(a.part_acc + (((int64_t)h * a.slots + slot) * a.row_pad + r) * D + dim) = x;
       }
     } else {
 #pragma unroll
@@ -185,8 +186,8 @@ __device__ inline void write_rows(const PagedAttendArgs& a, int b, int h, int nu
   }
   if (half != 0 || row >= a.rows) return;
   if (joined) {
-    a.part_max[((int64_t)h * a.row_pad + row) * a.parts + number] = live ? m : NEG_INF;
-    a.part_sum[((int64_t)h * a.row_pad + row) * a.parts + number] = sum;
+    a.part_max[((int64_t)h * a.row_pad + row) * a.slots + slot] = live ? m : NEG_INF;
+    a.part_sum[((int64_t)h * a.row_pad + row) * a.slots + slot] = sum;
     return;
   }
   int64_t at_out, at_lse;
@@ -209,6 +210,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
   const int b = part.sequence;
   if (b < 0) return;
   tell_parts(a, part);
+  const int slot = part_slot(part);
   const PagedStep step(a, b);
   const PagedHead q(a, b, h);
   const int row = block0 + 32 * wave + (lane & 31);
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
     if (TURNS && !second && left == 0) __syncthreads();  // the second group's last slot
   }
 
-  write_rows<DT>(a, b, h, number, part.count > 1, block0 + 32 * wave, see.live, m, l, o,
+  write_rows<DT>(a, b, h, slot, block0 + 32 * wave, see.live, m, l, o,
                  reinterpret_cast<float*>(lds_raw) + wave * 32 * O_STRIDE);
 }
 

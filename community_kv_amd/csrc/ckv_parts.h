@@ -25,6 +25,7 @@ struct Part {
   int first;       // number of the sequence's first part
   int count;       // the sequence's parts
   int rows;        // rows of a part
+  int whole;       // earlier sequences that are one part
 };
 
 __device__ inline int wave_sum_i32(int v) {
@@ -69,22 +70,24 @@ __device__ inline Part find_part(const Lengths& c, int parts, int part, int want
   const int size = part_size(c, parts);
   if (parts <= c.batch()) {
     const int b = wanted < 0 ? part : wanted;
-    return Part{b, 0, b, 1, size};
+    return Part{b, 0, b, 1, size, b};
   }
   const int lane = threadIdx.x & 63;
-  int before = 0;
+  int before = 0, whole = 0;
   for (int b0 = 0; b0 < c.batch(); b0 += 64) {
     const int mine = b0 + lane < c.batch() ? parts_of_sequence(c(b0 + lane), size) : 0;
     const int end = before + wave_inclusive_scan(mine);  // parts up to and with this lane's sequence
     const uint64_t hit = wanted < 0 ? __ballot(mine > 0 && part < end) : __ballot(b0 + lane == wanted);
+    const uint64_t single = __ballot(mine == 1);
     if (hit) {
       const int at = __ffsll((unsigned long long)hit) - 1;
       const int count = __builtin_amdgcn_readlane(mine, at), first = __builtin_amdgcn_readlane(end, at) - count;
-      return Part{b0 + at, part - first, first, count, size};
+      return Part{b0 + at, part - first, first, count, size, whole + (int)__popcll(single & ((1ull << at) - 1))};
     }
     before = __builtin_amdgcn_readlane(end, 63);
+    whole += __popcll(single);
   }
-  return Part{-1, 0, 0, 0, size};
+  return Part{-1, 0, 0, 0, size, 0};
 }
 
 }  // namespace ckv

@@ -245,3 +245,32 @@ def test_commit_c_entry_counts(device, counts, tokens, with_path):
     oracle.commit([tokens] * 3 if counts is None else counts, path)
     assert np.array_equal(cache.lengths.cpu().numpy(), oracle.lengths)
     assert np.array_equal(_host(cache.key_pages), oracle.keys) and np.array_equal(_host(cache.value_pages), oracle.values)
+
+
+# ------------------------------------------------------------------------------------------ workspaces
+
+@pytest.mark.parametrize("batch,heads,group,tokens,long", [(70, 4, 1, 1, [5]), (70, 4, 1, 1, [0, 33, 64, 69]), (40, 8, 3, 9, [1, 39]),
+                                                           (18, 8, 2, 65, [17]), (18, 8, 2, 65, [0, 9]), (18, 2, 4, 130, [3, 4, 5, 6, 7]),
+                                                           (3, 2, 4, 70, [0, 1, 2]), (3, 2, 1, 1, [0, 2])])
+def test_workspace_of_mixed_batches(device, batch, heads, group, tokens, long):
+    """Sequences that are cut among ones that are not: results as the oracle's, nothing behind the workspace written."""
+    print(f"mixed batch {batch} {heads} x {group} x {tokens} long={long}", flush=True)
+    gen = torch.Generator().manual_seed(batch + tokens)
+    lengths = [int(x) for x in torch.randint(0, 60, (batch,), generator=gen)]
+    for i, b in enumerate(long):
+        lengths[b] = 3000 - 700 * i
+    cache = _cache(device, gen, lengths=lengths, heads=heads, room=tokens, page=32, capacity=8192)
+    query = torch.randn(batch, heads * group, tokens, D, generator=gen).to(BF16)
+    on = query.to(device)
+    size = nat.lib().ckv_paged_attention_workspace_bytes(cache._ref, heads * group, tokens, 0)
+    assert size > 0
+    out = torch.empty(batch, tokens, heads * group, D, dtype=BF16, device=device)
+    lse = torch.empty(batch, heads * group, tokens, device=device)
+    workspace = torch.full((size + 65536,), 0x5A, dtype=torch.uint8, device=device)
+    args = nat.PAGED_ATTENTION_ARGS.pack(on.data_ptr(), *on.stride()[:3], 0, 0, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
+                                         0, heads * group, tokens, 0, SCALE, 0)
+    assert nat.lib().ckv_paged_attention(cache._ref, args, torch.cuda.current_stream(device).cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert bool((workspace[size:] == 0x5A).all())
+    want, tol = op.Paged.of(cache).attend(0, _host(query), scale=SCALE)
+    assert (np.abs(_host(lse) - want[1]) <= tol[1]).all() and (np.abs(_host(out) - want[0]) <= tol[0]).all()

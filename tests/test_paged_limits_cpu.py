@@ -1,0 +1,26 @@
+"""Paged KV cache without a GPU: workspace sizes, refusals of gradients."""
+
+from __future__ import annotations
+
+import pytest
+
+from tests.test_paged_cpu import _c_cache, lib  # noqa: F401 (a fixture)
+
+
+@pytest.mark.parametrize("batch,heads,query_heads,tokens,pages", [(64, 8, 32, 512, 64), (64, 8, 32, 512, 128), (64, 8, 32, 1, 2048),
+                                                                  (24, 8, 32, 64, 256), (200, 1, 1, 1, 128)])
+def test_workspace_holds_the_parts_of_cut_sequences_alone(lib, batch, heads, query_heads, tokens, pages):  # noqa: F811
+    """Parts are cut for 512 workgroups (one token) or 256, or a batch that fills the chip gets batch / 2 more than
+    sequences at most, none over 32 units of 128 rows or fewer.  Each of the parts above the sequences cuts one more of them at
+    most, so twice as many have 32-bit outputs and two sums a query row."""
+    c = _c_cache(lib, batch=batch, kv_heads=heads, table_pages=pages, page_size=64)
+    rows = (tokens * (query_heads // heads) + 15) // 16 * 16
+    blocks = -(-rows // 256) if rows > 32 else 1
+    want = (512 if rows == 16 else 256) // (heads * blocks)
+    if want >= (2 * batch if rows > 32 else batch + 1):  # the kernel of many query rows is cut later
+        parts = want
+    else:
+        parts = batch + (min(want, batch // 2) if pages * 64 > 32 * 128 else 0)
+    slots = min(parts, 2 * (parts - batch))
+    size = lib.ckv_paged_attention_workspace_bytes(c, query_heads, tokens, 0)
+    assert (size > 0) == (slots > 0) and size <= slots * heads * rows * (128 + 2) * 4 + 8 * batch + 64
