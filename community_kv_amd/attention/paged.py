@@ -29,6 +29,7 @@ import ctypes
 from dataclasses import dataclass, field
 
 import torch
+from torch.autograd import forward_ad
 
 from community_kv_amd import _native as nat
 from community_kv_amd.attention.quantized import _rows
@@ -312,6 +313,13 @@ def _counts_vector(counts: torch.Tensor, batch: int, device: int) -> torch.Tenso
     return counts.contiguous()
 
 
+def _refuse_tangents(**tensors: torch.Tensor | None) -> None:
+    """Inside a forward_ad level (its number is negative outside, which a call looks at first)."""
+    for name, tensor in tensors.items():
+        if tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None:
+            raise RuntimeError(f"{name} carries a tangent; the paged cache has no forward-mode derivative")
+
+
 def _check_step(cache: PagedKVCache, layer: int, name: str, tensor: torch.Tensor) -> torch.Size:
     shape = tensor.shape
     layers, batch, _, _, device = cache._facts
@@ -375,6 +383,9 @@ def paged_append(cache: PagedKVCache, key: torch.Tensor, value: torch.Tensor, *,
     Tokens whose row is past the capacity or has no page are dropped and raise the
     overflow flag (``assert_no_overflow``)."""
     layers, batch, heads, capacity, device = cache._facts
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(key=key, value=value, query=query, key_pages=cache.key_pages, value_pages=cache.value_pages,
+                         cosines=None if rotary is None else rotary.cosines, sines=None if rotary is None else rotary.sines)
     shape, kind = key.shape, key.dtype
     dtype = _DTYPES.get(kind)
     if (dtype is None or value.dtype != kind or value.shape != shape or len(shape) != 4 or shape[1] != heads or
@@ -440,6 +451,8 @@ def paged_attention(query: torch.Tensor, cache: PagedKVCache, *, softmax_scale: 
     may be as large as products of finite queries and keys in 32 bits are, times the
     scale; an lse beyond 32 bits is infinite."""
     _, batch, kv_heads, _, device = cache._facts
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(query=query, key_pages=cache.key_pages, value_pages=cache.value_pages)
     _, heads, tokens, _ = _check_step(cache, layer, "query", query)
     if query.dtype != cache.key_pages.dtype:
         raise TypeError(f"query must use the cache's {cache.dtype}, not {query.dtype}")

@@ -3,8 +3,11 @@
 from __future__ import annotations
 
 import pytest
+import torch
+from torch.autograd import forward_ad
 
-from tests.test_paged_cpu import _c_cache, lib  # noqa: F401 (a fixture)
+from community_kv_amd import PagedKVCache, RotaryTable, paged_append, paged_attention
+from tests.test_paged_cpu import _c_cache, _cache, _table, _tensors, lib  # noqa: F401 (a fixture)
 
 
 @pytest.mark.parametrize("batch,heads,query_heads,tokens,pages", [(64, 8, 32, 512, 64), (64, 8, 32, 512, 128), (64, 8, 32, 1, 2048),
@@ -24,3 +27,26 @@ def test_workspace_holds_the_parts_of_cut_sequences_alone(lib, batch, heads, que
     slots = min(parts, 2 * (parts - batch))
     size = lib.ckv_paged_attention_workspace_bytes(c, query_heads, tokens, 0)
     assert (size > 0) == (slots > 0) and size <= slots * heads * rows * (128 + 2) * 4 + 8 * batch + 64
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives would be lost: every tensor that goes into the result is looked at; others pass."""
+    cache, x, q = _cache(dtype=torch.float16), torch.zeros(2, 2, 3, 128, dtype=torch.float16), torch.zeros(2, 4, 3, 128, dtype=torch.float16)
+    with forward_ad.dual_level():
+        x_dual, q_dual = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, q))
+        table = _table()
+        dual_table = RotaryTable(forward_ad.make_dual(table.cosines, table.sines), table.sines)
+        dual_pages = PagedKVCache(**(_tensors(cache) | dict(value_pages=forward_ad.make_dual(cache.value_pages,
+                                                                                            torch.ones_like(cache.value_pages)))))
+        for call in (lambda: paged_append(cache, x_dual, x), lambda: paged_append(cache, x, x_dual),
+                     lambda: paged_append(cache, x, x, query=q_dual, rotary=table),
+                     lambda: paged_append(cache, x, x, query=q, rotary=dual_table), lambda: paged_append(dual_pages, x, x),
+                     lambda: paged_attention(q_dual, cache, softmax_scale=1.0),
+                     lambda: paged_attention(q, dual_pages, softmax_scale=1.0)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                call()
+        for call in (lambda: paged_append(cache, x, x, query=q, rotary=table), lambda: paged_attention(q, cache, softmax_scale=1.0)):
+            with pytest.raises(RuntimeError, match="GPU"):
+                call()
