@@ -51,6 +51,8 @@ def _expect(name: str, tensor: torch.Tensor, dtype: torch.dtype, shape: tuple[in
         raise ValueError(f"{name} must be contiguous")
     if tensor.device != device:
         raise ValueError(f"{name} must be on {device}")
+    if tensor.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient; the paged cache has no backward pass (use torch.no_grad())")
 
 
 @dataclass(frozen=True, eq=False)

@@ -50,3 +50,28 @@ def test_tangents_are_refused():
         for call in (lambda: paged_append(cache, x, x, query=q, rotary=table), lambda: paged_attention(q, cache, softmax_scale=1.0)):
             with pytest.raises(RuntimeError, match="GPU"):
                 call()
+
+
+@pytest.mark.parametrize("name", ["key_pages", "value_pages"])
+def test_pages_that_require_a_gradient_are_refused(name):
+    """They are written in place, past autograd; under no_grad nobody asks for one."""
+    good = _tensors(_cache())
+    good[name] = torch.zeros_like(good[name]).requires_grad_()
+    with pytest.raises(RuntimeError, match="gradient"):
+        PagedKVCache(**good)
+    with torch.no_grad():
+        PagedKVCache(**good)
+
+
+def test_rotation_tables_that_require_a_gradient_are_refused():
+    angles = torch.rand(128, 64)
+    for cosines, sines in ((angles.clone().requires_grad_(), angles), (angles, angles.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="gradient"):
+            RotaryTable(cosines, sines)
+        with torch.no_grad():
+            RotaryTable(cosines, sines)
+    frequencies = torch.rand(16).requires_grad_()
+    with pytest.raises(RuntimeError, match="gradient"):
+        RotaryTable.from_frequencies(frequencies, 10)
+    with torch.no_grad():
+        assert RotaryTable.from_frequencies(frequencies, 10).positions == 10
