@@ -49,10 +49,12 @@ __device__ inline f32x16_t mfma32(uint4 a, uint4 b, f32x16_t c) {
   }
 }
 
-// Largest of three without the moves that quiet a NaN first; a NaN operand is passed over.
-__device__ inline float max3(float x, float y, float z) {
+// Largest of three without the moves that quiet a NaN first; a NaN operand is passed over.  The compiler keeps its own
+// reads of a matrix product far enough behind it, but does not see those in inline assembly: `behind`, an unused operand,
+// is the result of a read that it does see, of the products that these maxima are of.
+__device__ inline float max3(float x, float y, float z, float behind) {
   float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z), "v"(behind));
   return r;
 }
 
@@ -349,16 +351,18 @@ __global__ __launch_bounds__(64 * W, 2) void paged_rows_kernel(const PagedAttend
         for (int v = 0; v < 16; ++v) sc[i][v] = bits >> (8 * (v >> 2) + (v & 3)) & 1u ? sc[i][v] : NEG_INF;
       }
     }
+    const float read = __builtin_amdgcn_fmed3f(sc[0][15], sc[NI - 1][15], 0.0f);
     float tops[2 * NI];
 #pragma unroll
     for (int x = 0; x < 2 * NI; ++x) {
       const f32x16_t& v = sc[x >> 1];
       const int e = 8 * (x & 1);
-      tops[x] = max3(max3(v[e], v[e + 1], v[e + 2]), max3(v[e + 3], v[e + 4], v[e + 5]), max3(v[e + 6], v[e + 7], v[e + 7]));
+      tops[x] = max3(max3(v[e], v[e + 1], v[e + 2], read), max3(v[e + 3], v[e + 4], v[e + 5], read),
+                     max3(v[e + 6], v[e + 7], v[e + 7], read), read);
     }
     float all = tops[0];
 #pragma unroll
-    for (int x = 1; x < 2 * NI; ++x) all = max3(all, tops[x], tops[x]);
+    for (int x = 1; x < 2 * NI; ++x) all = max3(all, tops[x], tops[x], read);
     const float top = max_xor32(all);
     if (__ballot(top > limit) != 0) {
       const float t = top > limit ? top : m;  // a query's own scores alone decide
