@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from community_kv_amd import DraftTree, RotaryTable, paged_append, paged_attention
+from community_kv_amd import DraftTree, PagedKVCache, RotaryTable, paged_append, paged_attention
 from community_kv_amd import _native as nat
 from oracle import paged as op
 from tests.test_gpu_paged import BF16, D, F16, HALF_STEP, LARGE, SCALE, _cache, _host, _i32, _parents
@@ -274,3 +274,44 @@ def test_workspace_of_mixed_batches(device, batch, heads, group, tokens, long):
     assert bool((workspace[size:] == 0x5A).all())
     want, tol = op.Paged.of(cache).attend(0, _host(query), scale=SCALE)
     assert (np.abs(_host(lse) - want[1]) <= tol[1]).all() and (np.abs(_host(out) - want[0]) <= tol[0]).all()
+
+
+# ------------------------------------------------------------------------------------------ far places
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_far_rows_weigh_what_they_should(device, dtype):
+    """Nine million rows of key 0 in pages up to beyond 2^32 elements weigh 1 each; a few keys far apart, and the step's own
+    token, weigh e^16 each, about as much as all of the others together: each part of the sum shows in the result.
+
+    A lane adds at most 2^15 terms of a part, each with half a step of a sum below 2: 2^-24.  So its share, and with it the
+    sum, is off by at most 2^-9 of itself, and twice that where a probability next to a larger one is rounded too."""
+    print(f"far rows {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(35)
+    pages, heads = 140_000, 2  # 2.3 G elements a layer
+    cache = PagedKVCache.allocate(layers=2, batch=1, kv_heads=heads, capacity=pages * 64, page_size=64, dtype=dtype, device=device)
+    cache.page_table.copy_(cache.page_table.flip(1).clone())
+    n = pages * 64 - 3
+    cache.lengths.fill_(n)
+    far = [0, 77, 64 * 9_000 + 5, 64 * 70_000, 64 * 130_001 + 63, n - 1]  # pages 139,999 to 0
+    assert ((2 * pages - 1) * heads * 64 * D) > 2 ** 32
+    value = torch.randn(heads, len(far) + 1, D, generator=gen).to(dtype)
+    key = torch.zeros(heads, 1, D, dtype=dtype)
+    key[..., 0] = 16.0
+    for layer in range(2):
+        for i, r in enumerate(far):
+            page, at = int(cache.page_table[0, r // 64]), r % 64
+            cache.key_pages[layer, page, :, at, 0] = 16.0 if layer else -3.0  # the other layer's rows are others
+            cache.value_pages[layer, page, :, at] = value[:, i].to(device)
+    paged_append(cache, key[None].to(device), value[None, :, -1:].to(device), layer=1)
+    query = torch.zeros(1, heads, 40, D, dtype=dtype, device=device)
+    query[..., 0] = 1.0
+    rows = n - len(far)
+    z = rows + (len(far) + 1) * np.exp(16.0)
+    want = np.exp(16.0) / z * _host(value).sum(1)
+    size = np.exp(16.0) / z * np.abs(_host(value)).sum(1)
+    for tokens in (1, 40):  # few query rows, many
+        out, lse = paged_attention(query[:, :, :tokens], cache, layer=1, softmax_scale=1.0, counts=_i32([1], device))
+        torch.cuda.synchronize()
+        assert (np.abs(_host(lse)[0, :, 0] - np.log(z)) <= 2.0 ** -8).all()
+        assert (np.abs(_host(out)[0, 0] - want) <= (2.0 ** -8 + 2 * HALF_STEP[dtype]) * size + 2.0 ** -25).all()
+        assert not out[0, 1:].any() and bool(lse[0, :, 1:].isneginf().all())
