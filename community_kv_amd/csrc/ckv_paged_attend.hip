@@ -131,7 +131,7 @@ __device__ inline void add_step(const PagedAttendArgs& a, const float* sc, const
 // Keys and values go from memory into operands without LDS: each is used by one
 // wave alone.  Bound by memory on long caches: a token over 8 sequences of up to
 // 131k rows, 32/8 heads, in 418 us, 5.8 TB/s, where reading alone reaches 6.1;
-// by latency on short ones (one sequence of 300 rows: 7.1 us).  Two tiles of
+// by latency on short ones (one sequence of 300 rows: 7.3 us).  Two tiles of
 // query rows share what is read; four spill.
 template <int DT, int RT>
 __global__ __launch_bounds__(64 * WAVES, 2) void paged_split_kernel(const PagedAttendArgs a) {

@@ -11,12 +11,12 @@
 // sees whole is masked by a bit a row and lane.
 //
 // Bound by the matrix cores together with the softmax beside them: 2,048 queries
-// over 32k rows (32/8 heads, bf16) take 967 to 1,003 us from card to card, 1,060 to
-// 1,100 TFLOP/s, where a library product of 16,384^3 reaches 1,373 on the faster card.
+// over 32k rows (32/8 heads, bf16) take 971 to 1,015 us from card to card, 1,050 to
+// 1,097 TFLOP/s, where a library product of 16,384^3 reaches 1,373 on the faster card.
 // The products alone took 787 us and the softmax alone 615 before the last two steps;
 // what the one does not hide of the other is the rest.  The matrix cores are busy 60 %
 // of the cycles at the 1.75 to 1.85 GHz that the card keeps under this load.  8 trees of 64
-// tokens over 4k to 16k rows each: 108 to 121 us, 3.0 TB/s; there each workgroup
+// tokens over 4k to 16k rows each: 109 to 119 us, 2.7 to 3.0 TB/s; there each workgroup
 // walks some 38 tiles of its own, 2 us each, and its first rows, its outputs and the
 // join take a quarter of the time.
 //
